@@ -2,9 +2,11 @@
 
 All compute lives in `lib/libq4b200.so` (CUDA, built by `qwen38_metal_b200.build`); this package is the
 host-side mirror of the reference's projection interface over that library's C ABI
-(`include/q4b200.h`). There is no CPU or PyTorch compute path: without the library, or without a
+(`include/q4b200.h`), and of the attention calls that stand between projections (`include/q4b_attention.h`). There is no CPU or PyTorch compute path: without the library, or without a
 B200, constructing a runtime raises.
 """
-from .runtime import CudaRuntime, DeviceBuffer, MappedQ4AffineJob, Q4RuntimeError  # noqa: F401
+from .runtime import (CudaRuntime, DeviceBuffer, KvCache, KvTable, MappedQ4AffineJob, Q4RuntimeError, Rotary,  # noqa: F401
+                      rotary_frequencies)
 
-__all__ = ["CudaRuntime", "DeviceBuffer", "MappedQ4AffineJob", "Q4RuntimeError"]
+__all__ = ["CudaRuntime", "DeviceBuffer", "KvCache", "KvTable", "MappedQ4AffineJob", "Q4RuntimeError", "Rotary",
+           "rotary_frequencies"]

@@ -1,4 +1,4 @@
-"""ctypes prototypes of include/q4b200.h and include/q4b_weights.h. The library is required: there is no fallback."""
+"""ctypes prototypes of include/q4b200.h, include/q4b_weights.h and include/q4b_attention.h. The library is required: there is no fallback."""
 from __future__ import annotations
 
 import ctypes as C
@@ -70,7 +70,36 @@ class Peers(C.Structure):
     _fields_ = [("world", C.c_uint32), ("rank", C.c_uint32), ("flags", C.c_void_p * 8), ("cand", C.c_void_p * 8)]
 
 
+class RotaryScaling(C.Structure):
+    """q4b_rotary_scaling: how rotary frequencies are stretched."""
+
+    _fields_ = [
+        ("kind", C.c_uint32), ("reserved", C.c_uint32), ("factor", C.c_double), ("original_length", C.c_double),
+        ("fast_turns", C.c_double), ("slow_turns", C.c_double), ("attention_factor", C.c_double),
+    ]
+
+
+class Kv(C.Structure):
+    """q4b_kv_cache: one layer's paged keys and values."""
+
+    _fields_ = [
+        ("format", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("page_tokens", C.c_uint32),
+        ("pages", C.c_uint32), ("reserved", C.c_uint32), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+        ("page_stride", C.c_uint64), ("head_stride", C.c_uint64), ("token_stride", C.c_uint64),
+    ]
+
+
+class Table(C.Structure):
+    """q4b_kv_table: which pages hold a sequence."""
+
+    _fields_ = [("pages_dev", C.c_void_p), ("sequences", C.c_uint32), ("pages_per_sequence", C.c_uint32), ("row_stride", C.c_uint64)]
+
+
 X_BF16, X_SWIGLU, X_RMS = 0, 1, 2
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+KV_FORMATS = {"bf16": 0, "int8": 1, "e4m3": 2}
 
 _lib = None
 
@@ -132,6 +161,12 @@ def load() -> C.CDLL:
         "q4b_chain_phase_count": [vp, P(u32)],
         "q4b_matvec_noalloc": [i32, vp, u64, vp, vp, vp, u64, vp, vp],
         "q4b_shard_free": [vp, u32],
+        "q4b_rotary_frequencies": [u32, C.c_double, P(RotaryScaling), P(C.c_double), P(C.c_double)],
+        "q4b_rotary_create": [vp, P(C.c_double), u32, i32, C.c_double, P(vp)],
+        "q4b_rotary_device": [vp, vp, vp, i32, u64, u64, u32, u32, vp, vp, i32, u64, vp],
+        "q4b_kv_write_device": [vp, P(Kv), P(Table), vp, vp, u64, vp, u64, vp, u64, i32, vp, vp],
+        "q4b_kv_read_device": [vp, P(Kv), P(Table), vp, vp, u64, vp, u64, vp, u64, i32, vp],
+        "q4b_attention_device": [vp, P(Kv), P(Table), vp, vp, i32, u64, u32, u32, C.c_float, vp, i32, u64, vp],
         "q4b_store_open": [C.c_char_p, P(vp)],
         "q4b_store_tensor_count": [vp, P(u64)],
         "q4b_store_shard_count": [vp, P(u64)],
@@ -171,6 +206,8 @@ def load() -> C.CDLL:
         getattr(lib, name).restype = None
     lib.q4b_chain_destroy.argtypes = [vp]
     lib.q4b_chain_destroy.restype = None
+    lib.q4b_rotary_destroy.argtypes = [vp]
+    lib.q4b_rotary_destroy.restype = None
     lib.q4b_chain_max_k.argtypes = []
     lib.q4b_chain_max_k.restype = C.c_uint64
     lib.q4b_noalloc_last_error.argtypes = []
@@ -201,4 +238,10 @@ WEIGHTS_EXPORTS = [
     "q4b_weights_store", "q4b_weights_shard_count", "q4b_weights_device_bytes", "q4b_weights_q4_matrix",
     "q4b_weights_jobs", "q4b_weights_matvec_batch", "q4b_weights_matmul_batch", "q4b_weights_argmax_batch",
     "q4b_weights_mlp_batch", "q4b_weights_dequantized_row",
+]
+
+# include/q4b_attention.h
+ATTENTION_EXPORTS = [
+    "q4b_rotary_frequencies", "q4b_rotary_create", "q4b_rotary_destroy", "q4b_rotary_device", "q4b_kv_write_device",
+    "q4b_kv_read_device", "q4b_attention_device",
 ]

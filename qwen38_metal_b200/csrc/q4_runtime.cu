@@ -17,6 +17,7 @@
 #include <string>
 #include <vector>
 
+#include "q4_attention.h"
 #include "q4_kernels.h"
 #include "q4_stack.h"
 
@@ -181,18 +182,19 @@ struct q4b_runtime {
 extern "C" uint32_t q4k_gemv_occupancy(int column_tiles, int aligned);
 
 namespace {
+constexpr int kInputErrorWord = 16;  // of error_flag: a word that no kernel looks at (the first one makes chains give up)
+}  // namespace
 
-struct DeviceGuard {
-    int prev = -1;
-    explicit DeviceGuard(int device) {
-        cudaGetDevice(&prev);
-        if (prev != device) cudaSetDevice(device);
-        else prev = -1;
-    }
-    ~DeviceGuard() {
-        if (prev >= 0) cudaSetDevice(prev);
-    }
-};
+namespace q4 {
+RuntimeView runtime_view(q4b_runtime *rt) {
+    int *flags = (int *)rt->error_flag.ptr;
+    return {&rt->mu, rt->device, rt->sm_count, flags, flags + kInputErrorWord, nullptr, nullptr, &rt->launches};
+}
+}  // namespace q4
+
+namespace {
+
+using q4::DeviceGuard;
 
 int check_rt(q4b_runtime *rt) {
     if (!rt) return fail(Q4B_INVALID_ARGUMENT, "runtime handle is null");
@@ -2095,7 +2097,13 @@ extern "C" int q4b_device_status(q4b_runtime *rt) {
     DeviceGuard guard(rt->device);
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return fail(Q4B_COMMAND_FAILED, "CUDA command failed: %s", cudaGetErrorString(e));
-    return finish(rt, rt->stream);
+    if (int st = finish(rt, rt->stream)) return st;
+    int input = 0;
+    int *word = (int *)rt->error_flag.ptr + kInputErrorWord;
+    Q4B_CUDA(cudaMemcpy(&input, word, sizeof input, cudaMemcpyDeviceToHost), "status download");
+    if (!input) return Q4B_OK;
+    Q4B_CUDA(cudaMemset(word, 0, sizeof input), "status reset");
+    return fail(Q4B_TENSOR_OUT_OF_RANGE, "a sequence, position, length or page number of an attention call is outside its page table or cache");
 }
 
 extern "C" int q4b_launch_count(q4b_runtime *rt, uint64_t *launches) {

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from functools import cached_property
 
 import numpy as np
 
@@ -68,6 +69,82 @@ def _jobs(jobs) -> "C.Array":
     for i, j in enumerate(jobs):
         arr[i] = j.to_c()
     return arr
+
+
+@dataclass(frozen=True)
+class KvCache:
+    """One layer's paged cache of keys and values in device memory of the caller's (q4b_kv_cache): addresses as integers, strides
+    in bytes, all 0 for [pages][kv_heads][page_tokens][head_dim] without gaps; scales [pages][kv_heads][page_tokens] fp32."""
+
+    format: str  # "bf16", "int8", "e4m3"
+    kv_heads: int
+    head_dim: int
+    page_tokens: int
+    pages: int
+    k: int
+    v: int
+    k_scales: int = 0
+    v_scales: int = 0
+    page_stride: int = 0
+    head_stride: int = 0
+    token_stride: int = 0
+
+    @cached_property
+    def c(self) -> capi.Kv:
+        if self.format not in capi.KV_FORMATS:
+            raise Q4RuntimeError(13, f"unknown cache format {self.format}")
+        return capi.Kv(capi.KV_FORMATS[self.format], self.kv_heads, self.head_dim, self.page_tokens, self.pages, 0, self.k or None,
+                       self.v or None, self.k_scales or None, self.v_scales or None, self.page_stride, self.head_stride,
+                       self.token_stride)
+
+
+@dataclass(frozen=True)
+class KvTable:
+    """Page table (q4b_kv_table): int32 page numbers [sequences][row_stride] in device memory; row_stride 0: pages_per_sequence."""
+
+    pages: int
+    sequences: int
+    pages_per_sequence: int
+    row_stride: int = 0
+
+    @cached_property
+    def c(self) -> capi.Table:
+        return capi.Table(self.pages or None, self.sequences, self.pages_per_sequence, self.row_stride)
+
+
+def rotary_frequencies(rotary_dim: int, base: float, scaling: dict | None = None) -> tuple[np.ndarray, float]:
+    """Radians per token of every pair in 64 bits, and the factor on cosine and sine (q4b_rotary_frequencies). scaling: None or
+    {"kind": "linear" | "ntk" | "yarn", "factor": f, and for yarn "original_length": n[, "fast_turns", "slow_turns",
+    "attention_factor"]}."""
+    cs = None
+    if scaling is not None:
+        kind = scaling.get("kind", "none")
+        if kind not in capi.ROTARY_SCALINGS:
+            raise Q4RuntimeError(13, f"unknown rotary scaling {kind}")
+        cs = capi.RotaryScaling(capi.ROTARY_SCALINGS[kind], 0, *(float(scaling.get(n, d)) for n, d in (
+            ("factor", 1.0), ("original_length", 0.0), ("fast_turns", 0.0), ("slow_turns", 0.0), ("attention_factor", 0.0))))
+    freq, factor = np.zeros(max(int(rotary_dim) // 2, 1), dtype=np.float64), C.c_double()
+    _check(capi.load().q4b_rotary_frequencies(rotary_dim, base, C.byref(cs) if cs is not None else None,
+                                              freq.ctypes.data_as(C.POINTER(C.c_double)), C.byref(factor)))
+    return freq, factor.value
+
+
+class Rotary:
+    """Rotary frequencies kept on a device (q4b_rotary)."""
+
+    def __init__(self, rt: "CudaRuntime", handle):
+        self._lib, self._h = rt._lib, handle
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            self._lib.q4b_rotary_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class CudaRuntime:
@@ -251,6 +328,48 @@ class CudaRuntime:
 
     def rms_unit_bf16_device(self, in_ptr: int, rows: int, n: int, eps: float, out_ptr: int, stream: int = 0) -> None:
         _check(self._lib.q4b_rms_unit_bf16_device(self._h, in_ptr, rows, n, eps, out_ptr, stream))
+
+    # -- attention (include/q4b_attention.h) -----------------------------------------------------
+    def rotary_create(self, rotary_dim: int, base: float = 10000.0, layout: str = "half", scaling: dict | None = None,
+                      inv_freq=None, attention_factor: float = 1.0) -> Rotary:
+        """Frequencies for `rotary_device` and `kv_write_device`: `base` and `scaling` as in `rotary_frequencies`, or the caller's
+        own `inv_freq` (radians per token of each pair) and `attention_factor`."""
+        if layout not in capi.ROTARY_LAYOUTS:
+            raise Q4RuntimeError(13, f"unknown rotary layout {layout}")
+        if inv_freq is None:
+            inv_freq, attention_factor = rotary_frequencies(rotary_dim, base, scaling)
+        freq = np.ascontiguousarray(inv_freq, dtype=np.float64).reshape(-1)
+        if freq.size * 2 != rotary_dim and rotary_dim > 0 and rotary_dim % 2 == 0:
+            raise Q4RuntimeError(6, f"inv_freq has {freq.size} elements, expected {rotary_dim // 2}")
+        handle = C.c_void_p()
+        _check(self._lib.q4b_rotary_create(self._h, freq.ctypes.data_as(C.POINTER(C.c_double)), rotary_dim,
+                                           capi.ROTARY_LAYOUTS[layout], attention_factor, C.byref(handle)))
+        return Rotary(self, handle)
+
+    def rotary_device(self, rotary: Rotary, x_ptr: int, x_dtype: int, x_stride: int, tokens: int, heads: int, head_dim: int,
+                      positions_ptr: int, out_ptr: int, out_dtype: int, out_stride: int, stream: int = 0) -> None:
+        """Turn the queries (or keys) of `tokens` tokens by their positions; strides in values. In place if out_ptr is x_ptr."""
+        _check(self._lib.q4b_rotary_device(self._h, rotary._h, x_ptr, x_dtype, x_stride, tokens, heads, head_dim, positions_ptr,
+                                           out_ptr, out_dtype, out_stride, stream))
+
+    def kv_write_device(self, cache: KvCache, table: KvTable, positions_ptr: int, sequences_ptr: int, tokens: int, k_ptr: int,
+                        k_stride: int, v_ptr: int, v_stride: int, dtype: int, rotary: Rotary | None = None, stream: int = 0) -> None:
+        """Quantise new keys (turned first if `rotary` is given) and values into the cache. sequences_ptr 0: the table's sequences
+        have equal runs of tokens; k_ptr or v_ptr 0: that side is left alone."""
+        _check(self._lib.q4b_kv_write_device(self._h, cache.c, table.c, positions_ptr, sequences_ptr or None, tokens, k_ptr or None,
+                                             k_stride, v_ptr or None, v_stride, dtype, rotary._h if rotary is not None else None, stream))
+
+    def kv_read_device(self, cache: KvCache, table: KvTable, positions_ptr: int, sequences_ptr: int, tokens: int, k_ptr: int,
+                       k_stride: int, v_ptr: int, v_stride: int, dtype: int, stream: int = 0) -> None:
+        """What the cache holds for these tokens, as numbers."""
+        _check(self._lib.q4b_kv_read_device(self._h, cache.c, table.c, positions_ptr, sequences_ptr or None, tokens, k_ptr or None,
+                                            k_stride, v_ptr or None, v_stride, dtype, stream))
+
+    def attention_device(self, cache: KvCache, table: KvTable, lengths_ptr: int, q_ptr: int, q_dtype: int, q_stride: int, heads: int,
+                         q_tokens: int, scale: float, out_ptr: int, out_dtype: int, out_stride: int, stream: int = 0) -> None:
+        """Attention of the last q_tokens tokens of every sequence over its cache."""
+        _check(self._lib.q4b_attention_device(self._h, cache.c, table.c, lengths_ptr, q_ptr, q_dtype, q_stride, heads, q_tokens, scale,
+                                              out_ptr, out_dtype, out_stride, stream))
 
     # -- persistent decode chain ----------------------------------------------------------------------
     def arena_create(self, nbytes: int) -> tuple[int, bytes]:
