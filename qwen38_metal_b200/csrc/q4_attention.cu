@@ -3,113 +3,775 @@
 //
 //     out = sum_j p_j v_j / sum_j p_j,   p_j = e^(scale q.k_j)
 //
-// The plain form: a block per query row, a warp per token at a time, one pass with the running maximum and sum of every warp,
-// joined through shared memory. Everything in 32 bits.
-#include "q4_attention.h"
-
+// Every key and value is read once from memory for eight query rows (token, head) that share its key head: at one byte a value that is
+// 12 to 16 operations a byte, so memory is the bound, and the kernel is built around keeping loads in flight.
+//
+//   * One block per SM, eight warps, each with a ring of its own in shared memory. Tiles of 16 tokens (they never cross a page)
+//     go round the warps; a warp's first lane asks for keys and values of its next tiles with tensor copies, past the end of an
+//     item too, so that 190 KB stay in flight per SM while results are joined. No warp waits for another one inside an item.
+//   * Both products run on m16n8k16 MMAs with eight query rows: rows 0...7 of the left operand hold the upper halves of the eight
+//     rows' factors, rows 8...15 the lower halves, so that the sum of the two accumulators is a product of factors of 16 bits or more
+//     (two bf16 numbers, error 2^-17; two fp16 numbers for 8-bit caches, 2^-22), at no cost: the rows would be empty.
+//   * 8-bit codes become fp16 exactly. Which 16 dimensions an MMA multiplies is free as long as queries and keys agree, so that a
+//     lane takes whole 16-byte pieces of a key row; values are read transposed as pairs of bytes, which gives the lane a pair of
+//     dimensions, one for each of two MMAs.
+//   * One pass: every warp keeps a running maximum, sum and result of each row in registers. The scale of a token's values goes into its
+//     weight: weights are kept relative to the largest weight times scale so far (its power of two), and stay in fp16's range whatever the
+//     scales are.
+//   * The work of all sequences is cut into equal shares by every block for itself (q4_attention_plan.h), from the lengths in device memory:
+//     a captured graph follows them. Results of an item cut over several blocks are joined in order by the last one.
 #include <cuda_fp8.h>
 
+#include <atomic>
+
+#include "q4_attention.h"
+#include "q4_attention_plan.h"
 #include "q4_device.cuh"
+#include "q4_tensor_map.h"
 
 namespace q4 {
 
-constexpr uint32_t kWarps = 8;
+constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;
+constexpr uint32_t kRoundDims = 64;             // dimensions joined at a time
+constexpr uint32_t kRoundPitch = kRoundDims + 16;  // floats between rows of the join buffer: lanes of a store fall into different banks
+constexpr uint32_t kMostPieces = 256;           // of an item (blocks of the grid)
+constexpr uint32_t kLeastRun = 16;              // tiles: shorter runs cost more in joining than they save
+// 8-bit caches: weights go up to 2^15, near the end of fp16's range, so that their lower halves keep 16 bits of weights down to
+// 2^-23 of the largest one (and 2^-39 of it below)
+constexpr float kWeightLift = 14.f;
+constexpr unsigned long long kWaitLimitNs = 200ull * 1000 * 1000, kLateLimitNs = 1000 * 1000;
+constexpr uint32_t kSharedLimit = 227 * 1024;
 
-__device__ __forceinline__ void cache8(const uint8_t *row, uint32_t d, uint32_t format, float scale, float (&v)[8]) {
-    if (format == 0u) {
-        const uint4 a = __ldcg(reinterpret_cast<const uint4 *>(row + 2 * d));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-        return;
+template <int FMT, int HDP>
+struct Shape {
+    static constexpr uint32_t kRow = HDP * (FMT == 0 ? 2 : 1);       // bytes of a token's row in shared memory
+    static constexpr uint32_t kSeg = kRow < 128 ? kRow : 128;        // bytes of it that one copy brings
+    static constexpr uint32_t kSegs = kRow / kSeg;
+    static constexpr uint32_t kTile = kTileTokens * kRow;            // a tile of keys or of values
+    static constexpr uint32_t kPieces = kSeg / 64;                   // 16-byte pieces of a segment a lane takes from a key row
+    static constexpr uint32_t kMmas = HDP / 16;                      // per 8 tokens of scores
+    static constexpr uint32_t kChunks = kRow / 16;                   // 16-byte pieces of a row
+    static constexpr uint32_t kChunkDims = FMT == 0 ? 8 : 16;
+    static constexpr uint32_t kAcc = HDP / 8;                        // accumulators of four numbers
+    // shared memory: rings, their scales, barriers, the join buffer, and small arrays
+    static constexpr uint32_t kJoin = kWarps * kAttentionRows * kRoundPitch * 4;
+    static constexpr uint32_t kWeights = kMostPieces * kAttentionRows * 4;  // over the join buffer
+    static constexpr uint32_t kSmall = 2048;
+    static constexpr uint32_t kFit = (kSharedLimit - 1024 - kJoin - kSmall) / (kWarps * (kTile + 64 + 8));
+    static constexpr uint32_t kSlots = kFit < 16 ? kFit : 16;        // of a warp's ring: keys and values of tiles in turn
+    static constexpr uint32_t kRing = kWarps * kSlots * kTile;
+    static constexpr uint32_t kShared = 1024 + kRing + kWarps * kSlots * (64 + 8) + kJoin + kSmall;
+    static_assert(kSlots >= 2 && kWeights <= kJoin, "");
+};
+
+// ---- small pieces ----
+
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last place; below 2^-126: zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 p = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+
+// Two numbers as upper and lower halves: a = hi + lo up to 2^-17 (bf16) or 2^-22 (fp16, numbers up to 2).
+template <int FMT>
+__device__ __forceinline__ void split(float a, float b, uint32_t &hi, uint32_t &lo) {
+    if (FMT == 0) {
+        hi = pack_bf16(a, b);
+        lo = pack_bf16(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+    } else {
+        hi = pack_f16(a, b);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+        lo = pack_f16(a - f.x, b - f.y);
     }
-    const uint2 a = __ldcg(reinterpret_cast<const uint2 *>(row + d));
-    const uint32_t w[2] = {a.x, a.y};
+}
+
+template <int FMT>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (FMT == 0)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        mma_f16_16816(d, a[0], a[1], a[2], a[3], b0, b1);
+}
+
+// Bytes 0 and 2, and bytes 1 and 3, of a word of int8 codes as fp16: 0x6400 | u is 1024 + u, with u = code + 128.
+__device__ __forceinline__ uint32_t int8_even(uint32_t w) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((w & 0x00ff00ffu) ^ 0x64806480u), "r"(0x64806480u));
+    return r;
+}
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {  // the lower two bytes
+    uint32_t r;
+    asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
+    return r;
+}
+
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded: after the limit the call is reported as failed and goes on with what is there, with a shorter limit for what follows.
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, unsigned long long &limit, int *error_flag) {
+    if (mbar_try(bar, parity)) return;
+    unsigned long long begin = 0;
+    for (uint32_t spin = 1; spin != 0; ++spin) {
+        if (mbar_try(bar, parity)) return;
+        if ((spin & 255u) == 0) {
+            unsigned long long now;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (begin == 0) begin = now;
+            if (now - begin > limit) break;
+        }
+    }
+    limit = kLateLimitNs;
+    *error_flag = 1;
+}
+
+__device__ __forceinline__ void copy_tile(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int token, int head, int page) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(token),
+                 "r"(head), "r"(page)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_bytes(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// ---- a block's share ----
+
+struct Geometry {
+    uint32_t chunks;  // items of a key head: eight query rows each
+    uint32_t heads;   // items of a sequence = key heads * chunks
+    uint32_t rows;    // query rows of a key head
+    uint32_t group;   // query heads of a key head
+};
+
+__device__ __forceinline__ int64_t length_of(const AttentionParams &p, uint32_t s) {
+    const int64_t n = __ldcg(p.lengths + s), most = (int64_t)p.kv.per_sequence * p.kv.page_tokens;
+    return n < 0 ? 0 : n > most ? most : n;
+}
+
+using Cursor = AttentionCursor;
+
+struct Share {
+    bool any;
+    Cursor at;
+    AttentionCut cut;
+};
+
+__device__ __forceinline__ uint64_t warp_scan(uint64_t v, uint32_t lane) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const uint32_t pair = (w[i / 4] >> (i % 4 * 8)) & 0xffffu;
-        if (format == 1u) {
-            v[i] = (float)(int8_t)(pair & 0xffu) * scale;
-            v[i + 1] = (float)(int8_t)(pair >> 8) * scale;
-        } else {
-            const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E4M3)));
-            v[i] = f.x * scale;
-            v[i + 1] = f.y * scale;
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint64_t o = __shfl_up_sync(0xffffffffu, v, off);
+        if (lane >= (uint32_t)off) v += o;
+    }
+    return v;
+}
+
+// All threads. `scratch`: 2 * kWarps + 8 words of 64 bits in shared memory.
+__device__ Share share_of_block(const AttentionParams &p, const Geometry &g, uint64_t *scratch) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, sequences = p.kv.sequences;
+    uint64_t tiles = 0, items = 0;
+    for (uint32_t s = threadIdx.x; s < sequences; s += kThreads) {
+        const int64_t raw = __ldcg(p.lengths + s), n = length_of(p, s);
+        if (raw != n && blockIdx.x == 0) *p.kv.input_error = 1;
+        tiles += attention_tiles(n);
+        items += n > 0;
+    }
+    tiles = __shfl_sync(0xffffffffu, warp_scan(tiles, lane), 31);
+    items = __shfl_sync(0xffffffffu, warp_scan(items, lane), 31);
+    if (lane == 0) scratch[warp] = tiles, scratch[kWarps + warp] = items;
+    __syncthreads();
+    tiles = items = 0;
+    for (uint32_t w = 0; w < kWarps; ++w) tiles += scratch[w], items += scratch[kWarps + w];
+    tiles *= g.heads;
+    items *= g.heads;
+    Share share;
+    share.any = false;
+    share.at = Cursor{};
+    if (tiles == 0) return share;
+    share.cut = attention_cut(tiles, items, gridDim.x, kLeastRun);
+    const AttentionCut &cut = share.cut;
+    const uint64_t target = cut.whole ? blockIdx.x : blockIdx.x * cut.run;
+    if (!cut.whole && target >= tiles) return share;
+    // the sequence that holds piece or tile number `target`
+    uint64_t before = 0;
+    for (uint32_t base = 0; base < sequences; base += kThreads) {
+        const uint32_t s = base + threadIdx.x;
+        const uint32_t t = s < sequences ? attention_tiles(length_of(p, s)) : 0u;
+        const uint64_t weight = attention_weight(cut, t, g.heads);
+        const uint64_t scan = warp_scan(weight, lane);
+        __syncthreads();
+        if (lane == 31) scratch[warp] = scan;
+        if (threadIdx.x == 0) scratch[2 * kWarps] = ~0ull;
+        __syncthreads();
+        uint64_t start = before + scan - weight, all = before;
+        for (uint32_t w = 0; w < kWarps; ++w) {
+            if (w < warp) start += scratch[w];
+            all += scratch[w];
+        }
+        if (target >= start && target < start + weight) {
+            scratch[2 * kWarps] = s;
+            scratch[2 * kWarps + 1] = start;
+        }
+        __syncthreads();
+        if (scratch[2 * kWarps] != ~0ull) {
+            share.any = true;
+            break;
+        }
+        before = all;
+    }
+    if (!share.any) return share;
+    const uint32_t s = (uint32_t)scratch[2 * kWarps];
+    const uint64_t start = scratch[2 * kWarps + 1];
+    share.at.start(cut, s, length_of(p, s), start, target - start, tiles);
+    __syncthreads();
+    return share;
+}
+
+// ---- asking for tiles ----
+
+// What a warp asks for, ahead of what it multiplies: keys, then values, of its tiles in order. The page number of the tile that is
+// next is read when the tile before it is asked for.
+template <int FMT, int HDP>
+struct Asker {
+    using S = Shape<FMT, HDP>;
+    Cursor at;
+    uint32_t tile, head, page, place, slot;
+    bool more, values;
+
+    __device__ __forceinline__ void look(const AttentionParams &p, const Geometry &g, uint32_t warp) {
+        while (tile >= at.end) {
+            if (!at.next([&](uint32_t i) { return length_of(p, i); }, p.kv.sequences, g.heads)) {
+                more = false;
+                return;
+            }
+            tile = at.begin + warp;
+        }
+        const uint32_t per = p.kv.page_tokens / kTileTokens;
+        head = at.item / g.chunks;
+        place = tile % per * kTileTokens;
+        page = (uint32_t)__ldcg(p.kv.table + (uint64_t)at.s * p.kv.row_stride + tile / per);
+    }
+    __device__ __forceinline__ void start(const Share &share, const AttentionParams &p, const Geometry &g, uint32_t warp) {
+        at = share.at;
+        tile = at.begin + warp;
+        slot = 0;
+        more = true;
+        values = false;
+        look(p, g, warp);
+    }
+    __device__ __forceinline__ void ask(const AttentionParams &p, const Geometry &g, const CUtensorMap *k_map, const CUtensorMap *v_map, uint32_t ring, uint32_t scales, uint32_t bars,
+                                        uint32_t warp, uint32_t lane) {
+        if (!more) return;
+        if (lane == 0) {
+            const uint32_t bar = bars + slot * 8, dst = ring + slot * S::kTile, sc = scales + slot * 64;
+            const bool there = page < p.kv.pages;
+            const CUtensorMap *map = values ? v_map : k_map;
+            // (a page outside the cache is outside the tensor map too: such copies bring zeros)
+            const int at_page = (int)(there ? page : p.kv.pages);
+            uint32_t bytes = S::kTile;
+            if (FMT != 0 && there) bytes += 64;
+            if (!there) {
+                *p.kv.input_error = 1;
+                if (FMT != 0) {
+                    for (uint32_t i = 0; i < 64; i += 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sc + i), "r"(0u) : "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+            }
+            mbar_expect(bar, bytes);
+#pragma unroll
+            for (uint32_t i = 0; i < S::kSegs; ++i) copy_tile(dst + i * (kTileTokens * S::kSeg), map, bar, (int)(i * S::kSeg / (FMT == 0 ? 2 : 1)), (int)place, (int)head, at_page);
+            if (FMT != 0 && there)
+                copy_bytes(sc, (values ? p.kv.v_scales : p.kv.k_scales) + ((uint64_t)page * p.kv.kv_heads + head) * p.kv.page_tokens + place, 64, bar);
+        }
+        slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+        if (values) {
+            tile += kWarps;
+            look(p, g, warp);
+        }
+        values = !values;
+    }
+};
+
+template <int FMT>
+__device__ __forceinline__ bool not_finite(uint32_t w, uint32_t byte) {  // the value that begins at this byte of a word
+    if (FMT == 0) return ((w >> (byte * 8)) & 0x7f80u) == 0x7f80u;
+    return ((w >> (byte * 8)) & 0x7fu) == 0x7fu;
+}
+
+// ---- the kernel ----
+
+template <int FMT, int HDP>
+__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ Geometry g, const __grid_constant__ CUtensorMap k_map,
+                                                                const __grid_constant__ CUtensorMap v_map) {
+    using S = Shape<FMT, HDP>;
+    extern __shared__ uint8_t shared_raw[];
+    const uint32_t raw = (uint32_t)__cvta_generic_to_shared(shared_raw), pad = (1024u - (raw & 1023u)) & 1023u;
+    uint8_t *const shared = shared_raw + pad;
+    float *const join = reinterpret_cast<float *>(shared + S::kRing + kWarps * S::kSlots * (64 + 8));
+    float *const small = join + S::kJoin / 4;
+    float *const tops = small, *const sums = small + kWarps * kAttentionRows;  // [warp][row]
+    float *const totals = small + 2 * kWarps * kAttentionRows;                 // [row] sum, [row] maximum of joined pieces
+    uint64_t *const scratch = reinterpret_cast<uint64_t *>(small + 2 * kWarps * kAttentionRows + 2 * kAttentionRows);
+    uint32_t *const arrived = reinterpret_cast<uint32_t *>(scratch + 2 * kWarps + 8);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row = lane >> 2, quad = lane & 3u;
+    const uint32_t ring = raw + pad + warp * S::kSlots * S::kTile;
+    const uint32_t scales = raw + pad + S::kRing + warp * S::kSlots * 64, bars = raw + pad + S::kRing + kWarps * S::kSlots * 64 + warp * S::kSlots * 8;
+    if (lane == 0)
+        for (uint32_t i = 0; i < S::kSlots; ++i) mbar_init(bars + i * 8, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
+    grid_dependency_wait();
+    grid_dependents_launch();
+
+    const Share share = share_of_block(p, g, scratch);
+    if (share.any) {
+        Asker<FMT, HDP> asker;
+        asker.start(share, p, g, warp);
+        for (uint32_t i = 0; i < S::kSlots; ++i) asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
+        uint32_t slot = 0, parity = 0;
+        unsigned long long limit_ns = kWaitLimitNs;
+        Cursor at = share.at;
+        do {
+            // ---- queries of the item, split into halves, in the order in which key rows are read ----
+            const uint32_t head = at.item / g.chunks, chunk = at.item % g.chunks;
+            const uint32_t r = chunk * kAttentionRows + row, draft = r / g.group;
+            const bool live = r < g.rows;
+            // tokens that the row sees
+            const int32_t limit = live ? at.length - (int32_t)p.q_tokens + 1 + (int32_t)draft : 0;
+            uint32_t qa[S::kMmas][4];
+            float row_scale = p.scale * 1.4426950408889634f;
+            {
+                float q[S::kMmas][4];
+                const uint64_t base = ((uint64_t)at.s * p.q_tokens + draft) * p.q_stride + ((uint64_t)head * g.group + r % g.group) * p.kv.head_dim;
+                uint32_t amax = 0;
+#pragma unroll
+                for (uint32_t m = 0; m < S::kMmas; ++m) {
+                    // four values for each MMA: a 16-byte piece of a key row holds 8 or 16 of them
+                    constexpr uint32_t kPer = S::kChunkDims / 4;
+                    const uint32_t piece = m / kPer, seg = piece / S::kPieces;
+                    const uint32_t d = (seg * (S::kSeg / 16) + quad * S::kPieces + piece % S::kPieces) * S::kChunkDims + m % kPer * 4;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (live && d < p.kv.head_dim) {
+                        if (p.q_is_f32) {
+                            v = __ldcg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + base + d));
+                        } else {
+                            const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.q) + base + d));
+                            v = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+                        }
+                    }
+                    q[m][0] = v.x, q[m][1] = v.y, q[m][2] = v.z, q[m][3] = v.w;
+                    if (FMT != 0)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) amax = max(amax, __float_as_uint(q[m][i]) & 0x7fffffffu);
+                }
+                float unit = 1.f;
+                if (FMT != 0) {
+                    // fp16 halves: the row is scaled by a power of two that brings its largest value into [1, 2)
+                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                    const uint32_t e = min(max(amax >> 23, 1u), 254u);
+                    unit = e == 254u ? __uint_as_float(0x00400000u) : __uint_as_float((254u - e) << 23);
+                    row_scale *= __uint_as_float(e << 23);
+                }
+#pragma unroll
+                for (uint32_t m = 0; m < S::kMmas; ++m) {
+                    // int8 codes are taken from a word as bytes 0 and 2, 1 and 3, the others in order
+                    constexpr int i1 = FMT == 1 ? 2 : 1, i2 = FMT == 1 ? 1 : 2;
+                    split<FMT>(q[m][0] * unit, q[m][i1] * unit, qa[m][0], qa[m][1]);
+                    split<FMT>(q[m][i2] * unit, q[m][3] * unit, qa[m][2], qa[m][3]);
+                }
+            }
+            float acc[S::kAcc][4];
+#pragma unroll
+            for (uint32_t i = 0; i < S::kAcc; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+            float top = -INFINITY, sum = 0.f;     // of the scores, in powers of two; sum: of this lane's tokens
+            float weight_top = -INFINITY;         // 8-bit: of the scores plus the exponents of the values' scales
+
+            for (uint32_t tile = at.begin + warp; tile < at.end; tile += kWarps) {
+                const int32_t token = (int32_t)(tile * kTileTokens);
+                const bool edge = token + (int32_t)kTileTokens > at.length - (int32_t)p.q_tokens + 1;  // some rows do not see all of it
+                // ---- scores of 16 tokens ----
+                float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
+                {
+                    const uint32_t base = ring + slot * S::kTile;
+#pragma unroll
+                    for (uint32_t seg = 0; seg < S::kSegs; ++seg)
+#pragma unroll
+                        for (uint32_t c = 0; c < S::kPieces; ++c) {
+                            const uint32_t piece = quad * S::kPieces + c, turn = S::kSeg == 128 ? row : row >> 1 & 3u;
+                            const uint32_t at_piece = base + seg * (kTileTokens * S::kSeg) + row * S::kSeg + ((piece ^ turn) << 4);
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) {
+                                const uint4 w = lds_v4(at_piece + n * 8 * S::kSeg);
+                                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+                                if (FMT == 0) {
+                                    const uint32_t m = (seg * S::kPieces + c) * 2;
+                                    mma<FMT>(s[n], qa[m], word[0], word[1]);
+                                    mma<FMT>(s[n], qa[m + 1], word[2], word[3]);
+                                } else {
+#pragma unroll
+                                    for (uint32_t i = 0; i < 4; ++i) {
+                                        const uint32_t m = (seg * S::kPieces + c) * 4 + i;
+                                        if (FMT == 1) mma<FMT>(s[n], qa[m], int8_even(word[i]), int8_even(word[i] >> 8));
+                                        else mma<FMT>(s[n], qa[m], e4m3_pair(word[i]), e4m3_pair(word[i] >> 16));
+                                    }
+                                }
+                            }
+                        }
+                }
+                // this lane's four: tokens 2 quad, + 1, + 8, + 9 of the tile, row `row`
+                float x[4] = {s[0][0] + s[0][2], s[0][1] + s[0][3], s[1][0] + s[1][2], s[1][1] + s[1][3]};
+                if (FMT != 0) {
+                    const uint2 a = lds_v2(scales + slot * 64 + quad * 8), b = lds_v2(scales + slot * 64 + 32 + quad * 8);
+                    x[0] *= __uint_as_float(a.x), x[1] *= __uint_as_float(a.y), x[2] *= __uint_as_float(b.x), x[3] *= __uint_as_float(b.y);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] *= row_scale;
+                __syncwarp();  // the slot has been read
+                asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
+                slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+                parity ^= slot == 0;
+                if (edge)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (token + (int32_t)quad * 2 + (i & 1) + (i >> 1) * 8 >= limit) x[i] = -INFINITY;
+                // ---- weights ----
+                mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
+                float frac[4], lift[4];  // 8-bit: scale of the token's values = frac * 2^lift
+                if (FMT != 0) {
+                    const uint2 a = lds_v2(scales + slot * 64 + quad * 8), b = lds_v2(scales + slot * 64 + 32 + quad * 8);
+                    const uint32_t bits[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t e = bits[i] >> 23 & 0xffu;
+                        // below 2^-126: times 2^126; infinities and NaNs as they are
+                        lift[i] = (float)((int)max(e, 1u) - 127);
+                        frac[i] = e == 0 ? __uint_as_float(bits[i]) * 0x1p126f : e == 255 ? __uint_as_float(bits[i]) : __uint_as_float((bits[i] & 0x807fffffu) | 0x3f800000u);
+                    }
+                }
+                float high = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), weight_high = 0.f;
+                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
+                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+                bool rise = high > top;
+                if (FMT != 0) {
+                    weight_high = fmaxf(fmaxf(x[0] + lift[0], x[1] + lift[1]), fmaxf(x[2] + lift[2], x[3] + lift[3]));
+                    weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 1));
+                    weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 2));
+                    rise = rise || weight_high > weight_top;
+                }
+                if (__any_sync(0xffffffffu, rise)) {
+                    if (high > top) {
+                        sum *= exp2_fast(top - high);  // (2^-inf is 0)
+                        if (FMT == 0) weight_high = top;
+                        top = high;
+                    } else if (FMT == 0) {
+                        weight_high = top;
+                    }
+                    float keep;
+                    if (FMT == 0) {
+                        keep = weight_high == top ? 1.f : exp2_fast(weight_high - top);
+                    } else {
+                        keep = weight_high > weight_top ? exp2_fast(weight_top - weight_high) : 1.f;
+                        weight_top = fmaxf(weight_top, weight_high);
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < S::kAcc; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[i][j] *= keep;
+                }
+                const float base = top == -INFINITY ? 0.f : top, weight_base = weight_top == -INFINITY ? 0.f : weight_top;
+                float weight[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = exp2_fast(x[i] - base);
+                    sum += e;
+                    // (a token that the row does not see: its scale may be anything)
+                    weight[i] = FMT == 0 ? e : x[i] == -INFINITY ? 0.f : exp2_fast(x[i] + lift[i] - weight_base + kWeightLift) * frac[i];
+                }
+                uint32_t pa[4];
+                split<FMT>(weight[0], weight[1], pa[0], pa[1]);
+                split<FMT>(weight[2], weight[3], pa[2], pa[3]);
+                // ---- values ----
+                {
+                    const uint32_t base_v = ring + slot * S::kTile;
+                    // Behind the sequence's end rows hold anything: zeros are taken for them. Among draft tokens a value that is not finite may
+                    // be seen by some rows only; a weight of zero does not take it out of a sum, so it is taken out of the MMA and
+                    // added below to the rows that see it.
+                    const int32_t behind = at.length - token;  // tokens of the tile from here on do not exist
+                    bool odd_values = false;
+                    if (FMT != 1 && edge && p.q_tokens > 1) {
+                        for (uint32_t i = lane * 16; i < S::kTile; i += 512) {
+                            const uint4 w = lds_v4(base_v + i);
+                            const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+                            if ((int32_t)(i / S::kSeg % kTileTokens) < behind)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                                    for (int b = 0; b < 4; b += FMT == 0 ? 2 : 1) odd_values = odd_values || not_finite<FMT>(word[j], b);
+                        }
+                        odd_values = __any_sync(0xffffffffu, odd_values);
+                    }
+                    const uint32_t matrix = lane >> 3, line = (lane & 7u) + (matrix & 1u) * 8, turn = S::kSeg == 128 ? line & 7u : line >> 1 & 3u;
+#pragma unroll
+                    for (uint32_t c = 0; c < S::kChunks; c += 2) {
+                        const uint32_t seg = c / (S::kSeg / 16), piece = c % (S::kSeg / 16) + (matrix >> 1);
+                        uint32_t v[4];
+                        ldmatrix_x4_trans(v, base_v + seg * (kTileTokens * S::kSeg) + line * S::kSeg + ((piece ^ turn) << 4));
+                        if (edge) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int32_t t = (int32_t)quad * 2 + (i & 1) * 8;
+                                v[i] &= (t < behind ? 0xffffu : 0u) | (t + 1 < behind ? 0xffff0000u : 0u);
+                                if (FMT != 1 && odd_values)
+#pragma unroll
+                                    for (int b = 0; b < 4; b += FMT == 0 ? 2 : 1)
+                                        if (not_finite<FMT>(v[i], b)) v[i] &= ~((FMT == 0 ? 0xffffu : 0xffu) << (b * 8));
+                            }
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < 2; ++i) {
+                            const uint32_t b0 = v[2 * i], b1 = v[2 * i + 1];
+                            if (FMT == 0) {
+                                mma<FMT>(acc[c + i], pa, b0, b1);
+                            } else if (FMT == 1) {
+                                mma<FMT>(acc[(c + i) * 2], pa, int8_even(b0), int8_even(b1));
+                                mma<FMT>(acc[(c + i) * 2 + 1], pa, int8_even(b0 >> 8), int8_even(b1 >> 8));
+                            } else {
+                                mma<FMT>(acc[(c + i) * 2], pa, e4m3_pair(__byte_perm(b0, 0, 0x4420)), e4m3_pair(__byte_perm(b1, 0, 0x4420)));
+                                mma<FMT>(acc[(c + i) * 2 + 1], pa, e4m3_pair(__byte_perm(b0, 0, 0x4431)), e4m3_pair(__byte_perm(b1, 0, 0x4431)));
+                            }
+                        }
+                    }
+                    if (FMT != 1 && odd_values) {
+#pragma unroll
+                        for (uint32_t i = 0; i < S::kAcc; ++i)
+#pragma unroll
+                            for (uint32_t j = 0; j < 2; ++j) {
+                                const uint32_t d = FMT == 0 ? i * 8 + quad * 2 + j : i / 2 * 16 + quad * 4 + j * 2 + (i & 1u);
+                                const uint32_t byte = d * (FMT == 0 ? 2 : 1), seg = byte / S::kSeg, piece = byte % S::kSeg / 16;
+                                for (int32_t t = 0; t < (int32_t)kTileTokens && token + t < limit; ++t) {
+                                    const uint32_t swap = S::kSeg == 128 ? (uint32_t)t & 7u : (uint32_t)t >> 1 & 3u;
+                                    const uint32_t w = lds_u32((base_v + seg * (kTileTokens * S::kSeg) + (uint32_t)t * S::kSeg + ((piece ^ swap) << 4) + byte % 16) & ~3u);
+                                    if (not_finite<FMT>(w, byte & 3u)) acc[i][j] += FMT == 0 ? __uint_as_float((w >> ((byte & 3u) * 8)) << 16) : __uint_as_float(0x7fc00000u);
+                                }
+                            }
+                    }
+                }
+                __syncwarp();
+                asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
+                slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+                parity ^= slot == 0;
+            }
+
+            // ---- join the warps' results ----
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (quad == 0) {
+                tops[warp * kAttentionRows + row] = top;
+                sums[warp * kAttentionRows + row] = sum;
+            }
+            __syncthreads();
+            float all_top = -INFINITY;
+            for (uint32_t w = 0; w < kWarps; ++w) all_top = fmaxf(all_top, tops[w * kAttentionRows + row]);
+            {
+                // (a warp without tiles, and rows that see nothing, have zeros)
+                float factor = top == -INFINITY ? 0.f : exp2_fast(FMT == 0 ? top - all_top : weight_top - all_top - kWeightLift);
+                if (FMT != 0 && weight_top == -INFINITY) factor = 0.f;
+                // infinities and NaNs of rows whose scores are all -infinity stay visible through their sum
+#pragma unroll
+                for (uint32_t i = 0; i < S::kAcc; ++i) {
+                    acc[i][0] = (acc[i][0] + acc[i][2]) * factor;
+                    acc[i][1] = (acc[i][1] + acc[i][3]) * factor;
+                }
+            }
+            const bool cut = !at.whole_item();
+            uint32_t owner, contributors;
+            at.contributors(share.cut, blockIdx.x, &owner, &contributors);
+            // a partial result: rows, then maxima, then sums
+            float *const part = p.parts + ((uint64_t)blockIdx.x * 2 + (blockIdx.x == owner ? 1 : 0)) * (kAttentionRows * (kMaxHeadDim + 2));
+            const uint32_t jr = threadIdx.x >> 4 & 7u, jd = (threadIdx.x & 15u) * 4;  // row and dimensions that a thread joins
+            const uint32_t j_row = chunk * kAttentionRows + jr, j_draft = j_row / g.group;
+            const bool j_live = j_row < g.rows;
+            const uint64_t out_row = ((uint64_t)at.s * p.q_tokens + j_draft) * p.out_stride + ((uint64_t)head * g.group + j_row % g.group) * p.kv.head_dim;
+            const bool j_empty = at.length - (int32_t)p.q_tokens + 1 + (int32_t)j_draft <= 0;
+#pragma unroll
+            for (uint32_t round = 0; round < HDP / kRoundDims; ++round) {
+                float *const mine = join + (warp * kAttentionRows + row) * kRoundPitch;
+                if (FMT == 0) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kRoundDims / 8; ++i)
+                        *reinterpret_cast<float2 *>(mine + i * 8 + quad * 2) = make_float2(acc[round * (kRoundDims / 8) + i][0], acc[round * (kRoundDims / 8) + i][1]);
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < kRoundDims / 16; ++i) {
+                        const uint32_t a = round * (kRoundDims / 8) + i * 2;
+                        *reinterpret_cast<float4 *>(mine + i * 16 + quad * 4) = make_float4(acc[a][0], acc[a + 1][0], acc[a][1], acc[a + 1][1]);
+                    }
+                }
+                __syncthreads();
+                if (threadIdx.x < 128) {
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float row_top = -INFINITY, total = 0.f;
+                    for (uint32_t w = 0; w < kWarps; ++w) row_top = fmaxf(row_top, tops[w * kAttentionRows + jr]);
+                    for (uint32_t w = 0; w < kWarps; ++w) {
+                        const float4 v = *reinterpret_cast<const float4 *>(join + (w * kAttentionRows + jr) * kRoundPitch + jd);
+                        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+                        const float t = tops[w * kAttentionRows + jr];
+                        total += sums[w * kAttentionRows + jr] * (t == -INFINITY ? 1.f : exp2_fast(t - row_top));
+                    }
+                    const uint32_t d = round * kRoundDims + jd;
+                    if (cut) {
+                        *reinterpret_cast<float4 *>(part + jr * HDP + d) = o;
+                        if (round == 0 && jd == 0) {
+                            part[kAttentionRows * HDP + jr] = row_top;
+                            part[kAttentionRows * (HDP + 1) + jr] = total;
+                        }
+                    } else if (j_live && d < p.kv.head_dim) {
+                        const float by = j_empty ? 0.f : 1.f / total;
+                        const float v[4] = {j_empty ? 0.f : o.x * by, j_empty ? 0.f : o.y * by, j_empty ? 0.f : o.z * by, j_empty ? 0.f : o.w * by};
+                        if (p.out_is_f32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + out_row + d) = make_float4(v[0], v[1], v[2], v[3]);
+                        else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + out_row + d) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+                    }
+                }
+                __syncthreads();
+            }
+            if (cut) {
+                // ---- the last block of an item joins its partial results, in the order of the tiles ----
+                __threadfence();
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    const uint32_t before = atomicAdd(p.counters + owner, 1u);
+                    *arrived = before + 1 == contributors;
+                    if (*arrived) p.counters[owner] = 0;
+                    __threadfence();
+                }
+                __syncthreads();
+                if (*arrived) {
+                    auto part_of = [&](uint32_t i) { return p.parts + ((uint64_t)(owner + i) * 2 + (i == 0 ? 1 : 0)) * (kAttentionRows * (kMaxHeadDim + 2)); };
+                    float *const weights = join;  // [piece][row]
+                    for (uint32_t i = threadIdx.x; i < contributors * kAttentionRows; i += kThreads) weights[i] = __ldcg(part_of(i / kAttentionRows) + kAttentionRows * HDP + i % kAttentionRows);
+                    __syncthreads();
+                    if (warp < kAttentionRows) {  // a warp per row
+                        float best = -INFINITY, total = 0.f;
+                        for (uint32_t i = lane; i < contributors; i += 32) best = fmaxf(best, weights[i * kAttentionRows + warp]);
+#pragma unroll
+                        for (int off = 16; off > 0; off >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, off));
+                        for (uint32_t i = lane; i < contributors; i += 32) {
+                            const float t = weights[i * kAttentionRows + warp];
+                            const float f = t == -INFINITY ? 0.f : exp2_fast(t - best);
+                            total += __ldcg(part_of(i) + kAttentionRows * (HDP + 1) + warp) * (t == -INFINITY ? 1.f : f);
+                            weights[i * kAttentionRows + warp] = f;
+                        }
+#pragma unroll
+                        for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+                        if (lane == 0) totals[warp] = total;
+                    }
+                    __syncthreads();
+                    for (uint32_t i = threadIdx.x; i < kAttentionRows * HDP / 4; i += kThreads) {
+                        const uint32_t rr = i / (HDP / 4), d = i % (HDP / 4) * 4, q_row = chunk * kAttentionRows + rr, q_draft = q_row / g.group;
+                        if (q_row >= g.rows || d >= p.kv.head_dim) continue;
+                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                        for (uint32_t k = 0; k < contributors; ++k) {
+                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_of(k) + rr * HDP + d));
+                            const float f = weights[k * kAttentionRows + rr];
+                            o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+                        }
+                        const bool empty = at.length - (int32_t)p.q_tokens + 1 + (int32_t)q_draft <= 0;
+                        const float by = 1.f / totals[rr];
+                        const float v[4] = {empty ? 0.f : o.x * by, empty ? 0.f : o.y * by, empty ? 0.f : o.z * by, empty ? 0.f : o.w * by};
+                        const uint64_t to = ((uint64_t)at.s * p.q_tokens + q_draft) * p.out_stride + ((uint64_t)head * g.group + q_row % g.group) * p.kv.head_dim + d;
+                        if (p.out_is_f32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to) = make_float4(v[0], v[1], v[2], v[3]);
+                        else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + to) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+                    }
+                    __syncthreads();
+                }
+            }
+        } while (at.next([&](uint32_t i) { return length_of(p, i); }, p.kv.sequences, g.heads));
+    }
+
+    // ---- sequences without tokens ----
+    for (uint32_t s = blockIdx.x; s < p.kv.sequences; s += gridDim.x) {
+        if (__ldcg(p.lengths + s) > 0) continue;
+        const uint32_t width = p.heads * p.kv.head_dim / 4;
+        for (uint32_t i = threadIdx.x; i < width * p.q_tokens; i += kThreads) {
+            const uint64_t to = ((uint64_t)s * p.q_tokens + i / width) * p.out_stride + (uint64_t)(i % width) * 4;
+            if (p.out_is_f32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to) = make_float4(0.f, 0.f, 0.f, 0.f);
+            else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + to) = make_uint2(0u, 0u);
         }
     }
 }
 
-__global__ void __launch_bounds__(kWarps * 32) attention_kernel(const AttentionParams p) {
-    __shared__ float part[kWarps][kMaxHeadDim], tops[kWarps], sums[kWarps];
-    grid_dependency_wait();
-    grid_dependents_launch();
-    const KvView &kv = p.kv;
-    const uint32_t row = blockIdx.x, head = blockIdx.y, s = row / p.q_tokens, i = row % p.q_tokens;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, d = lane * 8u;
-    const uint32_t kv_head = head / (p.heads / kv.kv_heads);
-    int64_t length = __ldcg(p.lengths + s);
-    const int64_t most = (int64_t)kv.per_sequence * kv.page_tokens;
-    if (length < 0 || length > most) {
-        if (threadIdx.x == 0) *kv.input_error = 1;
-        length = length < 0 ? 0 : most;
+// ---- host ----
+
+// Rows of the cache as [page][head][token][value]; copies of 16 tokens by one segment.
+template <int FMT, int HDP>
+bool encode_map(EncodeTiledFn encode, CUtensorMap *map, const KvView &kv, const uint8_t *pool) {
+    using S = Shape<FMT, HDP>;
+    const cuuint64_t dims[4] = {kv.head_dim, kv.page_tokens, kv.kv_heads, kv.pages};
+    const cuuint64_t strides[3] = {kv.token_stride, kv.head_stride, kv.page_stride};
+    const cuuint32_t box[4] = {S::kSeg / (FMT == 0 ? 2 : 1), kTileTokens, 1, 1}, step[4] = {1, 1, 1, 1};
+    return encode(map, FMT == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t *>(pool), dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, S::kSeg == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int FMT, int HDP>
+cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t stream) {
+    using S = Shape<FMT, HDP>;
+    const EncodeTiledFn encode = encode_tiled_fn();
+    CUtensorMap maps[2];
+    if (!encode || !encode_map<FMT, HDP>(encode, &maps[0], p.kv, p.kv.k) || !encode_map<FMT, HDP>(encode, &maps[1], p.kv, p.kv.v)) return cudaErrorInvalidValue;
+    static std::atomic<uint64_t> ready{0};  // a bit for each device: the attribute is the kernel's, once set it stays
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(attention_kernel<FMT, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kShared);
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    const int64_t seen = length - p.q_tokens + 1 + i;
-    const bool has = d < kv.head_dim;
-    float q[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const uint64_t at = row * p.q_stride + (uint64_t)head * kv.head_dim + d;
-    if (has)
-        for (int j = 0; j < 8; ++j)
-            q[j] = p.q_is_f32 ? __ldcg(static_cast<const float *>(p.q) + at + j) : __uint_as_float((uint32_t)__ldcg(static_cast<const uint16_t *>(p.q) + at + j) << 16);
-    float top = -INFINITY, sum = 0.f;
-    for (int64_t t = warp; t < seen; t += kWarps) {
-        const uint32_t entry = (uint32_t)t / kv.page_tokens, slot = (uint32_t)t % kv.page_tokens;
-        const uint32_t page = (uint32_t)__ldcg(kv.table + (uint64_t)s * kv.row_stride + entry);
-        const bool there = page < kv.pages;
-        if (!there && lane == 0) *kv.input_error = 1;
-        float k[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (there && has) {
-            const uint64_t off = (uint64_t)page * kv.page_stride + (uint64_t)kv_head * kv.head_stride + (uint64_t)slot * kv.token_stride;
-            const uint64_t sc = ((uint64_t)page * kv.kv_heads + kv_head) * kv.page_tokens + slot;
-            cache8(kv.k + off, d, kv.format, kv.format ? __ldcg(kv.k_scales + sc) : 1.f, k);
-            cache8(kv.v + off, d, kv.format, kv.format ? __ldcg(kv.v_scales + sc) : 1.f, v);
-        }
-        float dot = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dot = fmaf(q[j], k[j], dot);
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-        dot *= p.scale;
-        const float next = fmaxf(top, dot);
-        const float keep = next == -INFINITY ? 1.f : expf(top - next), w = expf(dot - next);
-        sum = sum * keep + w;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = o[j] * keep + w * v[j];
-        top = next;
-    }
-    if (has)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) part[warp][d + j] = o[j];
-    if (lane == 0) tops[warp] = top, sums[warp] = sum;
-    __syncthreads();
-    float all = -INFINITY, total = 0.f;
-    for (uint32_t w = 0; w < kWarps; ++w) all = fmaxf(all, tops[w]);
-    const float base = all == -INFINITY ? 0.f : all;
-    for (uint32_t w = 0; w < kWarps; ++w) total += sums[w] * expf(tops[w] - base);
-    for (uint32_t e = threadIdx.x; e < kv.head_dim; e += blockDim.x) {
-        float r = 0.f;
-        for (uint32_t w = 0; w < kWarps; ++w) r += part[w][e] * expf(tops[w] - base);
-        r = seen > 0 ? r / total : 0.f;
-        const uint64_t to = row * p.out_stride + (uint64_t)head * kv.head_dim + e;
-        if (p.out_is_f32) static_cast<float *>(p.out)[to] = r;
-        else static_cast<__nv_bfloat16 *>(p.out)[to] = __float2bfloat16_rn(r);
-    }
+    Geometry g;
+    g.group = p.heads / p.kv.kv_heads;
+    g.rows = g.group * p.q_tokens;
+    g.chunks = (g.rows + kAttentionRows - 1) / kAttentionRows;
+    g.heads = p.kv.kv_heads * g.chunks;
+    return launch_dependent(attention_kernel<FMT, HDP>, dim3(sm_count < kMostPieces ? sm_count : kMostPieces), kThreads, S::kShared, stream, p, g, maps[0], maps[1]);
+}
+
+template <int FMT>
+cudaError_t launch_dim(const AttentionParams &p, uint32_t sm_count, cudaStream_t stream) {
+    if (p.kv.head_dim <= 64) return launch<FMT, 64>(p, sm_count, stream);
+    if (p.kv.head_dim <= 128) return launch<FMT, 128>(p, sm_count, stream);
+    return launch<FMT, 256>(p, sm_count, stream);
 }
 
 }  // namespace q4
 
-extern "C" cudaError_t q4k_attention(const q4::AttentionParams *p, uint32_t, cudaStream_t stream) {
-    return q4::launch_dependent(q4::attention_kernel, dim3(p->kv.sequences * p->q_tokens, p->heads), q4::kWarps * 32, 0, stream, *p);
+extern "C" size_t q4k_attention_part_floats(uint32_t sm_count) { return (size_t)sm_count * 2 * q4::kAttentionRows * (q4::kMaxHeadDim + 2); }
+
+extern "C" cudaError_t q4k_attention(const q4::AttentionParams *p, uint32_t sm_count, cudaStream_t stream) {
+    if (p->kv.format == 0u) return q4::launch_dim<0>(*p, sm_count, stream);
+    if (p->kv.format == 1u) return q4::launch_dim<1>(*p, sm_count, stream);
+    return q4::launch_dim<2>(*p, sm_count, stream);
 }

@@ -46,6 +46,7 @@
 
 #include "q4_decomp.h"
 #include "q4_kernels.h"
+#include "q4_tensor_map.h"
 
 #include "q4_device.cuh"
 
@@ -852,21 +853,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) q4_
 
 namespace {
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled_fn() {
-    static const EncodeTiledFn fn = [] {
-        void *sym = nullptr;
-        cudaDriverEntryPointQueryResult qres;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) == cudaSuccess &&
-            qres == cudaDriverEntryPointSuccess)
-            return reinterpret_cast<EncodeTiledFn>(sym);
-        return static_cast<EncodeTiledFn>(nullptr);
-    }();
-    return fn;
-}
+using q4::EncodeTiledFn;
+using q4::encode_tiled_fn;
 
 // packed weights as a byte matrix [n][k/2] from the tensor's address rounded down to 16 bytes (TMA needs that;
 // the row pitch k/2 is a multiple of 32): 64-byte swizzled rows when the tensor is aligned, 80-byte windows else.

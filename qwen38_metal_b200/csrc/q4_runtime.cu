@@ -140,7 +140,7 @@ struct q4b_runtime {
     uint32_t gemv_ctas[3][2] = {{0, 0}, {0, 0}, {0, 0}};  // [column tiles][aligned] resident warps per SM
     uint32_t max_workers = 0;
     std::vector<void *> arenas, peer_arenas;
-    Pool trace, gemm_x, gemm_parts, gemm_counters, error_flag;
+    Pool trace, gemm_x, gemm_parts, gemm_counters, error_flag, attention_parts, attention_counters;
     uint64_t gemm_failures_seen = 0;  // rt->failures when the GEMM's tile counters were last known to be zero
     uint32_t gemm_min_m = 16;  // activation rows from which the tensor-core GEMM takes over (when the short-batch kernel does not apply)
     uint32_t rows_max_m = 16;  // activation rows per launch of the short-batch kernel (0: never use it)
@@ -188,7 +188,7 @@ constexpr int kInputErrorWord = 16;  // of error_flag: a word that no kernel loo
 namespace q4 {
 RuntimeView runtime_view(q4b_runtime *rt) {
     int *flags = (int *)rt->error_flag.ptr;
-    return {&rt->mu, rt->device, rt->sm_count, flags, flags + kInputErrorWord, nullptr, nullptr, &rt->launches};
+    return {&rt->mu, rt->device, rt->sm_count, flags, flags + kInputErrorWord, (float *)rt->attention_parts.ptr, (unsigned int *)rt->attention_counters.ptr, &rt->launches};
 }
 }  // namespace q4
 
@@ -791,6 +791,10 @@ extern "C" int q4b_runtime_create(int device_ordinal, q4b_runtime **out) {
     if (e == cudaSuccess) e = rt->gemm_parts.ensure(q4_gemm_most_partial_floats((uint32_t)rt->sm_count / 2u) * 4, true);
     if (e == cudaSuccess) e = rt->gemm_counters.ensure((size_t)q4_gemm_most_counters((uint32_t)rt->sm_count / 2u) * 4);
     if (e == cudaSuccess) e = cudaMemset(rt->gemm_counters.ptr, 0, rt->gemm_counters.capacity);
+    // partial results of attention items that are cut over blocks (two 8 KB slots a block)
+    if (e == cudaSuccess) e = rt->attention_parts.ensure(q4k_attention_part_floats((uint32_t)rt->sm_count) * 4, true);
+    if (e == cudaSuccess) e = rt->attention_counters.ensure((size_t)rt->sm_count * 4);
+    if (e == cudaSuccess) e = cudaMemset(rt->attention_counters.ptr, 0, rt->attention_counters.capacity);
     // (memsets return before they are done, and the runtime's stream does not wait for the default one)
     if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
     if (const char *unf = getenv("Q4B_MLP_UNFUSED")) rt->mlp_unfused = strtol(unf, nullptr, 10) != 0;
@@ -826,7 +830,7 @@ extern "C" void q4b_runtime_destroy(q4b_runtime *rt) {
         if (s.ptr) cudaFree(s.ptr);
     for (void *p : rt->peer_arenas) cudaIpcCloseMemHandle(p);
     for (void *p : rt->arenas) cudaFree(p);
-    Pool *pools[] = {&rt->rows_partials, &rt->rows_counters, &rt->gemm_x, &rt->gemm_parts, &rt->gemm_counters, &rt->error_flag, &rt->trace, &rt->x_in, &rt->xp, &rt->xsum, &rt->row_inv, &rt->partials, &rt->counters, &rt->logits, &rt->amax_v,
+    Pool *pools[] = {&rt->attention_parts, &rt->attention_counters, &rt->rows_partials, &rt->rows_counters, &rt->gemm_x, &rt->gemm_parts, &rt->gemm_counters, &rt->error_flag, &rt->trace, &rt->x_in, &rt->xp, &rt->xsum, &rt->row_inv, &rt->partials, &rt->counters, &rt->logits, &rt->amax_v,
                      &rt->amax_i, &rt->tokens, &rt->gate, &rt->up, &rt->hidden};
     for (Pool *p : pools) p->release();
     for (Pool &p : rt->outs) p.release();

@@ -122,7 +122,12 @@ def attention64(cache, lengths, q, q_tokens, scale):
     products in 32 bits add less than 256 * 2^-24 = 2^-16 of the sum of magnitudes, scaling and exponential 2^-16 of the score
     at most; so a score is off by d = 2^-14 scale sum |q k| at most, its weight by e^d - 1 < 1.06 d (d < 0.1) and the mean of the
     values by twice that of the mean of their magnitudes. Weights kept to 16 bits: 2^-16 of it; 32-bit sums of n terms in
-    blocks of 16 tokens, then of blocks: 2^-24 (16 + n / 16), and of partial results less than 2^-17."""
+    blocks of 16 tokens, then of blocks: 2^-24 (16 + n / 16), and of partial results less than 2^-17.
+
+    8-bit caches keep halves in fp16, whose smallest step is 2^-24: queries are scaled to a largest value of 1 or more, so a query is
+    off by 2^-16 of itself or by 2^-25 of the largest one, whichever is more: that adds 2^-25 scale max|q| sum |k| to d. Weights times
+    scales w_j = p_j scale_j are scaled so that the largest one's power of two is 2^14, and are off by 2^-16 of themselves or by 2^-39 of
+    twice the largest one (of a warp's, or smaller): that adds 2^-38 max w sum |code| to the result."""
     rows, heads, dim = q.shape
     group = heads // cache.kv_heads
     out = torch.zeros(rows, heads, dim, dtype=torch.float64, device="cuda")
@@ -132,7 +137,8 @@ def attention64(cache, lengths, q, q_tokens, scale):
             continue
         at = torch.arange(n, dtype=torch.int32, device="cuda")
         seq = torch.full_like(at, s)
-        k, v = cache.held(0, seq, at)[0], cache.held(1, seq, at)[0]
+        k = cache.held(0, seq, at)[0]
+        v, raw, v_scales = cache.held(1, seq, at)
         for i in range(q_tokens):
             seen = n - q_tokens + 1 + i
             if seen <= 0:
@@ -141,11 +147,17 @@ def attention64(cache, lengths, q, q_tokens, scale):
             score = torch.einsum("hgd,thd->hgt", x, k[:seen]) * scale
             size = torch.einsum("hgd,thd->hgt", x.abs(), k[:seen].abs()) * abs(scale)
             p = torch.softmax(score, -1)
+            steps = 0.0
+            if v_scales is not None:
+                size = size + 2.0 ** -11 * abs(scale) * torch.einsum("hg,th->hgt", x.abs().amax(-1), k[:seen].abs().sum(-1))
+                codes = raw[:seen].view(POOLS[cache.fmt]).double().abs().sum(0)
+                steps = 2.0 ** -38 * (p * v_scales[:seen].double().T[:, None]).amax(-1)[..., None] * codes[:, None]
+                steps = steps.reshape(heads, dim)
             out[s * q_tokens + i] = torch.einsum("hgt,thd->hgd", p, v[:seen]).reshape(heads, dim)
             mean = torch.einsum("hgt,thd->hgd", p, v[:seen].abs()).reshape(heads, dim)
             off = 2.12 * 2.0 ** -14 * size.amax(-1) + 2.0 ** -16 + 2.0 ** -24 * (16 + seen / 16) + 2.0 ** -17
             assert float((2.0 ** -14 * size.amax(-1)).max()) < 0.1
-            bound[s * q_tokens + i] = mean * off.reshape(heads, 1)
+            bound[s * q_tokens + i] = mean * off.reshape(heads, 1) + steps
     return out, bound
 
 
