@@ -7,17 +7,18 @@
 // 12 to 16 operations a byte, so memory is the bound, and the kernel is built around keeping loads in flight.
 //
 //   * One block per SM, eight warps, each with a ring of its own in shared memory. Tiles of 16 tokens (they never cross a page)
-//     go round the warps; a warp's first lane asks for keys and values of its next tiles with tensor copies, past the end of an
-//     item too, so that 190 KB stay in flight per SM while results are joined. No warp waits for another one inside an item.
+//     go round the warps, two at a time for 8-bit caches; a warp asks for keys and values of its next tiles with tensor copies, past the
+//     end of an item too, so that 190 KB stay in flight per SM while results are joined. No warp waits for another one inside an item.
 //   * Both products run on m16n8k16 MMAs with eight query rows: rows 0...7 of the left operand hold the upper halves of the eight
 //     rows' factors, rows 8...15 the lower halves, so that the sum of the two accumulators is a product of factors of 16 bits or more
 //     (two bf16 numbers, error 2^-17; two fp16 numbers for 8-bit caches, 2^-22), at no cost: the rows would be empty.
 //   * 8-bit codes become fp16 exactly. Which 16 dimensions an MMA multiplies is free as long as queries and keys agree, so that a
 //     lane takes whole 16-byte pieces of a key row; values are read transposed as pairs of bytes, which gives the lane a pair of
 //     dimensions, one for each of two MMAs.
-//   * One pass: every warp keeps a running maximum, sum and result of each row in registers. The scale of a token's values goes into its
-//     weight: weights are kept relative to the largest weight times scale so far (its power of two), and stay in fp16's range whatever the
-//     scales are.
+//   * One pass: every warp keeps a sum and a result of each row in registers, relative to a power of two that is raised when a score lies 8
+//     above it, which is seldom after the first tiles (raising it with every maximum cost 128 multiplications a tile). The scale of a
+//     token's values goes into its weight; weights times scales have a reference of their own, so that they stay in fp16's range
+//     whatever the scales are.
 //   * The work of all sequences is cut into equal shares by every block for itself (q4_attention_plan.h), from the lengths in device memory:
 //     a captured graph follows them. Results of an item cut over several blocks are joined in order by the last one.
 #include <cuda_fp8.h>
@@ -36,9 +37,12 @@ constexpr uint32_t kRoundDims = 64;             // dimensions joined at a time
 constexpr uint32_t kRoundPitch = kRoundDims + 16;  // floats between rows of the join buffer: lanes of a store fall into different banks
 constexpr uint32_t kMostPieces = 256;           // of an item (blocks of the grid)
 constexpr uint32_t kLeastRun = 16;              // tiles: shorter runs cost more in joining than they save
-// 8-bit caches: weights go up to 2^15, near the end of fp16's range, so that their lower halves keep 16 bits of weights down to
-// 2^-23 of the largest one (and 2^-39 of it below)
-constexpr float kWeightLift = 14.f;
+constexpr float kNone = -3.0e38f;               // a reference below all scores: the row has seen nothing
+constexpr float kHeadroom = 8.f;                // how far above its reference a score may lie, in powers of two
+// 8-bit caches: a weight times scale is brought to 2^11 when it becomes the reference and may grow to 2^15, near the end of fp16's
+// range, so that lower halves keep 16 bits of weights down to 2^-19 of the largest one (and 2^-35 of it below)
+constexpr int kWeightExponent = 11;
+constexpr float kMostWeight = 32768.f;
 constexpr unsigned long long kWaitLimitNs = 200ull * 1000 * 1000, kLateLimitNs = 1000 * 1000;
 constexpr uint32_t kSharedLimit = 227 * 1024;
 
@@ -53,15 +57,17 @@ struct Shape {
     static constexpr uint32_t kChunks = kRow / 16;                   // 16-byte pieces of a row
     static constexpr uint32_t kChunkDims = FMT == 0 ? 8 : 16;
     static constexpr uint32_t kAcc = HDP / 8;                        // accumulators of four numbers
-    // shared memory: rings, their scales, barriers, the join buffer, and small arrays
+    static constexpr uint32_t kStep = FMT == 0 ? 1 : 2;              // tiles a warp multiplies at a time
+    // shared memory: rings, their scales, barriers, queries, the join buffer, and small arrays
+    static constexpr uint32_t kQueries = kMmas * 32 * 16;
     static constexpr uint32_t kJoin = kWarps * kAttentionRows * kRoundPitch * 4;
     static constexpr uint32_t kWeights = kMostPieces * kAttentionRows * 4;  // over the join buffer
     static constexpr uint32_t kSmall = 2048;
-    static constexpr uint32_t kFit = (kSharedLimit - 1024 - kJoin - kSmall) / (kWarps * (kTile + 64 + 8));
+    static constexpr uint32_t kFit = (kSharedLimit - 1024 - kQueries - kJoin - kSmall) / (kWarps * (kTile + 64 + 8));
     static constexpr uint32_t kSlots = kFit < 16 ? kFit : 16;        // of a warp's ring: keys and values of tiles in turn
     static constexpr uint32_t kRing = kWarps * kSlots * kTile;
-    static constexpr uint32_t kShared = 1024 + kRing + kWarps * kSlots * (64 + 8) + kJoin + kSmall;
-    static_assert(kSlots >= 2 && kWeights <= kJoin, "");
+    static constexpr uint32_t kShared = 1024 + kRing + kWarps * kSlots * (64 + 8) + kQueries + kJoin + kSmall;
+    static_assert(kSlots > kStep && kWeights <= kJoin, "");
 };
 
 // ---- small pieces ----
@@ -160,6 +166,8 @@ struct Geometry {
     uint32_t heads;   // items of a sequence = key heads * chunks
     uint32_t rows;    // query rows of a key head
     uint32_t group;   // query heads of a key head
+    uint32_t per;     // tiles of a page, and the division by it as a product: tile / per = (tile * inverse >> 32) >> shift
+    uint32_t inverse, shift;
 };
 
 __device__ __forceinline__ int64_t length_of(const AttentionParams &p, uint32_t s) {
@@ -247,14 +255,16 @@ __device__ Share share_of_block(const AttentionParams &p, const Geometry &g, uin
 
 // ---- asking for tiles ----
 
-// What a warp asks for, ahead of what it multiplies: keys, then values, of its tiles in order. The page number of the tile that is
-// next is read when the tile before it is asked for.
+// What a warp asks for, ahead of what it multiplies: keys of its next kStep tiles, then their values. Page numbers of the tiles that
+// come next are read when the ones before have been asked for. A step's second tile may lie behind the segment's end: such a copy
+// starts outside the tensor map and brings zeros.
 template <int FMT, int HDP>
 struct Asker {
     using S = Shape<FMT, HDP>;
     Cursor at;
-    uint32_t tile, head, page, place, slot;
-    bool more, values;
+    uint32_t tile, head, slot, step;
+    uint32_t page[S::kStep], place[S::kStep];
+    bool more;
 
     __device__ __forceinline__ void look(const AttentionParams &p, const Geometry &g, uint32_t warp) {
         while (tile >= at.end) {
@@ -262,51 +272,54 @@ struct Asker {
                 more = false;
                 return;
             }
-            tile = at.begin + warp;
+            tile = at.begin + warp * S::kStep;
         }
-        const uint32_t per = p.kv.page_tokens / kTileTokens;
-        head = at.item / g.chunks;
-        place = tile % per * kTileTokens;
-        page = (uint32_t)__ldcg(p.kv.table + (uint64_t)at.s * p.kv.row_stride + tile / per);
+        head = g.chunks == 1 ? at.item : at.item / g.chunks;
+        const int32_t *table = p.kv.table + (uint64_t)at.s * p.kv.row_stride;
+#pragma unroll
+        for (uint32_t i = 0; i < S::kStep; ++i) {
+            const uint32_t entry = g.per == 1 ? tile + i : __umulhi(tile + i, g.inverse) >> g.shift;
+            place[i] = (tile + i - entry * g.per) * kTileTokens;
+            page[i] = tile + i < at.end ? (uint32_t)__ldcg(table + entry) : ~0u;
+        }
     }
     __device__ __forceinline__ void start(const Share &share, const AttentionParams &p, const Geometry &g, uint32_t warp) {
         at = share.at;
-        tile = at.begin + warp;
-        slot = 0;
+        tile = at.begin + warp * S::kStep;
+        slot = step = 0;
         more = true;
-        values = false;
         look(p, g, warp);
     }
+    // Lane i brings segment i of the rows, the next one the scales.
     __device__ __forceinline__ void ask(const AttentionParams &p, const Geometry &g, const CUtensorMap *k_map, const CUtensorMap *v_map, uint32_t ring, uint32_t scales, uint32_t bars,
                                         uint32_t warp, uint32_t lane) {
         if (!more) return;
-        if (lane == 0) {
-            const uint32_t bar = bars + slot * 8, dst = ring + slot * S::kTile, sc = scales + slot * 64;
-            const bool there = page < p.kv.pages;
-            const CUtensorMap *map = values ? v_map : k_map;
-            // (a page outside the cache is outside the tensor map too: such copies bring zeros)
-            const int at_page = (int)(there ? page : p.kv.pages);
-            uint32_t bytes = S::kTile;
-            if (FMT != 0 && there) bytes += 64;
-            if (!there) {
-                *p.kv.input_error = 1;
-                if (FMT != 0) {
-                    for (uint32_t i = 0; i < 64; i += 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sc + i), "r"(0u) : "memory");
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
+        const bool values = step >= S::kStep;
+        uint32_t at_page = page[0], at_place = place[0];
+        bool last = tile + 1 >= at.end;
+        if (S::kStep == 2 && (step & 1u)) at_page = page[1], at_place = place[1];
+        const uint32_t bar = bars + slot * 8, dst = ring + slot * S::kTile, sc = scales + slot * 64;
+        const bool there = at_page < p.kv.pages;
+        if (!there) {
+            // (behind the segment's end, or no page of the cache)
+            if (lane == 0 && !(S::kStep == 2 && (step & 1u) && last)) *p.kv.input_error = 1;
+            if (FMT != 0) {
+                if (lane < 16) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sc + lane * 4), "r"(0u) : "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
             }
-            mbar_expect(bar, bytes);
-#pragma unroll
-            for (uint32_t i = 0; i < S::kSegs; ++i) copy_tile(dst + i * (kTileTokens * S::kSeg), map, bar, (int)(i * S::kSeg / (FMT == 0 ? 2 : 1)), (int)place, (int)head, at_page);
-            if (FMT != 0 && there)
-                copy_bytes(sc, (values ? p.kv.v_scales : p.kv.k_scales) + ((uint64_t)page * p.kv.kv_heads + head) * p.kv.page_tokens + place, 64, bar);
         }
+        if (lane == 0) mbar_expect(bar, S::kTile + (FMT != 0 && there ? 64u : 0u));
+        if (lane < S::kSegs)
+            copy_tile(dst + lane * (kTileTokens * S::kSeg), values ? v_map : k_map, bar, (int)(lane * S::kSeg / (FMT == 0 ? 2 : 1)), (int)at_place, (int)head, (int)(there ? at_page : p.kv.pages));
+        if (FMT != 0 && lane == S::kSegs && there)
+            copy_bytes(sc, (values ? p.kv.v_scales : p.kv.k_scales) + ((uint64_t)at_page * p.kv.kv_heads + head) * p.kv.page_tokens + at_place, 64, bar);
         slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-        if (values) {
-            tile += kWarps;
+        if (++step == 2 * S::kStep) {
+            step = 0;
+            tile += kWarps * S::kStep;
             look(p, g, warp);
         }
-        values = !values;
     }
 };
 
@@ -322,18 +335,22 @@ template <int FMT, int HDP>
 __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ Geometry g, const __grid_constant__ CUtensorMap k_map,
                                                                 const __grid_constant__ CUtensorMap v_map) {
     using S = Shape<FMT, HDP>;
+    constexpr uint32_t kStep = S::kStep;
     extern __shared__ uint8_t shared_raw[];
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(shared_raw), pad = (1024u - (raw & 1023u)) & 1023u;
     uint8_t *const shared = shared_raw + pad;
-    float *const join = reinterpret_cast<float *>(shared + S::kRing + kWarps * S::kSlots * (64 + 8));
+    uint4 *const queries = reinterpret_cast<uint4 *>(shared + S::kRing + kWarps * S::kSlots * (64 + 8));  // left operands: [MMA][lane]
+    float *const join = reinterpret_cast<float *>(queries) + S::kQueries / 4;
     float *const small = join + S::kJoin / 4;
     float *const tops = small, *const sums = small + kWarps * kAttentionRows;  // [warp][row]
-    float *const totals = small + 2 * kWarps * kAttentionRows;                 // [row] sum, [row] maximum of joined pieces
-    uint64_t *const scratch = reinterpret_cast<uint64_t *>(small + 2 * kWarps * kAttentionRows + 2 * kAttentionRows);
+    float *const totals = small + 2 * kWarps * kAttentionRows;                 // [row]
+    float *const row_scales = totals + kAttentionRows;                         // [row] scale of the scores, in powers of two
+    uint64_t *const scratch = reinterpret_cast<uint64_t *>(row_scales + kAttentionRows);
     uint32_t *const arrived = reinterpret_cast<uint32_t *>(scratch + 2 * kWarps + 8);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row = lane >> 2, quad = lane & 3u;
     const uint32_t ring = raw + pad + warp * S::kSlots * S::kTile;
     const uint32_t scales = raw + pad + S::kRing + warp * S::kSlots * 64, bars = raw + pad + S::kRing + kWarps * S::kSlots * 64 + warp * S::kSlots * 8;
+    const uint32_t queries_at = raw + pad + S::kRing + kWarps * S::kSlots * (64 + 8) + lane * 16;
     if (lane == 0)
         for (uint32_t i = 0; i < S::kSlots; ++i) mbar_init(bars + i * 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -350,253 +367,301 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         unsigned long long limit_ns = kWaitLimitNs;
         Cursor at = share.at;
         do {
-            // ---- queries of the item, split into halves, in the order in which key rows are read ----
+            // ---- queries of the item: warp w brings row w, split into halves, in the order in which key rows are read ----
             const uint32_t head = at.item / g.chunks, chunk = at.item % g.chunks;
-            const uint32_t r = chunk * kAttentionRows + row, draft = r / g.group;
-            const bool live = r < g.rows;
-            // tokens that the row sees
-            const int32_t limit = live ? at.length - (int32_t)p.q_tokens + 1 + (int32_t)draft : 0;
-            uint32_t qa[S::kMmas][4];
-            float row_scale = p.scale * 1.4426950408889634f;
             {
-                float q[S::kMmas][4];
-                const uint64_t base = ((uint64_t)at.s * p.q_tokens + draft) * p.q_stride + ((uint64_t)head * g.group + r % g.group) * p.kv.head_dim;
-                uint32_t amax = 0;
+                const uint32_t r = chunk * kAttentionRows + warp, d = lane * 8;
+                float q[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (r < g.rows && d < p.kv.head_dim) {
+                    const uint64_t base = ((uint64_t)at.s * p.q_tokens + r / g.group) * p.q_stride + ((uint64_t)head * g.group + r % g.group) * p.kv.head_dim + d;
+                    if (p.q_is_f32) {
+                        const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + base);
+                        const float4 v = __ldcg(f), w = __ldcg(f + 1);
+                        q[0] = v.x, q[1] = v.y, q[2] = v.z, q[3] = v.w, q[4] = w.x, q[5] = w.y, q[6] = w.z, q[7] = w.w;
+                    } else {
+                        const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + base));
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (uint32_t m = 0; m < S::kMmas; ++m) {
-                    // four values for each MMA: a 16-byte piece of a key row holds 8 or 16 of them
-                    constexpr uint32_t kPer = S::kChunkDims / 4;
-                    const uint32_t piece = m / kPer, seg = piece / S::kPieces;
-                    const uint32_t d = (seg * (S::kSeg / 16) + quad * S::kPieces + piece % S::kPieces) * S::kChunkDims + m % kPer * 4;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (live && d < p.kv.head_dim) {
-                        if (p.q_is_f32) {
-                            v = __ldcg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + base + d));
-                        } else {
-                            const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.q) + base + d));
-                            v = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-                        }
+                        for (int i = 0; i < 4; ++i) q[2 * i] = __uint_as_float(w[i] << 16), q[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
                     }
-                    q[m][0] = v.x, q[m][1] = v.y, q[m][2] = v.z, q[m][3] = v.w;
-                    if (FMT != 0)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) amax = max(amax, __float_as_uint(q[m][i]) & 0x7fffffffu);
                 }
-                float unit = 1.f;
+                float unit = 1.f, row_scale = p.scale * 1.4426950408889634f;
                 if (FMT != 0) {
                     // fp16 halves: the row is scaled by a power of two that brings its largest value into [1, 2)
-                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                    const uint32_t e = min(max(amax >> 23, 1u), 254u);
+                    uint32_t amax = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(q[i]) & 0x7fffffffu);
+                    const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, amax) >> 23, 1u), 254u);
                     unit = e == 254u ? __uint_as_float(0x00400000u) : __uint_as_float((254u - e) << 23);
                     row_scale *= __uint_as_float(e << 23);
                 }
+                if (d < HDP) {
+                    // four values are one lane's part of an MMA; a 16-byte piece of a key row holds 8 or 16
+                    constexpr uint32_t kPer = S::kChunkDims / 4;
+                    const uint32_t piece = d / S::kChunkDims, seg = piece / (S::kSeg / 16), in_seg = piece % (S::kSeg / 16);
+                    const uint32_t m = (seg * S::kPieces + in_seg % S::kPieces) * kPer + d % S::kChunkDims / 4, to = warp * 4 + in_seg / S::kPieces;
 #pragma unroll
-                for (uint32_t m = 0; m < S::kMmas; ++m) {
-                    // int8 codes are taken from a word as bytes 0 and 2, 1 and 3, the others in order
-                    constexpr int i1 = FMT == 1 ? 2 : 1, i2 = FMT == 1 ? 1 : 2;
-                    split<FMT>(q[m][0] * unit, q[m][i1] * unit, qa[m][0], qa[m][1]);
-                    split<FMT>(q[m][i2] * unit, q[m][3] * unit, qa[m][2], qa[m][3]);
+                    for (int i = 0; i < 2; ++i) {
+                        // int8 codes are taken from a word as bytes 0 and 2, 1 and 3, the others in order
+                        constexpr int i1 = FMT == 1 ? 2 : 1, i2 = FMT == 1 ? 1 : 2;
+                        uint4 a;
+                        split<FMT>(q[4 * i] * unit, q[4 * i + i1] * unit, a.x, a.y);
+                        split<FMT>(q[4 * i + i2] * unit, q[4 * i + 3] * unit, a.z, a.w);
+                        queries[(m + i) * 32 + to] = a;
+                    }
                 }
+                if (lane == 0) row_scales[warp] = row_scale;
             }
+            __syncthreads();
+            const float row_scale = row_scales[row];
+            // tokens of the segment that all rows see, that this row sees, and that exist
+            const int32_t end_token = (int32_t)(at.end * kTileTokens), existing = min(at.length, end_token);
+            const int32_t sure = min(at.length - (int32_t)p.q_tokens + 1, end_token);
+            const uint32_t r = chunk * kAttentionRows + row;
+            const int32_t limit = r < g.rows ? min(at.length - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group), end_token) : 0;
             float acc[S::kAcc][4];
 #pragma unroll
             for (uint32_t i = 0; i < S::kAcc; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-            float top = -INFINITY, sum = 0.f;     // of the scores, in powers of two; sum: of this lane's tokens
-            float weight_top = -INFINITY;         // 8-bit: of the scores plus the exponents of the values' scales
+            float top = kNone, sum = 0.f;                     // reference of the row's scores; sum of this lane's weights
+            float weight_top = kNone, lift = 0.f, most = 0.f;  // 8-bit: reference of weights times scales, 2^(top - weight_top), and what they may be
 
-            for (uint32_t tile = at.begin + warp; tile < at.end; tile += kWarps) {
+            for (uint32_t tile = at.begin + warp * kStep; tile < at.end; tile += kWarps * kStep) {
                 const int32_t token = (int32_t)(tile * kTileTokens);
-                const bool edge = token + (int32_t)kTileTokens > at.length - (int32_t)p.q_tokens + 1;  // some rows do not see all of it
-                // ---- scores of 16 tokens ----
-                float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-                mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
-                {
-                    const uint32_t base = ring + slot * S::kTile;
+                const bool edge = token + (int32_t)(kStep * kTileTokens) > sure;  // some rows do not see all of it
+                // ---- scores ----
+                uint32_t key_slot[kStep], value_slot[kStep];
 #pragma unroll
-                    for (uint32_t seg = 0; seg < S::kSegs; ++seg)
+                for (uint32_t i = 0; i < kStep; ++i) {
+                    mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
+                    key_slot[i] = slot;
+                    slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+                    parity ^= slot == 0;
+                }
+                float s[2 * kStep][4];
 #pragma unroll
-                        for (uint32_t c = 0; c < S::kPieces; ++c) {
-                            const uint32_t piece = quad * S::kPieces + c, turn = S::kSeg == 128 ? row : row >> 1 & 3u;
-                            const uint32_t at_piece = base + seg * (kTileTokens * S::kSeg) + row * S::kSeg + ((piece ^ turn) << 4);
+                for (uint32_t n = 0; n < 2 * kStep; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-                            for (int n = 0; n < 2; ++n) {
-                                const uint4 w = lds_v4(at_piece + n * 8 * S::kSeg);
-                                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-                                if (FMT == 0) {
-                                    const uint32_t m = (seg * S::kPieces + c) * 2;
-                                    mma<FMT>(s[n], qa[m], word[0], word[1]);
-                                    mma<FMT>(s[n], qa[m + 1], word[2], word[3]);
-                                } else {
+                for (uint32_t seg = 0; seg < S::kSegs; ++seg)
 #pragma unroll
-                                    for (uint32_t i = 0; i < 4; ++i) {
-                                        const uint32_t m = (seg * S::kPieces + c) * 4 + i;
-                                        if (FMT == 1) mma<FMT>(s[n], qa[m], int8_even(word[i]), int8_even(word[i] >> 8));
-                                        else mma<FMT>(s[n], qa[m], e4m3_pair(word[i]), e4m3_pair(word[i] >> 16));
-                                    }
-                                }
+                    for (uint32_t c = 0; c < S::kPieces; ++c) {
+                        const uint32_t piece = quad * S::kPieces + c, turn = S::kSeg == 128 ? row : row >> 1 & 3u;
+                        const uint32_t within = seg * (kTileTokens * S::kSeg) + row * S::kSeg + ((piece ^ turn) << 4);
+                        constexpr uint32_t kPer = S::kChunkDims / 4;
+                        const uint32_t m = (seg * S::kPieces + c) * kPer;
+                        uint32_t word[2 * kStep][4];
+#pragma unroll
+                        for (uint32_t n = 0; n < 2 * kStep; ++n) {
+                            const uint4 w = lds_v4(ring + key_slot[n / 2] * S::kTile + within + n % 2 * 8 * S::kSeg);
+                            word[n][0] = w.x, word[n][1] = w.y, word[n][2] = w.z, word[n][3] = w.w;
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < kPer; ++i) {
+                            const uint4 w = lds_v4(queries_at + (m + i) * 512);
+                            const uint32_t qa[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (uint32_t n = 0; n < 2 * kStep; ++n) {
+                                if (FMT == 0) mma<FMT>(s[n], qa, word[n][2 * i], word[n][2 * i + 1]);
+                                else if (FMT == 1) mma<FMT>(s[n], qa, int8_even(word[n][i]), int8_even(word[n][i] >> 8));
+                                else mma<FMT>(s[n], qa, e4m3_pair(word[n][i]), e4m3_pair(word[n][i] >> 16));
                             }
                         }
-                }
-                // this lane's four: tokens 2 quad, + 1, + 8, + 9 of the tile, row `row`
-                float x[4] = {s[0][0] + s[0][2], s[0][1] + s[0][3], s[1][0] + s[1][2], s[1][1] + s[1][3]};
-                if (FMT != 0) {
-                    const uint2 a = lds_v2(scales + slot * 64 + quad * 8), b = lds_v2(scales + slot * 64 + 32 + quad * 8);
-                    x[0] *= __uint_as_float(a.x), x[1] *= __uint_as_float(a.y), x[2] *= __uint_as_float(b.x), x[3] *= __uint_as_float(b.y);
-                }
+                    }
+                // this lane's: tokens 2 quad, + 1, + 8, + 9 of each tile, row `row`
+                float x[4 * kStep];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] *= row_scale;
-                __syncwarp();  // the slot has been read
-                asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
-                slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-                parity ^= slot == 0;
+                for (uint32_t n = 0; n < 2 * kStep; ++n) {
+                    x[2 * n] = (s[n][0] + s[n][2]) * row_scale;
+                    x[2 * n + 1] = (s[n][1] + s[n][3]) * row_scale;
+                    if (FMT != 0) {
+                        const uint2 k = lds_v2(scales + key_slot[n / 2] * 64 + n % 2 * 32 + quad * 8);
+                        x[2 * n] *= __uint_as_float(k.x), x[2 * n + 1] *= __uint_as_float(k.y);
+                    }
+                }
+                __syncwarp();  // the slots have been read
+#pragma unroll
+                for (uint32_t i = 0; i < kStep; ++i) asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
                 if (edge)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (token + (int32_t)quad * 2 + (i & 1) + (i >> 1) * 8 >= limit) x[i] = -INFINITY;
+                    for (uint32_t i = 0; i < 4 * kStep; ++i)
+                        if (token + (int32_t)(i / 2 * 8 + quad * 2 + i % 2) >= limit) x[i] = -INFINITY;
                 // ---- weights ----
-                mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
-                float frac[4], lift[4];  // 8-bit: scale of the token's values = frac * 2^lift
-                if (FMT != 0) {
-                    const uint2 a = lds_v2(scales + slot * 64 + quad * 8), b = lds_v2(scales + slot * 64 + 32 + quad * 8);
-                    const uint32_t bits[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t e = bits[i] >> 23 & 0xffu;
-                        // below 2^-126: times 2^126; infinities and NaNs as they are
-                        lift[i] = (float)((int)max(e, 1u) - 127);
-                        frac[i] = e == 0 ? __uint_as_float(bits[i]) * 0x1p126f : e == 255 ? __uint_as_float(bits[i]) : __uint_as_float((bits[i] & 0x807fffffu) | 0x3f800000u);
+                for (uint32_t i = 0; i < kStep; ++i) {
+                    mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
+                    value_slot[i] = slot;
+                    slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+                    parity ^= slot == 0;
+                }
+                float value_scale[FMT == 0 ? 1 : 4 * kStep], weight[4 * kStep];
+                if (FMT != 0)
+#pragma unroll
+                    for (uint32_t n = 0; n < 2 * kStep; ++n) {
+                        const uint2 v = lds_v2(scales + value_slot[n / 2] * 64 + n % 2 * 32 + quad * 8);
+                        value_scale[2 * n] = __uint_as_float(v.x), value_scale[2 * n + 1] = __uint_as_float(v.y);
+                        // (a token that the row does not see: its scale may be anything)
+                        if (edge) {
+                            if (x[2 * n] == -INFINITY) value_scale[2 * n] = 0.f;
+                            if (x[2 * n + 1] == -INFINITY) value_scale[2 * n + 1] = 0.f;
+                        }
                     }
+                float high = x[0], weight_high = 0.f;
+#pragma unroll
+                for (uint32_t i = 1; i < 4 * kStep; ++i) high = fmaxf(high, x[i]);
+#pragma unroll
+                for (uint32_t i = 0; i < 4 * kStep; ++i) {
+                    weight[i] = exp2_fast(x[i] - top);
+                    if (FMT != 0) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
                 }
-                float high = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), weight_high = 0.f;
-                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
-                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
-                bool rise = high > top;
-                if (FMT != 0) {
-                    weight_high = fmaxf(fmaxf(x[0] + lift[0], x[1] + lift[1]), fmaxf(x[2] + lift[2], x[3] + lift[3]));
-                    weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 1));
-                    weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 2));
-                    rise = rise || weight_high > weight_top;
-                }
-                if (__any_sync(0xffffffffu, rise)) {
-                    if (high > top) {
-                        sum *= exp2_fast(top - high);  // (2^-inf is 0)
-                        if (FMT == 0) weight_high = top;
+                if (__any_sync(0xffffffffu, high - top > kHeadroom || (FMT != 0 && weight_high > most))) {
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+                    float keep = 1.f;
+                    if (high - top > kHeadroom) {
+                        high = ceilf(high);
+                        keep = exp2_fast(top - high);
+                        sum *= keep;
                         top = high;
-                    } else if (FMT == 0) {
-                        weight_high = top;
+                        if (FMT != 0) {
+                            lift = weight_top == kNone ? 0.f : exp2_fast(top - weight_top);
+                            most = lift > 0.f ? kMostWeight / lift : 0.f;
+                            keep = 1.f;
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < 4 * kStep; ++i) weight[i] = exp2_fast(x[i] - top);
                     }
-                    float keep;
-                    if (FMT == 0) {
-                        keep = weight_high == top ? 1.f : exp2_fast(weight_high - top);
-                    } else {
-                        keep = weight_high > weight_top ? exp2_fast(weight_top - weight_high) : 1.f;
-                        weight_top = fmaxf(weight_top, weight_high);
+                    if (FMT != 0) {
+                        weight_high = 0.f;
+#pragma unroll
+                        for (uint32_t i = 0; i < 4 * kStep; ++i) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
+                        weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 1));
+                        weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 2));
+                        if (weight_high > most) {
+                            const int e = (int)(__float_as_uint(weight_high) >> 23) - 126;  // weight_high < 2^e
+                            const float next = top + (float)max(e - kWeightExponent, -126);
+                            keep = weight_top == kNone ? 0.f : exp2_fast(weight_top - next);
+                            weight_top = next;
+                            lift = exp2_fast(top - weight_top);
+                            most = kMostWeight / lift;
+                        }
                     }
 #pragma unroll
                     for (uint32_t i = 0; i < S::kAcc; ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) acc[i][j] *= keep;
                 }
-                const float base = top == -INFINITY ? 0.f : top, weight_base = weight_top == -INFINITY ? 0.f : weight_top;
-                float weight[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = exp2_fast(x[i] - base);
-                    sum += e;
-                    // (a token that the row does not see: its scale may be anything)
-                    weight[i] = FMT == 0 ? e : x[i] == -INFINITY ? 0.f : exp2_fast(x[i] + lift[i] - weight_base + kWeightLift) * frac[i];
-                }
-                uint32_t pa[4];
-                split<FMT>(weight[0], weight[1], pa[0], pa[1]);
-                split<FMT>(weight[2], weight[3], pa[2], pa[3]);
-                // ---- values ----
-                {
-                    const uint32_t base_v = ring + slot * S::kTile;
-                    // Behind the sequence's end rows hold anything: zeros are taken for them. Among draft tokens a value that is not finite may
-                    // be seen by some rows only; a weight of zero does not take it out of a sum, so it is taken out of the MMA and
-                    // added below to the rows that see it.
-                    const int32_t behind = at.length - token;  // tokens of the tile from here on do not exist
-                    bool odd_values = false;
-                    if (FMT != 1 && edge && p.q_tokens > 1) {
-                        for (uint32_t i = lane * 16; i < S::kTile; i += 512) {
-                            const uint4 w = lds_v4(base_v + i);
-                            const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-                            if ((int32_t)(i / S::kSeg % kTileTokens) < behind)
-#pragma unroll
-                                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                                    for (int b = 0; b < 4; b += FMT == 0 ? 2 : 1) odd_values = odd_values || not_finite<FMT>(word[j], b);
-                        }
-                        odd_values = __any_sync(0xffffffffu, odd_values);
+                for (uint32_t i = 0; i < 4 * kStep; ++i) {
+                    if (FMT != 0) {
+                        sum += weight[i];
+                        weight[i] *= value_scale[i] * lift;
                     }
-                    const uint32_t matrix = lane >> 3, line = (lane & 7u) + (matrix & 1u) * 8, turn = S::kSeg == 128 ? line & 7u : line >> 1 & 3u;
+                }
+                uint32_t pa[kStep][4];
 #pragma unroll
-                    for (uint32_t c = 0; c < S::kChunks; c += 2) {
-                        const uint32_t seg = c / (S::kSeg / 16), piece = c % (S::kSeg / 16) + (matrix >> 1);
-                        uint32_t v[4];
-                        ldmatrix_x4_trans(v, base_v + seg * (kTileTokens * S::kSeg) + line * S::kSeg + ((piece ^ turn) << 4));
-                        if (edge) {
+                for (uint32_t i = 0; i < kStep; ++i) {
+                    split<FMT>(weight[4 * i], weight[4 * i + 1], pa[i][0], pa[i][1]);
+                    split<FMT>(weight[4 * i + 2], weight[4 * i + 3], pa[i][2], pa[i][3]);
+                    // bf16: the weights as they are multiplied, so that they add up to one whatever the halves cut off
+                    if (FMT == 0)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int32_t t = (int32_t)quad * 2 + (i & 1) * 8;
-                                v[i] &= (t < behind ? 0xffffu : 0u) | (t + 1 < behind ? 0xffff0000u : 0u);
-                                if (FMT != 1 && odd_values)
+                        for (int j = 0; j < 4; j += 2)
+                            sum += (__uint_as_float(pa[i][j] << 16) + __uint_as_float(pa[i][j + 1] << 16)) +
+                                   (__uint_as_float(pa[i][j] & 0xffff0000u) + __uint_as_float(pa[i][j + 1] & 0xffff0000u));
+                }
+                // ---- values ----
+                if (edge) {
+                    // Rows behind the sequence's end hold anything: zeros are put in their place. Among draft tokens a value that is not
+                    // finite may be seen by some rows only, and a weight of zero does not take it out of a sum: it is added here to the
+                    // rows that see it, and becomes a zero too.
 #pragma unroll
-                                    for (int b = 0; b < 4; b += FMT == 0 ? 2 : 1)
-                                        if (not_finite<FMT>(v[i], b)) v[i] &= ~((FMT == 0 ? 0xffffu : 0xffu) << (b * 8));
+                    for (uint32_t i = 0; i < kStep; ++i) {
+                        const uint32_t base = ring + value_slot[i] * S::kTile;
+                        const int32_t first = token + (int32_t)(i * kTileTokens);
+                        if (FMT != 1 && p.q_tokens > 1) {
+                            bool odd = false;
+                            for (uint32_t b = lane * 16; b < S::kTile; b += 512) {
+                                const uint4 w = lds_v4(base + b);
+                                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+                                if (first + (int32_t)(b / S::kSeg % kTileTokens) < existing)
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                                        for (int k = 0; k < 4; k += FMT == 0 ? 2 : 1) odd = odd || not_finite<FMT>(word[j], k);
+                            }
+                            if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+                                for (uint32_t c = 0; c < S::kAcc; ++c)
+#pragma unroll
+                                    for (uint32_t j = 0; j < 2; ++j) {
+                                        const uint32_t d = FMT == 0 ? c * 8 + quad * 2 + j : c / 2 * 16 + quad * 4 + j * 2 + (c & 1u);
+                                        const uint32_t byte = d * (FMT == 0 ? 2 : 1), seg = byte / S::kSeg, piece = byte % S::kSeg / 16;
+                                        for (int32_t t = 0; t < (int32_t)kTileTokens && first + t < limit; ++t) {
+                                            const uint32_t swap = S::kSeg == 128 ? (uint32_t)t & 7u : (uint32_t)t >> 1 & 3u;
+                                            const uint32_t w = lds_u32((base + seg * (kTileTokens * S::kSeg) + (uint32_t)t * S::kSeg + ((piece ^ swap) << 4) + byte % 16) & ~3u);
+                                            if (not_finite<FMT>(w, byte & 3u)) acc[c][j] += FMT == 0 ? __uint_as_float((w >> ((byte & 3u) * 8)) << 16) : __uint_as_float(0x7fc00000u);
+                                        }
+                                    }
+                                __syncwarp();
+                                for (uint32_t b = lane * 16; b < S::kTile; b += 512) {
+                                    const uint4 w = lds_v4(base + b);
+                                    uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                                        for (int k = 0; k < 4; k += FMT == 0 ? 2 : 1)
+                                            if (not_finite<FMT>(word[j], k)) word[j] &= ~((FMT == 0 ? 0xffffu : 0xffu) << (k * 8));
+                                    sts_v4(base + b, make_uint4(word[0], word[1], word[2], word[3]));
+                                }
                             }
                         }
+                        for (uint32_t b = lane * 16; b < S::kTile; b += 512)
+                            if (first + (int32_t)(b / S::kSeg % kTileTokens) >= existing) sts_v4(base + b, make_uint4(0u, 0u, 0u, 0u));
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into these slots
+                    __syncwarp();
+                }
+                const uint32_t matrix = lane >> 3, line = (lane & 7u) + (matrix & 1u) * 8, turn = S::kSeg == 128 ? line & 7u : line >> 1 & 3u;
+#pragma unroll
+                for (uint32_t c = 0; c < S::kChunks; c += 2) {
+                    const uint32_t seg = c / (S::kSeg / 16), piece = c % (S::kSeg / 16) + (matrix >> 1);
+                    const uint32_t within = seg * (kTileTokens * S::kSeg) + line * S::kSeg + ((piece ^ turn) << 4);
+#pragma unroll
+                    for (uint32_t t = 0; t < kStep; ++t) {
+                        uint32_t v[4];
+                        ldmatrix_x4_trans(v, ring + value_slot[t] * S::kTile + within);
 #pragma unroll
                         for (uint32_t i = 0; i < 2; ++i) {
                             const uint32_t b0 = v[2 * i], b1 = v[2 * i + 1];
                             if (FMT == 0) {
-                                mma<FMT>(acc[c + i], pa, b0, b1);
+                                mma<FMT>(acc[c + i], pa[t], b0, b1);
                             } else if (FMT == 1) {
-                                mma<FMT>(acc[(c + i) * 2], pa, int8_even(b0), int8_even(b1));
-                                mma<FMT>(acc[(c + i) * 2 + 1], pa, int8_even(b0 >> 8), int8_even(b1 >> 8));
+                                mma<FMT>(acc[(c + i) * 2], pa[t], int8_even(b0), int8_even(b1));
+                                mma<FMT>(acc[(c + i) * 2 + 1], pa[t], int8_even(b0 >> 8), int8_even(b1 >> 8));
                             } else {
-                                mma<FMT>(acc[(c + i) * 2], pa, e4m3_pair(__byte_perm(b0, 0, 0x4420)), e4m3_pair(__byte_perm(b1, 0, 0x4420)));
-                                mma<FMT>(acc[(c + i) * 2 + 1], pa, e4m3_pair(__byte_perm(b0, 0, 0x4431)), e4m3_pair(__byte_perm(b1, 0, 0x4431)));
+                                mma<FMT>(acc[(c + i) * 2], pa[t], e4m3_pair(__byte_perm(b0, 0, 0x4420)), e4m3_pair(__byte_perm(b1, 0, 0x4420)));
+                                mma<FMT>(acc[(c + i) * 2 + 1], pa[t], e4m3_pair(__byte_perm(b0, 0, 0x4431)), e4m3_pair(__byte_perm(b1, 0, 0x4431)));
                             }
                         }
                     }
-                    if (FMT != 1 && odd_values) {
-#pragma unroll
-                        for (uint32_t i = 0; i < S::kAcc; ++i)
-#pragma unroll
-                            for (uint32_t j = 0; j < 2; ++j) {
-                                const uint32_t d = FMT == 0 ? i * 8 + quad * 2 + j : i / 2 * 16 + quad * 4 + j * 2 + (i & 1u);
-                                const uint32_t byte = d * (FMT == 0 ? 2 : 1), seg = byte / S::kSeg, piece = byte % S::kSeg / 16;
-                                for (int32_t t = 0; t < (int32_t)kTileTokens && token + t < limit; ++t) {
-                                    const uint32_t swap = S::kSeg == 128 ? (uint32_t)t & 7u : (uint32_t)t >> 1 & 3u;
-                                    const uint32_t w = lds_u32((base_v + seg * (kTileTokens * S::kSeg) + (uint32_t)t * S::kSeg + ((piece ^ swap) << 4) + byte % 16) & ~3u);
-                                    if (not_finite<FMT>(w, byte & 3u)) acc[i][j] += FMT == 0 ? __uint_as_float((w >> ((byte & 3u) * 8)) << 16) : __uint_as_float(0x7fc00000u);
-                                }
-                            }
-                    }
                 }
                 __syncwarp();
-                asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
-                slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-                parity ^= slot == 0;
+#pragma unroll
+                for (uint32_t i = 0; i < kStep; ++i) asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
             }
 
             // ---- join the warps' results ----
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             if (quad == 0) {
-                tops[warp * kAttentionRows + row] = top;
+                tops[warp * kAttentionRows + row] = top == kNone ? -INFINITY : top;
                 sums[warp * kAttentionRows + row] = sum;
             }
             __syncthreads();
             float all_top = -INFINITY;
             for (uint32_t w = 0; w < kWarps; ++w) all_top = fmaxf(all_top, tops[w * kAttentionRows + row]);
             {
-                // (a warp without tiles, and rows that see nothing, have zeros)
-                float factor = top == -INFINITY ? 0.f : exp2_fast(FMT == 0 ? top - all_top : weight_top - all_top - kWeightLift);
-                if (FMT != 0 && weight_top == -INFINITY) factor = 0.f;
-                // infinities and NaNs of rows whose scores are all -infinity stay visible through their sum
+                // (a warp without tiles, and rows that see nothing, have zeros; a row whose scores are NaNs keeps those)
+                const float factor = top == kNone || (FMT != 0 && weight_top == kNone) ? 0.f : exp2_fast((FMT == 0 ? top : weight_top) - all_top);
 #pragma unroll
                 for (uint32_t i = 0; i < S::kAcc; ++i) {
                     acc[i][0] = (acc[i][0] + acc[i][2]) * factor;
@@ -756,6 +821,11 @@ cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t str
     g.rows = g.group * p.q_tokens;
     g.chunks = (g.rows + kAttentionRows - 1) / kAttentionRows;
     g.heads = p.kv.kv_heads * g.chunks;
+    // tile / per for tiles below 2^27: 2^(32 + shift) / per rounded up has an error below per <= 2^(shift + 1), less than 2^(5 + shift)
+    g.per = p.kv.page_tokens / kTileTokens;
+    g.shift = 0;
+    while ((2u << g.shift) < g.per) ++g.shift;
+    g.inverse = g.per == 1 ? 0 : (uint32_t)(((1ull << (32 + g.shift)) + g.per - 1) / g.per);
     return launch_dependent(attention_kernel<FMT, HDP>, dim3(sm_count < kMostPieces ? sm_count : kMostPieces), kThreads, S::kShared, stream, p, g, maps[0], maps[1]);
 }
 
