@@ -12,9 +12,9 @@
 //   * Both products run on m16n8k16 MMAs with eight query rows: rows 0...7 of the left operand hold the upper halves of the eight
 //     rows' factors, rows 8...15 the lower halves, so that the sum of the two accumulators is a product of factors of 16 bits or more
 //     (two bf16 numbers, error 2^-17; two fp16 numbers for 8-bit caches, 2^-22), at no cost: the rows would be empty.
-//   * 8-bit codes become fp16 exactly. Which 16 dimensions an MMA multiplies is free as long as queries and keys agree, so that a
-//     lane takes whole 16-byte pieces of a key row; values are read transposed as pairs of bytes, which gives the lane a pair of
-//     dimensions, one for each of two MMAs.
+//   * Queries against int8 keys run on whole-number MMAs as they lie in memory, four 8-bit digits of every query; other 8-bit codes become
+//     fp16 exactly. Which dimensions an MMA multiplies is free as long as queries and keys agree, so that a lane takes whole 16-byte pieces
+//     of a key row; values are read transposed as pairs of bytes, which gives the lane a pair of dimensions, one for each of two MMAs.
 //   * One pass: every warp keeps a sum and a result of each row in registers, relative to a power of two that is raised when a score lies 8
 //     above it, which is seldom after the first tiles (raising it with every maximum cost 128 multiplications a tile). The scale of a
 //     token's values goes into its weight; weights times scales have a reference of their own, so that they stay in fp16's range
@@ -63,11 +63,12 @@ struct Shape {
     static constexpr uint32_t kJoin = kWarps * kAttentionRows * kRoundPitch * 4;
     static constexpr uint32_t kWeights = kMostPieces * kAttentionRows * 4;  // over the join buffer
     static constexpr uint32_t kSmall = 2048;
-    static constexpr uint32_t kFit = (kSharedLimit - 1024 - kQueries - kJoin - kSmall) / (kWarps * (kTile + 64 + 8));
-    static constexpr uint32_t kSlots = kFit < 16 ? kFit : 16;        // of a warp's ring: keys and values of tiles in turn
-    static constexpr uint32_t kRing = kWarps * kSlots * kTile;
-    static constexpr uint32_t kShared = 1024 + kRing + kWarps * kSlots * (64 + 8) + kQueries + kJoin + kSmall;
-    static_assert(kSlots > kStep && kWeights <= kJoin, "");
+    static constexpr uint32_t kSlot = kStep * kTile, kSlotScales = kStep * 64;
+    static constexpr uint32_t kFit = (kSharedLimit - 1024 - kQueries - kJoin - kSmall) / (kWarps * (kSlot + kSlotScales + 8));
+    static constexpr uint32_t kSlots = kFit < 8 ? kFit : 8;          // of a warp's ring: keys and values of its steps in turn
+    static constexpr uint32_t kRing = kWarps * kSlots * kSlot, kScales = kWarps * kSlots * kSlotScales, kBars = (kWarps * kSlots * 8 + 15) / 16 * 16;
+    static constexpr uint32_t kShared = 1024 + kRing + kScales + kBars + kQueries + kJoin + kSmall;
+    static_assert(kSlots >= 2 && kWeights <= kJoin && kStep * (kSegs + 1) <= 32, "");
 };
 
 // ---- small pieces ----
@@ -108,6 +109,23 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
         mma_f16_16816(d, a[0], a[1], a[2], a[3], b0, b1);
+}
+
+// Queries against int8 codes: whole-number MMAs of four signed 8-bit digits of each query, two digits to a call.
+__device__ __forceinline__ void split_digits(const float (&q)[8], uint4 &upper, uint4 &lower) {
+    uint32_t word[4][2] = {{0u, 0u}, {0u, 0u}, {0u, 0u}, {0u, 0u}};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        int v = __float2int_rn(q[i] * 0x1p29f);  // |q| < 2
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int digit = k == 3 ? v : (int)(int8_t)(v & 0xff);
+            word[k][i / 4] |= ((uint32_t)digit & 0xffu) << (i % 4 * 8);
+            v = (v - digit) >> 8;
+        }
+    }
+    upper = make_uint4(word[3][0], word[2][0], word[3][1], word[2][1]);
+    lower = make_uint4(word[1][0], word[0][0], word[1][1], word[0][1]);
 }
 
 // Bytes 0 and 2, and bytes 1 and 3, of a word of int8 codes as fp16: 0x6400 | u is 1024 + u, with u = code + 128.
@@ -255,71 +273,71 @@ __device__ Share share_of_block(const AttentionParams &p, const Geometry &g, uin
 
 // ---- asking for tiles ----
 
-// What a warp asks for, ahead of what it multiplies: keys of its next kStep tiles, then their values. Page numbers of the tiles that
-// come next are read when the ones before have been asked for. A step's second tile may lie behind the segment's end: such a copy
-// starts outside the tensor map and brings zeros.
+// What a warp asks for, ahead of what it multiplies: keys of its next kStep tiles into one slot, then their values into the next.
+// Lane i * kSegs + j brings segment j of tile i, the lanes behind those the scales. Page numbers are read one step ahead. A step's
+// second tile may lie behind the segment's end: such a copy starts outside the tensor map and brings zeros.
 template <int FMT, int HDP>
 struct Asker {
     using S = Shape<FMT, HDP>;
+    static constexpr uint32_t kCopies = S::kStep * S::kSegs;
     Cursor at;
-    uint32_t tile, head, slot, step;
-    uint32_t page[S::kStep], place[S::kStep];
-    bool more;
+    uint32_t tile, head, slot, page, place;  // page and place: of this lane's tile
+    bool more, values;
 
-    __device__ __forceinline__ void look(const AttentionParams &p, const Geometry &g, uint32_t warp) {
+    __device__ __forceinline__ static uint32_t mine(uint32_t lane) { return lane < kCopies ? lane / S::kSegs : (lane - kCopies) % S::kStep; }
+    __device__ __forceinline__ void look(const AttentionParams &p, const Geometry &g, uint32_t warp, uint32_t lane) {
         while (tile >= at.end) {
             if (!at.next([&](uint32_t i) { return length_of(p, i); }, p.kv.sequences, g.heads)) {
                 more = false;
                 return;
             }
             tile = at.begin + warp * S::kStep;
+            head = g.chunks == 1 ? at.item : at.item / g.chunks;
         }
-        head = g.chunks == 1 ? at.item : at.item / g.chunks;
-        const int32_t *table = p.kv.table + (uint64_t)at.s * p.kv.row_stride;
-#pragma unroll
-        for (uint32_t i = 0; i < S::kStep; ++i) {
-            const uint32_t entry = g.per == 1 ? tile + i : __umulhi(tile + i, g.inverse) >> g.shift;
-            place[i] = (tile + i - entry * g.per) * kTileTokens;
-            page[i] = tile + i < at.end ? (uint32_t)__ldcg(table + entry) : ~0u;
-        }
+        const uint32_t t = tile + mine(lane), entry = g.per == 1 ? t : __umulhi(t, g.inverse) >> g.shift;
+        place = (t - entry * g.per) * kTileTokens;
+        page = t < at.end ? (uint32_t)__ldcg(p.kv.table + (uint64_t)at.s * p.kv.row_stride + entry) : ~0u;
     }
-    __device__ __forceinline__ void start(const Share &share, const AttentionParams &p, const Geometry &g, uint32_t warp) {
+    __device__ __forceinline__ void start(const Share &share, const AttentionParams &p, const Geometry &g, uint32_t warp, uint32_t lane) {
         at = share.at;
         tile = at.begin + warp * S::kStep;
-        slot = step = 0;
+        head = at.item / g.chunks;
+        slot = 0;
         more = true;
-        look(p, g, warp);
+        values = false;
+        look(p, g, warp, lane);
     }
-    // Lane i brings segment i of the rows, the next one the scales.
     __device__ __forceinline__ void ask(const AttentionParams &p, const Geometry &g, const CUtensorMap *k_map, const CUtensorMap *v_map, uint32_t ring, uint32_t scales, uint32_t bars,
                                         uint32_t warp, uint32_t lane) {
         if (!more) return;
-        const bool values = step >= S::kStep;
-        uint32_t at_page = page[0], at_place = place[0];
-        bool last = tile + 1 >= at.end;
-        if (S::kStep == 2 && (step & 1u)) at_page = page[1], at_place = place[1];
-        const uint32_t bar = bars + slot * 8, dst = ring + slot * S::kTile, sc = scales + slot * 64;
-        const bool there = at_page < p.kv.pages;
-        if (!there) {
-            // (behind the segment's end, or no page of the cache)
-            if (lane == 0 && !(S::kStep == 2 && (step & 1u) && last)) *p.kv.input_error = 1;
+        const uint32_t bar = bars + slot * 8;
+        const bool there = page < p.kv.pages;
+        const uint32_t absent = __ballot_sync(0xffffffffu, !there);
+        uint32_t bytes = S::kSlot + (FMT == 0 ? 0u : S::kSlotScales);
+        if (absent) {
+            // behind the segment's end, or no page of the cache
+            if (!there && tile + mine(lane) < at.end) *p.kv.input_error = 1;
             if (FMT != 0) {
-                if (lane < 16) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sc + lane * 4), "r"(0u) : "memory");
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                bytes -= 64 * __popc(absent >> kCopies & ((1u << S::kStep) - 1));
+                if (!there && lane >= kCopies && lane < kCopies + S::kStep) {
+                    for (uint32_t i = 0; i < 64; i += 16) sts_v4(scales + slot * S::kSlotScales + (lane - kCopies) * 64 + i, make_uint4(0u, 0u, 0u, 0u));
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
                 __syncwarp();
             }
         }
-        if (lane == 0) mbar_expect(bar, S::kTile + (FMT != 0 && there ? 64u : 0u));
-        if (lane < S::kSegs)
-            copy_tile(dst + lane * (kTileTokens * S::kSeg), values ? v_map : k_map, bar, (int)(lane * S::kSeg / (FMT == 0 ? 2 : 1)), (int)at_place, (int)head, (int)(there ? at_page : p.kv.pages));
-        if (FMT != 0 && lane == S::kSegs && there)
-            copy_bytes(sc, (values ? p.kv.v_scales : p.kv.k_scales) + ((uint64_t)at_page * p.kv.kv_heads + head) * p.kv.page_tokens + at_place, 64, bar);
+        if (lane == 0) mbar_expect(bar, bytes);
+        if (lane < kCopies)
+            copy_tile(ring + slot * S::kSlot + lane * (kTileTokens * S::kSeg), values ? v_map : k_map, bar, (int)(lane % S::kSegs * S::kSeg / (FMT == 0 ? 2 : 1)), (int)place, (int)head,
+                      (int)(there ? page : p.kv.pages));
+        else if (FMT != 0 && lane < kCopies + S::kStep && there)
+            copy_bytes(scales + slot * S::kSlotScales + (lane - kCopies) * 64, (values ? p.kv.v_scales : p.kv.k_scales) + ((uint64_t)page * p.kv.kv_heads + head) * p.kv.page_tokens + place, 64, bar);
         slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-        if (++step == 2 * S::kStep) {
-            step = 0;
+        if (values) {
             tile += kWarps * S::kStep;
-            look(p, g, warp);
+            look(p, g, warp, lane);
         }
+        values = !values;
     }
 };
 
@@ -339,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     extern __shared__ uint8_t shared_raw[];
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(shared_raw), pad = (1024u - (raw & 1023u)) & 1023u;
     uint8_t *const shared = shared_raw + pad;
-    uint4 *const queries = reinterpret_cast<uint4 *>(shared + S::kRing + kWarps * S::kSlots * (64 + 8));  // left operands: [MMA][lane]
+    uint4 *const queries = reinterpret_cast<uint4 *>(shared + S::kRing + S::kScales + S::kBars);  // left operands: [MMA][lane]
     float *const join = reinterpret_cast<float *>(queries) + S::kQueries / 4;
     float *const small = join + S::kJoin / 4;
     float *const tops = small, *const sums = small + kWarps * kAttentionRows;  // [warp][row]
@@ -348,9 +366,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     uint64_t *const scratch = reinterpret_cast<uint64_t *>(row_scales + kAttentionRows);
     uint32_t *const arrived = reinterpret_cast<uint32_t *>(scratch + 2 * kWarps + 8);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row = lane >> 2, quad = lane & 3u;
-    const uint32_t ring = raw + pad + warp * S::kSlots * S::kTile;
-    const uint32_t scales = raw + pad + S::kRing + warp * S::kSlots * 64, bars = raw + pad + S::kRing + kWarps * S::kSlots * 64 + warp * S::kSlots * 8;
-    const uint32_t queries_at = raw + pad + S::kRing + kWarps * S::kSlots * (64 + 8) + lane * 16;
+    const uint32_t ring = raw + pad + warp * S::kSlots * S::kSlot, scales = raw + pad + S::kRing + warp * S::kSlots * S::kSlotScales;
+    const uint32_t bars = raw + pad + S::kRing + S::kScales + warp * S::kSlots * 8, queries_at = raw + pad + S::kRing + S::kScales + S::kBars + lane * 16;
     if (lane == 0)
         for (uint32_t i = 0; i < S::kSlots; ++i) mbar_init(bars + i * 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -361,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const Share share = share_of_block(p, g, scratch);
     if (share.any) {
         Asker<FMT, HDP> asker;
-        asker.start(share, p, g, warp);
+        asker.start(share, p, g, warp, lane);
         for (uint32_t i = 0; i < S::kSlots; ++i) asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
         uint32_t slot = 0, parity = 0;
         unsigned long long limit_ns = kWaitLimitNs;
@@ -387,28 +404,35 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 }
                 float unit = 1.f, row_scale = p.scale * 1.4426950408889634f;
                 if (FMT != 0) {
-                    // fp16 halves: the row is scaled by a power of two that brings its largest value into [1, 2)
+                    // fp16 halves, whole numbers: the row is scaled by a power of two that brings its largest value into [1, 2)
                     uint32_t amax = 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(q[i]) & 0x7fffffffu);
-                    const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, amax) >> 23, 1u), 254u);
+                    amax = __reduce_max_sync(0xffffffffu, amax);
+                    const uint32_t e = min(max(amax >> 23, 1u), 254u);
                     unit = e == 254u ? __uint_as_float(0x00400000u) : __uint_as_float((254u - e) << 23);
                     row_scale *= __uint_as_float(e << 23);
+                    if (FMT == 1) row_scale *= 0x1p-29f;
+                    if (amax >= 0x7f800000u) row_scale = __uint_as_float(0x7fc00000u);  // whole numbers hold no NaN
                 }
                 if (d < HDP) {
-                    // four values are one lane's part of an MMA; a 16-byte piece of a key row holds 8 or 16
+                    // a lane's part of an MMA is four values, of a whole-number one eight; a 16-byte piece of a key row holds 8 or 16
                     constexpr uint32_t kPer = S::kChunkDims / 4;
                     const uint32_t piece = d / S::kChunkDims, seg = piece / (S::kSeg / 16), in_seg = piece % (S::kSeg / 16);
                     const uint32_t m = (seg * S::kPieces + in_seg % S::kPieces) * kPer + d % S::kChunkDims / 4, to = warp * 4 + in_seg / S::kPieces;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        // int8 codes are taken from a word as bytes 0 and 2, 1 and 3, the others in order
-                        constexpr int i1 = FMT == 1 ? 2 : 1, i2 = FMT == 1 ? 1 : 2;
-                        uint4 a;
-                        split<FMT>(q[4 * i] * unit, q[4 * i + i1] * unit, a.x, a.y);
-                        split<FMT>(q[4 * i + i2] * unit, q[4 * i + 3] * unit, a.z, a.w);
-                        queries[(m + i) * 32 + to] = a;
+                    for (int i = 0; i < 8; ++i) q[i] *= unit;
+                    uint4 a, b;
+                    if (FMT == 1) {
+                        split_digits(q, a, b);
+                    } else {
+                        split<FMT>(q[0], q[1], a.x, a.y);
+                        split<FMT>(q[2], q[3], a.z, a.w);
+                        split<FMT>(q[4], q[5], b.x, b.y);
+                        split<FMT>(q[6], q[7], b.z, b.w);
                     }
+                    queries[m * 32 + to] = a;
+                    queries[(m + 1) * 32 + to] = b;
                 }
                 if (lane == 0) row_scales[warp] = row_scale;
             }
@@ -429,74 +453,76 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 const int32_t token = (int32_t)(tile * kTileTokens);
                 const bool edge = token + (int32_t)(kStep * kTileTokens) > sure;  // some rows do not see all of it
                 // ---- scores ----
-                uint32_t key_slot[kStep], value_slot[kStep];
+                mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
+                float x[4 * kStep];  // this lane's: tokens 2 quad, + 1, + 8, + 9 of each tile, row `row`
+                {
+                    const uint32_t keys = ring + slot * S::kSlot;
+                    float s[2 * kStep][4];
+                    int upper[2 * kStep][4], lower[2 * kStep][4];  // int8: products with digits 3 and 2, and with 1 and 0
 #pragma unroll
-                for (uint32_t i = 0; i < kStep; ++i) {
-                    mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
-                    key_slot[i] = slot;
-                    slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-                    parity ^= slot == 0;
-                }
-                float s[2 * kStep][4];
+                    for (uint32_t n = 0; n < 2 * kStep; ++n) {
+                        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+                        upper[n][0] = upper[n][1] = upper[n][2] = upper[n][3] = lower[n][0] = lower[n][1] = lower[n][2] = lower[n][3] = 0;
+                    }
 #pragma unroll
-                for (uint32_t n = 0; n < 2 * kStep; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+                    for (uint32_t seg = 0; seg < S::kSegs; ++seg)
 #pragma unroll
-                for (uint32_t seg = 0; seg < S::kSegs; ++seg)
-#pragma unroll
-                    for (uint32_t c = 0; c < S::kPieces; ++c) {
-                        const uint32_t piece = quad * S::kPieces + c, turn = S::kSeg == 128 ? row : row >> 1 & 3u;
-                        const uint32_t within = seg * (kTileTokens * S::kSeg) + row * S::kSeg + ((piece ^ turn) << 4);
-                        constexpr uint32_t kPer = S::kChunkDims / 4;
-                        const uint32_t m = (seg * S::kPieces + c) * kPer;
-                        uint32_t word[2 * kStep][4];
-#pragma unroll
-                        for (uint32_t n = 0; n < 2 * kStep; ++n) {
-                            const uint4 w = lds_v4(ring + key_slot[n / 2] * S::kTile + within + n % 2 * 8 * S::kSeg);
-                            word[n][0] = w.x, word[n][1] = w.y, word[n][2] = w.z, word[n][3] = w.w;
-                        }
-#pragma unroll
-                        for (uint32_t i = 0; i < kPer; ++i) {
-                            const uint4 w = lds_v4(queries_at + (m + i) * 512);
-                            const uint32_t qa[4] = {w.x, w.y, w.z, w.w};
+                        for (uint32_t c = 0; c < S::kPieces; ++c) {
+                            const uint32_t piece = quad * S::kPieces + c, turn = S::kSeg == 128 ? row : row >> 1 & 3u;
+                            const uint32_t within = seg * (kTileTokens * S::kSeg) + row * S::kSeg + ((piece ^ turn) << 4);
+                            constexpr uint32_t kPer = S::kChunkDims / 4;
+                            const uint32_t m = (seg * S::kPieces + c) * kPer;
+                            uint32_t word[2 * kStep][4];
 #pragma unroll
                             for (uint32_t n = 0; n < 2 * kStep; ++n) {
-                                if (FMT == 0) mma<FMT>(s[n], qa, word[n][2 * i], word[n][2 * i + 1]);
-                                else if (FMT == 1) mma<FMT>(s[n], qa, int8_even(word[n][i]), int8_even(word[n][i] >> 8));
-                                else mma<FMT>(s[n], qa, e4m3_pair(word[n][i]), e4m3_pair(word[n][i] >> 16));
+                                const uint4 w = lds_v4(keys + n / 2 * S::kTile + within + n % 2 * 8 * S::kSeg);
+                                word[n][0] = w.x, word[n][1] = w.y, word[n][2] = w.z, word[n][3] = w.w;
+                            }
+#pragma unroll
+                            for (uint32_t i = 0; i < kPer; ++i) {
+                                const uint4 w = lds_v4(queries_at + (m + i) * 512);
+                                const uint32_t qa[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                                for (uint32_t n = 0; n < 2 * kStep; ++n) {
+                                    if (FMT == 0) mma<FMT>(s[n], qa, word[n][2 * i], word[n][2 * i + 1]);
+                                    else if (FMT == 1) mma_s8s8_16832(i % 2 == 0 ? upper[n] : lower[n], qa[0], qa[1], qa[2], qa[3], word[n][i / 2 * 2], word[n][i / 2 * 2 + 1]);
+                                    else mma<FMT>(s[n], qa, e4m3_pair(word[n][i]), e4m3_pair(word[n][i] >> 16));
+                                }
                             }
                         }
-                    }
-                // this lane's: tokens 2 quad, + 1, + 8, + 9 of each tile, row `row`
-                float x[4 * kStep];
 #pragma unroll
-                for (uint32_t n = 0; n < 2 * kStep; ++n) {
-                    x[2 * n] = (s[n][0] + s[n][2]) * row_scale;
-                    x[2 * n + 1] = (s[n][1] + s[n][3]) * row_scale;
-                    if (FMT != 0) {
-                        const uint2 k = lds_v2(scales + key_slot[n / 2] * 64 + n % 2 * 32 + quad * 8);
-                        x[2 * n] *= __uint_as_float(k.x), x[2 * n + 1] *= __uint_as_float(k.y);
+                    for (uint32_t n = 0; n < 2 * kStep; ++n) {
+                        if (FMT == 1) {
+                            // a sum of 256 products is below 2^22, so two digits' sums fit 32 bits
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                x[2 * n + j] = fmaf((float)(upper[n][j] * 256 + upper[n][j + 2]), 65536.f, (float)(lower[n][j] * 256 + lower[n][j + 2])) * row_scale;
+                        } else {
+                            x[2 * n] = (s[n][0] + s[n][2]) * row_scale;
+                            x[2 * n + 1] = (s[n][1] + s[n][3]) * row_scale;
+                        }
+                        if (FMT != 0) {
+                            const uint2 k = lds_v2(scales + slot * S::kSlotScales + n * 32 + quad * 8);
+                            x[2 * n] *= __uint_as_float(k.x), x[2 * n + 1] *= __uint_as_float(k.y);
+                        }
                     }
                 }
-                __syncwarp();  // the slots have been read
-#pragma unroll
-                for (uint32_t i = 0; i < kStep; ++i) asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
+                __syncwarp();  // the slot has been read
+                asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
+                slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+                parity ^= slot == 0;
                 if (edge)
 #pragma unroll
                     for (uint32_t i = 0; i < 4 * kStep; ++i)
                         if (token + (int32_t)(i / 2 * 8 + quad * 2 + i % 2) >= limit) x[i] = -INFINITY;
                 // ---- weights ----
-#pragma unroll
-                for (uint32_t i = 0; i < kStep; ++i) {
-                    mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
-                    value_slot[i] = slot;
-                    slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-                    parity ^= slot == 0;
-                }
+                mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
+                const uint32_t held = ring + slot * S::kSlot;
                 float value_scale[FMT == 0 ? 1 : 4 * kStep], weight[4 * kStep];
                 if (FMT != 0)
 #pragma unroll
                     for (uint32_t n = 0; n < 2 * kStep; ++n) {
-                        const uint2 v = lds_v2(scales + value_slot[n / 2] * 64 + n % 2 * 32 + quad * 8);
+                        const uint2 v = lds_v2(scales + slot * S::kSlotScales + n * 32 + quad * 8);
                         value_scale[2 * n] = __uint_as_float(v.x), value_scale[2 * n + 1] = __uint_as_float(v.y);
                         // (a token that the row does not see: its scale may be anything)
                         if (edge) {
@@ -575,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     // rows that see it, and becomes a zero too.
 #pragma unroll
                     for (uint32_t i = 0; i < kStep; ++i) {
-                        const uint32_t base = ring + value_slot[i] * S::kTile;
+                        const uint32_t base = held + i * S::kTile;
                         const int32_t first = token + (int32_t)(i * kTileTokens);
                         if (FMT != 1 && p.q_tokens > 1) {
                             bool odd = false;
@@ -628,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll
                     for (uint32_t t = 0; t < kStep; ++t) {
                         uint32_t v[4];
-                        ldmatrix_x4_trans(v, ring + value_slot[t] * S::kTile + within);
+                        ldmatrix_x4_trans(v, held + t * S::kTile + within);
 #pragma unroll
                         for (uint32_t i = 0; i < 2; ++i) {
                             const uint32_t b0 = v[2 * i], b1 = v[2 * i + 1];
@@ -645,8 +671,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     }
                 }
                 __syncwarp();
-#pragma unroll
-                for (uint32_t i = 0; i < kStep; ++i) asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
+                asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
+                slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+                parity ^= slot == 0;
             }
 
             // ---- join the warps' results ----
