@@ -35,7 +35,6 @@ namespace q4 {
 constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;
 constexpr uint32_t kRoundDims = 64;             // dimensions joined at a time
 constexpr uint32_t kRoundPitch = kRoundDims + 16;  // floats between rows of the join buffer: lanes of a store fall into different banks
-constexpr uint32_t kMostPieces = 256;           // of an item (blocks of the grid)
 constexpr uint32_t kLeastRun = 16;              // tiles: shorter runs cost more in joining than they save
 constexpr float kNone = -3.0e38f;               // a reference below all scores: the row has seen nothing
 constexpr float kHeadroom = 8.f;                // how far above its reference a score may lie, in powers of two
@@ -61,14 +60,13 @@ struct Shape {
     // shared memory: rings, their scales, barriers, queries, the join buffer, and small arrays
     static constexpr uint32_t kQueries = kMmas * 32 * 16;
     static constexpr uint32_t kJoin = kWarps * kAttentionRows * kRoundPitch * 4;
-    static constexpr uint32_t kWeights = kMostPieces * kAttentionRows * 4;  // over the join buffer
     static constexpr uint32_t kSmall = 2048;
     static constexpr uint32_t kSlot = kStep * kTile, kSlotScales = kStep * 64;
     static constexpr uint32_t kFit = (kSharedLimit - 1024 - kQueries - kJoin - kSmall) / (kWarps * (kSlot + kSlotScales + 8));
     static constexpr uint32_t kSlots = kFit < 8 ? kFit : 8;          // of a warp's ring: keys and values of its steps in turn
     static constexpr uint32_t kRing = kWarps * kSlots * kSlot, kScales = kWarps * kSlots * kSlotScales, kBars = (kWarps * kSlots * 8 + 15) / 16 * 16;
     static constexpr uint32_t kShared = 1024 + kRing + kScales + kBars + kQueries + kJoin + kSmall;
-    static_assert(kSlots >= 2 && kWeights <= kJoin && kStep * (kSegs + 1) <= 32, "");
+    static_assert(kSlots >= 2 && kStep * (kSegs + 1) <= 32, "");
 };
 
 // ---- small pieces ----
@@ -184,8 +182,7 @@ struct Geometry {
     uint32_t heads;   // items of a sequence = key heads * chunks
     uint32_t rows;    // query rows of a key head
     uint32_t group;   // query heads of a key head
-    uint32_t per;     // tiles of a page, and the division by it as a product: tile / per = (tile * inverse >> 32) >> shift
-    uint32_t inverse, shift;
+    AttentionPages pages;
 };
 
 __device__ __forceinline__ int64_t length_of(const AttentionParams &p, uint32_t s) {
@@ -210,64 +207,79 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t v, uint32_t lane) {
     return v;
 }
 
-// All threads. `scratch`: 2 * kWarps + 8 words of 64 bits in shared memory.
-__device__ Share share_of_block(const AttentionParams &p, const Geometry &g, uint64_t *scratch) {
+// All threads. `scratch`: 3 * kWarps + 2 words of 64 bits in shared memory. Up to 32 sequences every warp finds it by itself.
+__device__ __forceinline__ Share share_of_block(const AttentionParams &p, const Geometry &g, uint64_t *scratch) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, sequences = p.kv.sequences;
-    uint64_t tiles = 0, items = 0;
-    for (uint32_t s = threadIdx.x; s < sequences; s += kThreads) {
-        const int64_t raw = __ldcg(p.lengths + s), n = length_of(p, s);
+    const bool few = sequences <= 32;
+    const uint32_t mine = few ? lane : threadIdx.x, stride = few ? 32 : kThreads;
+    uint64_t tiles = 0;
+    uint32_t items = 0, longest = 0, own = 0;  // own: tiles of the thread's first sequence
+    for (uint32_t s = mine; s < sequences; s += stride) {
+        const int64_t raw = __ldcg(p.lengths + s), most = (int64_t)p.kv.per_sequence * p.kv.page_tokens, n = raw < 0 ? 0 : raw > most ? most : raw;
         if (raw != n && blockIdx.x == 0) *p.kv.input_error = 1;
-        tiles += attention_tiles(n);
-        items += n > 0;
+        const uint32_t t = attention_tiles(n);
+        if (s == mine) own = t;
+        tiles += t;
+        items += t > 0;
+        longest = max(longest, t);
     }
-    tiles = __shfl_sync(0xffffffffu, warp_scan(tiles, lane), 31);
-    items = __shfl_sync(0xffffffffu, warp_scan(items, lane), 31);
-    if (lane == 0) scratch[warp] = tiles, scratch[kWarps + warp] = items;
-    __syncthreads();
-    tiles = items = 0;
-    for (uint32_t w = 0; w < kWarps; ++w) tiles += scratch[w], items += scratch[kWarps + w];
-    tiles *= g.heads;
-    items *= g.heads;
+    uint64_t scan = warp_scan(tiles, lane);
+    tiles = __shfl_sync(0xffffffffu, scan, 31);
+    items = __reduce_add_sync(0xffffffffu, items);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (!few) {
+        if (lane == 0) scratch[warp] = tiles, scratch[kWarps + warp] = items, scratch[2 * kWarps + warp] = longest;
+        __syncthreads();
+        tiles = items = longest = 0;
+        for (uint32_t w = 0; w < kWarps; ++w) {
+            tiles += scratch[w];
+            items += (uint32_t)scratch[kWarps + w];
+            longest = max(longest, (uint32_t)scratch[2 * kWarps + w]);
+        }
+    }
     Share share;
     share.any = false;
     share.at = Cursor{};
     if (tiles == 0) return share;
-    share.cut = attention_cut(tiles, items, gridDim.x, kLeastRun);
+    share.cut = attention_cut(tiles * g.heads, (uint64_t)items * g.heads, longest, gridDim.x, kLeastRun);
     const AttentionCut &cut = share.cut;
-    const uint64_t target = cut.whole ? blockIdx.x : blockIdx.x * cut.run;
-    if (!cut.whole && target >= tiles) return share;
+    const uint64_t target = attention_target(cut, blockIdx.x);
+    if (cut.mode != kEqualPieces && target >= cut.tiles) return share;
     // the sequence that holds piece or tile number `target`
-    uint64_t before = 0;
-    for (uint32_t base = 0; base < sequences; base += kThreads) {
-        const uint32_t s = base + threadIdx.x;
-        const uint32_t t = s < sequences ? attention_tiles(length_of(p, s)) : 0u;
-        const uint64_t weight = attention_weight(cut, t, g.heads);
-        const uint64_t scan = warp_scan(weight, lane);
-        __syncthreads();
-        if (lane == 31) scratch[warp] = scan;
-        if (threadIdx.x == 0) scratch[2 * kWarps] = ~0ull;
-        __syncthreads();
-        uint64_t start = before + scan - weight, all = before;
-        for (uint32_t w = 0; w < kWarps; ++w) {
-            if (w < warp) start += scratch[w];
-            all += scratch[w];
+    uint64_t start = 0;
+    uint32_t s = 0;
+    bool found = false;
+    if (few) {
+        const uint64_t weight = attention_weight(cut, own, g.heads), to = warp_scan(weight, lane);
+        const uint32_t hit = __ballot_sync(0xffffffffu, target >= to - weight && target < to);
+        found = hit != 0;
+        s = found ? __ffs(hit) - 1 : 0;
+        start = __shfl_sync(0xffffffffu, to - weight, s);
+    } else {
+        uint64_t before = 0;
+        for (uint32_t base = 0; base < sequences && !found; base += kThreads) {
+            const uint32_t i = base + threadIdx.x;
+            const uint32_t t = base == 0 ? own : i < sequences ? attention_tiles(length_of(p, i)) : 0u;
+            const uint64_t weight = attention_weight(cut, t, g.heads);
+            const uint64_t to = warp_scan(weight, lane);
+            __syncthreads();
+            if (lane == 31) scratch[warp] = to;
+            if (threadIdx.x == 0) scratch[kWarps] = ~0ull;
+            __syncthreads();
+            uint64_t from = before + to - weight;
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                if (w < warp) from += scratch[w];
+                before += scratch[w];
+            }
+            if (target >= from && target < from + weight) scratch[kWarps] = i, scratch[kWarps + 1] = from;
+            __syncthreads();
+            found = scratch[kWarps] != ~0ull;
+            s = (uint32_t)scratch[kWarps];
+            start = scratch[kWarps + 1];
         }
-        if (target >= start && target < start + weight) {
-            scratch[2 * kWarps] = s;
-            scratch[2 * kWarps + 1] = start;
-        }
         __syncthreads();
-        if (scratch[2 * kWarps] != ~0ull) {
-            share.any = true;
-            break;
-        }
-        before = all;
     }
-    if (!share.any) return share;
-    const uint32_t s = (uint32_t)scratch[2 * kWarps];
-    const uint64_t start = scratch[2 * kWarps + 1];
-    share.at.start(cut, s, length_of(p, s), start, target - start, tiles);
-    __syncthreads();
+    if (found) share.any = share.at.start(cut, target, s, start, [&](uint32_t i) { return length_of(p, i); }, sequences, g.heads);
     return share;
 }
 
@@ -294,8 +306,8 @@ struct Asker {
             tile = at.begin + warp * S::kStep;
             head = g.chunks == 1 ? at.item : at.item / g.chunks;
         }
-        const uint32_t t = tile + mine(lane), entry = g.per == 1 ? t : __umulhi(t, g.inverse) >> g.shift;
-        place = (t - entry * g.per) * kTileTokens;
+        const uint32_t t = tile + mine(lane), entry = g.pages.page_of(t);
+        place = (t - entry * g.pages.per) * kTileTokens;
         page = t < at.end ? (uint32_t)__ldcg(p.kv.table + (uint64_t)at.s * p.kv.row_stride + entry) : ~0u;
     }
     __device__ __forceinline__ void start(const Share &share, const AttentionParams &p, const Geometry &g, uint32_t warp, uint32_t lane) {
@@ -361,10 +373,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     float *const join = reinterpret_cast<float *>(queries) + S::kQueries / 4;
     float *const small = join + S::kJoin / 4;
     float *const tops = small, *const sums = small + kWarps * kAttentionRows;  // [warp][row]
-    float *const totals = small + 2 * kWarps * kAttentionRows;                 // [row]
-    float *const row_scales = totals + kAttentionRows;                         // [row] scale of the scores, in powers of two
+    float *const row_scales = small + 2 * kWarps * kAttentionRows;             // [row] scale of the scores, in powers of two
     uint64_t *const scratch = reinterpret_cast<uint64_t *>(row_scales + kAttentionRows);
-    uint32_t *const arrived = reinterpret_cast<uint32_t *>(scratch + 2 * kWarps + 8);
+    uint32_t *const arrived = reinterpret_cast<uint32_t *>(scratch + 3 * kWarps + 2);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row = lane >> 2, quad = lane & 3u;
     const uint32_t ring = raw + pad + warp * S::kSlots * S::kSlot, scales = raw + pad + S::kRing + warp * S::kSlots * S::kSlotScales;
     const uint32_t bars = raw + pad + S::kRing + S::kScales + warp * S::kSlots * 8, queries_at = raw + pad + S::kRing + S::kScales + S::kBars + lane * 16;
@@ -676,126 +687,120 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 parity ^= slot == 0;
             }
 
-            // ---- join the warps' results ----
+            // ---- join the warps' results; then, in the last block of a cut item, those of the blocks ----
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (quad == 0) {
-                tops[warp * kAttentionRows + row] = top == kNone ? -INFINITY : top;
-                sums[warp * kAttentionRows + row] = sum;
-            }
-            __syncthreads();
-            float all_top = -INFINITY;
-            for (uint32_t w = 0; w < kWarps; ++w) all_top = fmaxf(all_top, tops[w * kAttentionRows + row]);
-            {
-                // (a warp without tiles, and rows that see nothing, have zeros; a row whose scores are NaNs keeps those)
-                const float factor = top == kNone || (FMT != 0 && weight_top == kNone) ? 0.f : exp2_fast((FMT == 0 ? top : weight_top) - all_top);
+            // what of the row's result a lane holds: dimensions 16 i + 4 quad ... + 3 (bf16, at first: 16 i + 2 quad, + 1, + 8, + 9)
+            float4 o[HDP / 16];
 #pragma unroll
-                for (uint32_t i = 0; i < S::kAcc; ++i) {
-                    acc[i][0] = (acc[i][0] + acc[i][2]) * factor;
-                    acc[i][1] = (acc[i][1] + acc[i][3]) * factor;
-                }
+            for (uint32_t i = 0; i < HDP / 16; ++i) {
+                const float *a = acc[2 * i], *b = acc[2 * i + 1];
+                o[i] = FMT == 0 ? make_float4(a[0] + a[2], a[1] + a[3], b[0] + b[2], b[1] + b[3]) : make_float4(a[0] + a[2], b[0] + b[2], a[1] + a[3], b[1] + b[3]);
             }
+            if (top == kNone) top = -INFINITY;
+            float o_top = FMT == 0 ? top : weight_top == kNone ? -INFINITY : weight_top;
             const bool cut = !at.whole_item();
             uint32_t owner, contributors;
             at.contributors(share.cut, blockIdx.x, &owner, &contributors);
             // a partial result: rows, then maxima, then sums
-            float *const part = p.parts + ((uint64_t)blockIdx.x * 2 + (blockIdx.x == owner ? 1 : 0)) * (kAttentionRows * (kMaxHeadDim + 2));
+            constexpr uint32_t kPart = kAttentionRows * (kMaxHeadDim + 2);
+            float *const part = p.parts + ((uint64_t)blockIdx.x * 2 + (blockIdx.x == owner ? 1 : 0)) * kPart;
             const uint32_t jr = threadIdx.x >> 4 & 7u, jd = (threadIdx.x & 15u) * 4;  // row and dimensions that a thread joins
             const uint32_t j_row = chunk * kAttentionRows + jr, j_draft = j_row / g.group;
-            const bool j_live = j_row < g.rows;
+            const bool j_live = j_row < g.rows, j_empty = at.length - (int32_t)p.q_tokens + 1 + (int32_t)j_draft <= 0;
             const uint64_t out_row = ((uint64_t)at.s * p.q_tokens + j_draft) * p.out_stride + ((uint64_t)head * g.group + j_row % g.group) * p.kv.head_dim;
-            const bool j_empty = at.length - (int32_t)p.q_tokens + 1 + (int32_t)j_draft <= 0;
+            bool partial = cut;
+            while (true) {
+                if (quad == 0) {
+                    tops[warp * kAttentionRows + row] = top;
+                    sums[warp * kAttentionRows + row] = sum;
+                }
+                __syncthreads();
+                float all_top = -INFINITY;
 #pragma unroll
-            for (uint32_t round = 0; round < HDP / kRoundDims; ++round) {
-                float *const mine = join + (warp * kAttentionRows + row) * kRoundPitch;
-                if (FMT == 0) {
+                for (uint32_t w = 0; w < kWarps; ++w) all_top = fmaxf(all_top, tops[w * kAttentionRows + row]);
+                // (a warp without tiles, and rows that see nothing, have zeros; a row whose scores are NaNs keeps those)
+                const float factor = o_top == -INFINITY ? 0.f : exp2_fast(o_top - all_top);
+                float row_top = -INFINITY, total = 0.f;
 #pragma unroll
-                    for (uint32_t i = 0; i < kRoundDims / 8; ++i)
-                        *reinterpret_cast<float2 *>(mine + i * 8 + quad * 2) = make_float2(acc[round * (kRoundDims / 8) + i][0], acc[round * (kRoundDims / 8) + i][1]);
-                } else {
+                for (uint32_t w = 0; w < kWarps; ++w) row_top = fmaxf(row_top, tops[w * kAttentionRows + jr]);
+#pragma unroll
+                for (uint32_t w = 0; w < kWarps; ++w) {
+                    const float t = tops[w * kAttentionRows + jr];
+                    total += sums[w * kAttentionRows + jr] * (t == -INFINITY ? 1.f : exp2_fast(t - row_top));
+                }
+                const float by = 1.f / total;
+#pragma unroll
+                for (uint32_t round = 0; round < HDP / kRoundDims; ++round) {
+                    float *const mine = join + (warp * kAttentionRows + row) * kRoundPitch;
 #pragma unroll
                     for (uint32_t i = 0; i < kRoundDims / 16; ++i) {
-                        const uint32_t a = round * (kRoundDims / 8) + i * 2;
-                        *reinterpret_cast<float4 *>(mine + i * 16 + quad * 4) = make_float4(acc[a][0], acc[a + 1][0], acc[a][1], acc[a + 1][1]);
-                    }
-                }
-                __syncthreads();
-                if (threadIdx.x < 128) {
-                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                    float row_top = -INFINITY, total = 0.f;
-                    for (uint32_t w = 0; w < kWarps; ++w) row_top = fmaxf(row_top, tops[w * kAttentionRows + jr]);
-                    for (uint32_t w = 0; w < kWarps; ++w) {
-                        const float4 v = *reinterpret_cast<const float4 *>(join + (w * kAttentionRows + jr) * kRoundPitch + jd);
-                        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
-                        const float t = tops[w * kAttentionRows + jr];
-                        total += sums[w * kAttentionRows + jr] * (t == -INFINITY ? 1.f : exp2_fast(t - row_top));
-                    }
-                    const uint32_t d = round * kRoundDims + jd;
-                    if (cut) {
-                        *reinterpret_cast<float4 *>(part + jr * HDP + d) = o;
-                        if (round == 0 && jd == 0) {
-                            part[kAttentionRows * HDP + jr] = row_top;
-                            part[kAttentionRows * (HDP + 1) + jr] = total;
+                        float4 v = o[round * (kRoundDims / 16) + i];
+                        v.x *= factor, v.y *= factor, v.z *= factor, v.w *= factor;
+                        if (FMT == 0 && partial == cut) {
+                            *reinterpret_cast<float2 *>(mine + i * 16 + quad * 2) = make_float2(v.x, v.y);
+                            *reinterpret_cast<float2 *>(mine + i * 16 + 8 + quad * 2) = make_float2(v.z, v.w);
+                        } else {
+                            *reinterpret_cast<float4 *>(mine + i * 16 + quad * 4) = v;
                         }
-                    } else if (j_live && d < p.kv.head_dim) {
-                        const float by = j_empty ? 0.f : 1.f / total;
-                        const float v[4] = {j_empty ? 0.f : o.x * by, j_empty ? 0.f : o.y * by, j_empty ? 0.f : o.z * by, j_empty ? 0.f : o.w * by};
-                        if (p.out_is_f32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + out_row + d) = make_float4(v[0], v[1], v[2], v[3]);
-                        else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + out_row + d) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
                     }
+                    __syncthreads();
+                    if (threadIdx.x < 128) {
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (uint32_t w = 0; w < kWarps; ++w) {
+                            const float4 a = *reinterpret_cast<const float4 *>(join + (w * kAttentionRows + jr) * kRoundPitch + jd);
+                            v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
+                        }
+                        const uint32_t d = round * kRoundDims + jd;
+                        if (partial) {
+                            if (j_live) *reinterpret_cast<float4 *>(part + jr * HDP + d) = v;
+                            if (round == 0 && jd == 0) {
+                                part[kAttentionRows * HDP + jr] = row_top;
+                                part[kAttentionRows * (HDP + 1) + jr] = total;
+                            }
+                        } else if (j_live && d < p.kv.head_dim) {
+                            v = j_empty ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * by, v.y * by, v.z * by, v.w * by);
+                            if (p.out_is_f32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + out_row + d) = v;
+                            else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + out_row + d) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+                        }
+                    }
+                    if (round + 1 < HDP / kRoundDims) __syncthreads();
                 }
+                if (partial) __threadfence();
                 __syncthreads();
-            }
-            if (cut) {
-                // ---- the last block of an item joins its partial results, in the order of the tiles ----
-                __threadfence();
-                __syncthreads();
+                if (!partial) break;
                 if (threadIdx.x == 0) {
-                    const uint32_t before = atomicAdd(p.counters + owner, 1u);
-                    *arrived = before + 1 == contributors;
+                    *arrived = atomicAdd(p.counters + owner, 1u) + 1 == contributors;
                     if (*arrived) p.counters[owner] = 0;
                     __threadfence();
                 }
                 __syncthreads();
-                if (*arrived) {
-                    auto part_of = [&](uint32_t i) { return p.parts + ((uint64_t)(owner + i) * 2 + (i == 0 ? 1 : 0)) * (kAttentionRows * (kMaxHeadDim + 2)); };
-                    float *const weights = join;  // [piece][row]
-                    for (uint32_t i = threadIdx.x; i < contributors * kAttentionRows; i += kThreads) weights[i] = __ldcg(part_of(i / kAttentionRows) + kAttentionRows * HDP + i % kAttentionRows);
-                    __syncthreads();
-                    if (warp < kAttentionRows) {  // a warp per row
-                        float best = -INFINITY, total = 0.f;
-                        for (uint32_t i = lane; i < contributors; i += 32) best = fmaxf(best, weights[i * kAttentionRows + warp]);
+                if (!*arrived) break;
+                // partial results in the order of the tiles: warp w adds up those of blocks w, w + 8, ...
+                partial = false;
+                const float *const parts = p.parts + (uint64_t)owner * 2 * kPart;
+                auto part_of = [&](uint32_t i) { return parts + (i * 2 + (i == 0 ? 1 : 0)) * kPart; };
+                top = -INFINITY;
+                sum = 0.f;
 #pragma unroll
-                        for (int off = 16; off > 0; off >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, off));
-                        for (uint32_t i = lane; i < contributors; i += 32) {
-                            const float t = weights[i * kAttentionRows + warp];
-                            const float f = t == -INFINITY ? 0.f : exp2_fast(t - best);
-                            total += __ldcg(part_of(i) + kAttentionRows * (HDP + 1) + warp) * (t == -INFINITY ? 1.f : f);
-                            weights[i * kAttentionRows + warp] = f;
-                        }
+                for (uint32_t i = 0; i < HDP / 16; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                for (uint32_t i = warp; i < contributors; i += kWarps) top = fmaxf(top, __ldcg(part_of(i) + kAttentionRows * HDP + row));
+                o_top = top;
+                for (uint32_t i = warp; i < contributors; i += kWarps) {
+                    const float *const from = part_of(i);
+                    const float t = __ldcg(from + kAttentionRows * HDP + row), l = __ldcg(from + kAttentionRows * (HDP + 1) + row);
+                    float4 v[HDP / 16];
+                    if (chunk * kAttentionRows + row < g.rows) {
 #pragma unroll
-                        for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-                        if (lane == 0) totals[warp] = total;
+                        for (uint32_t j = 0; j < HDP / 16; ++j) v[j] = __ldcg(reinterpret_cast<const float4 *>(from + row * HDP + j * 16 + quad * 4));
+                        const float f = t == -INFINITY ? 0.f : exp2_fast(t - top);
+                        sum += t == -INFINITY ? l : l * f;
+#pragma unroll
+                        for (uint32_t j = 0; j < HDP / 16; ++j)
+                            o[j].x = fmaf(v[j].x, f, o[j].x), o[j].y = fmaf(v[j].y, f, o[j].y), o[j].z = fmaf(v[j].z, f, o[j].z), o[j].w = fmaf(v[j].w, f, o[j].w);
                     }
-                    __syncthreads();
-                    for (uint32_t i = threadIdx.x; i < kAttentionRows * HDP / 4; i += kThreads) {
-                        const uint32_t rr = i / (HDP / 4), d = i % (HDP / 4) * 4, q_row = chunk * kAttentionRows + rr, q_draft = q_row / g.group;
-                        if (q_row >= g.rows || d >= p.kv.head_dim) continue;
-                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                        for (uint32_t k = 0; k < contributors; ++k) {
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_of(k) + rr * HDP + d));
-                            const float f = weights[k * kAttentionRows + rr];
-                            o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
-                        }
-                        const bool empty = at.length - (int32_t)p.q_tokens + 1 + (int32_t)q_draft <= 0;
-                        const float by = 1.f / totals[rr];
-                        const float v[4] = {empty ? 0.f : o.x * by, empty ? 0.f : o.y * by, empty ? 0.f : o.z * by, empty ? 0.f : o.w * by};
-                        const uint64_t to = ((uint64_t)at.s * p.q_tokens + q_draft) * p.out_stride + ((uint64_t)head * g.group + q_row % g.group) * p.kv.head_dim + d;
-                        if (p.out_is_f32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to) = make_float4(v[0], v[1], v[2], v[3]);
-                        else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + to) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-                    }
-                    __syncthreads();
                 }
             }
         } while (at.next([&](uint32_t i) { return length_of(p, i); }, p.kv.sequences, g.heads));
@@ -848,12 +853,8 @@ cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t str
     g.rows = g.group * p.q_tokens;
     g.chunks = (g.rows + kAttentionRows - 1) / kAttentionRows;
     g.heads = p.kv.kv_heads * g.chunks;
-    // tile / per for tiles below 2^27: 2^(32 + shift) / per rounded up has an error below per <= 2^(shift + 1), less than 2^(5 + shift)
-    g.per = p.kv.page_tokens / kTileTokens;
-    g.shift = 0;
-    while ((2u << g.shift) < g.per) ++g.shift;
-    g.inverse = g.per == 1 ? 0 : (uint32_t)(((1ull << (32 + g.shift)) + g.per - 1) / g.per);
-    return launch_dependent(attention_kernel<FMT, HDP>, dim3(sm_count < kMostPieces ? sm_count : kMostPieces), kThreads, S::kShared, stream, p, g, maps[0], maps[1]);
+    g.pages = attention_pages(p.kv.page_tokens);
+    return launch_dependent(attention_kernel<FMT, HDP>, dim3(sm_count), kThreads, S::kShared, stream, p, g, maps[0], maps[1]);
 }
 
 template <int FMT>

@@ -19,20 +19,44 @@ constexpr uint32_t kAttentionRows = 8;  // query rows of an item
 
 Q4_PLAN_FN uint32_t attention_tiles(int64_t length) { return length > 0 ? (uint32_t)((length + kTileTokens - 1) / kTileTokens) : 0u; }
 
-// The cut of a call, the same in every block.
-struct AttentionCut {
-    uint64_t run;      // tiles of a block's share, or of a piece at most
-    uint32_t whole;    // 1: every block takes one piece of one item; 0: blocks take equal runs through all tiles
+// tile / per for tiles below 2^27, as a product: 2^(32 + shift) / per rounded up is off by less than per <= 2^(shift + 1).
+struct AttentionPages {
+    uint32_t per, inverse, shift;  // tiles of a page
+    Q4_PLAN_FN uint32_t page_of(uint32_t tile) const { return per == 1 ? tile : (uint32_t)((uint64_t)tile * inverse >> 32) >> shift; }
+};
+inline AttentionPages attention_pages(uint32_t page_tokens) {
+    AttentionPages d = {page_tokens / kTileTokens, 0, 0};
+    while ((2ull << d.shift) < d.per) ++d.shift;
+    if (d.per > 1) d.inverse = (uint32_t)(((1ull << (32 + d.shift)) + d.per - 1) / d.per);
+    return d;
+}
+
+enum AttentionMode : uint32_t {
+    kEqualRuns = 0,    // blocks take equal runs through the tiles of all items
+    kEqualPieces = 1,  // every item is cut into equal pieces, a block takes one
+    kWholeItems = 2    // blocks take the items whose middle lies in their run
 };
 
-// `tiles`: of all items; `items`: those that have any. With few items every item is cut into equal pieces, one to a block: no block
-// has a second start or an uneven rest. pieces <= tiles / run + items <= blocks holds for run >= tiles / (blocks - items).
-Q4_PLAN_FN AttentionCut attention_cut(uint64_t tiles, uint64_t items, uint32_t blocks, uint32_t least) {
+// The cut of a call, the same in every block.
+struct AttentionCut {
+    uint64_t tiles;  // of all items
+    uint64_t run;    // tiles of a block's run, or of a piece at most
+    uint32_t mode;
+};
+
+// `tiles`: of all items, `items`: those that have any, `longest`: tiles of the longest one.
+//   * Few items are cut into pieces: no block has a second start or an uneven rest. pieces <= tiles / run + items <= blocks
+//     holds for run >= tiles / (blocks - items).
+//   * Items that are short against a run stay whole: what a block does more than another is less than joining cut items takes.
+//   * Otherwise all blocks take the same number of tiles.
+Q4_PLAN_FN AttentionCut attention_cut(uint64_t tiles, uint64_t items, uint32_t longest, uint32_t blocks, uint32_t least) {
     AttentionCut c;
-    c.whole = items * 2 <= blocks ? 1u : 0u;
-    const uint64_t by = c.whole ? blocks - items : blocks;
+    c.tiles = tiles;
+    c.mode = items * 2 <= blocks ? kEqualPieces : kEqualRuns;
+    const uint64_t by = c.mode == kEqualPieces ? blocks - items : blocks;
     c.run = (tiles + by - 1) / by;
-    if (c.run < least) c.run = least;
+    if (c.mode == kEqualRuns && (longest <= 2 * least || longest <= c.run / 16)) c.mode = kWholeItems;
+    if (c.mode != kWholeItems && c.run < least) c.run = least;
     return c;
 }
 
@@ -40,28 +64,38 @@ Q4_PLAN_FN uint64_t attention_pieces(const AttentionCut &c, uint32_t tiles) { re
 
 // What a sequence counts for in the search for a block's start: its pieces, or its tiles, in all items.
 Q4_PLAN_FN uint64_t attention_weight(const AttentionCut &c, uint32_t tiles, uint32_t items) {
-    return (c.whole ? attention_pieces(c, tiles) : (uint64_t)tiles) * items;
+    return (c.mode == kEqualPieces ? attention_pieces(c, tiles) : (uint64_t)tiles) * items;
 }
+
+// Where block `block` starts, in those; past the end: it has nothing to do.
+Q4_PLAN_FN uint64_t attention_target(const AttentionCut &c, uint32_t block) { return c.mode == kEqualPieces ? block : block * c.run; }
 
 // Walks the segments of a block's share: tiles [begin, end) of an item. `items` of a sequence, `lengths(s)` its tokens.
 struct AttentionCursor {
     uint32_t s, item, begin, end, tiles;
     uint32_t piece, pieces;  // of an item cut into equal pieces
     int32_t length;
-    uint64_t left;   // tiles of the share from `begin` on
-    uint64_t first;  // equal runs: number of the sequence's first tile among the tiles of all items
+    uint64_t left;   // tiles of the share from `begin` on; whole items: where the block's run ends
+    uint64_t first;  // runs: number of the sequence's first tile among the tiles of all items
+    uint32_t whole;
 
-    Q4_PLAN_FN void close() { end = (uint64_t)(tiles - begin) < left ? tiles : begin + (uint32_t)left; }
+    Q4_PLAN_FN void close() { end = whole || (uint64_t)(tiles - begin) < left ? tiles : begin + (uint32_t)left; }
+    Q4_PLAN_FN bool mine() const { return first + (uint64_t)item * tiles + tiles / 2 < left; }  // whole items: middle in the run
 
-    // Start of the block's share, which begins `local` pieces or tiles into sequence s; `before`: those of the sequences in front.
-    Q4_PLAN_FN void start(const AttentionCut &cut, uint32_t sequence, int64_t tokens, uint64_t before, uint64_t local, uint64_t all_tiles) {
+    // Start of the block's share, which lies `target - before` pieces or tiles into sequence `sequence`; `before`: those of the
+    // sequences in front. False: whole items, and none has its middle in the block's run.
+    template <typename Lengths>
+    Q4_PLAN_FN bool start(const AttentionCut &cut, uint64_t target, uint32_t sequence, uint64_t before, const Lengths &lengths, uint32_t sequences, uint32_t items) {
+        const int64_t tokens = lengths(sequence);
+        const uint64_t local = target - before;
         s = sequence;
         length = (int32_t)tokens;
         tiles = attention_tiles(tokens);
         first = before;
         piece = 0;
         pieces = 1;
-        if (cut.whole) {
+        whole = cut.mode == kWholeItems;
+        if (cut.mode == kEqualPieces) {
             pieces = (uint32_t)attention_pieces(cut, tiles);
             item = (uint32_t)(local / pieces);
             piece = (uint32_t)(local % pieces);
@@ -70,26 +104,37 @@ struct AttentionCursor {
         } else {
             item = (uint32_t)(local / tiles);
             begin = (uint32_t)(local % tiles);
-            left = all_tiles - (before + local) < cut.run ? all_tiles - (before + local) : cut.run;
+            left = cut.tiles - target < cut.run ? cut.tiles - target : cut.run;
+            if (whole) {
+                left += target;
+                const bool behind = begin > tiles / 2;  // its middle lies in the run before
+                begin = 0;
+                if (behind) return next(lengths, sequences, items);
+                if (!mine()) return false;
+            }
         }
         close();
+        return true;
     }
 
     template <typename Lengths>
     Q4_PLAN_FN bool next(const Lengths &lengths, uint32_t sequences, uint32_t items) {
-        left -= end - begin;
-        if (left == 0) return false;
+        if (!whole) {
+            left -= end - begin;
+            if (left == 0) return false;
+        }
         begin = 0;
         if (++item == items) {
             item = 0;
             first += (uint64_t)tiles * items;
             do {
-                if (++s >= sequences) return false;  // (never: `left` counts tiles that exist)
+                if (++s >= sequences) return false;
                 const int64_t tokens = lengths(s);
                 length = (int32_t)tokens;
                 tiles = attention_tiles(tokens);
             } while (tiles == 0);
         }
+        if (whole && !mine()) return false;
         close();
         return true;
     }
@@ -99,11 +144,9 @@ struct AttentionCursor {
     // Blocks owner ... owner + contributors - 1 work on the item. A block is the owner of one cut item at most, its share's last
     // one, and one of the others of one at most, its first: two places for partial results are enough, place 1 for an owner.
     Q4_PLAN_FN void contributors(const AttentionCut &cut, uint32_t block, uint32_t *owner, uint32_t *count) const {
-        if (cut.whole) {
-            *owner = block - piece;
-            *count = pieces;
-            return;
-        }
+        *owner = block - piece;
+        *count = pieces;
+        if (cut.mode != kEqualRuns) return;
         const uint64_t from = first + (uint64_t)item * tiles;
         *owner = (uint32_t)(from / cut.run);
         *count = (uint32_t)((from + tiles - 1) / cut.run) - *owner + 1;

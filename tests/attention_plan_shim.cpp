@@ -4,21 +4,24 @@ extern "C" {
 // All blocks' segments, seven numbers each: block, sequence, item, begin, end, owner, contributors. Returns how many.
 uint64_t shim_attention_plan(const int64_t *lengths, uint32_t sequences, uint32_t items, uint32_t blocks, uint32_t least, uint64_t *out, uint64_t most) {
     uint64_t tiles = 0, live = 0, n = 0;
+    uint32_t longest = 0;
     for (uint32_t s = 0; s < sequences; ++s) {
-        tiles += q4::attention_tiles(lengths[s]);
-        live += lengths[s] > 0;
+        const uint32_t t = q4::attention_tiles(lengths[s]);
+        tiles += t;
+        live += t > 0;
+        longest = t > longest ? t : longest;
     }
     if (tiles == 0) return 0;
-    tiles *= items;
-    const q4::AttentionCut cut = q4::attention_cut(tiles, live * items, blocks, least);
+    const q4::AttentionCut cut = q4::attention_cut(tiles * items, live * items, longest, blocks, least);
+    auto length = [&](uint32_t i) { return lengths[i]; };
     for (uint32_t b = 0; b < blocks; ++b) {
-        const uint64_t target = cut.whole ? b : b * cut.run;
+        const uint64_t target = q4::attention_target(cut, b);
         uint64_t before = 0;
         for (uint32_t s = 0; s < sequences; ++s) {
             const uint64_t weight = q4::attention_weight(cut, q4::attention_tiles(lengths[s]), items);
             if (target >= before && target < before + weight) {
                 q4::AttentionCursor c;
-                c.start(cut, s, lengths[s], before, target - before, tiles);
+                if (!c.start(cut, target, s, before, length, sequences, items)) break;
                 do {
                     if (n == most) return n;
                     uint32_t owner, count;
@@ -26,7 +29,7 @@ uint64_t shim_attention_plan(const int64_t *lengths, uint32_t sequences, uint32_
                     const uint64_t row[7] = {b, c.s, c.item, c.begin, c.end, owner, count};
                     for (int i = 0; i < 7; ++i) out[n * 7 + i] = row[i];
                     ++n;
-                } while (c.next([&](uint32_t i) { return lengths[i]; }, sequences, items));
+                } while (c.next(length, sequences, items));
                 break;
             }
             before += weight;
@@ -34,4 +37,5 @@ uint64_t shim_attention_plan(const int64_t *lengths, uint32_t sequences, uint32_
     }
     return n;
 }
+uint32_t shim_attention_page_of(uint32_t page_tokens, uint32_t tile) { return q4::attention_pages(page_tokens).page_of(tile); }
 }

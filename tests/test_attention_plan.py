@@ -70,3 +70,22 @@ def test_few_items_are_cut_evenly(shim):
     plan = _plan(shim, [5000] * 75, 1, 148)
     sizes = np.bincount(plan[:, 0], weights=plan[:, 4] - plan[:, 3])
     assert sizes.max() - np.sort(sizes)[1] <= 1  # equal runs but for the last one
+
+
+def test_short_items_stay_whole(shim):
+    plan = _plan(shim, [60] * 28, 4, 148)  # 112 items of four tiles: a block each
+    assert len(plan) == 112 and len(set(plan[:, 0])) == 112 and set(plan[:, 6]) == {1}
+    plan = _plan(shim, [100] * 300, 8, 148)
+    assert set(plan[:, 6]) == {1}
+    sizes = np.bincount(plan[:, 0], weights=plan[:, 4] - plan[:, 3], minlength=148)
+    run = -(-300 * 8 * 7 // 148)  # (the last block has what is left)
+    assert sizes.max() <= run + 7 and np.sort(sizes)[1] >= run - 7 and sizes.sum() == 300 * 8 * 7
+
+
+def test_division_by_page_size(shim):
+    rng = np.random.default_rng(3)
+    for per in [1, 2, 3, 4, 5, 6, 7, 12, 16, 31, 33, 1000, 4095, 65535, 65536]:
+        tiles = [0, 1, per - 1, per, per + 1, 2 ** 27 - 1, 2 ** 27 - per] + rng.integers(0, 2 ** 27, 200).tolist()
+        tiles += [per * k + d for k in rng.integers(1, 2 ** 27 // per, 50).tolist() for d in (-1, 0)]
+        for t in tiles:
+            assert shim.shim_attention_page_of(16 * per, int(t)) == t // per
