@@ -6,19 +6,22 @@
 // Every key and value is read once from memory for eight query rows (token, head) that share its key head: at one byte a value that is
 // 12 to 16 operations a byte, so memory is the bound, and the kernel is built around keeping loads in flight.
 //
-//   * One block per SM, eight warps, each with a ring of its own in shared memory. Tiles of 16 tokens (they never cross a page)
-//     go round the warps, two at a time for 8-bit caches; a warp asks for keys and values of its next tiles with tensor copies, past the
-//     end of an item too, so that 190 KB stay in flight per SM while results are joined. No warp waits for another one inside an item.
-//   * Both products run on m16n8k16 MMAs with eight query rows: rows 0...7 of the left operand hold the upper halves of the eight
-//     rows' factors, rows 8...15 the lower halves, so that the sum of the two accumulators is a product of factors of 16 bits or more
-//     (two bf16 numbers, error 2^-17; two fp16 numbers for 8-bit caches, 2^-22), at no cost: the rows would be empty.
+//   * One block per SM: eight warps that multiply and one that asks for tiles with tensor copies into a ring in shared memory, keys of up
+//     to 128 tokens and their values in turn, past the end of an item too: 190 KB are in flight while results are written. A page has a
+//     whole number of the 16-token tiles that a copy brings.
+//   * Warp w has the scores of 16 tokens, hands their weights on through shared memory, and then adds up one eighth of the dimensions
+//     of the values for all 128 tokens: one barrier for 128 tokens, and a result lies in one warp's registers. (Warps that kept whole
+//     results of tokens of their own needed 128 registers for them and four rounds through shared memory to join them: 3 us for
+//     every item, 8 for a cut one.)
+//   * Both products run on MMAs with eight query rows: rows 0...7 of the left operand hold the upper halves of the eight rows' factors,
+//     rows 8...15 the lower halves, so that the sum of the two accumulators is a product of factors of 16 bits or more (two bf16
+//     numbers, error 2^-17; two fp16 numbers for 8-bit caches, 2^-22), at no cost: the rows would be empty.
 //   * Queries against int8 keys run on whole-number MMAs as they lie in memory, four 8-bit digits of every query; other 8-bit codes become
 //     fp16 exactly. Which dimensions an MMA multiplies is free as long as queries and keys agree, so that a lane takes whole 16-byte pieces
 //     of a key row; values are read transposed as pairs of bytes, which gives the lane a pair of dimensions, one for each of two MMAs.
-//   * One pass: every warp keeps a sum and a result of each row in registers, relative to a power of two that is raised when a score lies 8
-//     above it, which is seldom after the first tiles (raising it with every maximum cost 128 multiplications a tile). The scale of a
-//     token's values goes into its weight; weights times scales have a reference of their own, so that they stay in fp16's range
-//     whatever the scales are.
+//   * One pass: sums and results are relative to a power of two for each row that is raised when a score lies 8 above it, which is seldom
+//     after the first tiles. The scale of a token's values goes into its weight; weights times scales have a reference of their own, so
+//     that they stay in fp16's range whatever the scales are.
 //   * The work of all sequences is cut into equal shares by every block for itself (q4_attention_plan.h), from the lengths in device memory:
 //     a captured graph follows them. Results of an item cut over several blocks are joined in order by the last one.
 #include <cuda_fp8.h>
@@ -32,10 +35,9 @@
 
 namespace q4 {
 
-constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;
-constexpr uint32_t kRoundDims = 64;             // dimensions joined at a time
-constexpr uint32_t kRoundPitch = kRoundDims + 16;  // floats between rows of the join buffer: lanes of a store fall into different banks
+constexpr uint32_t kWarps = 8, kMultipliers = kWarps * 32, kThreads = kMultipliers + 32;  // the last warp asks for tiles
 constexpr uint32_t kLeastRun = 16;              // tiles: shorter runs cost more in joining than they save
+constexpr uint32_t kBatch = 8;                  // partial results that are asked for at a time
 constexpr float kNone = -3.0e38f;               // a reference below all scores: the row has seen nothing
 constexpr float kHeadroom = 8.f;                // how far above its reference a score may lie, in powers of two
 // 8-bit caches: a weight times scale is brought to 2^11 when it becomes the reference and may grow to 2^15, near the end of fp16's
@@ -50,23 +52,26 @@ struct Shape {
     static constexpr uint32_t kRow = HDP * (FMT == 0 ? 2 : 1);       // bytes of a token's row in shared memory
     static constexpr uint32_t kSeg = kRow < 128 ? kRow : 128;        // bytes of it that one copy brings
     static constexpr uint32_t kSegs = kRow / kSeg;
-    static constexpr uint32_t kTile = kTileTokens * kRow;            // a tile of keys or of values
+    static constexpr uint32_t kTile = kTileTokens * kRow;            // 16 tokens' keys or values
+    static constexpr uint32_t kSlot = kWarps * kTile;                // of the ring: keys, or values, of 128 tokens
     static constexpr uint32_t kPieces = kSeg / 64;                   // 16-byte pieces of a segment a lane takes from a key row
     static constexpr uint32_t kMmas = HDP / 16;                      // per 8 tokens of scores
-    static constexpr uint32_t kChunks = kRow / 16;                   // 16-byte pieces of a row
-    static constexpr uint32_t kChunkDims = FMT == 0 ? 8 : 16;
-    static constexpr uint32_t kAcc = HDP / 8;                        // accumulators of four numbers
-    static constexpr uint32_t kStep = FMT == 0 ? 1 : 2;              // tiles a warp multiplies at a time
-    // shared memory: rings, their scales, barriers, queries, the join buffer, and small arrays
+    static constexpr uint32_t kChunkDims = FMT == 0 ? 8 : 16;        // of a 16-byte piece
+    static constexpr uint32_t kValueWarps = HDP / kChunkDims < kWarps ? HDP / kChunkDims : kWarps;  // that have dimensions of the values
+    static constexpr uint32_t kWarpDims = HDP / kValueWarps;
+    static constexpr uint32_t kChunks = kWarpDims / kChunkDims;      // of a warp
+    static constexpr uint32_t kAcc = kWarpDims / 8;                  // accumulators of four numbers
+    static constexpr uint32_t kOwn = kWarpDims / 4;                  // numbers of a row's result in a lane
+    static constexpr bool kQueriesStay = FMT == 1 || HDP < 256;      // in registers
+    // shared memory: ring, scales of its keys and values, weights, queries, barriers, small arrays
+    static constexpr uint32_t kScales = FMT == 0 ? 0 : 2 * kWarps * 64;  // of a slot
     static constexpr uint32_t kQueries = kMmas * 32 * 16;
-    static constexpr uint32_t kJoin = kWarps * kAttentionRows * kRoundPitch * 4;
+    static constexpr uint32_t kWeights = 2 * kWarps * 32 * 16;
     static constexpr uint32_t kSmall = 2048;
-    static constexpr uint32_t kSlot = kStep * kTile, kSlotScales = kStep * 64;
-    static constexpr uint32_t kFit = (kSharedLimit - 1024 - kQueries - kJoin - kSmall) / (kWarps * (kSlot + kSlotScales + 8));
-    static constexpr uint32_t kSlots = kFit < 8 ? kFit : 8;          // of a warp's ring: keys and values of its steps in turn
-    static constexpr uint32_t kRing = kWarps * kSlots * kSlot, kScales = kWarps * kSlots * kSlotScales, kBars = (kWarps * kSlots * 8 + 15) / 16 * 16;
-    static constexpr uint32_t kShared = 1024 + kRing + kScales + kBars + kQueries + kJoin + kSmall;
-    static_assert(kSlots >= 2 && kStep * (kSegs + 1) <= 32, "");
+    static constexpr uint32_t kFit = (kSharedLimit - 1024 - kQueries - kWeights - kSmall) / (kSlot + kScales + 16);
+    static constexpr uint32_t kSlots = (kFit < 16 ? kFit : 16) & (FMT == 0 ? ~0u : ~1u);  // 8-bit: keys in even ones
+    static constexpr uint32_t kShared = 1024 + kSlots * (kSlot + kScales + 16) + kQueries + kWeights + kSmall;
+    static_assert(kSlots >= 2 && kWarps * kSegs <= 32, "");
 };
 
 // ---- small pieces ----
@@ -138,12 +143,16 @@ __device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {  // the lower two by
     return r;
 }
 
+__device__ __forceinline__ void ldmatrix_x2_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+}
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
@@ -166,14 +175,29 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, unsigne
     *error_flag = 1;
 }
 
+// Barrier of the warps that multiply; the second one tells whether any thread brought `true`.
+__device__ __forceinline__ void multipliers_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(kMultipliers) : "memory"); }
+__device__ __forceinline__ bool multipliers_any(bool mine) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t)mine), "n"(kMultipliers) : "memory");
+    return any != 0;
+}
+
 __device__ __forceinline__ void copy_tile(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int token, int head, int page) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(token),
                  "r"(head), "r"(page)
                  : "memory");
 }
-__device__ __forceinline__ void copy_bytes(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+__device__ __forceinline__ void copy_whole_tile(uint32_t dst, const CUtensorMap *map, uint32_t bar, int token, int head, int page) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %3, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(token),
+                 "r"(head), "r"(page)
+                 : "memory");
 }
+// 16 bytes, or zeros; counted by a barrier when they and the thread's others have arrived
+__device__ __forceinline__ void copy_16_or_zeros(uint32_t dst, const void *src, bool wanted) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(wanted ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
 
 // ---- a block's share ----
 
@@ -182,6 +206,7 @@ struct Geometry {
     uint32_t heads;   // items of a sequence = key heads * chunks
     uint32_t rows;    // query rows of a key head
     uint32_t group;   // query heads of a key head
+    uint32_t whole_rows;  // a copy brings all segments of 16 rows, else one of them
     AttentionPages pages;
 };
 
@@ -207,7 +232,9 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t v, uint32_t lane) {
     return v;
 }
 
-// All threads. `scratch`: 3 * kWarps + 2 words of 64 bits in shared memory. Up to 32 sequences every warp finds it by itself.
+constexpr uint32_t kAllWarps = kThreads / 32;
+
+// All threads. `scratch`: 3 * kAllWarps + 2 words of 64 bits in shared memory. Up to 32 sequences every warp finds it by itself.
 __device__ __forceinline__ Share share_of_block(const AttentionParams &p, const Geometry &g, uint64_t *scratch) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, sequences = p.kv.sequences;
     const bool few = sequences <= 32;
@@ -228,13 +255,13 @@ __device__ __forceinline__ Share share_of_block(const AttentionParams &p, const 
     items = __reduce_add_sync(0xffffffffu, items);
     longest = __reduce_max_sync(0xffffffffu, longest);
     if (!few) {
-        if (lane == 0) scratch[warp] = tiles, scratch[kWarps + warp] = items, scratch[2 * kWarps + warp] = longest;
+        if (lane == 0) scratch[warp] = tiles, scratch[kAllWarps + warp] = items, scratch[2 * kAllWarps + warp] = longest;
         __syncthreads();
         tiles = items = longest = 0;
-        for (uint32_t w = 0; w < kWarps; ++w) {
+        for (uint32_t w = 0; w < kAllWarps; ++w) {
             tiles += scratch[w];
-            items += (uint32_t)scratch[kWarps + w];
-            longest = max(longest, (uint32_t)scratch[2 * kWarps + w]);
+            items += (uint32_t)scratch[kAllWarps + w];
+            longest = max(longest, (uint32_t)scratch[2 * kAllWarps + w]);
         }
     }
     Share share;
@@ -264,18 +291,18 @@ __device__ __forceinline__ Share share_of_block(const AttentionParams &p, const 
             const uint64_t to = warp_scan(weight, lane);
             __syncthreads();
             if (lane == 31) scratch[warp] = to;
-            if (threadIdx.x == 0) scratch[kWarps] = ~0ull;
+            if (threadIdx.x == 0) scratch[kAllWarps] = ~0ull;
             __syncthreads();
             uint64_t from = before + to - weight;
-            for (uint32_t w = 0; w < kWarps; ++w) {
+            for (uint32_t w = 0; w < kAllWarps; ++w) {
                 if (w < warp) from += scratch[w];
                 before += scratch[w];
             }
-            if (target >= from && target < from + weight) scratch[kWarps] = i, scratch[kWarps + 1] = from;
+            if (target >= from && target < from + weight) scratch[kAllWarps] = i, scratch[kAllWarps + 1] = from;
             __syncthreads();
-            found = scratch[kWarps] != ~0ull;
-            s = (uint32_t)scratch[kWarps];
-            start = scratch[kWarps + 1];
+            found = scratch[kAllWarps] != ~0ull;
+            s = (uint32_t)scratch[kAllWarps];
+            start = scratch[kAllWarps + 1];
         }
         __syncthreads();
     }
@@ -283,80 +310,75 @@ __device__ __forceinline__ Share share_of_block(const AttentionParams &p, const 
     return share;
 }
 
-// ---- asking for tiles ----
-
-// What a warp asks for, ahead of what it multiplies: keys of its next kStep tiles into one slot, then their values into the next.
-// Lane i * kSegs + j brings segment j of tile i, the lanes behind those the scales. Page numbers are read one step ahead. A step's
-// second tile may lie behind the segment's end: such a copy starts outside the tensor map and brings zeros.
-template <int FMT, int HDP>
-struct Asker {
-    using S = Shape<FMT, HDP>;
-    static constexpr uint32_t kCopies = S::kStep * S::kSegs;
-    Cursor at;
-    uint32_t tile, head, slot, page, place;  // page and place: of this lane's tile
-    bool more, values;
-
-    __device__ __forceinline__ static uint32_t mine(uint32_t lane) { return lane < kCopies ? lane / S::kSegs : (lane - kCopies) % S::kStep; }
-    __device__ __forceinline__ void look(const AttentionParams &p, const Geometry &g, uint32_t warp, uint32_t lane) {
-        while (tile >= at.end) {
-            if (!at.next([&](uint32_t i) { return length_of(p, i); }, p.kv.sequences, g.heads)) {
-                more = false;
-                return;
-            }
-            tile = at.begin + warp * S::kStep;
-            head = g.chunks == 1 ? at.item : at.item / g.chunks;
-        }
-        const uint32_t t = tile + mine(lane), entry = g.pages.page_of(t);
-        place = (t - entry * g.pages.per) * kTileTokens;
-        page = t < at.end ? (uint32_t)__ldcg(p.kv.table + (uint64_t)at.s * p.kv.row_stride + entry) : ~0u;
-    }
-    __device__ __forceinline__ void start(const Share &share, const AttentionParams &p, const Geometry &g, uint32_t warp, uint32_t lane) {
-        at = share.at;
-        tile = at.begin + warp * S::kStep;
-        head = at.item / g.chunks;
-        slot = 0;
-        more = true;
-        values = false;
-        look(p, g, warp, lane);
-    }
-    __device__ __forceinline__ void ask(const AttentionParams &p, const Geometry &g, const CUtensorMap *k_map, const CUtensorMap *v_map, uint32_t ring, uint32_t scales, uint32_t bars,
-                                        uint32_t warp, uint32_t lane) {
-        if (!more) return;
-        const uint32_t bar = bars + slot * 8;
-        const bool there = page < p.kv.pages;
-        const uint32_t absent = __ballot_sync(0xffffffffu, !there);
-        uint32_t bytes = S::kSlot + (FMT == 0 ? 0u : S::kSlotScales);
-        if (absent) {
-            // behind the segment's end, or no page of the cache
-            if (!there && tile + mine(lane) < at.end) *p.kv.input_error = 1;
-            if (FMT != 0) {
-                bytes -= 64 * __popc(absent >> kCopies & ((1u << S::kStep) - 1));
-                if (!there && lane >= kCopies && lane < kCopies + S::kStep) {
-                    for (uint32_t i = 0; i < 64; i += 16) sts_v4(scales + slot * S::kSlotScales + (lane - kCopies) * 64 + i, make_uint4(0u, 0u, 0u, 0u));
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
-                __syncwarp();
-            }
-        }
-        if (lane == 0) mbar_expect(bar, bytes);
-        if (lane < kCopies)
-            copy_tile(ring + slot * S::kSlot + lane * (kTileTokens * S::kSeg), values ? v_map : k_map, bar, (int)(lane % S::kSegs * S::kSeg / (FMT == 0 ? 2 : 1)), (int)place, (int)head,
-                      (int)(there ? page : p.kv.pages));
-        else if (FMT != 0 && lane < kCopies + S::kStep && there)
-            copy_bytes(scales + slot * S::kSlotScales + (lane - kCopies) * 64, (values ? p.kv.v_scales : p.kv.k_scales) + ((uint64_t)page * p.kv.kv_heads + head) * p.kv.page_tokens + place, 64, bar);
-        slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-        if (values) {
-            tile += kWarps * S::kStep;
-            look(p, g, warp, lane);
-        }
-        values = !values;
-    }
-};
-
 template <int FMT>
 __device__ __forceinline__ bool not_finite(uint32_t w, uint32_t byte) {  // the value that begins at this byte of a word
     if (FMT == 0) return ((w >> (byte * 8)) & 0x7f80u) == 0x7f80u;
     return ((w >> (byte * 8)) & 0x7fu) == 0x7fu;
+}
+
+// A slot of the ring and the phase of its barriers.
+template <uint32_t N>
+struct Turn {
+    uint32_t slot = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        slot = slot + 1 == N ? 0 : slot + 1;
+        phase ^= slot == 0;
+    }
+};
+
+// ---- the warp that asks for tiles ----
+
+// A lane brings a tile, or one segment of it where rows are not a whole number of segments; scales come in 16-byte pieces, two a lane.
+// Page numbers are read while the slot that comes next is still in use.
+template <int FMT, int HDP>
+__device__ __forceinline__ void ask_for_tiles(const AttentionParams &p, const Geometry &g, Cursor at, const CUtensorMap *k_map, const CUtensorMap *v_map, uint32_t ring, uint32_t scales,
+                                              uint32_t full, uint32_t empty, uint32_t lane) {
+    using S = Shape<FMT, HDP>;
+    const uint32_t per = g.whole_rows ? 1 : S::kSegs, mine = lane / per, seg = lane % per;
+    const auto lengths = [&](uint32_t i) { return length_of(p, i); };
+    unsigned long long limit_ns = kWaitLimitNs;
+    Turn<S::kSlots> turn;
+    do {
+        const uint32_t head = at.item / g.chunks;
+        const int32_t *const table = p.kv.table + (uint64_t)at.s * p.kv.row_stride;
+        uint32_t entry = g.pages.page_of(at.begin + mine);
+        uint32_t page = at.begin + mine < at.end ? (uint32_t)__ldcg(table + entry) : 0u;
+        for (uint32_t tile = at.begin; tile < at.end; tile += kWarps) {
+            const uint32_t count = min(at.end - tile, kWarps);
+            const bool wanted = mine < count, there = page < p.kv.pages;
+            // (a page outside the cache is outside the tensor map too: such copies bring zeros)
+            const uint32_t now = there ? page : p.kv.pages, place = (tile + mine - entry * g.pages.per) * kTileTokens;
+            if (wanted && !there) *p.kv.input_error = 1;
+            const uint32_t next = tile + kWarps + mine;
+            if (next < at.end) {
+                entry = g.pages.page_of(next);
+                page = (uint32_t)__ldcg(table + entry);
+            }
+#pragma unroll
+            for (uint32_t values = 0; values < 2; ++values) {
+                mbar_wait(empty + turn.slot * 8, turn.phase ^ 1u, limit_ns, p.error_flag);
+                const uint32_t bar = full + turn.slot * 8, dst = ring + turn.slot * S::kSlot;
+                if (lane == 0) mbar_expect(bar, count * S::kTile);
+                __syncwarp();
+                if (wanted) {
+                    if (S::kSegs > 1 && g.whole_rows) copy_whole_tile(dst + lane * S::kTile, values ? v_map : k_map, bar, (int)place, (int)head, (int)now);
+                    else copy_tile(dst + lane * (kTileTokens * S::kSeg), values ? v_map : k_map, bar, (int)(seg * S::kSeg / (FMT == 0 ? 2 : 1)), (int)place, (int)head, (int)now);
+                }
+                if (FMT != 0 && values == 0) {
+                    // lane 4 i + j: 16-byte piece j of tile i's scales, of keys and of values
+                    const uint32_t of = lane / 4, of_page = __shfl_sync(0xffffffffu, now, of * per), of_place = __shfl_sync(0xffffffffu, place, of * per);
+                    const bool here = of < count && of_page < p.kv.pages;
+                    const uint64_t from = here ? ((uint64_t)of_page * p.kv.kv_heads + head) * p.kv.page_tokens + of_place + lane % 4 * 4 : 0;
+                    const uint32_t sc = scales + turn.slot * S::kScales + lane * 16;
+                    copy_16_or_zeros(sc, p.kv.k_scales + from, here);
+                    copy_16_or_zeros(sc + kWarps * 64, p.kv.v_scales + from, here);
+                    copies_arrive(bar);
+                }
+                turn.next();
+            }
+        }
+    } while (at.next(lengths, p.kv.sequences, g.heads));
+    if (FMT != 0) asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---- the kernel ----
@@ -365,54 +387,63 @@ template <int FMT, int HDP>
 __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ Geometry g, const __grid_constant__ CUtensorMap k_map,
                                                                 const __grid_constant__ CUtensorMap v_map) {
     using S = Shape<FMT, HDP>;
-    constexpr uint32_t kStep = S::kStep;
     extern __shared__ uint8_t shared_raw[];
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(shared_raw), pad = (1024u - (raw & 1023u)) & 1023u;
-    uint8_t *const shared = shared_raw + pad;
-    uint4 *const queries = reinterpret_cast<uint4 *>(shared + S::kRing + S::kScales + S::kBars);  // left operands: [MMA][lane]
-    float *const join = reinterpret_cast<float *>(queries) + S::kQueries / 4;
-    float *const small = join + S::kJoin / 4;
-    float *const tops = small, *const sums = small + kWarps * kAttentionRows;  // [warp][row]
-    float *const row_scales = small + 2 * kWarps * kAttentionRows;             // [row] scale of the scores, in powers of two
+    const uint32_t ring = raw + pad, scales = ring + S::kSlots * S::kSlot, weights = scales + S::kSlots * S::kScales, queries = weights + S::kWeights, full = queries + S::kQueries,
+                   empty = full + S::kSlots * 8;
+    float *const small = reinterpret_cast<float *>(shared_raw + (empty + S::kSlots * 8 - raw));
+    float *const highs = small, *const weight_highs = small + kWarps * kAttentionRows, *const sums = small + 2 * kWarps * kAttentionRows;  // [warp][row]
+    float *const row_scales = small + 3 * kWarps * kAttentionRows;                                                                         // [row] scale of the scores, in powers of two
     uint64_t *const scratch = reinterpret_cast<uint64_t *>(row_scales + kAttentionRows);
-    uint32_t *const arrived = reinterpret_cast<uint32_t *>(scratch + 3 * kWarps + 2);
+    uint32_t *const arrived = reinterpret_cast<uint32_t *>(scratch + 3 * kAllWarps + 2);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row = lane >> 2, quad = lane & 3u;
-    const uint32_t ring = raw + pad + warp * S::kSlots * S::kSlot, scales = raw + pad + S::kRing + warp * S::kSlots * S::kSlotScales;
-    const uint32_t bars = raw + pad + S::kRing + S::kScales + warp * S::kSlots * 8, queries_at = raw + pad + S::kRing + S::kScales + S::kBars + lane * 16;
-    if (lane == 0)
-        for (uint32_t i = 0; i < S::kSlots; ++i) mbar_init(bars + i * 8, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncwarp();
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < S::kSlots; ++i) {
+            mbar_init(full + i * 8, FMT != 0 && i % 2 == 0 ? 33 : 1);  // the tile copies; the lanes' scales
+            mbar_init(empty + i * 8, kWarps);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
     grid_dependency_wait();
     grid_dependents_launch();
 
     const Share share = share_of_block(p, g, scratch);
-    if (share.any) {
-        Asker<FMT, HDP> asker;
-        asker.start(share, p, g, warp, lane);
-        for (uint32_t i = 0; i < S::kSlots; ++i) asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
-        uint32_t slot = 0, parity = 0;
+    const auto lengths = [&](uint32_t i) { return length_of(p, i); };
+    if (share.any && warp == kWarps) {
+        ask_for_tiles<FMT, HDP>(p, g, share.at, &k_map, &v_map, ring, scales, full, empty, lane);
+    } else if (share.any) {
+        Turn<S::kSlots> turn;
         unsigned long long limit_ns = kWaitLimitNs;
+        uint32_t weights_at = weights;  // one of two buffers
         Cursor at = share.at;
+        // eight values of query row `warp` of an item
+        float q[8];
+        const auto load_query = [&](const Cursor &c) {
+            const uint32_t r = c.item % g.chunks * kAttentionRows + warp, d = lane * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = 0.f;
+            if (r < g.rows && d < p.kv.head_dim) {
+                const uint64_t base = ((uint64_t)c.s * p.q_tokens + r / g.group) * p.q_stride + ((uint64_t)(c.item / g.chunks) * g.group + r % g.group) * p.kv.head_dim + d;
+                if (p.q_is_f32) {
+                    const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + base);
+                    const float4 v = __ldcg(f), w = __ldcg(f + 1);
+                    q[0] = v.x, q[1] = v.y, q[2] = v.z, q[3] = v.w, q[4] = w.x, q[5] = w.y, q[6] = w.z, q[7] = w.w;
+                } else {
+                    const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + base));
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) q[2 * i] = __uint_as_float(w[i] << 16), q[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                }
+            }
+        };
+        load_query(at);
+        bool more;
         do {
-            // ---- queries of the item: warp w brings row w, split into halves, in the order in which key rows are read ----
+            // ---- queries of the item: warp w splits row w into halves, in the order in which key rows are read ----
             const uint32_t head = at.item / g.chunks, chunk = at.item % g.chunks;
             {
-                const uint32_t r = chunk * kAttentionRows + warp, d = lane * 8;
-                float q[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (r < g.rows && d < p.kv.head_dim) {
-                    const uint64_t base = ((uint64_t)at.s * p.q_tokens + r / g.group) * p.q_stride + ((uint64_t)head * g.group + r % g.group) * p.kv.head_dim + d;
-                    if (p.q_is_f32) {
-                        const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + base);
-                        const float4 v = __ldcg(f), w = __ldcg(f + 1);
-                        q[0] = v.x, q[1] = v.y, q[2] = v.z, q[3] = v.w, q[4] = w.x, q[5] = w.y, q[6] = w.z, q[7] = w.w;
-                    } else {
-                        const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + base));
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) q[2 * i] = __uint_as_float(w[i] << 16), q[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-                    }
-                }
+                const uint32_t d = lane * 8;
                 float unit = 1.f, row_scale = p.scale * 1.4426950408889634f;
                 if (FMT != 0) {
                     // fp16 halves, whole numbers: the row is scaled by a power of two that brings its largest value into [1, 2)
@@ -430,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     // a lane's part of an MMA is four values, of a whole-number one eight; a 16-byte piece of a key row holds 8 or 16
                     constexpr uint32_t kPer = S::kChunkDims / 4;
                     const uint32_t piece = d / S::kChunkDims, seg = piece / (S::kSeg / 16), in_seg = piece % (S::kSeg / 16);
-                    const uint32_t m = (seg * S::kPieces + in_seg % S::kPieces) * kPer + d % S::kChunkDims / 4, to = warp * 4 + in_seg / S::kPieces;
+                    const uint32_t m = (seg * S::kPieces + in_seg % S::kPieces) * kPer + d % S::kChunkDims / 4, to = queries + (m * 32 + warp * 4 + in_seg / S::kPieces) * 16;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) q[i] *= unit;
                     uint4 a, b;
@@ -442,69 +473,74 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         split<FMT>(q[4], q[5], b.x, b.y);
                         split<FMT>(q[6], q[7], b.z, b.w);
                     }
-                    queries[m * 32 + to] = a;
-                    queries[(m + 1) * 32 + to] = b;
+                    sts_v4(to, a);
+                    sts_v4(to + 512, b);
                 }
                 if (lane == 0) row_scales[warp] = row_scale;
             }
-            __syncthreads();
+            multipliers_sync();
             const float row_scale = row_scales[row];
+            uint32_t qa[S::kMmas][4];  // (where registers are short, read again for every tile)
+            const auto fetch_query = [&](uint32_t m) {
+                const uint4 w = lds_v4(queries + (m * 32 + lane) * 16);
+                qa[m][0] = w.x, qa[m][1] = w.y, qa[m][2] = w.z, qa[m][3] = w.w;
+            };
+            if (S::kQueriesStay)
+#pragma unroll
+                for (uint32_t m = 0; m < S::kMmas; ++m) fetch_query(m);
+            Cursor ahead = at;
+            more = ahead.next(lengths, p.kv.sequences, g.heads);
+            if (more) load_query(ahead);
             // tokens of the segment that all rows see, that this row sees, and that exist
             const int32_t end_token = (int32_t)(at.end * kTileTokens), existing = min(at.length, end_token);
             const int32_t sure = min(at.length - (int32_t)p.q_tokens + 1, end_token);
             const uint32_t r = chunk * kAttentionRows + row;
-            const int32_t limit = r < g.rows ? min(at.length - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group), end_token) : 0;
+            const bool live = r < g.rows;
+            const int32_t limit = live ? min(at.length - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group), end_token) : 0;
             float acc[S::kAcc][4];
 #pragma unroll
             for (uint32_t i = 0; i < S::kAcc; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-            float top = kNone, sum = 0.f;                     // reference of the row's scores; sum of this lane's weights
+            float top = kNone, sum = 0.f;                      // reference of the row's scores; sum of this lane's weights
             float weight_top = kNone, lift = 0.f, most = 0.f;  // 8-bit: reference of weights times scales, 2^(top - weight_top), and what they may be
 
-            for (uint32_t tile = at.begin + warp * kStep; tile < at.end; tile += kWarps * kStep) {
-                const int32_t token = (int32_t)(tile * kTileTokens);
-                const bool edge = token + (int32_t)(kStep * kTileTokens) > sure;  // some rows do not see all of it
+            for (uint32_t tile = at.begin; tile < at.end; tile += kWarps) {
+                const uint32_t count = min(at.end - tile, kWarps);  // tiles of 16 tokens; this warp's scores are those of tile + warp
                 // ---- scores ----
-                mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
-                float x[4 * kStep];  // this lane's: tokens 2 quad, + 1, + 8, + 9 of each tile, row `row`
-                {
-                    const uint32_t keys = ring + slot * S::kSlot;
-                    float s[2 * kStep][4];
-                    int upper[2 * kStep][4], lower[2 * kStep][4];  // int8: products with digits 3 and 2, and with 1 and 0
-#pragma unroll
-                    for (uint32_t n = 0; n < 2 * kStep; ++n) {
-                        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-                        upper[n][0] = upper[n][1] = upper[n][2] = upper[n][3] = lower[n][0] = lower[n][1] = lower[n][2] = lower[n][3] = 0;
-                    }
+                mbar_wait(full + turn.slot * 8, turn.phase, limit_ns, p.error_flag);
+                float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // tokens 2 quad, + 1, + 8, + 9, row `row`
+                float value_scale[4] = {0.f, 0.f, 0.f, 0.f};
+                if (warp < count) {
+                    const uint32_t keys = ring + turn.slot * S::kSlot + warp * S::kTile;
+                    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                    int upper[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, lower[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};  // int8: products with digits 3 and 2, and with 1 and 0
 #pragma unroll
                     for (uint32_t seg = 0; seg < S::kSegs; ++seg)
 #pragma unroll
                         for (uint32_t c = 0; c < S::kPieces; ++c) {
-                            const uint32_t piece = quad * S::kPieces + c, turn = S::kSeg == 128 ? row : row >> 1 & 3u;
-                            const uint32_t within = seg * (kTileTokens * S::kSeg) + row * S::kSeg + ((piece ^ turn) << 4);
+                            const uint32_t piece = quad * S::kPieces + c, swap = S::kSeg == 128 ? row : row >> 1 & 3u;
+                            const uint32_t from = keys + seg * (kTileTokens * S::kSeg) + row * S::kSeg + ((piece ^ swap) << 4);
                             constexpr uint32_t kPer = S::kChunkDims / 4;
                             const uint32_t m = (seg * S::kPieces + c) * kPer;
-                            uint32_t word[2 * kStep][4];
+                            if (!S::kQueriesStay)
 #pragma unroll
-                            for (uint32_t n = 0; n < 2 * kStep; ++n) {
-                                const uint4 w = lds_v4(keys + n / 2 * S::kTile + within + n % 2 * 8 * S::kSeg);
-                                word[n][0] = w.x, word[n][1] = w.y, word[n][2] = w.z, word[n][3] = w.w;
-                            }
+                                for (uint32_t i = 0; i < kPer; ++i) fetch_query(m + i);
 #pragma unroll
-                            for (uint32_t i = 0; i < kPer; ++i) {
-                                const uint4 w = lds_v4(queries_at + (m + i) * 512);
-                                const uint32_t qa[4] = {w.x, w.y, w.z, w.w};
+                            for (uint32_t n = 0; n < 2; ++n) {
+                                const uint4 w = lds_v4(from + n * 8 * S::kSeg);
+                                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                                for (uint32_t n = 0; n < 2 * kStep; ++n) {
-                                    if (FMT == 0) mma<FMT>(s[n], qa, word[n][2 * i], word[n][2 * i + 1]);
-                                    else if (FMT == 1) mma_s8s8_16832(i % 2 == 0 ? upper[n] : lower[n], qa[0], qa[1], qa[2], qa[3], word[n][i / 2 * 2], word[n][i / 2 * 2 + 1]);
-                                    else mma<FMT>(s[n], qa, e4m3_pair(word[n][i]), e4m3_pair(word[n][i] >> 16));
+                                for (uint32_t i = 0; i < kPer; ++i) {
+                                    if (FMT == 0) mma<FMT>(s[n], qa[m + i], word[2 * i % 4], word[(2 * i + 1) % 4]);
+                                    else if (FMT == 1) mma_s8s8_16832(i % 2 == 0 ? upper[n] : lower[n], qa[m + i][0], qa[m + i][1], qa[m + i][2], qa[m + i][3], word[i / 2 * 2], word[i / 2 * 2 + 1]);
+                                    else mma<FMT>(s[n], qa[m + i], e4m3_pair(word[i]), e4m3_pair(word[i] >> 16));
                                 }
                             }
                         }
+                    const uint32_t sc = scales + turn.slot * S::kScales + warp * 64 + quad * 8;
 #pragma unroll
-                    for (uint32_t n = 0; n < 2 * kStep; ++n) {
+                    for (uint32_t n = 0; n < 2; ++n) {
                         if (FMT == 1) {
-                            // a sum of 256 products is below 2^22, so two digits' sums fit 32 bits
+                            // a sum of 256 products is at most 2^22, so two digits' sums fit 32 bits
 #pragma unroll
                             for (int j = 0; j < 2; ++j)
                                 x[2 * n + j] = fmaf((float)(upper[n][j] * 256 + upper[n][j + 2]), 65536.f, (float)(lower[n][j] * 256 + lower[n][j + 2])) * row_scale;
@@ -513,45 +549,59 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             x[2 * n + 1] = (s[n][1] + s[n][3]) * row_scale;
                         }
                         if (FMT != 0) {
-                            const uint2 k = lds_v2(scales + slot * S::kSlotScales + n * 32 + quad * 8);
+                            const uint2 k = lds_v2(sc + n * 32), v = lds_v2(sc + kWarps * 64 + n * 32);
                             x[2 * n] *= __uint_as_float(k.x), x[2 * n + 1] *= __uint_as_float(k.y);
+                            value_scale[2 * n] = __uint_as_float(v.x), value_scale[2 * n + 1] = __uint_as_float(v.y);
                         }
                     }
+                    const int32_t token = (int32_t)((tile + warp) * kTileTokens);
+                    if (token + (int32_t)kTileTokens > sure)  // some rows do not see all of it
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (token + (int32_t)quad * 2 + i % 2 + i / 2 * 8 >= limit) {
+                                x[i] = -INFINITY;
+                                value_scale[i] = 0.f;  // (it may be anything)
+                            }
                 }
-                __syncwarp();  // the slot has been read
-                asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
-                slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-                parity ^= slot == 0;
-                if (edge)
-#pragma unroll
-                    for (uint32_t i = 0; i < 4 * kStep; ++i)
-                        if (token + (int32_t)(i / 2 * 8 + quad * 2 + i % 2) >= limit) x[i] = -INFINITY;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty + turn.slot * 8);
+                turn.next();
                 // ---- weights ----
-                mbar_wait(bars + slot * 8, parity, limit_ns, p.error_flag);
-                const uint32_t held = ring + slot * S::kSlot;
-                float value_scale[FMT == 0 ? 1 : 4 * kStep], weight[4 * kStep];
-                if (FMT != 0)
+                float high = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), weight[4], weight_high = 0.f;
 #pragma unroll
-                    for (uint32_t n = 0; n < 2 * kStep; ++n) {
-                        const uint2 v = lds_v2(scales + slot * S::kSlotScales + n * 32 + quad * 8);
-                        value_scale[2 * n] = __uint_as_float(v.x), value_scale[2 * n + 1] = __uint_as_float(v.y);
-                        // (a token that the row does not see: its scale may be anything)
-                        if (edge) {
-                            if (x[2 * n] == -INFINITY) value_scale[2 * n] = 0.f;
-                            if (x[2 * n + 1] == -INFINITY) value_scale[2 * n + 1] = 0.f;
-                        }
-                    }
-                float high = x[0], weight_high = 0.f;
-#pragma unroll
-                for (uint32_t i = 1; i < 4 * kStep; ++i) high = fmaxf(high, x[i]);
-#pragma unroll
-                for (uint32_t i = 0; i < 4 * kStep; ++i) {
+                for (int i = 0; i < 4; ++i) {
                     weight[i] = exp2_fast(x[i] - top);
                     if (FMT != 0) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
                 }
-                if (__any_sync(0xffffffffu, high - top > kHeadroom || (FMT != 0 && weight_high > most))) {
+                uint32_t pa[4];
+                float of_tile;
+                const auto pass_on = [&]() {
+                    float w[4];
+                    of_tile = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = FMT == 0 ? weight[i] : weight[i] * (value_scale[i] * lift);
+                    split<FMT>(w[0], w[1], pa[0], pa[1]);
+                    split<FMT>(w[2], w[3], pa[2], pa[3]);
+                    if (FMT == 0) {
+                        // bf16: the weights as they are multiplied, so that they add up to one whatever the halves cut off
+#pragma unroll
+                        for (int j = 0; j < 4; j += 2)
+                            of_tile += (__uint_as_float(pa[j] << 16) + __uint_as_float(pa[j + 1] << 16)) + (__uint_as_float(pa[j] & 0xffff0000u) + __uint_as_float(pa[j + 1] & 0xffff0000u));
+                    } else {
+                        of_tile = (weight[0] + weight[1]) + (weight[2] + weight[3]);
+                    }
+                    sts_v4(weights_at + (warp * 32 + lane) * 16, make_uint4(pa[0], pa[1], pa[2], pa[3]));
+                };
+                pass_on();
+                if (multipliers_any(high - top > kHeadroom || (FMT != 0 && weight_high > most))) {
+                    // a reference is raised, in all warps alike
                     high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
                     high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+                    if (quad == 0) highs[warp * kAttentionRows + row] = high;
+                    multipliers_sync();
+                    high = -INFINITY;
+#pragma unroll
+                    for (uint32_t w = 0; w < kWarps; ++w) high = fmaxf(high, highs[w * kAttentionRows + row]);
                     float keep = 1.f;
                     if (high - top > kHeadroom) {
                         high = ceilf(high);
@@ -564,14 +614,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             keep = 1.f;
                         }
 #pragma unroll
-                        for (uint32_t i = 0; i < 4 * kStep; ++i) weight[i] = exp2_fast(x[i] - top);
+                        for (int i = 0; i < 4; ++i) weight[i] = exp2_fast(x[i] - top);
                     }
                     if (FMT != 0) {
                         weight_high = 0.f;
 #pragma unroll
-                        for (uint32_t i = 0; i < 4 * kStep; ++i) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
+                        for (int i = 0; i < 4; ++i) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
                         weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 1));
                         weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 2));
+                        if (quad == 0) weight_highs[warp * kAttentionRows + row] = weight_high;
+                        multipliers_sync();
+                        weight_high = 0.f;
+#pragma unroll
+                        for (uint32_t w = 0; w < kWarps; ++w) weight_high = fmaxf(weight_high, weight_highs[w * kAttentionRows + row]);
                         if (weight_high > most) {
                             const int e = (int)(__float_as_uint(weight_high) >> 23) - 126;  // weight_high < 2^e
                             const float next = top + (float)max(e - kWeightExponent, -126);
@@ -585,225 +640,214 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     for (uint32_t i = 0; i < S::kAcc; ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) acc[i][j] *= keep;
+                    pass_on();
+                    multipliers_sync();
                 }
+                sum += of_tile;
+                // ---- values: this warp's dimensions, all tokens ----
+                mbar_wait(full + turn.slot * 8, turn.phase, limit_ns, p.error_flag);
+                if (warp < S::kValueWarps) {
+                    const uint32_t held = ring + turn.slot * S::kSlot;
+                    const uint32_t matrix = lane >> 3, line = (lane & 7u) + (matrix & 1u) * 8, swap = S::kSeg == 128 ? line & 7u : line >> 1 & 3u;
+                    uint32_t from[(S::kChunks + 1) / 2];  // in a tile, for each pair of chunks
 #pragma unroll
-                for (uint32_t i = 0; i < 4 * kStep; ++i) {
-                    if (FMT != 0) {
-                        sum += weight[i];
-                        weight[i] *= value_scale[i] * lift;
+                    for (uint32_t c = 0; c < (S::kChunks + 1) / 2; ++c) {
+                        const uint32_t piece = warp * S::kChunks + 2 * c + (S::kChunks > 1 ? matrix >> 1 : 0u), seg = piece / (S::kSeg / 16);
+                        from[c] = held + seg * (kTileTokens * S::kSeg) + line * S::kSeg + ((piece % (S::kSeg / 16) ^ swap) << 4);
                     }
-                }
-                uint32_t pa[kStep][4];
+                    const auto add_tile = [&](uint32_t t, bool edge) {
+                        const uint4 w = lds_v4(weights_at + (t * 32 + lane) * 16);
+                        const uint32_t wa[4] = {w.x, w.y, w.z, w.w};
+                        uint32_t v[(S::kChunks + 1) / 2][4];
 #pragma unroll
-                for (uint32_t i = 0; i < kStep; ++i) {
-                    split<FMT>(weight[4 * i], weight[4 * i + 1], pa[i][0], pa[i][1]);
-                    split<FMT>(weight[4 * i + 2], weight[4 * i + 3], pa[i][2], pa[i][3]);
-                    // bf16: the weights as they are multiplied, so that they add up to one whatever the halves cut off
-                    if (FMT == 0)
-#pragma unroll
-                        for (int j = 0; j < 4; j += 2)
-                            sum += (__uint_as_float(pa[i][j] << 16) + __uint_as_float(pa[i][j + 1] << 16)) +
-                                   (__uint_as_float(pa[i][j] & 0xffff0000u) + __uint_as_float(pa[i][j + 1] & 0xffff0000u));
-                }
-                // ---- values ----
-                if (edge) {
-                    // Rows behind the sequence's end hold anything: zeros are put in their place. Among draft tokens a value that is not
-                    // finite may be seen by some rows only, and a weight of zero does not take it out of a sum: it is added here to the
-                    // rows that see it, and becomes a zero too.
-#pragma unroll
-                    for (uint32_t i = 0; i < kStep; ++i) {
-                        const uint32_t base = held + i * S::kTile;
-                        const int32_t first = token + (int32_t)(i * kTileTokens);
-                        if (FMT != 1 && p.q_tokens > 1) {
+                        for (uint32_t c = 0; c < (S::kChunks + 1) / 2; ++c) {
+                            if (S::kChunks > 1) ldmatrix_x4_trans(v[c], from[c] + t * S::kTile);
+                            else ldmatrix_x2_trans(v[c], from[c] + t * S::kTile);
+                        }
+                        const int32_t first = (int32_t)((tile + t) * kTileTokens);
+                        if (edge) {
+                            // Rows behind the sequence's end hold anything: zeros are taken for them. Among draft tokens a value that is not
+                            // finite may be seen by some rows only, and a weight of zero does not take it out of a sum: it is taken out
+                            // here and added to the rows that see it.
                             bool odd = false;
-                            for (uint32_t b = lane * 16; b < S::kTile; b += 512) {
-                                const uint4 w = lds_v4(base + b);
-                                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-                                if (first + (int32_t)(b / S::kSeg % kTileTokens) < existing)
 #pragma unroll
-                                    for (int j = 0; j < 4; ++j)
+                            for (uint32_t c = 0; c < (S::kChunks + 1) / 2; ++c)
 #pragma unroll
-                                        for (int k = 0; k < 4; k += FMT == 0 ? 2 : 1) odd = odd || not_finite<FMT>(word[j], k);
-                            }
-                            if (__any_sync(0xffffffffu, odd)) {
+                                for (uint32_t i = 0; i < (S::kChunks > 1 ? 4 : 2); ++i) {
+                                    const int32_t k = first + (int32_t)(quad * 2 + i % 2 * 8);
+                                    v[c][i] &= (k < existing ? 0xffffu : 0u) | (k + 1 < existing ? 0xffff0000u : 0u);
+                                    if (FMT != 1 && p.q_tokens > 1)
 #pragma unroll
-                                for (uint32_t c = 0; c < S::kAcc; ++c)
+                                        for (int b = 0; b < 4; b += FMT == 0 ? 2 : 1)
+                                            if (not_finite<FMT>(v[c][i], b)) {
+                                                odd = true;
+                                                v[c][i] &= ~((FMT == 0 ? 0xffffu : 0xffu) << (b * 8));
+                                            }
+                                }
+                            if (FMT != 1 && __any_sync(0xffffffffu, odd)) {
+#pragma unroll
+                                for (uint32_t i = 0; i < S::kAcc; ++i)
 #pragma unroll
                                     for (uint32_t j = 0; j < 2; ++j) {
-                                        const uint32_t d = FMT == 0 ? c * 8 + quad * 2 + j : c / 2 * 16 + quad * 4 + j * 2 + (c & 1u);
+                                        const uint32_t d = warp * S::kWarpDims + (FMT == 0 ? i * 8 + quad * 2 + j : i / 2 * 16 + quad * 4 + j * 2 + (i & 1u));
                                         const uint32_t byte = d * (FMT == 0 ? 2 : 1), seg = byte / S::kSeg, piece = byte % S::kSeg / 16;
-                                        for (int32_t t = 0; t < (int32_t)kTileTokens && first + t < limit; ++t) {
-                                            const uint32_t swap = S::kSeg == 128 ? (uint32_t)t & 7u : (uint32_t)t >> 1 & 3u;
-                                            const uint32_t w = lds_u32((base + seg * (kTileTokens * S::kSeg) + (uint32_t)t * S::kSeg + ((piece ^ swap) << 4) + byte % 16) & ~3u);
-                                            if (not_finite<FMT>(w, byte & 3u)) acc[c][j] += FMT == 0 ? __uint_as_float((w >> ((byte & 3u) * 8)) << 16) : __uint_as_float(0x7fc00000u);
+                                        for (int32_t k = 0; k < (int32_t)kTileTokens && first + k < limit; ++k) {
+                                            const uint32_t turned = S::kSeg == 128 ? (uint32_t)k & 7u : (uint32_t)k >> 1 & 3u;
+                                            const uint32_t e = lds_u32((held + t * S::kTile + seg * (kTileTokens * S::kSeg) + (uint32_t)k * S::kSeg + ((piece ^ turned) << 4) + byte % 16) & ~3u);
+                                            if (not_finite<FMT>(e, byte & 3u)) acc[i][j] += FMT == 0 ? __uint_as_float((e >> ((byte & 3u) * 8)) << 16) : __uint_as_float(0x7fc00000u);
                                         }
                                     }
                                 __syncwarp();
-                                for (uint32_t b = lane * 16; b < S::kTile; b += 512) {
-                                    const uint4 w = lds_v4(base + b);
-                                    uint32_t word[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                                        for (int k = 0; k < 4; k += FMT == 0 ? 2 : 1)
-                                            if (not_finite<FMT>(word[j], k)) word[j] &= ~((FMT == 0 ? 0xffffu : 0xffu) << (k * 8));
-                                    sts_v4(base + b, make_uint4(word[0], word[1], word[2], word[3]));
-                                }
                             }
                         }
-                        for (uint32_t b = lane * 16; b < S::kTile; b += 512)
-                            if (first + (int32_t)(b / S::kSeg % kTileTokens) >= existing) sts_v4(base + b, make_uint4(0u, 0u, 0u, 0u));
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into these slots
-                    __syncwarp();
-                }
-                const uint32_t matrix = lane >> 3, line = (lane & 7u) + (matrix & 1u) * 8, turn = S::kSeg == 128 ? line & 7u : line >> 1 & 3u;
 #pragma unroll
-                for (uint32_t c = 0; c < S::kChunks; c += 2) {
-                    const uint32_t seg = c / (S::kSeg / 16), piece = c % (S::kSeg / 16) + (matrix >> 1);
-                    const uint32_t within = seg * (kTileTokens * S::kSeg) + line * S::kSeg + ((piece ^ turn) << 4);
-#pragma unroll
-                    for (uint32_t t = 0; t < kStep; ++t) {
-                        uint32_t v[4];
-                        ldmatrix_x4_trans(v, held + t * S::kTile + within);
-#pragma unroll
-                        for (uint32_t i = 0; i < 2; ++i) {
-                            const uint32_t b0 = v[2 * i], b1 = v[2 * i + 1];
+                        for (uint32_t c = 0; c < S::kChunks; ++c) {
+                            const uint32_t b0 = v[c / 2][c % 2 * 2], b1 = v[c / 2][c % 2 * 2 + 1];
                             if (FMT == 0) {
-                                mma<FMT>(acc[c + i], pa[t], b0, b1);
+                                mma<FMT>(acc[c], wa, b0, b1);
                             } else if (FMT == 1) {
-                                mma<FMT>(acc[(c + i) * 2], pa[t], int8_even(b0), int8_even(b1));
-                                mma<FMT>(acc[(c + i) * 2 + 1], pa[t], int8_even(b0 >> 8), int8_even(b1 >> 8));
+                                mma<FMT>(acc[2 * c], wa, int8_even(b0), int8_even(b1));
+                                mma<FMT>(acc[2 * c + 1], wa, int8_even(b0 >> 8), int8_even(b1 >> 8));
                             } else {
-                                mma<FMT>(acc[(c + i) * 2], pa[t], e4m3_pair(__byte_perm(b0, 0, 0x4420)), e4m3_pair(__byte_perm(b1, 0, 0x4420)));
-                                mma<FMT>(acc[(c + i) * 2 + 1], pa[t], e4m3_pair(__byte_perm(b0, 0, 0x4431)), e4m3_pair(__byte_perm(b1, 0, 0x4431)));
+                                mma<FMT>(acc[2 * c], wa, e4m3_pair(__byte_perm(b0, 0, 0x4420)), e4m3_pair(__byte_perm(b1, 0, 0x4420)));
+                                mma<FMT>(acc[2 * c + 1], wa, e4m3_pair(__byte_perm(b0, 0, 0x4431)), e4m3_pair(__byte_perm(b1, 0, 0x4431)));
                             }
                         }
+                    };
+                    const uint32_t plain = (uint32_t)max(min(sure - (int32_t)(tile * kTileTokens), (int32_t)(count * kTileTokens)), 0) / kTileTokens;  // tiles that all rows see
+                    if (plain == kWarps) {
+#pragma unroll
+                        for (uint32_t t = 0; t < kWarps; ++t) add_tile(t, false);
+                    } else {
+#pragma unroll 1
+                        for (uint32_t t = 0; t < count; ++t) add_tile(t, t >= plain);
                     }
                 }
                 __syncwarp();
-                asker.ask(p, g, &k_map, &v_map, ring, scales, bars, warp, lane);
-                slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-                parity ^= slot == 0;
+                if (lane == 0) mbar_arrive(empty + turn.slot * 8);
+                turn.next();
+                weights_at = weights_at == weights ? weights + S::kWeights / 2 : weights;
             }
 
-            // ---- join the warps' results; then, in the last block of a cut item, those of the blocks ----
+            // ---- the segment's result ----
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            // what of the row's result a lane holds: dimensions 16 i + 4 quad ... + 3 (bf16, at first: 16 i + 2 quad, + 1, + 8, + 9)
-            float4 o[HDP / 16];
+            if (quad == 0) sums[warp * kAttentionRows + row] = sum;
+            multipliers_sync();
+            float total = 0.f;
 #pragma unroll
-            for (uint32_t i = 0; i < HDP / 16; ++i) {
-                const float *a = acc[2 * i], *b = acc[2 * i + 1];
-                o[i] = FMT == 0 ? make_float4(a[0] + a[2], a[1] + a[3], b[0] + b[2], b[1] + b[3]) : make_float4(a[0] + a[2], b[0] + b[2], a[1] + a[3], b[1] + b[3]);
-            }
-            if (top == kNone) top = -INFINITY;
-            float o_top = FMT == 0 ? top : weight_top == kNone ? -INFINITY : weight_top;
-            const bool cut = !at.whole_item();
-            uint32_t owner, contributors;
-            at.contributors(share.cut, blockIdx.x, &owner, &contributors);
-            // a partial result: rows, then maxima, then sums
-            constexpr uint32_t kPart = kAttentionRows * (kMaxHeadDim + 2);
-            float *const part = p.parts + ((uint64_t)blockIdx.x * 2 + (blockIdx.x == owner ? 1 : 0)) * kPart;
-            const uint32_t jr = threadIdx.x >> 4 & 7u, jd = (threadIdx.x & 15u) * 4;  // row and dimensions that a thread joins
-            const uint32_t j_row = chunk * kAttentionRows + jr, j_draft = j_row / g.group;
-            const bool j_live = j_row < g.rows, j_empty = at.length - (int32_t)p.q_tokens + 1 + (int32_t)j_draft <= 0;
-            const uint64_t out_row = ((uint64_t)at.s * p.q_tokens + j_draft) * p.out_stride + ((uint64_t)head * g.group + j_row % g.group) * p.kv.head_dim;
-            bool partial = cut;
-            while (true) {
-                if (quad == 0) {
-                    tops[warp * kAttentionRows + row] = top;
-                    sums[warp * kAttentionRows + row] = sum;
-                }
-                __syncthreads();
-                float all_top = -INFINITY;
+            for (uint32_t w = 0; w < kWarps; ++w) total += sums[w * kAttentionRows + row];
+            // numbers of the row: bf16: dimensions 8 i + 2 quad, + 1; 8-bit: 16 i + 4 quad ... + 3, from the warp's first on
+            float o[S::kOwn];
+            const float unlift = FMT == 0 ? 1.f : weight_top == kNone ? 0.f : exp2_fast(weight_top - top);
 #pragma unroll
-                for (uint32_t w = 0; w < kWarps; ++w) all_top = fmaxf(all_top, tops[w * kAttentionRows + row]);
-                // (a warp without tiles, and rows that see nothing, have zeros; a row whose scores are NaNs keeps those)
-                const float factor = o_top == -INFINITY ? 0.f : exp2_fast(o_top - all_top);
-                float row_top = -INFINITY, total = 0.f;
+            for (uint32_t i = 0; i < S::kAcc; ++i)
 #pragma unroll
-                for (uint32_t w = 0; w < kWarps; ++w) row_top = fmaxf(row_top, tops[w * kAttentionRows + jr]);
+                for (int j = 0; j < 2; ++j) o[FMT == 0 ? 2 * i + j : i / 2 * 4 + 2 * j + i % 2] = (acc[i][j] + acc[i][j + 2]) * unlift;
+            constexpr uint32_t kGroup = FMT == 0 ? 2 : 4;  // numbers beside each other
+            const auto dim_of = [&](uint32_t i) { return warp * S::kWarpDims + i / kGroup * (4 * kGroup) + quad * kGroup + i % kGroup; };
+            bool write = true;
+            if (!at.whole_item()) {
+                // ---- one of an item's partial results: the last block joins them, in the order of the tiles ----
+                uint32_t owner, contributors;
+                at.contributors(share.cut, blockIdx.x, &owner, &contributors);
+                constexpr uint32_t kPart = kAttentionRows * (kMaxHeadDim + 2);  // rows, then maxima, then sums
+                float *const part = p.parts + ((uint64_t)blockIdx.x * 2 + (blockIdx.x == owner ? 1 : 0)) * kPart;
+                if (live && warp < S::kValueWarps) {
 #pragma unroll
-                for (uint32_t w = 0; w < kWarps; ++w) {
-                    const float t = tops[w * kAttentionRows + jr];
-                    total += sums[w * kAttentionRows + jr] * (t == -INFINITY ? 1.f : exp2_fast(t - row_top));
-                }
-                const float by = 1.f / total;
-#pragma unroll
-                for (uint32_t round = 0; round < HDP / kRoundDims; ++round) {
-                    float *const mine = join + (warp * kAttentionRows + row) * kRoundPitch;
-#pragma unroll
-                    for (uint32_t i = 0; i < kRoundDims / 16; ++i) {
-                        float4 v = o[round * (kRoundDims / 16) + i];
-                        v.x *= factor, v.y *= factor, v.z *= factor, v.w *= factor;
-                        if (FMT == 0 && partial == cut) {
-                            *reinterpret_cast<float2 *>(mine + i * 16 + quad * 2) = make_float2(v.x, v.y);
-                            *reinterpret_cast<float2 *>(mine + i * 16 + 8 + quad * 2) = make_float2(v.z, v.w);
-                        } else {
-                            *reinterpret_cast<float4 *>(mine + i * 16 + quad * 4) = v;
-                        }
+                    for (uint32_t i = 0; i < S::kOwn; i += kGroup) {
+                        float *const to = part + row * HDP + dim_of(i);
+                        if (FMT == 0) *reinterpret_cast<float2 *>(to) = make_float2(o[i], o[i + 1]);
+                        else *reinterpret_cast<float4 *>(to) = make_float4(o[i], o[i + 1], o[i + 2 < S::kOwn ? i + 2 : i], o[i + 3 < S::kOwn ? i + 3 : i]);
                     }
-                    __syncthreads();
-                    if (threadIdx.x < 128) {
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                        for (uint32_t w = 0; w < kWarps; ++w) {
-                            const float4 a = *reinterpret_cast<const float4 *>(join + (w * kAttentionRows + jr) * kRoundPitch + jd);
-                            v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
-                        }
-                        const uint32_t d = round * kRoundDims + jd;
-                        if (partial) {
-                            if (j_live) *reinterpret_cast<float4 *>(part + jr * HDP + d) = v;
-                            if (round == 0 && jd == 0) {
-                                part[kAttentionRows * HDP + jr] = row_top;
-                                part[kAttentionRows * (HDP + 1) + jr] = total;
-                            }
-                        } else if (j_live && d < p.kv.head_dim) {
-                            v = j_empty ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * by, v.y * by, v.z * by, v.w * by);
-                            if (p.out_is_f32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + out_row + d) = v;
-                            else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + out_row + d) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-                        }
-                    }
-                    if (round + 1 < HDP / kRoundDims) __syncthreads();
                 }
-                if (partial) __threadfence();
-                __syncthreads();
-                if (!partial) break;
+                if (warp == 0 && quad == 0) {
+                    part[kAttentionRows * HDP + row] = top == kNone ? -INFINITY : top;
+                    part[kAttentionRows * (HDP + 1) + row] = total;
+                }
+                __threadfence();
+                multipliers_sync();
                 if (threadIdx.x == 0) {
                     *arrived = atomicAdd(p.counters + owner, 1u) + 1 == contributors;
                     if (*arrived) p.counters[owner] = 0;
                     __threadfence();
                 }
-                __syncthreads();
-                if (!*arrived) break;
-                // partial results in the order of the tiles: warp w adds up those of blocks w, w + 8, ...
-                partial = false;
-                const float *const parts = p.parts + (uint64_t)owner * 2 * kPart;
-                auto part_of = [&](uint32_t i) { return parts + (i * 2 + (i == 0 ? 1 : 0)) * kPart; };
-                top = -INFINITY;
-                sum = 0.f;
+                multipliers_sync();
+                write = *arrived;
+                if (write && live && warp < S::kValueWarps) {
+                    const float *const parts = p.parts + (uint64_t)owner * 2 * kPart;
+                    float best = -INFINITY;
+                    total = 0.f;
 #pragma unroll
-                for (uint32_t i = 0; i < HDP / 16; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                for (uint32_t i = warp; i < contributors; i += kWarps) top = fmaxf(top, __ldcg(part_of(i) + kAttentionRows * HDP + row));
-                o_top = top;
-                for (uint32_t i = warp; i < contributors; i += kWarps) {
-                    const float *const from = part_of(i);
-                    const float t = __ldcg(from + kAttentionRows * HDP + row), l = __ldcg(from + kAttentionRows * (HDP + 1) + row);
-                    float4 v[HDP / 16];
-                    if (chunk * kAttentionRows + row < g.rows) {
+                    for (uint32_t i = 0; i < S::kOwn; ++i) o[i] = 0.f;
+                    for (uint32_t k0 = 0; k0 < contributors; k0 += kBatch) {
+                        float t[kBatch], l[kBatch], v[kBatch][S::kOwn];
 #pragma unroll
-                        for (uint32_t j = 0; j < HDP / 16; ++j) v[j] = __ldcg(reinterpret_cast<const float4 *>(from + row * HDP + j * 16 + quad * 4));
-                        const float f = t == -INFINITY ? 0.f : exp2_fast(t - top);
-                        sum += t == -INFINITY ? l : l * f;
+                        for (uint32_t k = 0; k < kBatch; ++k) {
+                            t[k] = -INFINITY;
+                            l[k] = 0.f;
+                            if (k0 + k < contributors) {
+                                const float *const from = parts + ((k0 + k) * 2 + (k0 + k == 0 ? 1 : 0)) * kPart;
+                                t[k] = __ldcg(from + kAttentionRows * HDP + row);
+                                l[k] = __ldcg(from + kAttentionRows * (HDP + 1) + row);
 #pragma unroll
-                        for (uint32_t j = 0; j < HDP / 16; ++j)
-                            o[j].x = fmaf(v[j].x, f, o[j].x), o[j].y = fmaf(v[j].y, f, o[j].y), o[j].z = fmaf(v[j].z, f, o[j].z), o[j].w = fmaf(v[j].w, f, o[j].w);
+                                for (uint32_t i = 0; i < S::kOwn; i += kGroup) {
+                                    const float *const at_dim = from + row * HDP + dim_of(i);
+                                    if (FMT == 0) {
+                                        const float2 a = __ldcg(reinterpret_cast<const float2 *>(at_dim));
+                                        v[k][i] = a.x, v[k][i + 1] = a.y;
+                                    } else {
+                                        const float4 a = __ldcg(reinterpret_cast<const float4 *>(at_dim));
+                                        v[k][i] = a.x, v[k][i + 1] = a.y, v[k][(i + 2) % S::kOwn] = a.z, v[k][(i + 3) % S::kOwn] = a.w;
+                                    }
+                                }
+                            } else {
+#pragma unroll
+                                for (uint32_t i = 0; i < S::kOwn; ++i) v[k][i] = 0.f;
+                            }
+                        }
+                        float next = best;
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) next = fmaxf(next, t[k]);
+                        const float keep = best == next ? 1.f : exp2_fast(best - next);
+                        best = next;
+                        total *= keep;
+#pragma unroll
+                        for (uint32_t i = 0; i < S::kOwn; ++i) o[i] *= keep;
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) {
+                            // (rows of a piece that saw nothing have zeros; rows whose scores are NaNs keep those)
+                            const float f = t[k] == -INFINITY ? 0.f : exp2_fast(t[k] - best);
+                            total += t[k] == -INFINITY ? l[k] : l[k] * f;
+#pragma unroll
+                            for (uint32_t i = 0; i < S::kOwn; ++i) o[i] = fmaf(v[k][i], f, o[i]);
+                        }
                     }
                 }
             }
-        } while (at.next([&](uint32_t i) { return length_of(p, i); }, p.kv.sequences, g.heads));
+            if (write && live && warp < S::kValueWarps) {
+                const bool none = at.length - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group) <= 0;
+                const float by = 1.f / total;
+                const uint64_t base = ((uint64_t)at.s * p.q_tokens + r / g.group) * p.out_stride + ((uint64_t)head * g.group + r % g.group) * p.kv.head_dim;
+#pragma unroll
+                for (uint32_t i = 0; i < S::kOwn; ++i) o[i] = none ? 0.f : o[i] * by;
+#pragma unroll
+                for (uint32_t i = 0; i < S::kOwn; i += kGroup) {
+                    const uint32_t d = dim_of(i);
+                    if (d >= p.kv.head_dim) continue;
+                    if (p.out_is_f32) {
+                        float *const to = static_cast<float *>(p.out) + base + d;
+                        if (FMT == 0) *reinterpret_cast<float2 *>(to) = make_float2(o[i], o[i + 1]);
+                        else *reinterpret_cast<float4 *>(to) = make_float4(o[i], o[i + 1], o[i + 2 < S::kOwn ? i + 2 : i], o[i + 3 < S::kOwn ? i + 3 : i]);
+                    } else {
+                        uint16_t *const to = static_cast<uint16_t *>(p.out) + base + d;
+                        if (FMT == 0) *reinterpret_cast<uint32_t *>(to) = pack_bf16(o[i], o[i + 1]);
+                        else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2 < S::kOwn ? i + 2 : i], o[i + 3 < S::kOwn ? i + 3 : i]));
+                    }
+                }
+            }
+            at = ahead;
+        } while (more);
     }
 
     // ---- sequences without tokens ----
@@ -820,15 +864,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 
 // ---- host ----
 
-// Rows of the cache as [page][head][token][value]; copies of 16 tokens by one segment.
+// Rows of the cache as [page][head][token][value], or [page][head][segment][token][value in it]; copies of 16 tokens by one segment, or all.
 template <int FMT, int HDP>
-bool encode_map(EncodeTiledFn encode, CUtensorMap *map, const KvView &kv, const uint8_t *pool) {
+bool encode_map(EncodeTiledFn encode, CUtensorMap *map, const KvView &kv, const uint8_t *pool, bool whole_rows) {
     using S = Shape<FMT, HDP>;
+    constexpr uint32_t kSegValues = S::kSeg / (FMT == 0 ? 2 : 1);
+    const CUtensorMapDataType type = FMT == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const CUtensorMapSwizzle swizzle = S::kSeg == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+    if (whole_rows && S::kSegs > 1) {
+        const cuuint64_t dims[5] = {kSegValues, kv.page_tokens, kv.head_dim / kSegValues, kv.kv_heads, kv.pages};
+        const cuuint64_t strides[4] = {kv.token_stride, S::kSeg, kv.head_stride, kv.page_stride};
+        const cuuint32_t box[5] = {kSegValues, kTileTokens, S::kSegs, 1, 1};
+        return encode(map, type, 5, const_cast<uint8_t *>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
     const cuuint64_t dims[4] = {kv.head_dim, kv.page_tokens, kv.kv_heads, kv.pages};
     const cuuint64_t strides[3] = {kv.token_stride, kv.head_stride, kv.page_stride};
-    const cuuint32_t box[4] = {S::kSeg / (FMT == 0 ? 2 : 1), kTileTokens, 1, 1}, step[4] = {1, 1, 1, 1};
-    return encode(map, FMT == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t *>(pool), dims, strides, box, step,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, S::kSeg == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const cuuint32_t box[4] = {kSegValues, kTileTokens, 1, 1};
+    return encode(map, type, 4, const_cast<uint8_t *>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -837,7 +891,8 @@ cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t str
     using S = Shape<FMT, HDP>;
     const EncodeTiledFn encode = encode_tiled_fn();
     CUtensorMap maps[2];
-    if (!encode || !encode_map<FMT, HDP>(encode, &maps[0], p.kv, p.kv.k) || !encode_map<FMT, HDP>(encode, &maps[1], p.kv, p.kv.v)) return cudaErrorInvalidValue;
+    const bool whole_rows = p.kv.head_dim * (FMT == 0 ? 2 : 1) % S::kSeg == 0;
+    if (!encode || !encode_map<FMT, HDP>(encode, &maps[0], p.kv, p.kv.k, whole_rows) || !encode_map<FMT, HDP>(encode, &maps[1], p.kv, p.kv.v, whole_rows)) return cudaErrorInvalidValue;
     static std::atomic<uint64_t> ready{0};  // a bit for each device: the attribute is the kernel's, once set it stays
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
@@ -854,6 +909,7 @@ cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t str
     g.chunks = (g.rows + kAttentionRows - 1) / kAttentionRows;
     g.heads = p.kv.kv_heads * g.chunks;
     g.pages = attention_pages(p.kv.page_tokens);
+    g.whole_rows = whole_rows || S::kSegs == 1;
     return launch_dependent(attention_kernel<FMT, HDP>, dim3(sm_count), kThreads, S::kShared, stream, p, g, maps[0], maps[1]);
 }
 
