@@ -6,22 +6,24 @@
 // Every key and value is read once from memory for eight query rows (token, head) that share its key head: at one byte a value that is
 // 12 to 16 operations a byte, so memory is the bound, and the kernel is built around keeping loads in flight.
 //
-//   * One block per SM: eight warps that multiply and one that asks for tiles with tensor copies into a ring in shared memory, keys of up
-//     to 128 tokens and their values in turn, past the end of an item too: 190 KB are in flight while results are written. A page has a
-//     whole number of the 16-token tiles that a copy brings.
-//   * Warp w has the scores of 16 tokens, hands their weights on through shared memory, and then adds up one eighth of the dimensions
-//     of the values for all 128 tokens: one barrier for 128 tokens, and a result lies in one warp's registers. (Warps that kept whole
-//     results of tokens of their own needed 128 registers for them and four rounds through shared memory to join them: 3 us for
-//     every item, 8 for a cut one.)
+//   * One block per SM: eight warps that multiply and one that asks for tiles with tensor copies into a ring in shared memory, keys of
+//     128 tokens (256 where rows are short) and their values in turn, past the end of an item too: 190 KB are in flight while results
+//     are written. A page has a whole number of the 16-token rows that a copy brings; copies of single segments of rows, and scales as
+//     copies of their own, were more than the copy engine takes (1100 of 4300 cycles for 128 tokens).
+//   * Warp w has the scores of an eighth of the tile's tokens, hands their weights on through shared memory, and then adds up an eighth of
+//     the dimensions of the values for all of them: one barrier for a tile, and a result lies in few registers. (Warps that kept whole
+//     results of tokens of their own needed 128 registers for them and four rounds through shared memory to join them: 3 us for every
+//     item, 8 for a cut one. Two groups of four warps that took turns at tiles were no faster on long contexts and slower on others.)
 //   * Both products run on MMAs with eight query rows: rows 0...7 of the left operand hold the upper halves of the eight rows' factors,
 //     rows 8...15 the lower halves, so that the sum of the two accumulators is a product of factors of 16 bits or more (two bf16
 //     numbers, error 2^-17; two fp16 numbers for 8-bit caches, 2^-22), at no cost: the rows would be empty.
-//   * Queries against int8 keys run on whole-number MMAs as they lie in memory, four 8-bit digits of every query; other 8-bit codes become
-//     fp16 exactly. Which dimensions an MMA multiplies is free as long as queries and keys agree, so that a lane takes whole 16-byte pieces
-//     of a key row; values are read transposed as pairs of bytes, which gives the lane a pair of dimensions, one for each of two MMAs.
+//   * int8 codes are multiplied as they lie in memory, by whole-number MMAs with four 8-bit digits of every query, and of every weight.
+//     e4m3 codes become fp16 exactly. Which dimensions (or tokens) an MMA multiplies is free as long as its operands agree, so that a
+//     lane takes whole 16-byte pieces of a key row; values are read transposed as pairs of bytes, which gives the lane a pair of
+//     dimensions, one for each of two MMAs, and a byte permutation for each brings four tokens into a register.
 //   * One pass: sums and results are relative to a power of two for each row that is raised when a score lies 8 above it, which is seldom
 //     after the first tiles. The scale of a token's values goes into its weight; weights times scales have a reference of their own, so
-//     that they stay in fp16's range whatever the scales are.
+//     that they stay in range whatever the scales are.
 //   * The work of all sequences is cut into equal shares by every block for itself (q4_attention_plan.h), from the lengths in device memory:
 //     a captured graph follows them. Results of an item cut over several blocks are joined in order by the last one.
 #include <cuda_fp8.h>
@@ -40,38 +42,44 @@ constexpr uint32_t kLeastRun = 16;              // tiles: shorter runs cost more
 constexpr uint32_t kBatch = 8;                  // partial results that are asked for at a time
 constexpr float kNone = -3.0e38f;               // a reference below all scores: the row has seen nothing
 constexpr float kHeadroom = 8.f;                // how far above its reference a score may lie, in powers of two
-// 8-bit caches: a weight times scale is brought to 2^11 when it becomes the reference and may grow to 2^15, near the end of fp16's
-// range, so that lower halves keep 16 bits of weights down to 2^-19 of the largest one (and 2^-35 of it below)
-constexpr int kWeightExponent = 11;
-constexpr float kMostWeight = 32768.f;
+// 8-bit caches: a weight times scale is brought below 2^11 (int8: 2^26) when it becomes the reference and may grow to 2^15 (2^30). As fp16
+// halves, up to the end of fp16's range, weights keep 16 bits down to 2^-19 of the largest one (and 2^-35 of it below); as whole
+// numbers they are off by half at most, 2^-26 of the largest one.
+template <int FMT>
+struct Weights {
+    static constexpr int kExponent = FMT == 1 ? 26 : 11;
+    static constexpr float kMost = FMT == 1 ? 1073741824.f : 32768.f;
+};
 constexpr unsigned long long kWaitLimitNs = 200ull * 1000 * 1000, kLateLimitNs = 1000 * 1000;
 constexpr uint32_t kSharedLimit = 227 * 1024;
 
 template <int FMT, int HDP>
 struct Shape {
     static constexpr uint32_t kRow = HDP * (FMT == 0 ? 2 : 1);       // bytes of a token's row in shared memory
-    static constexpr uint32_t kSeg = kRow < 128 ? kRow : 128;        // bytes of it that one copy brings
+    static constexpr uint32_t kSeg = kRow < 128 ? kRow : 128;        // swizzled together
     static constexpr uint32_t kSegs = kRow / kSeg;
-    static constexpr uint32_t kTile = kTileTokens * kRow;            // 16 tokens' keys or values
-    static constexpr uint32_t kSlot = kWarps * kTile;                // of the ring: keys, or values, of 128 tokens
+    static constexpr uint32_t kSub = kTileTokens * kRow;             // 16 tokens' keys or values
+    static constexpr uint32_t kOwnSubs = kRow > 128 ? 1 : 2;         // of a tile, whose scores a warp has
+    static constexpr uint32_t kSubs = kWarps * kOwnSubs;             // of a tile
+    static constexpr uint32_t kSlot = kSubs * kSub;                  // of the ring: keys, or values, of a tile
     static constexpr uint32_t kPieces = kSeg / 64;                   // 16-byte pieces of a segment a lane takes from a key row
     static constexpr uint32_t kMmas = HDP / 16;                      // per 8 tokens of scores
     static constexpr uint32_t kChunkDims = FMT == 0 ? 8 : 16;        // of a 16-byte piece
     static constexpr uint32_t kValueWarps = HDP / kChunkDims < kWarps ? HDP / kChunkDims : kWarps;  // that have dimensions of the values
     static constexpr uint32_t kWarpDims = HDP / kValueWarps;
-    static constexpr uint32_t kChunks = kWarpDims / kChunkDims;      // of a warp
+    static constexpr uint32_t kChunks = kWarpDims / kChunkDims;
     static constexpr uint32_t kAcc = kWarpDims / 8;                  // accumulators of four numbers
     static constexpr uint32_t kOwn = kWarpDims / 4;                  // numbers of a row's result in a lane
-    static constexpr bool kQueriesStay = FMT == 1 || HDP < 256;      // in registers
+    static constexpr bool kQueriesStay = HDP < 256;      // in registers
     // shared memory: ring, scales of its keys and values, weights, queries, barriers, small arrays
-    static constexpr uint32_t kScales = FMT == 0 ? 0 : 2 * kWarps * 64;  // of a slot
+    static constexpr uint32_t kScales = FMT == 0 ? 0 : 2 * kSubs * 64;  // of a slot
     static constexpr uint32_t kQueries = kMmas * 32 * 16;
-    static constexpr uint32_t kWeights = 2 * kWarps * 32 * 16;
+    static constexpr uint32_t kWeights = kSubs * 32 * 16;               // of a tile; there are two
     static constexpr uint32_t kSmall = 2048;
-    static constexpr uint32_t kFit = (kSharedLimit - 1024 - kQueries - kWeights - kSmall) / (kSlot + kScales + 16);
+    static constexpr uint32_t kFit = (kSharedLimit - 1024 - kQueries - 2 * kWeights - kSmall) / (kSlot + kScales + 16);
     static constexpr uint32_t kSlots = (kFit < 16 ? kFit : 16) & (FMT == 0 ? ~0u : ~1u);  // 8-bit: keys in even ones
-    static constexpr uint32_t kShared = 1024 + kSlots * (kSlot + kScales + 16) + kQueries + kWeights + kSmall;
-    static_assert(kSlots >= 2 && kWarps * kSegs <= 32, "");
+    static constexpr uint32_t kShared = 1024 + kSlots * (kSlot + kScales + 16) + kQueries + 2 * kWeights + kSmall;
+    static_assert(kSlots >= 2 && kSubs * kSegs <= 32, "");
 };
 
 // ---- small pieces ----
@@ -131,11 +139,24 @@ __device__ __forceinline__ void split_digits(const float (&q)[8], uint4 &upper, 
     lower = make_uint4(word[1][0], word[0][0], word[1][1], word[0][1]);
 }
 
-// Bytes 0 and 2, and bytes 1 and 3, of a word of int8 codes as fp16: 0x6400 | u is 1024 + u, with u = code + 128.
-__device__ __forceinline__ uint32_t int8_even(uint32_t w) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((w & 0x00ff00ffu) ^ 0x64806480u), "r"(0x64806480u));
-    return r;
+// A number from the sums of products with its factor's four digits. Sums of up to 256 products of 8-bit numbers are at most 2^22, which
+// small_int_to_float takes; the conversion unit (8 cycles an instruction) would be busy for a fifth of the time.
+__device__ __forceinline__ float of_digits(int d3, int d2, int d1, int d0) {
+    return fmaf(fmaf(small_int_to_float(d3), 256.f, small_int_to_float(d2)), 65536.f, fmaf(small_int_to_float(d1), 256.f, small_int_to_float(d0)));
+}
+
+// The four signed digits of four whole numbers 0 ... 2^30, a word for each digit from the highest on. With 128 added to its lower three
+// digits, a number's bytes are its digits, each but the highest plus 128.
+__device__ __forceinline__ void weight_digits(const float (&w)[4], uint32_t (&digit)[4]) {
+    uint32_t n[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = (uint32_t)__float2int_rn(w[i]) + 0x00808080u;
+    const uint32_t low01 = __byte_perm(n[0], n[1], 0x5140), low23 = __byte_perm(n[2], n[3], 0x5140);    // bytes 0, 0, 1, 1
+    const uint32_t high01 = __byte_perm(n[0], n[1], 0x7362), high23 = __byte_perm(n[2], n[3], 0x7362);  // bytes 2, 2, 3, 3
+    digit[3] = __byte_perm(low01, low23, 0x5410) ^ 0x80808080u;
+    digit[2] = __byte_perm(low01, low23, 0x7632) ^ 0x80808080u;
+    digit[1] = __byte_perm(high01, high23, 0x5410) ^ 0x80808080u;
+    digit[0] = __byte_perm(high01, high23, 0x7632);
 }
 __device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {  // the lower two bytes
     uint32_t r;
@@ -343,13 +364,13 @@ __device__ __forceinline__ void ask_for_tiles(const AttentionParams &p, const Ge
         const int32_t *const table = p.kv.table + (uint64_t)at.s * p.kv.row_stride;
         uint32_t entry = g.pages.page_of(at.begin + mine);
         uint32_t page = at.begin + mine < at.end ? (uint32_t)__ldcg(table + entry) : 0u;
-        for (uint32_t tile = at.begin; tile < at.end; tile += kWarps) {
-            const uint32_t count = min(at.end - tile, kWarps);
+        for (uint32_t tile = at.begin; tile < at.end; tile += S::kSubs) {
+            const uint32_t count = min(at.end - tile, S::kSubs);
             const bool wanted = mine < count, there = page < p.kv.pages;
             // (a page outside the cache is outside the tensor map too: such copies bring zeros)
             const uint32_t now = there ? page : p.kv.pages, place = (tile + mine - entry * g.pages.per) * kTileTokens;
             if (wanted && !there) *p.kv.input_error = 1;
-            const uint32_t next = tile + kWarps + mine;
+            const uint32_t next = tile + S::kSubs + mine;
             if (next < at.end) {
                 entry = g.pages.page_of(next);
                 page = (uint32_t)__ldcg(table + entry);
@@ -358,20 +379,23 @@ __device__ __forceinline__ void ask_for_tiles(const AttentionParams &p, const Ge
             for (uint32_t values = 0; values < 2; ++values) {
                 mbar_wait(empty + turn.slot * 8, turn.phase ^ 1u, limit_ns, p.error_flag);
                 const uint32_t bar = full + turn.slot * 8, dst = ring + turn.slot * S::kSlot;
-                if (lane == 0) mbar_expect(bar, count * S::kTile);
+                if (lane == 0) mbar_expect(bar, count * S::kSub);
                 __syncwarp();
                 if (wanted) {
-                    if (S::kSegs > 1 && g.whole_rows) copy_whole_tile(dst + lane * S::kTile, values ? v_map : k_map, bar, (int)place, (int)head, (int)now);
+                    if (S::kSegs > 1 && g.whole_rows) copy_whole_tile(dst + lane * S::kSub, values ? v_map : k_map, bar, (int)place, (int)head, (int)now);
                     else copy_tile(dst + lane * (kTileTokens * S::kSeg), values ? v_map : k_map, bar, (int)(seg * S::kSeg / (FMT == 0 ? 2 : 1)), (int)place, (int)head, (int)now);
                 }
                 if (FMT != 0 && values == 0) {
-                    // lane 4 i + j: 16-byte piece j of tile i's scales, of keys and of values
-                    const uint32_t of = lane / 4, of_page = __shfl_sync(0xffffffffu, now, of * per), of_place = __shfl_sync(0xffffffffu, place, of * per);
-                    const bool here = of < count && of_page < p.kv.pages;
-                    const uint64_t from = here ? ((uint64_t)of_page * p.kv.kv_heads + head) * p.kv.page_tokens + of_place + lane % 4 * 4 : 0;
-                    const uint32_t sc = scales + turn.slot * S::kScales + lane * 16;
-                    copy_16_or_zeros(sc, p.kv.k_scales + from, here);
-                    copy_16_or_zeros(sc + kWarps * 64, p.kv.v_scales + from, here);
+                    // lane 4 i + j: 16-byte piece j of the scales of 16 tokens, of keys and of values
+#pragma unroll
+                    for (uint32_t of = lane / 4; of < S::kSubs; of += 8) {
+                        const uint32_t of_page = __shfl_sync(0xffffffffu, now, of * per), of_place = __shfl_sync(0xffffffffu, place, of * per);
+                        const bool here = of < count && of_page < p.kv.pages;
+                        const uint64_t from = here ? ((uint64_t)of_page * p.kv.kv_heads + head) * p.kv.page_tokens + of_place + lane % 4 * 4 : 0;
+                        const uint32_t sc = scales + turn.slot * S::kScales + of * 64 + lane % 4 * 16;
+                        copy_16_or_zeros(sc, p.kv.k_scales + from, here);
+                        copy_16_or_zeros(sc + S::kSubs * 64, p.kv.v_scales + from, here);
+                    }
                     copies_arrive(bar);
                 }
                 turn.next();
@@ -389,8 +413,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     using S = Shape<FMT, HDP>;
     extern __shared__ uint8_t shared_raw[];
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(shared_raw), pad = (1024u - (raw & 1023u)) & 1023u;
-    const uint32_t ring = raw + pad, scales = ring + S::kSlots * S::kSlot, weights = scales + S::kSlots * S::kScales, queries = weights + S::kWeights, full = queries + S::kQueries,
-                   empty = full + S::kSlots * 8;
+    const uint32_t ring = raw + pad, scales = ring + S::kSlots * S::kSlot, weights = scales + S::kSlots * S::kScales, queries = weights + 2 * S::kWeights,
+                   full = queries + S::kQueries, empty = full + S::kSlots * 8;
     float *const small = reinterpret_cast<float *>(shared_raw + (empty + S::kSlots * 8 - raw));
     float *const highs = small, *const weight_highs = small + kWarps * kAttentionRows, *const sums = small + 2 * kWarps * kAttentionRows;  // [warp][row]
     float *const row_scales = small + 3 * kWarps * kAttentionRows;                                                                         // [row] scale of the scores, in powers of two
@@ -415,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     } else if (share.any) {
         Turn<S::kSlots> turn;
         unsigned long long limit_ns = kWaitLimitNs;
-        uint32_t weights_at = weights;  // one of two buffers
+        uint32_t weights_at = weights;  // one of two
         Cursor at = share.at;
         // eight values of query row `warp` of an item
         float q[8];
@@ -440,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         load_query(at);
         bool more;
         do {
-            // ---- queries of the item: warp w splits row w into halves, in the order in which key rows are read ----
+            // ---- queries of the item: warp w splits row w into halves, or digits, in the order in which key rows are read ----
             const uint32_t head = at.item / g.chunks, chunk = at.item % g.chunks;
             {
                 const uint32_t d = lane * 8;
@@ -497,22 +521,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             const uint32_t r = chunk * kAttentionRows + row;
             const bool live = r < g.rows;
             const int32_t limit = live ? min(at.length - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group), end_token) : 0;
-            float acc[S::kAcc][4];
+            // Results. int8: o itself, from whole-number accumulators of a tile; else accumulators of the upper and lower halves
+            float o[FMT == 1 ? S::kOwn : 1], acc[FMT == 1 ? 1 : S::kAcc][4];
 #pragma unroll
-            for (uint32_t i = 0; i < S::kAcc; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+            for (uint32_t i = 0; i < (FMT == 1 ? S::kOwn : 1); ++i) o[i] = 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < (FMT == 1 ? 1 : S::kAcc); ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
             float top = kNone, sum = 0.f;                      // reference of the row's scores; sum of this lane's weights
             float weight_top = kNone, lift = 0.f, most = 0.f;  // 8-bit: reference of weights times scales, 2^(top - weight_top), and what they may be
 
-            for (uint32_t tile = at.begin; tile < at.end; tile += kWarps) {
-                const uint32_t count = min(at.end - tile, kWarps);  // tiles of 16 tokens; this warp's scores are those of tile + warp
+            for (uint32_t tile = at.begin; tile < at.end; tile += S::kSubs) {
+                const uint32_t count = min(at.end - tile, S::kSubs);  // of 16 tokens; this warp's scores are those of warp * kOwnSubs and on
                 // ---- scores ----
                 mbar_wait(full + turn.slot * 8, turn.phase, limit_ns, p.error_flag);
-                float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // tokens 2 quad, + 1, + 8, + 9, row `row`
-                float value_scale[4] = {0.f, 0.f, 0.f, 0.f};
-                if (warp < count) {
-                    const uint32_t keys = ring + turn.slot * S::kSlot + warp * S::kTile;
-                    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-                    int upper[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, lower[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};  // int8: products with digits 3 and 2, and with 1 and 0
+                float x[4 * S::kOwnSubs];  // tokens 2 quad, + 1, + 8, + 9 of each 16, row `row`
+                float value_scale[4 * S::kOwnSubs];
+#pragma unroll
+                for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) x[i] = -INFINITY, value_scale[i] = 0.f;
+                if (warp * S::kOwnSubs < count) {
+                    // (the last warp may multiply 16 tokens that are not there; they are left out below)
+                    const uint32_t keys = ring + turn.slot * S::kSlot + warp * S::kOwnSubs * S::kSub;
+                    float s[2 * S::kOwnSubs][4];
+                    int upper[2 * S::kOwnSubs][4], lower[2 * S::kOwnSubs][4];  // int8: products with digits 3 and 2, and with 1 and 0
+#pragma unroll
+                    for (uint32_t n = 0; n < 2 * S::kOwnSubs; ++n) {
+                        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+                        upper[n][0] = upper[n][1] = upper[n][2] = upper[n][3] = lower[n][0] = lower[n][1] = lower[n][2] = lower[n][3] = 0;
+                    }
 #pragma unroll
                     for (uint32_t seg = 0; seg < S::kSegs; ++seg)
 #pragma unroll
@@ -525,8 +560,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll
                                 for (uint32_t i = 0; i < kPer; ++i) fetch_query(m + i);
 #pragma unroll
-                            for (uint32_t n = 0; n < 2; ++n) {
-                                const uint4 w = lds_v4(from + n * 8 * S::kSeg);
+                            for (uint32_t n = 0; n < 2 * S::kOwnSubs; ++n) {
+                                const uint4 w = lds_v4(from + n / 2 * S::kSub + n % 2 * 8 * S::kSeg);
                                 const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                                 for (uint32_t i = 0; i < kPer; ++i) {
@@ -536,29 +571,27 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                                 }
                             }
                         }
-                    const uint32_t sc = scales + turn.slot * S::kScales + warp * 64 + quad * 8;
+                    const uint32_t sc = scales + turn.slot * S::kScales + warp * S::kOwnSubs * 64 + quad * 8;
 #pragma unroll
-                    for (uint32_t n = 0; n < 2; ++n) {
+                    for (uint32_t n = 0; n < 2 * S::kOwnSubs; ++n) {
                         if (FMT == 1) {
-                            // a sum of 256 products is at most 2^22, so two digits' sums fit 32 bits
 #pragma unroll
-                            for (int j = 0; j < 2; ++j)
-                                x[2 * n + j] = fmaf((float)(upper[n][j] * 256 + upper[n][j + 2]), 65536.f, (float)(lower[n][j] * 256 + lower[n][j + 2])) * row_scale;
+                            for (int j = 0; j < 2; ++j) x[2 * n + j] = of_digits(upper[n][j], upper[n][j + 2], lower[n][j], lower[n][j + 2]) * row_scale;
                         } else {
                             x[2 * n] = (s[n][0] + s[n][2]) * row_scale;
                             x[2 * n + 1] = (s[n][1] + s[n][3]) * row_scale;
                         }
                         if (FMT != 0) {
-                            const uint2 k = lds_v2(sc + n * 32), v = lds_v2(sc + kWarps * 64 + n * 32);
+                            const uint2 k = lds_v2(sc + n * 32), v = lds_v2(sc + S::kSubs * 64 + n * 32);
                             x[2 * n] *= __uint_as_float(k.x), x[2 * n + 1] *= __uint_as_float(k.y);
                             value_scale[2 * n] = __uint_as_float(v.x), value_scale[2 * n + 1] = __uint_as_float(v.y);
                         }
                     }
-                    const int32_t token = (int32_t)((tile + warp) * kTileTokens);
-                    if (token + (int32_t)kTileTokens > sure)  // some rows do not see all of it
+                    const int32_t token = (int32_t)((tile + warp * S::kOwnSubs) * kTileTokens);
+                    if (token + (int32_t)(S::kOwnSubs * kTileTokens) > sure)  // some rows do not see all of it
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (token + (int32_t)quad * 2 + i % 2 + i / 2 * 8 >= limit) {
+                        for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i)
+                            if (token + (int32_t)(quad * 2 + i % 2 + i / 2 * 8) >= limit) {
                                 x[i] = -INFINITY;
                                 value_scale[i] = 0.f;  // (it may be anything)
                             }
@@ -567,33 +600,53 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 if (lane == 0) mbar_arrive(empty + turn.slot * 8);
                 turn.next();
                 // ---- weights ----
-                float high = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), weight[4], weight_high = 0.f;
+                float high = x[0], weight[4 * S::kOwnSubs], weight_high = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (uint32_t i = 1; i < 4 * S::kOwnSubs; ++i) high = fmaxf(high, x[i]);
+#pragma unroll
+                for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) {
                     weight[i] = exp2_fast(x[i] - top);
                     if (FMT != 0) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
                 }
-                uint32_t pa[4];
                 float of_tile;
                 const auto pass_on = [&]() {
-                    float w[4];
                     of_tile = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = FMT == 0 ? weight[i] : weight[i] * (value_scale[i] * lift);
-                    split<FMT>(w[0], w[1], pa[0], pa[1]);
-                    split<FMT>(w[2], w[3], pa[2], pa[3]);
-                    if (FMT == 0) {
-                        // bf16: the weights as they are multiplied, so that they add up to one whatever the halves cut off
+                    for (uint32_t t = 0; t < S::kOwnSubs; ++t) {
+                        const uint32_t sub = warp * S::kOwnSubs + t;
+                        float w[4];
 #pragma unroll
-                        for (int j = 0; j < 4; j += 2)
-                            of_tile += (__uint_as_float(pa[j] << 16) + __uint_as_float(pa[j + 1] << 16)) + (__uint_as_float(pa[j] & 0xffff0000u) + __uint_as_float(pa[j + 1] & 0xffff0000u));
-                    } else {
-                        of_tile = (weight[0] + weight[1]) + (weight[2] + weight[3]);
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            w[i] = FMT == 0 ? weight[4 * t + i] : weight[4 * t + i] * (value_scale[4 * t + i] * lift);
+                            if (FMT != 0) of_tile += weight[4 * t + i];
+                        }
+                        uint32_t a[4];
+                        if (FMT == 1) {
+                            // of two 16s, one MMA's left operand: digits 3 and 2 of the first, of the second; another one's: digits 1 and 0.
+                            // What is no number spoils the sum of the weights, and with it the row.
+                            weight_digits(w, a);
+                            const uint32_t to = weights_at + sub / 2 * 1024 + lane * 16 + sub % 2 * 8;
+                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(a[0]), "r"(a[1]) : "memory");
+                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + 512), "r"(a[2]), "r"(a[3]) : "memory");
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; ++i)
+                                if (!(w[i] <= Weights<1>::kMost)) of_tile = __uint_as_float(0x7fc00000u);
+                        } else {
+                            split<FMT>(w[0], w[1], a[0], a[1]);
+                            split<FMT>(w[2], w[3], a[2], a[3]);
+                            if (FMT == 0) {
+                                // bf16: the weights as they are multiplied, so that they add up to one whatever the halves cut off
+#pragma unroll
+                                for (int j = 0; j < 4; j += 2)
+                                    of_tile += (__uint_as_float(a[j] << 16) + __uint_as_float(a[j + 1] << 16)) + (__uint_as_float(a[j] & 0xffff0000u) + __uint_as_float(a[j + 1] & 0xffff0000u));
+                            }
+                            sts_v4(weights_at + (sub * 32 + lane) * 16, make_uint4(a[0], a[1], a[2], a[3]));
+                        }
                     }
-                    sts_v4(weights_at + (warp * 32 + lane) * 16, make_uint4(pa[0], pa[1], pa[2], pa[3]));
                 };
-                pass_on();
-                if (multipliers_any(high - top > kHeadroom || (FMT != 0 && weight_high > most))) {
+                const bool rise = high - top > kHeadroom || (FMT != 0 && weight_high > most);
+                if (!__any_sync(0xffffffffu, rise)) pass_on();
+                if (multipliers_any(rise)) {
                     // a reference is raised, in all warps alike
                     high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
                     high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
@@ -610,16 +663,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         top = high;
                         if (FMT != 0) {
                             lift = weight_top == kNone ? 0.f : exp2_fast(top - weight_top);
-                            most = lift > 0.f ? kMostWeight / lift : 0.f;
+                            most = lift > 0.f ? Weights<FMT>::kMost / lift : 0.f;
                             keep = 1.f;
                         }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) weight[i] = exp2_fast(x[i] - top);
+                        for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) weight[i] = exp2_fast(x[i] - top);
                     }
                     if (FMT != 0) {
                         weight_high = 0.f;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
+                        for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
                         weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 1));
                         weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 2));
                         if (quad == 0) weight_highs[warp * kAttentionRows + row] = weight_high;
@@ -629,123 +682,179 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         for (uint32_t w = 0; w < kWarps; ++w) weight_high = fmaxf(weight_high, weight_highs[w * kAttentionRows + row]);
                         if (weight_high > most) {
                             const int e = (int)(__float_as_uint(weight_high) >> 23) - 126;  // weight_high < 2^e
-                            const float next = top + (float)max(e - kWeightExponent, -126);
+                            const float next = top + (float)max(e - Weights<FMT>::kExponent, -100);
                             keep = weight_top == kNone ? 0.f : exp2_fast(weight_top - next);
                             weight_top = next;
                             lift = exp2_fast(top - weight_top);
-                            most = kMostWeight / lift;
+                            most = Weights<FMT>::kMost / lift;
                         }
                     }
 #pragma unroll
-                    for (uint32_t i = 0; i < S::kAcc; ++i)
+                    for (uint32_t i = 0; i < (FMT == 1 ? S::kOwn : 1); ++i) o[i] *= keep;
+#pragma unroll
+                    for (uint32_t i = 0; i < (FMT == 1 ? 1 : S::kAcc); ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) acc[i][j] *= keep;
                     pass_on();
                     multipliers_sync();
                 }
                 sum += of_tile;
-                // ---- values: this warp's dimensions, all tokens ----
+                // ---- values: this warp's dimensions, all tokens of the tile ----
                 mbar_wait(full + turn.slot * 8, turn.phase, limit_ns, p.error_flag);
                 if (warp < S::kValueWarps) {
                     const uint32_t held = ring + turn.slot * S::kSlot;
                     const uint32_t matrix = lane >> 3, line = (lane & 7u) + (matrix & 1u) * 8, swap = S::kSeg == 128 ? line & 7u : line >> 1 & 3u;
-                    uint32_t from[(S::kChunks + 1) / 2];  // in a tile, for each pair of chunks
+                    constexpr uint32_t kPairs = (S::kChunks + 1) / 2;
+                    uint32_t from[kPairs];  // in 16 tokens, for each pair of chunks
 #pragma unroll
-                    for (uint32_t c = 0; c < (S::kChunks + 1) / 2; ++c) {
+                    for (uint32_t c = 0; c < kPairs; ++c) {
                         const uint32_t piece = warp * S::kChunks + 2 * c + (S::kChunks > 1 ? matrix >> 1 : 0u), seg = piece / (S::kSeg / 16);
                         from[c] = held + seg * (kTileTokens * S::kSeg) + line * S::kSeg + ((piece % (S::kSeg / 16) ^ swap) << 4);
                     }
-                    const auto add_tile = [&](uint32_t t, bool edge) {
-                        const uint4 w = lds_v4(weights_at + (t * 32 + lane) * 16);
-                        const uint32_t wa[4] = {w.x, w.y, w.z, w.w};
-                        uint32_t v[(S::kChunks + 1) / 2][4];
+                    const auto fetch = [&](uint32_t (&v)[kPairs][4], uint32_t t) {
 #pragma unroll
-                        for (uint32_t c = 0; c < (S::kChunks + 1) / 2; ++c) {
-                            if (S::kChunks > 1) ldmatrix_x4_trans(v[c], from[c] + t * S::kTile);
-                            else ldmatrix_x2_trans(v[c], from[c] + t * S::kTile);
-                        }
-                        const int32_t first = (int32_t)((tile + t) * kTileTokens);
-                        if (edge) {
-                            // Rows behind the sequence's end hold anything: zeros are taken for them. Among draft tokens a value that is not
-                            // finite may be seen by some rows only, and a weight of zero does not take it out of a sum: it is taken out
-                            // here and added to the rows that see it.
-                            bool odd = false;
-#pragma unroll
-                            for (uint32_t c = 0; c < (S::kChunks + 1) / 2; ++c)
-#pragma unroll
-                                for (uint32_t i = 0; i < (S::kChunks > 1 ? 4 : 2); ++i) {
-                                    const int32_t k = first + (int32_t)(quad * 2 + i % 2 * 8);
-                                    v[c][i] &= (k < existing ? 0xffffu : 0u) | (k + 1 < existing ? 0xffff0000u : 0u);
-                                    if (FMT != 1 && p.q_tokens > 1)
-#pragma unroll
-                                        for (int b = 0; b < 4; b += FMT == 0 ? 2 : 1)
-                                            if (not_finite<FMT>(v[c][i], b)) {
-                                                odd = true;
-                                                v[c][i] &= ~((FMT == 0 ? 0xffffu : 0xffu) << (b * 8));
-                                            }
-                                }
-                            if (FMT != 1 && __any_sync(0xffffffffu, odd)) {
-#pragma unroll
-                                for (uint32_t i = 0; i < S::kAcc; ++i)
-#pragma unroll
-                                    for (uint32_t j = 0; j < 2; ++j) {
-                                        const uint32_t d = warp * S::kWarpDims + (FMT == 0 ? i * 8 + quad * 2 + j : i / 2 * 16 + quad * 4 + j * 2 + (i & 1u));
-                                        const uint32_t byte = d * (FMT == 0 ? 2 : 1), seg = byte / S::kSeg, piece = byte % S::kSeg / 16;
-                                        for (int32_t k = 0; k < (int32_t)kTileTokens && first + k < limit; ++k) {
-                                            const uint32_t turned = S::kSeg == 128 ? (uint32_t)k & 7u : (uint32_t)k >> 1 & 3u;
-                                            const uint32_t e = lds_u32((held + t * S::kTile + seg * (kTileTokens * S::kSeg) + (uint32_t)k * S::kSeg + ((piece ^ turned) << 4) + byte % 16) & ~3u);
-                                            if (not_finite<FMT>(e, byte & 3u)) acc[i][j] += FMT == 0 ? __uint_as_float((e >> ((byte & 3u) * 8)) << 16) : __uint_as_float(0x7fc00000u);
-                                        }
-                                    }
-                                __syncwarp();
-                            }
-                        }
-#pragma unroll
-                        for (uint32_t c = 0; c < S::kChunks; ++c) {
-                            const uint32_t b0 = v[c / 2][c % 2 * 2], b1 = v[c / 2][c % 2 * 2 + 1];
-                            if (FMT == 0) {
-                                mma<FMT>(acc[c], wa, b0, b1);
-                            } else if (FMT == 1) {
-                                mma<FMT>(acc[2 * c], wa, int8_even(b0), int8_even(b1));
-                                mma<FMT>(acc[2 * c + 1], wa, int8_even(b0 >> 8), int8_even(b1 >> 8));
-                            } else {
-                                mma<FMT>(acc[2 * c], wa, e4m3_pair(__byte_perm(b0, 0, 0x4420)), e4m3_pair(__byte_perm(b1, 0, 0x4420)));
-                                mma<FMT>(acc[2 * c + 1], wa, e4m3_pair(__byte_perm(b0, 0, 0x4431)), e4m3_pair(__byte_perm(b1, 0, 0x4431)));
-                            }
+                        for (uint32_t c = 0; c < kPairs; ++c) {
+                            if (S::kChunks > 1) ldmatrix_x4_trans(v[c], from[c] + t * S::kSub);
+                            else ldmatrix_x2_trans(v[c], from[c] + t * S::kSub);
                         }
                     };
-                    const uint32_t plain = (uint32_t)max(min(sure - (int32_t)(tile * kTileTokens), (int32_t)(count * kTileTokens)), 0) / kTileTokens;  // tiles that all rows see
-                    if (plain == kWarps) {
+                    if constexpr (FMT == 1) {
+                        // 32 tokens to an MMA; those without a weight count as nothing whatever their codes are
+                        int upper[S::kAcc][4], lower[S::kAcc][4];
 #pragma unroll
-                        for (uint32_t t = 0; t < kWarps; ++t) add_tile(t, false);
-                    } else {
+                        for (uint32_t i = 0; i < S::kAcc; ++i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) upper[i][j] = lower[i][j] = 0;
+                        const auto add_pair = [&](uint32_t t) {
+                            const uint4 a = lds_v4(weights_at + (t * 64 + lane) * 16), b = lds_v4(weights_at + (t * 64 + 32 + lane) * 16);
+                            uint32_t v[kPairs][4], w[kPairs][4];
+                            fetch(v, 2 * t);
+                            fetch(w, 2 * t + 1);
+#pragma unroll
+                            for (uint32_t c = 0; c < S::kChunks; ++c) {
+                                const uint32_t v0 = v[c / 2][c % 2 * 2], v1 = v[c / 2][c % 2 * 2 + 1], w0 = w[c / 2][c % 2 * 2], w1 = w[c / 2][c % 2 * 2 + 1];
+#pragma unroll
+                                for (uint32_t i = 0; i < 2; ++i) {
+                                    const uint32_t pick = i == 0 ? 0x6420 : 0x7531, b0 = __byte_perm(v0, v1, pick), b1 = __byte_perm(w0, w1, pick);
+                                    mma_s8s8_16832(upper[2 * c + i], a.x, a.y, a.z, a.w, b0, b1);
+                                    mma_s8s8_16832(lower[2 * c + i], b.x, b.y, b.z, b.w, b0, b1);
+                                }
+                            }
+                        };
+                        if (count == S::kSubs) {
+#pragma unroll
+                            for (uint32_t t = 0; t < S::kSubs / 2; ++t) add_pair(t);
+                        } else {
 #pragma unroll 1
-                        for (uint32_t t = 0; t < count; ++t) add_tile(t, t >= plain);
+                            for (uint32_t t = 0; 2 * t < count; ++t) add_pair(t);
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < S::kOwn; ++i) {
+                            const uint32_t m = i / 4 * 2 + i % 2, j = i / 2 % 2;  // dimensions 4 quad ... + 3 of each 16: even, odd, even, odd
+                            o[i] += of_digits(upper[m][j], upper[m][j + 2], lower[m][j], lower[m][j + 2]);
+                        }
+                    } else {
+                        const auto add_sub = [&](uint32_t t, bool edge) {
+                            const uint4 w = lds_v4(weights_at + (t * 32 + lane) * 16);
+                            const uint32_t wa[4] = {w.x, w.y, w.z, w.w};
+                            uint32_t v[kPairs][4];
+                            fetch(v, t);
+                            const int32_t first = (int32_t)((tile + t) * kTileTokens);
+                            if (edge) {
+                                // Rows behind the sequence's end hold anything: zeros are taken for them. Among draft tokens a value that is not
+                                // finite may be seen by some rows only, and a weight of zero does not take it out of a sum: it is taken out
+                                // here and added to the rows that see it.
+                                bool odd = false;
+#pragma unroll
+                                for (uint32_t c = 0; c < kPairs; ++c)
+#pragma unroll
+                                    for (uint32_t i = 0; i < (S::kChunks > 1 ? 4 : 2); ++i) {
+                                        const int32_t k = first + (int32_t)(quad * 2 + i % 2 * 8);
+                                        v[c][i] &= (k < existing ? 0xffffu : 0u) | (k + 1 < existing ? 0xffff0000u : 0u);
+                                        if (p.q_tokens > 1)
+#pragma unroll
+                                            for (int b = 0; b < 4; b += FMT == 0 ? 2 : 1)
+                                                if (not_finite<FMT>(v[c][i], b)) {
+                                                    odd = true;
+                                                    v[c][i] &= ~((FMT == 0 ? 0xffffu : 0xffu) << (b * 8));
+                                                }
+                                    }
+                                if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+                                    for (uint32_t i = 0; i < S::kAcc; ++i)
+#pragma unroll
+                                        for (uint32_t j = 0; j < 2; ++j) {
+                                            const uint32_t d = warp * S::kWarpDims + (FMT == 0 ? i * 8 + quad * 2 + j : i / 2 * 16 + quad * 4 + j * 2 + (i & 1u));
+                                            const uint32_t byte = d * (FMT == 0 ? 2 : 1), seg = byte / S::kSeg, piece = byte % S::kSeg / 16;
+                                            for (int32_t k = 0; k < (int32_t)kTileTokens && first + k < limit; ++k) {
+                                                const uint32_t turned = S::kSeg == 128 ? (uint32_t)k & 7u : (uint32_t)k >> 1 & 3u;
+                                                const uint32_t e = lds_u32((held + t * S::kSub + seg * (kTileTokens * S::kSeg) + (uint32_t)k * S::kSeg + ((piece ^ turned) << 4) + byte % 16) & ~3u);
+                                                if (not_finite<FMT>(e, byte & 3u)) acc[i][j] += FMT == 0 ? __uint_as_float((e >> ((byte & 3u) * 8)) << 16) : __uint_as_float(0x7fc00000u);
+                                            }
+                                        }
+                                    __syncwarp();
+                                }
+                            }
+#pragma unroll
+                            for (uint32_t c = 0; c < S::kChunks; ++c) {
+                                const uint32_t b0 = v[c / 2][c % 2 * 2], b1 = v[c / 2][c % 2 * 2 + 1];
+                                if (FMT == 0) {
+                                    mma<FMT>(acc[c], wa, b0, b1);
+                                } else {
+                                    mma<FMT>(acc[2 * c], wa, e4m3_pair(__byte_perm(b0, 0, 0x4420)), e4m3_pair(__byte_perm(b1, 0, 0x4420)));
+                                    mma<FMT>(acc[2 * c + 1], wa, e4m3_pair(__byte_perm(b0, 0, 0x4431)), e4m3_pair(__byte_perm(b1, 0, 0x4431)));
+                                }
+                            }
+                        };
+                        const uint32_t plain = (uint32_t)max(min(sure - (int32_t)(tile * kTileTokens), (int32_t)(count * kTileTokens)), 0) / kTileTokens;  // 16s that all rows see
+                        if (plain == S::kSubs) {
+#pragma unroll
+                            for (uint32_t t = 0; t < S::kSubs; ++t) add_sub(t, false);
+                        } else {
+#pragma unroll 1
+                            for (uint32_t t = 0; t < count; ++t) add_sub(t, t >= plain);
+                        }
                     }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty + turn.slot * 8);
                 turn.next();
-                weights_at = weights_at == weights ? weights + S::kWeights / 2 : weights;
+                weights_at = weights_at == weights ? weights + S::kWeights : weights;
             }
 
             // ---- the segment's result ----
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             if (quad == 0) sums[warp * kAttentionRows + row] = sum;
+            // numbers of the row: bf16: dimensions 8 i + 2 quad, + 1; 8-bit: 16 i + 4 quad ... + 3, from the warp's first on
+            const bool holds = live && warp < S::kValueWarps;
+            float mine[S::kOwn];
+            {
+                const float unlift = FMT == 0 ? 1.f : weight_top == kNone ? 0.f : exp2_fast(weight_top - top);
+#pragma unroll
+                for (uint32_t i = 0; i < S::kOwn; ++i) {
+                    if constexpr (FMT == 1) {
+                        mine[i] = o[i] * unlift;
+                    } else {
+                        const uint32_t m = FMT == 0 ? i / 2 : i / 4 * 2 + i % 2, j = FMT == 0 ? i % 2 : i / 2 % 2;
+                        mine[i] = (acc[m][j] + acc[m][j + 2]) * unlift;
+                    }
+                }
+            }
+            if (top == kNone) top = -INFINITY;
+            constexpr uint32_t kBeside = FMT == 0 ? 2 : 4;  // numbers beside each other
+            const auto dim_of = [&](uint32_t i) { return warp * S::kWarpDims + i / kBeside * (4 * kBeside) + quad * kBeside + i % kBeside; };
+            const auto put = [&](float *row_at, const float (&v)[S::kOwn]) {
+#pragma unroll
+                for (uint32_t i = 0; i < S::kOwn; i += kBeside) {
+                    if (FMT == 0) *reinterpret_cast<float2 *>(row_at + dim_of(i)) = make_float2(v[i], v[i + 1]);
+                    else *reinterpret_cast<float4 *>(row_at + dim_of(i)) = make_float4(v[i], v[i + 1], v[(i + 2) % S::kOwn], v[(i + 3) % S::kOwn]);
+                }
+            };
             multipliers_sync();
             float total = 0.f;
 #pragma unroll
             for (uint32_t w = 0; w < kWarps; ++w) total += sums[w * kAttentionRows + row];
-            // numbers of the row: bf16: dimensions 8 i + 2 quad, + 1; 8-bit: 16 i + 4 quad ... + 3, from the warp's first on
-            float o[S::kOwn];
-            const float unlift = FMT == 0 ? 1.f : weight_top == kNone ? 0.f : exp2_fast(weight_top - top);
-#pragma unroll
-            for (uint32_t i = 0; i < S::kAcc; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) o[FMT == 0 ? 2 * i + j : i / 2 * 4 + 2 * j + i % 2] = (acc[i][j] + acc[i][j + 2]) * unlift;
-            constexpr uint32_t kGroup = FMT == 0 ? 2 : 4;  // numbers beside each other
-            const auto dim_of = [&](uint32_t i) { return warp * S::kWarpDims + i / kGroup * (4 * kGroup) + quad * kGroup + i % kGroup; };
             bool write = true;
             if (!at.whole_item()) {
                 // ---- one of an item's partial results: the last block joins them, in the order of the tiles ----
@@ -753,16 +862,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 at.contributors(share.cut, blockIdx.x, &owner, &contributors);
                 constexpr uint32_t kPart = kAttentionRows * (kMaxHeadDim + 2);  // rows, then maxima, then sums
                 float *const part = p.parts + ((uint64_t)blockIdx.x * 2 + (blockIdx.x == owner ? 1 : 0)) * kPart;
-                if (live && warp < S::kValueWarps) {
-#pragma unroll
-                    for (uint32_t i = 0; i < S::kOwn; i += kGroup) {
-                        float *const to = part + row * HDP + dim_of(i);
-                        if (FMT == 0) *reinterpret_cast<float2 *>(to) = make_float2(o[i], o[i + 1]);
-                        else *reinterpret_cast<float4 *>(to) = make_float4(o[i], o[i + 1], o[i + 2 < S::kOwn ? i + 2 : i], o[i + 3 < S::kOwn ? i + 3 : i]);
-                    }
-                }
+                if (holds) put(part + row * HDP, mine);
                 if (warp == 0 && quad == 0) {
-                    part[kAttentionRows * HDP + row] = top == kNone ? -INFINITY : top;
+                    part[kAttentionRows * HDP + row] = top;
                     part[kAttentionRows * (HDP + 1) + row] = total;
                 }
                 __threadfence();
@@ -774,12 +876,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 }
                 multipliers_sync();
                 write = *arrived;
-                if (write && live && warp < S::kValueWarps) {
+                if (write && holds) {
                     const float *const parts = p.parts + (uint64_t)owner * 2 * kPart;
                     float best = -INFINITY;
                     total = 0.f;
 #pragma unroll
-                    for (uint32_t i = 0; i < S::kOwn; ++i) o[i] = 0.f;
+                    for (uint32_t i = 0; i < S::kOwn; ++i) mine[i] = 0.f;
                     for (uint32_t k0 = 0; k0 < contributors; k0 += kBatch) {
                         float t[kBatch], l[kBatch], v[kBatch][S::kOwn];
 #pragma unroll
@@ -791,7 +893,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                                 t[k] = __ldcg(from + kAttentionRows * HDP + row);
                                 l[k] = __ldcg(from + kAttentionRows * (HDP + 1) + row);
 #pragma unroll
-                                for (uint32_t i = 0; i < S::kOwn; i += kGroup) {
+                                for (uint32_t i = 0; i < S::kOwn; i += kBeside) {
                                     const float *const at_dim = from + row * HDP + dim_of(i);
                                     if (FMT == 0) {
                                         const float2 a = __ldcg(reinterpret_cast<const float2 *>(at_dim));
@@ -813,36 +915,35 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         best = next;
                         total *= keep;
 #pragma unroll
-                        for (uint32_t i = 0; i < S::kOwn; ++i) o[i] *= keep;
+                        for (uint32_t i = 0; i < S::kOwn; ++i) mine[i] *= keep;
 #pragma unroll
                         for (uint32_t k = 0; k < kBatch; ++k) {
-                            // (rows of a piece that saw nothing have zeros; rows whose scores are NaNs keep those)
                             const float f = t[k] == -INFINITY ? 0.f : exp2_fast(t[k] - best);
                             total += t[k] == -INFINITY ? l[k] : l[k] * f;
 #pragma unroll
-                            for (uint32_t i = 0; i < S::kOwn; ++i) o[i] = fmaf(v[k][i], f, o[i]);
+                            for (uint32_t i = 0; i < S::kOwn; ++i) mine[i] = fmaf(v[k][i], f, mine[i]);
                         }
                     }
                 }
             }
-            if (write && live && warp < S::kValueWarps) {
+            if (write && holds) {
                 const bool none = at.length - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group) <= 0;
                 const float by = 1.f / total;
                 const uint64_t base = ((uint64_t)at.s * p.q_tokens + r / g.group) * p.out_stride + ((uint64_t)head * g.group + r % g.group) * p.kv.head_dim;
 #pragma unroll
-                for (uint32_t i = 0; i < S::kOwn; ++i) o[i] = none ? 0.f : o[i] * by;
+                for (uint32_t i = 0; i < S::kOwn; ++i) mine[i] = none ? 0.f : mine[i] * by;
 #pragma unroll
-                for (uint32_t i = 0; i < S::kOwn; i += kGroup) {
+                for (uint32_t i = 0; i < S::kOwn; i += kBeside) {
                     const uint32_t d = dim_of(i);
                     if (d >= p.kv.head_dim) continue;
                     if (p.out_is_f32) {
                         float *const to = static_cast<float *>(p.out) + base + d;
-                        if (FMT == 0) *reinterpret_cast<float2 *>(to) = make_float2(o[i], o[i + 1]);
-                        else *reinterpret_cast<float4 *>(to) = make_float4(o[i], o[i + 1], o[i + 2 < S::kOwn ? i + 2 : i], o[i + 3 < S::kOwn ? i + 3 : i]);
+                        if (FMT == 0) *reinterpret_cast<float2 *>(to) = make_float2(mine[i], mine[i + 1]);
+                        else *reinterpret_cast<float4 *>(to) = make_float4(mine[i], mine[i + 1], mine[(i + 2) % S::kOwn], mine[(i + 3) % S::kOwn]);
                     } else {
                         uint16_t *const to = static_cast<uint16_t *>(p.out) + base + d;
-                        if (FMT == 0) *reinterpret_cast<uint32_t *>(to) = pack_bf16(o[i], o[i + 1]);
-                        else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2 < S::kOwn ? i + 2 : i], o[i + 3 < S::kOwn ? i + 3 : i]));
+                        if (FMT == 0) *reinterpret_cast<uint32_t *>(to) = pack_bf16(mine[i], mine[i + 1]);
+                        else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16(mine[i], mine[i + 1]), pack_bf16(mine[(i + 2) % S::kOwn], mine[(i + 3) % S::kOwn]));
                     }
                 }
             }

@@ -126,8 +126,9 @@ def attention64(cache, lengths, q, q_tokens, scale):
 
     8-bit caches keep halves in fp16, whose smallest step is 2^-24: queries are scaled to a largest value of 1 or more, so a query is
     off by 2^-16 of itself or by 2^-25 of the largest one, whichever is more: that adds 2^-25 scale max|q| sum |k| to d. Weights times
-    scales w_j = p_j scale_j are scaled so that the largest one of a warp is 2^10 or more, and are off by 2^-16 of themselves or by
-    2^-25 2^-10 of that one: that adds 2^-35 max w sum |code| to the result."""
+    scales w_j = p_j scale_j are, for int8, whole numbers of which the largest one so far is 2^25 or more: off by half at most, 2^-26 of
+    the largest one; for e4m3 scaled so that the largest one is 2^10 or more, and off by 2^-16 of themselves or by 2^-25 2^-10 of it.
+    That adds 2^-26, 2^-35 max w sum |code| to the result."""
     rows, heads, dim = q.shape
     group = heads // cache.kv_heads
     out = torch.zeros(rows, heads, dim, dtype=torch.float64, device="cuda")
@@ -151,7 +152,7 @@ def attention64(cache, lengths, q, q_tokens, scale):
             if v_scales is not None:
                 size = size + 2.0 ** -11 * abs(scale) * torch.einsum("hg,th->hgt", x.abs().amax(-1), k[:seen].abs().sum(-1))
                 codes = raw[:seen].view(POOLS[cache.fmt]).double().abs().sum(0)
-                steps = 2.0 ** -35 * (p * v_scales[:seen].double().T[:, None]).amax(-1)[..., None] * codes[:, None]
+                steps = 2.0 ** (-26 if cache.fmt == "int8" else -35) * (p * v_scales[:seen].double().T[:, None]).amax(-1)[..., None] * codes[:, None]
                 steps = steps.reshape(heads, dim)
             out[s * q_tokens + i] = torch.einsum("hgt,thd->hgd", p, v[:seen]).reshape(heads, dim)
             mean = torch.einsum("hgt,thd->hgd", p, v[:seen].abs()).reshape(heads, dim)
