@@ -38,8 +38,8 @@
 namespace q4 {
 
 constexpr uint32_t kWarps = 8, kMultipliers = kWarps * 32, kThreads = kMultipliers + 32;  // the last warp asks for tiles
+constexpr uint32_t kMostBlocks = 256;           // of a launch
 constexpr uint32_t kLeastRun = 16;              // tiles: shorter runs cost more in joining than they save
-constexpr uint32_t kBatch = 8;                  // partial results that are asked for at a time
 constexpr float kNone = -3.0e38f;               // a reference below all scores: the row has seen nothing
 constexpr float kHeadroom = 8.f;                // how far above its reference a score may lie, in powers of two
 // 8-bit caches: a weight times scale is brought below 2^11 (int8: 2^26) when it becomes the reference and may grow to 2^15 (2^30). As fp16
@@ -79,7 +79,7 @@ struct Shape {
     static constexpr uint32_t kFit = (kSharedLimit - 1024 - kQueries - 2 * kWeights - kSmall) / (kSlot + kScales + 16);
     static constexpr uint32_t kSlots = (kFit < 16 ? kFit : 16) & (FMT == 0 ? ~0u : ~1u);  // 8-bit: keys in even ones
     static constexpr uint32_t kShared = 1024 + kSlots * (kSlot + kScales + 16) + kQueries + 2 * kWeights + kSmall;
-    static_assert(kSlots >= 2 && kSubs * kSegs <= 32, "");
+    static_assert(kSlots >= 2 && kSubs * kSegs <= 32 && 2 * kWeights >= kMostBlocks * kAttentionRows * 4, "");
 };
 
 // ---- small pieces ----
@@ -214,6 +214,9 @@ __device__ __forceinline__ void copy_whole_tile(uint32_t dst, const CUtensorMap 
                  "r"(head), "r"(page)
                  : "memory");
 }
+__device__ __forceinline__ void copy_bytes(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 // 16 bytes, or zeros; counted by a barrier when they and the thread's others have arrived
 __device__ __forceinline__ void copy_16_or_zeros(uint32_t dst, const void *src, bool wanted) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(wanted ? 16u : 0u) : "memory");
@@ -244,10 +247,10 @@ struct Share {
     AttentionCut cut;
 };
 
-__device__ __forceinline__ uint64_t warp_scan(uint64_t v, uint32_t lane) {
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v, uint32_t lane) {
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const uint64_t o = __shfl_up_sync(0xffffffffu, v, off);
+        const uint32_t o = __shfl_up_sync(0xffffffffu, v, off);
         if (lane >= (uint32_t)off) v += o;
     }
     return v;
@@ -255,79 +258,72 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t v, uint32_t lane) {
 
 constexpr uint32_t kAllWarps = kThreads / 32;
 
-// All threads. `scratch`: 3 * kAllWarps + 2 words of 64 bits in shared memory. Up to 32 sequences every warp finds it by itself.
-__device__ __forceinline__ Share share_of_block(const AttentionParams &p, const Geometry &g, uint64_t *scratch) {
+// All threads. `scratch`: 3 * kAllWarps words in shared memory. Up to 32 sequences every warp finds it by itself.
+__device__ __forceinline__ Share share_of_block(const AttentionParams &p, const Geometry &g, uint32_t *scratch) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, sequences = p.kv.sequences;
     const bool few = sequences <= 32;
     const uint32_t mine = few ? lane : threadIdx.x, stride = few ? 32 : kThreads;
-    uint64_t tiles = 0;
-    uint32_t items = 0, longest = 0, own = 0;  // own: tiles of the thread's first sequence
+    const int64_t most = (int64_t)p.kv.per_sequence * p.kv.page_tokens;
+    uint32_t tiles = 0, items = 0, longest = 0, own = 0;  // own: tiles of the thread's first sequence
+#pragma unroll 1
     for (uint32_t s = mine; s < sequences; s += stride) {
-        const int64_t raw = __ldcg(p.lengths + s), most = (int64_t)p.kv.per_sequence * p.kv.page_tokens, n = raw < 0 ? 0 : raw > most ? most : raw;
-        if (raw != n && blockIdx.x == 0) *p.kv.input_error = 1;
-        const uint32_t t = attention_tiles(n);
+        const int32_t raw = __ldcg(p.lengths + s);
+        const uint32_t t = attention_tiles(raw > most ? most : raw);
+        if ((raw < 0 || raw > most) && blockIdx.x == 0) *p.kv.input_error = 1;
         if (s == mine) own = t;
         tiles += t;
         items += t > 0;
         longest = max(longest, t);
     }
-    uint64_t scan = warp_scan(tiles, lane);
-    tiles = __shfl_sync(0xffffffffu, scan, 31);
+    tiles = __reduce_add_sync(0xffffffffu, tiles);
     items = __reduce_add_sync(0xffffffffu, items);
     longest = __reduce_max_sync(0xffffffffu, longest);
     if (!few) {
         if (lane == 0) scratch[warp] = tiles, scratch[kAllWarps + warp] = items, scratch[2 * kAllWarps + warp] = longest;
         __syncthreads();
-        tiles = items = longest = 0;
-        for (uint32_t w = 0; w < kAllWarps; ++w) {
-            tiles += scratch[w];
-            items += (uint32_t)scratch[kAllWarps + w];
-            longest = max(longest, (uint32_t)scratch[2 * kAllWarps + w]);
-        }
+        const bool has = lane < kAllWarps;
+        tiles = __reduce_add_sync(0xffffffffu, has ? scratch[lane] : 0u);
+        items = __reduce_add_sync(0xffffffffu, has ? scratch[kAllWarps + lane] : 0u);
+        longest = __reduce_max_sync(0xffffffffu, has ? scratch[2 * kAllWarps + lane] : 0u);
     }
     Share share;
     share.any = false;
     share.at = Cursor{};
     if (tiles == 0) return share;
-    share.cut = attention_cut(tiles * g.heads, (uint64_t)items * g.heads, longest, gridDim.x, kLeastRun);
-    const AttentionCut &cut = share.cut;
-    const uint64_t target = attention_target(cut, blockIdx.x);
-    if (cut.mode != kEqualPieces && target >= cut.tiles) return share;
-    // the sequence that holds piece or tile number `target`
-    uint64_t start = 0;
-    uint32_t s = 0;
-    bool found = false;
-    if (few) {
-        const uint64_t weight = attention_weight(cut, own, g.heads), to = warp_scan(weight, lane);
-        const uint32_t hit = __ballot_sync(0xffffffffu, target >= to - weight && target < to);
-        found = hit != 0;
-        s = found ? __ffs(hit) - 1 : 0;
-        start = __shfl_sync(0xffffffffu, to - weight, s);
-    } else {
-        uint64_t before = 0;
-        for (uint32_t base = 0; base < sequences && !found; base += kThreads) {
-            const uint32_t i = base + threadIdx.x;
-            const uint32_t t = base == 0 ? own : i < sequences ? attention_tiles(length_of(p, i)) : 0u;
-            const uint64_t weight = attention_weight(cut, t, g.heads);
-            const uint64_t to = warp_scan(weight, lane);
-            __syncthreads();
-            if (lane == 31) scratch[warp] = to;
-            if (threadIdx.x == 0) scratch[kAllWarps] = ~0ull;
-            __syncthreads();
-            uint64_t from = before + to - weight;
-            for (uint32_t w = 0; w < kAllWarps; ++w) {
-                if (w < warp) from += scratch[w];
-                before += scratch[w];
+    share.cut = attention_cut(tiles * g.heads, items * g.heads, longest, gridDim.x, kLeastRun);
+    uint32_t target;
+    if (!attention_target(share.cut, blockIdx.x, &target)) return share;
+    // the sequence that holds piece or tile number `target`; every warp finds it: first eight that do, of 256 at a time, then which of them
+    uint32_t base = 0, before = 0, hit = 0, s = 0, start = 0;
+    if (!few) {
+#pragma unroll 1
+        for (;; base += 256) {
+            uint32_t weight = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) {
+                const uint32_t i = base + lane * 8 + j;
+                weight += attention_weight(share.cut, i < sequences ? attention_tiles(length_of(p, i)) : 0u, g.heads);
             }
-            if (target >= from && target < from + weight) scratch[kAllWarps] = i, scratch[kAllWarps + 1] = from;
-            __syncthreads();
-            found = scratch[kAllWarps] != ~0ull;
-            s = (uint32_t)scratch[kAllWarps];
-            start = scratch[kAllWarps + 1];
+            const uint32_t to = before + warp_scan(weight, lane);
+            hit = __ballot_sync(0xffffffffu, target >= to - weight && target - (to - weight) < weight);
+            const uint32_t from = hit ? __ffs(hit) - 1 : 31;
+            before = __shfl_sync(0xffffffffu, hit ? to - weight : to, from);
+            if (hit) {
+                base += from * 8;
+                break;
+            }
+            if (sequences - base <= 256) return share;
         }
-        __syncthreads();
     }
-    if (found) share.any = share.at.start(cut, target, s, start, [&](uint32_t i) { return length_of(p, i); }, sequences, g.heads);
+    {
+        const uint32_t i = base + lane, t = few ? own : lane < 8 && i < sequences ? attention_tiles(length_of(p, i)) : 0u;
+        const uint32_t weight = attention_weight(share.cut, t, g.heads), to = before + warp_scan(weight, lane);
+        hit = __ballot_sync(0xffffffffu, target >= to - weight && target - (to - weight) < weight);
+        const uint32_t from = hit ? __ffs(hit) - 1 : 0;
+        s = base + from;
+        start = __shfl_sync(0xffffffffu, to - weight, from);
+    }
+    if (hit) share.any = share.at.start(share.cut, target, s, start, [&](uint32_t i) { return length_of(p, i); }, sequences, g.heads);
     return share;
 }
 
@@ -414,18 +410,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     extern __shared__ uint8_t shared_raw[];
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(shared_raw), pad = (1024u - (raw & 1023u)) & 1023u;
     const uint32_t ring = raw + pad, scales = ring + S::kSlots * S::kSlot, weights = scales + S::kSlots * S::kScales, queries = weights + 2 * S::kWeights,
-                   full = queries + S::kQueries, empty = full + S::kSlots * 8;
-    float *const small = reinterpret_cast<float *>(shared_raw + (empty + S::kSlots * 8 - raw));
+                   full = queries + S::kQueries, empty = full + S::kSlots * 8, joined = empty + S::kSlots * 8;
+    float *const small = reinterpret_cast<float *>(shared_raw + (joined + 16 - raw));
     float *const highs = small, *const weight_highs = small + kWarps * kAttentionRows, *const sums = small + 2 * kWarps * kAttentionRows;  // [warp][row]
     float *const row_scales = small + 3 * kWarps * kAttentionRows;                                                                         // [row] scale of the scores, in powers of two
-    uint64_t *const scratch = reinterpret_cast<uint64_t *>(row_scales + kAttentionRows);
-    uint32_t *const arrived = reinterpret_cast<uint32_t *>(scratch + 3 * kAllWarps + 2);
+    uint32_t *const scratch = reinterpret_cast<uint32_t *>(row_scales + kAttentionRows), *const joins = scratch + 3 * kAllWarps;  // joins: 2 of 6 words
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row = lane >> 2, quad = lane & 3u;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < S::kSlots; ++i) {
             mbar_init(full + i * 8, FMT != 0 && i % 2 == 0 ? 33 : 1);  // the tile copies; the lanes' scales
             mbar_init(empty + i * 8, kWarps);
         }
+        mbar_init(joined, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -462,6 +458,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             }
         };
         load_query(at);
+        constexpr uint32_t kPart = kAttentionRows * (kMaxHeadDim + 2);  // numbers of a partial result: rows, then maxima, then sums
+        uint32_t left_parts = 0;  // partial results this block has left: two at most
         bool more;
         do {
             // ---- queries of the item: warp w splits row w into halves, or digits, in the order in which key rows are read ----
@@ -600,17 +598,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 if (lane == 0) mbar_arrive(empty + turn.slot * 8);
                 turn.next();
                 // ---- weights ----
-                float high = x[0], weight[4 * S::kOwnSubs], weight_high = 0.f;
+                float high = x[0], weight[4 * S::kOwnSubs], of_tile;
 #pragma unroll
                 for (uint32_t i = 1; i < 4 * S::kOwnSubs; ++i) high = fmaxf(high, x[i]);
-#pragma unroll
-                for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) {
-                    weight[i] = exp2_fast(x[i] - top);
-                    if (FMT != 0) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
-                }
-                float of_tile;
-                const auto pass_on = [&]() {
+#pragma unroll 1
+                for (bool again = false;; again = true) {
+                    // as if the references were high enough; if they are not, for any warp, they are raised and all is done again
+                    float weight_high = 0.f;
                     of_tile = 0.f;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) {
+                        weight[i] = exp2_fast(x[i] - top);
+                        if (FMT != 0) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
+                    }
 #pragma unroll
                     for (uint32_t t = 0; t < S::kOwnSubs; ++t) {
                         const uint32_t sub = warp * S::kOwnSubs + t;
@@ -643,36 +643,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             sts_v4(weights_at + (sub * 32 + lane) * 16, make_uint4(a[0], a[1], a[2], a[3]));
                         }
                     }
-                };
-                const bool rise = high - top > kHeadroom || (FMT != 0 && weight_high > most);
-                if (!__any_sync(0xffffffffu, rise)) pass_on();
-                if (multipliers_any(rise)) {
-                    // a reference is raised, in all warps alike
-                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
-                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
-                    if (quad == 0) highs[warp * kAttentionRows + row] = high;
+                    if (!multipliers_any(!again && (high - top > kHeadroom || (FMT != 0 && weight_high > most)))) break;
+                    float now = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
+                    now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 2));
+                    if (quad == 0) highs[warp * kAttentionRows + row] = now;
                     multipliers_sync();
-                    high = -INFINITY;
+                    now = -INFINITY;
 #pragma unroll
-                    for (uint32_t w = 0; w < kWarps; ++w) high = fmaxf(high, highs[w * kAttentionRows + row]);
+                    for (uint32_t w = 0; w < kWarps; ++w) now = fmaxf(now, highs[w * kAttentionRows + row]);
                     float keep = 1.f;
-                    if (high - top > kHeadroom) {
-                        high = ceilf(high);
-                        keep = exp2_fast(top - high);
+                    if (now - top > kHeadroom) {
+                        now = ceilf(now);
+                        keep = exp2_fast(top - now);
                         sum *= keep;
-                        top = high;
-                        if (FMT != 0) {
-                            lift = weight_top == kNone ? 0.f : exp2_fast(top - weight_top);
-                            most = lift > 0.f ? Weights<FMT>::kMost / lift : 0.f;
-                            keep = 1.f;
-                        }
-#pragma unroll
-                        for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) weight[i] = exp2_fast(x[i] - top);
+                        top = now;
                     }
                     if (FMT != 0) {
                         weight_high = 0.f;
 #pragma unroll
-                        for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
+                        for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) weight_high = fmaxf(weight_high, exp2_fast(x[i] - top) * value_scale[i]);
                         weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 1));
                         weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 2));
                         if (quad == 0) weight_highs[warp * kAttentionRows + row] = weight_high;
@@ -680,14 +669,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         weight_high = 0.f;
 #pragma unroll
                         for (uint32_t w = 0; w < kWarps; ++w) weight_high = fmaxf(weight_high, weight_highs[w * kAttentionRows + row]);
-                        if (weight_high > most) {
+                        lift = weight_top == kNone ? 0.f : exp2_fast(top - weight_top);
+                        keep = 1.f;
+                        if (weight_high * lift > Weights<FMT>::kMost || (lift == 0.f && weight_high > 0.f)) {
                             const int e = (int)(__float_as_uint(weight_high) >> 23) - 126;  // weight_high < 2^e
                             const float next = top + (float)max(e - Weights<FMT>::kExponent, -100);
                             keep = weight_top == kNone ? 0.f : exp2_fast(weight_top - next);
                             weight_top = next;
                             lift = exp2_fast(top - weight_top);
-                            most = Weights<FMT>::kMost / lift;
                         }
+                        most = lift > 0.f ? Weights<FMT>::kMost / lift : 0.f;
                     }
 #pragma unroll
                     for (uint32_t i = 0; i < (FMT == 1 ? S::kOwn : 1); ++i) o[i] *= keep;
@@ -695,8 +686,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     for (uint32_t i = 0; i < (FMT == 1 ? 1 : S::kAcc); ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) acc[i][j] *= keep;
-                    pass_on();
-                    multipliers_sync();
                 }
                 sum += of_tile;
                 // ---- values: this warp's dimensions, all tokens of the tile ----
@@ -780,18 +769,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                                                 }
                                     }
                                 if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+                                    for (int32_t k = 0; k < (int32_t)kTileTokens && first + k < limit; ++k) {
+                                        const uint32_t turned = S::kSeg == 128 ? (uint32_t)k & 7u : (uint32_t)k >> 1 & 3u, at_token = held + t * S::kSub + (uint32_t)k * S::kSeg;
 #pragma unroll
-                                    for (uint32_t i = 0; i < S::kAcc; ++i)
+                                        for (uint32_t i = 0; i < S::kAcc; ++i)
 #pragma unroll
-                                        for (uint32_t j = 0; j < 2; ++j) {
-                                            const uint32_t d = warp * S::kWarpDims + (FMT == 0 ? i * 8 + quad * 2 + j : i / 2 * 16 + quad * 4 + j * 2 + (i & 1u));
-                                            const uint32_t byte = d * (FMT == 0 ? 2 : 1), seg = byte / S::kSeg, piece = byte % S::kSeg / 16;
-                                            for (int32_t k = 0; k < (int32_t)kTileTokens && first + k < limit; ++k) {
-                                                const uint32_t turned = S::kSeg == 128 ? (uint32_t)k & 7u : (uint32_t)k >> 1 & 3u;
-                                                const uint32_t e = lds_u32((held + t * S::kSub + seg * (kTileTokens * S::kSeg) + (uint32_t)k * S::kSeg + ((piece ^ turned) << 4) + byte % 16) & ~3u);
+                                            for (uint32_t j = 0; j < 2; ++j) {
+                                                const uint32_t d = warp * S::kWarpDims + (FMT == 0 ? i * 8 + quad * 2 + j : i / 2 * 16 + quad * 4 + j * 2 + (i & 1u));
+                                                const uint32_t byte = d * (FMT == 0 ? 2 : 1), piece = byte % S::kSeg / 16;
+                                                const uint32_t e = lds_u32((at_token + byte / S::kSeg * (kTileTokens * S::kSeg) + ((piece ^ turned) << 4) + byte % 16) & ~3u);
                                                 if (not_finite<FMT>(e, byte & 3u)) acc[i][j] += FMT == 0 ? __uint_as_float((e >> ((byte & 3u) * 8)) << 16) : __uint_as_float(0x7fc00000u);
                                             }
-                                        }
+                                    }
                                     __syncwarp();
                                 }
                             }
@@ -855,12 +845,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             float total = 0.f;
 #pragma unroll
             for (uint32_t w = 0; w < kWarps; ++w) total += sums[w * kAttentionRows + row];
-            bool write = true;
             if (!at.whole_item()) {
-                // ---- one of an item's partial results: the last block joins them, in the order of the tiles ----
+                // ---- a partial result; the block that is the last to leave one of an item joins them below ----
                 uint32_t owner, contributors;
                 at.contributors(share.cut, blockIdx.x, &owner, &contributors);
-                constexpr uint32_t kPart = kAttentionRows * (kMaxHeadDim + 2);  // rows, then maxima, then sums
                 float *const part = p.parts + ((uint64_t)blockIdx.x * 2 + (blockIdx.x == owner ? 1 : 0)) * kPart;
                 if (holds) put(part + row * HDP, mine);
                 if (warp == 0 && quad == 0) {
@@ -870,63 +858,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 __threadfence();
                 multipliers_sync();
                 if (threadIdx.x == 0) {
-                    *arrived = atomicAdd(p.counters + owner, 1u) + 1 == contributors;
-                    if (*arrived) p.counters[owner] = 0;
-                    __threadfence();
+                    uint32_t *const to = joins + left_parts * 6;
+                    const bool last = atomicAdd(p.counters + owner, 1u) + 1 == contributors;
+                    if (last) p.counters[owner] = 0;
+                    to[0] = last, to[1] = owner, to[2] = contributors, to[3] = at.s, to[4] = at.item, to[5] = (uint32_t)at.length;
                 }
-                multipliers_sync();
-                write = *arrived;
-                if (write && holds) {
-                    const float *const parts = p.parts + (uint64_t)owner * 2 * kPart;
-                    float best = -INFINITY;
-                    total = 0.f;
-#pragma unroll
-                    for (uint32_t i = 0; i < S::kOwn; ++i) mine[i] = 0.f;
-                    for (uint32_t k0 = 0; k0 < contributors; k0 += kBatch) {
-                        float t[kBatch], l[kBatch], v[kBatch][S::kOwn];
-#pragma unroll
-                        for (uint32_t k = 0; k < kBatch; ++k) {
-                            t[k] = -INFINITY;
-                            l[k] = 0.f;
-                            if (k0 + k < contributors) {
-                                const float *const from = parts + ((k0 + k) * 2 + (k0 + k == 0 ? 1 : 0)) * kPart;
-                                t[k] = __ldcg(from + kAttentionRows * HDP + row);
-                                l[k] = __ldcg(from + kAttentionRows * (HDP + 1) + row);
-#pragma unroll
-                                for (uint32_t i = 0; i < S::kOwn; i += kBeside) {
-                                    const float *const at_dim = from + row * HDP + dim_of(i);
-                                    if (FMT == 0) {
-                                        const float2 a = __ldcg(reinterpret_cast<const float2 *>(at_dim));
-                                        v[k][i] = a.x, v[k][i + 1] = a.y;
-                                    } else {
-                                        const float4 a = __ldcg(reinterpret_cast<const float4 *>(at_dim));
-                                        v[k][i] = a.x, v[k][i + 1] = a.y, v[k][(i + 2) % S::kOwn] = a.z, v[k][(i + 3) % S::kOwn] = a.w;
-                                    }
-                                }
-                            } else {
-#pragma unroll
-                                for (uint32_t i = 0; i < S::kOwn; ++i) v[k][i] = 0.f;
-                            }
-                        }
-                        float next = best;
-#pragma unroll
-                        for (uint32_t k = 0; k < kBatch; ++k) next = fmaxf(next, t[k]);
-                        const float keep = best == next ? 1.f : exp2_fast(best - next);
-                        best = next;
-                        total *= keep;
-#pragma unroll
-                        for (uint32_t i = 0; i < S::kOwn; ++i) mine[i] *= keep;
-#pragma unroll
-                        for (uint32_t k = 0; k < kBatch; ++k) {
-                            const float f = t[k] == -INFINITY ? 0.f : exp2_fast(t[k] - best);
-                            total += t[k] == -INFINITY ? l[k] : l[k] * f;
-#pragma unroll
-                            for (uint32_t i = 0; i < S::kOwn; ++i) mine[i] = fmaf(v[k][i], f, mine[i]);
-                        }
-                    }
-                }
-            }
-            if (write && holds) {
+                ++left_parts;
+            } else if (holds) {
                 const bool none = at.length - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group) <= 0;
                 const float by = 1.f / total;
                 const uint64_t base = ((uint64_t)at.s * p.q_tokens + r / g.group) * p.out_stride + ((uint64_t)head * g.group + r % g.group) * p.kv.head_dim;
@@ -949,6 +887,82 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             }
             at = ahead;
         } while (more);
+
+        // ---- partial results of cut items that are complete, joined in the order of the tiles ----
+        // They come by bulk copies into the ring, which is free now: plain loads took 14000 cycles for 36 pieces of 6 KB, copies 3000.
+        multipliers_sync();
+        float *const factors = reinterpret_cast<float *>(shared_raw + (weights - raw));  // [piece][row]
+        uint32_t phase = 0;
+#pragma unroll 1
+        for (uint32_t n = 0; n < left_parts; ++n) {
+            const uint32_t *const job = joins + n * 6;
+            if (!job[0]) continue;
+            const uint32_t owner = job[1], contributors = job[2], seq = job[3], head = job[4] / g.chunks, chunk = job[4] % g.chunks;
+            const uint32_t rows = min(g.rows - chunk * kAttentionRows, kAttentionRows), bytes = rows * HDP * 4, room = S::kSlots * S::kSlot / bytes;
+            // piece k lies 2 k - 1 places behind the owner's, which is the first one
+            const float *const first = p.parts + ((uint64_t)owner * 2 + 1) * kPart;
+            const auto piece = [&](uint32_t k) { return first + (k == 0 ? 0 : 2 * k - 1) * kPart; };
+            float4 sums_of[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};  // 16 bytes of the item's rows, and those 256 x 16 behind
+#pragma unroll 1
+            for (uint32_t done = 0; done < contributors; done += room) {
+                const uint32_t now = min(room, contributors - done);
+                if (done) multipliers_sync();  // those before have been read
+                if (threadIdx.x == 0) mbar_expect(joined, now * bytes);
+                for (uint32_t k = threadIdx.x; k < now; k += kMultipliers) {
+                    asm volatile("fence.proxy.async;" ::: "memory");
+                    copy_bytes(ring + k * bytes, piece(done + k), bytes, joined);
+                }
+                if (done == 0) {
+                    // a warp for each row; pieces that saw nothing have zeros, rows whose scores are NaNs keep those
+                    float best = -INFINITY, total = 0.f;
+#pragma unroll 1
+                    for (uint32_t k = lane; k < contributors; k += 32) best = fmaxf(best, __ldcg(piece(k) + kAttentionRows * HDP + warp));
+#pragma unroll
+                    for (int off = 16; off > 0; off >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, off));
+#pragma unroll 1
+                    for (uint32_t k = lane; k < contributors; k += 32) {
+                        const float t = __ldcg(piece(k) + kAttentionRows * HDP + warp), l = __ldcg(piece(k) + kAttentionRows * (HDP + 1) + warp);
+                        const float f = t == -INFINITY ? 0.f : exp2_fast(t - best);
+                        total += t == -INFINITY ? l : l * f;
+                        factors[k * kAttentionRows + warp] = f;
+                    }
+#pragma unroll
+                    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+                    if (lane == 0) sums[warp] = total;
+                    multipliers_sync();
+                }
+                mbar_wait(joined, phase, limit_ns, p.error_flag);
+                phase ^= 1u;
+#pragma unroll
+                for (uint32_t j = 0; j < 2; ++j) {
+                    const uint32_t i = threadIdx.x + j * kMultipliers;
+                    if (i * 16 >= bytes) continue;
+                    const uint32_t of = i / (HDP / 4);
+                    float4 o4 = sums_of[j];
+#pragma unroll 4
+                    for (uint32_t k = 0; k < now; ++k) {
+                        const uint4 w = lds_v4(ring + k * bytes + i * 16);
+                        const float f = factors[(done + k) * kAttentionRows + of];
+                        o4.x = fmaf(__uint_as_float(w.x), f, o4.x), o4.y = fmaf(__uint_as_float(w.y), f, o4.y);
+                        o4.z = fmaf(__uint_as_float(w.z), f, o4.z), o4.w = fmaf(__uint_as_float(w.w), f, o4.w);
+                    }
+                    sums_of[j] = o4;
+                }
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 2; ++j) {
+                const uint32_t i = threadIdx.x + j * kMultipliers, of = i / (HDP / 4), d = i % (HDP / 4) * 4;
+                if (i * 16 >= bytes || d >= p.kv.head_dim) continue;
+                const uint32_t r = chunk * kAttentionRows + of;
+                const bool none = (int32_t)job[5] - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group) <= 0;
+                const float by = 1.f / sums[of];
+                const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sums_of[j].x * by, sums_of[j].y * by, sums_of[j].z * by, sums_of[j].w * by);
+                const uint64_t to = ((uint64_t)seq * p.q_tokens + r / g.group) * p.out_stride + ((uint64_t)head * g.group + r % g.group) * p.kv.head_dim + d;
+                if (p.out_is_f32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to) = v;
+                else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + to) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+            }
+            multipliers_sync();  // factors and sums have been read
+        }
     }
 
     // ---- sequences without tokens ----
@@ -1011,7 +1025,7 @@ cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t str
     g.heads = p.kv.kv_heads * g.chunks;
     g.pages = attention_pages(p.kv.page_tokens);
     g.whole_rows = whole_rows || S::kSegs == 1;
-    return launch_dependent(attention_kernel<FMT, HDP>, dim3(sm_count), kThreads, S::kShared, stream, p, g, maps[0], maps[1]);
+    return launch_dependent(attention_kernel<FMT, HDP>, dim3(sm_count < kMostBlocks ? sm_count : kMostBlocks), kThreads, S::kShared, stream, p, g, maps[0], maps[1]);
 }
 
 template <int FMT>

@@ -407,6 +407,11 @@ extern "C" int q4b_attention_device(q4b_runtime *rt, const q4b_kv_cache *cache, 
     if (!std::isfinite(scale)) return fail(Q4B_INVALID_ARGUMENT, "scale is not finite");
     const uint64_t rows = (uint64_t)table->sequences * q_tokens;
     if (rows > kMaxTokens) return fail(Q4B_DIMENSION_OVERFLOW, "tokens exceed runtime limits");
+    // 16-token tiles of all key heads and groups of eight query rows, at the longest lengths: numbered in 32 bits
+    const uint64_t tiles = (uint64_t)table->pages_per_sequence * (cache->page_tokens / 16), chunks = ((uint64_t)(heads / cache->kv_heads) * q_tokens + 7) / 8;
+    uint64_t work;
+    if (!product(tiles, table->sequences, &work) || !product(work, cache->kv_heads * chunks, &work) || work > 0xffffffffull)
+        return fail(Q4B_DIMENSION_OVERFLOW, "sequences, heads and page table have room for 2^32 or more tiles of 16 tokens");
     Span q, out, lengths;
     if (int st = check_rows("queries", q_dev, q_dtype, rows, heads, cache->head_dim, q_stride, &q)) return st;
     if (int st = check_rows("output", out_dev, out_dtype, rows, heads, cache->head_dim, out_stride, &out)) return st;

@@ -37,10 +37,10 @@ enum AttentionMode : uint32_t {
     kWholeItems = 2    // blocks take the items whose middle lies in their run
 };
 
-// The cut of a call, the same in every block.
+// The cut of a call, the same in every block. All numbers of tiles fit 32 bits: the host refuses calls that could have more.
 struct AttentionCut {
-    uint64_t tiles;  // of all items
-    uint64_t run;    // tiles of a block's run, or of a piece at most
+    uint32_t tiles;  // of all items
+    uint32_t run;    // tiles of a block's run, or of a piece at most
     uint32_t mode;
 };
 
@@ -49,45 +49,49 @@ struct AttentionCut {
 //     holds for run >= tiles / (blocks - items).
 //   * Items that are short against a run stay whole: what a block does more than another is less than joining cut items takes.
 //   * Otherwise all blocks take the same number of tiles.
-Q4_PLAN_FN AttentionCut attention_cut(uint64_t tiles, uint64_t items, uint32_t longest, uint32_t blocks, uint32_t least) {
+Q4_PLAN_FN AttentionCut attention_cut(uint32_t tiles, uint32_t items, uint32_t longest, uint32_t blocks, uint32_t least) {
     AttentionCut c;
     c.tiles = tiles;
-    c.mode = items * 2 <= blocks ? kEqualPieces : kEqualRuns;
-    const uint64_t by = c.mode == kEqualPieces ? blocks - items : blocks;
-    c.run = (tiles + by - 1) / by;
+    c.mode = items <= blocks / 2 ? kEqualPieces : kEqualRuns;
+    const uint32_t by = c.mode == kEqualPieces ? blocks - items : blocks;
+    c.run = (tiles - 1) / by + 1;
     if (c.mode == kEqualRuns && (longest <= 2 * least || longest <= c.run / 16)) c.mode = kWholeItems;
     if (c.mode != kWholeItems && c.run < least) c.run = least;
     return c;
 }
 
-Q4_PLAN_FN uint64_t attention_pieces(const AttentionCut &c, uint32_t tiles) { return (tiles + c.run - 1) / c.run; }
+Q4_PLAN_FN uint32_t attention_pieces(const AttentionCut &c, uint32_t tiles) { return tiles == 0 ? 0 : (tiles - 1) / c.run + 1; }
 
 // What a sequence counts for in the search for a block's start: its pieces, or its tiles, in all items.
-Q4_PLAN_FN uint64_t attention_weight(const AttentionCut &c, uint32_t tiles, uint32_t items) {
-    return (c.mode == kEqualPieces ? attention_pieces(c, tiles) : (uint64_t)tiles) * items;
+Q4_PLAN_FN uint32_t attention_weight(const AttentionCut &c, uint32_t tiles, uint32_t items) {
+    return (c.mode == kEqualPieces ? attention_pieces(c, tiles) : tiles) * items;
 }
 
-// Where block `block` starts, in those; past the end: it has nothing to do.
-Q4_PLAN_FN uint64_t attention_target(const AttentionCut &c, uint32_t block) { return c.mode == kEqualPieces ? block : block * c.run; }
+// Where block `block` starts, in those. False: behind them, it has nothing to do.
+Q4_PLAN_FN bool attention_target(const AttentionCut &c, uint32_t block, uint32_t *target) {
+    const uint64_t to = c.mode == kEqualPieces ? block : (uint64_t)block * c.run;
+    *target = (uint32_t)to;
+    return c.mode == kEqualPieces || to < c.tiles;
+}
 
 // Walks the segments of a block's share: tiles [begin, end) of an item. `items` of a sequence, `lengths(s)` its tokens.
 struct AttentionCursor {
     uint32_t s, item, begin, end, tiles;
     uint32_t piece, pieces;  // of an item cut into equal pieces
     int32_t length;
-    uint64_t left;   // tiles of the share from `begin` on; whole items: where the block's run ends
-    uint64_t first;  // runs: number of the sequence's first tile among the tiles of all items
+    uint32_t left;   // tiles of the share from `begin` on; whole items: where the block's run ends
+    uint32_t first;  // runs: number of the sequence's first tile among the tiles of all items
     uint32_t whole;
 
-    Q4_PLAN_FN void close() { end = whole || (uint64_t)(tiles - begin) < left ? tiles : begin + (uint32_t)left; }
-    Q4_PLAN_FN bool mine() const { return first + (uint64_t)item * tiles + tiles / 2 < left; }  // whole items: middle in the run
+    Q4_PLAN_FN void close() { end = whole || tiles - begin < left ? tiles : begin + left; }
+    Q4_PLAN_FN bool mine() const { return first + item * tiles + tiles / 2 < left; }  // whole items: middle in the run
 
     // Start of the block's share, which lies `target - before` pieces or tiles into sequence `sequence`; `before`: those of the
     // sequences in front. False: whole items, and none has its middle in the block's run.
     template <typename Lengths>
-    Q4_PLAN_FN bool start(const AttentionCut &cut, uint64_t target, uint32_t sequence, uint64_t before, const Lengths &lengths, uint32_t sequences, uint32_t items) {
+    Q4_PLAN_FN bool start(const AttentionCut &cut, uint32_t target, uint32_t sequence, uint32_t before, const Lengths &lengths, uint32_t sequences, uint32_t items) {
         const int64_t tokens = lengths(sequence);
-        const uint64_t local = target - before;
+        const uint32_t local = target - before;
         s = sequence;
         length = (int32_t)tokens;
         tiles = attention_tiles(tokens);
@@ -95,24 +99,26 @@ struct AttentionCursor {
         piece = 0;
         pieces = 1;
         whole = cut.mode == kWholeItems;
+        if (cut.mode == kEqualPieces) pieces = attention_pieces(cut, tiles);
+        const uint32_t per = cut.mode == kEqualPieces ? pieces : tiles;
+        item = local / per;
+        begin = local - item * per;
+        left = cut.tiles - target < cut.run ? cut.tiles - target : cut.run;
+        bool behind = false;
         if (cut.mode == kEqualPieces) {
-            pieces = (uint32_t)attention_pieces(cut, tiles);
-            item = (uint32_t)(local / pieces);
-            piece = (uint32_t)(local % pieces);
-            begin = (uint32_t)((uint64_t)tiles * piece / pieces);
-            left = (uint32_t)((uint64_t)tiles * (piece + 1) / pieces) - begin;
-        } else {
-            item = (uint32_t)(local / tiles);
-            begin = (uint32_t)(local % tiles);
-            left = cut.tiles - target < cut.run ? cut.tiles - target : cut.run;
-            if (whole) {
-                left += target;
-                const bool behind = begin > tiles / 2;  // its middle lies in the run before
-                begin = 0;
-                if (behind) return next(lengths, sequences, items);
-                if (!mine()) return false;
-            }
+            // the first `longer` pieces have a tile more than the others
+            const uint32_t each = tiles / pieces, longer = tiles - each * pieces;
+            piece = begin;
+            begin = piece * each + (piece < longer ? piece : longer);
+            left = each + (piece < longer ? 1 : 0);
+        } else if (whole) {
+            left += target;
+            behind = begin > tiles / 2;  // its middle lies in the run before
+            begin = 0;
         }
+        end = tiles;  // (next looks at it)
+        if (behind) return next(lengths, sequences, items);
+        if (whole && !mine()) return false;
         close();
         return true;
     }
@@ -126,7 +132,7 @@ struct AttentionCursor {
         begin = 0;
         if (++item == items) {
             item = 0;
-            first += (uint64_t)tiles * items;
+            first += tiles * items;
             do {
                 if (++s >= sequences) return false;
                 const int64_t tokens = lengths(s);
@@ -147,9 +153,9 @@ struct AttentionCursor {
         *owner = block - piece;
         *count = pieces;
         if (cut.mode != kEqualRuns) return;
-        const uint64_t from = first + (uint64_t)item * tiles;
-        *owner = (uint32_t)(from / cut.run);
-        *count = (uint32_t)((from + tiles - 1) / cut.run) - *owner + 1;
+        const uint32_t from = first + item * tiles;
+        *owner = from / cut.run;
+        *count = (from + (tiles - 1)) / cut.run - *owner + 1;
     }
 };
 

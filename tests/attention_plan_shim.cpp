@@ -12,14 +12,15 @@ uint64_t shim_attention_plan(const int64_t *lengths, uint32_t sequences, uint32_
         longest = t > longest ? t : longest;
     }
     if (tiles == 0) return 0;
-    const q4::AttentionCut cut = q4::attention_cut(tiles * items, live * items, longest, blocks, least);
+    if (tiles * items > 0xffffffffull) return 0;
+    const q4::AttentionCut cut = q4::attention_cut((uint32_t)(tiles * items), (uint32_t)live * items, longest, blocks, least);
     auto length = [&](uint32_t i) { return lengths[i]; };
     for (uint32_t b = 0; b < blocks; ++b) {
-        const uint64_t target = q4::attention_target(cut, b);
-        uint64_t before = 0;
+        uint32_t target, before = 0;
+        if (!q4::attention_target(cut, b, &target)) continue;
         for (uint32_t s = 0; s < sequences; ++s) {
-            const uint64_t weight = q4::attention_weight(cut, q4::attention_tiles(lengths[s]), items);
-            if (target >= before && target < before + weight) {
+            const uint32_t weight = q4::attention_weight(cut, q4::attention_tiles(lengths[s]), items);
+            if (target >= before && target - before < weight) {
                 q4::AttentionCursor c;
                 if (!c.start(cut, target, s, before, length, sequences, items)) break;
                 do {

@@ -26,14 +26,14 @@ def shim():
 
 def _plan(lib, lengths, items, blocks):
     lengths = np.asarray(lengths, dtype=np.int64)
-    out = np.zeros((100000, 7), dtype=np.uint64)
+    out = np.zeros((300000, 7), dtype=np.uint64)
     n = lib.shim_attention_plan(lengths.ctypes.data, len(lengths), items, blocks, LEAST, out.ctypes.data, len(out))
     assert n < len(out)
     return out[:n].astype(np.int64)
 
 
 CASES = [([1], 1), ([37], 4), ([0, 0, 5, 0], 4), ([262144], 4), ([8200], 4), ([16] * 40, 2), ([17, 1, 0, 5000, 31], 3), ([0] * 600 + [40] + [0] * 500 + [1000], 8),
-         (list(range(500, 8000, 233)), 4), ([100] * 256, 8), ([3100 + 16 * i for i in range(128)], 8), ([1], 148), ([1], 149), ([1] * 74, 1), ([5000] * 75, 1), ([2147483647], 2)]
+         (list(range(500, 8000, 233)), 4), ([100] * 256, 8), ([3100 + 16 * i for i in range(128)], 8), ([1], 148), ([1], 149), ([1] * 74, 1), ([5000] * 75, 1), ([2147483647], 2), ([2147483647], 31), ([262144] * 511, 512)]
 
 
 @pytest.mark.parametrize("blocks", [1, 2, 7, 132, 148, 160])

@@ -196,6 +196,14 @@ def test_attention_refusals(lib, more, name):
     assert got[0] == name and got != NO_RUNTIME, got
 
 
+def test_more_tiles_than_32_bits_number_are_refused(lib):
+    big = _table(sequences=1 << 16, pages_per_sequence=1 << 14)  # 2^30 tiles of four heads
+    got = _attend(lib, table=big)
+    assert got[0] == "DimensionOverflow" and "2^32" in got[1]
+    assert _attend(lib, table=_table(sequences=(1 << 16) - 1, pages_per_sequence=1 << 14)) == NO_RUNTIME
+    assert _attend(lib, table=_table(sequences=(1 << 16) - 1, pages_per_sequence=1 << 14), q_tokens=2)[0] == "DimensionOverflow"
+
+
 def test_shared_memory_is_refused(lib):
     share = lambda got: got[0] == "InvalidArgument" and "share" in got[1]  # noqa: E731
     for at in (K, K + 64 * 4 * 16 * 256 - 16, V + 1024, KS, VS + 64):
