@@ -914,17 +914,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 }
                 if (done == 0) {
                     // a warp for each row; pieces that saw nothing have zeros, rows whose scores are NaNs keep those
-                    float best = -INFINITY, total = 0.f;
-#pragma unroll 1
-                    for (uint32_t k = lane; k < contributors; k += 32) best = fmaxf(best, __ldcg(piece(k) + kAttentionRows * HDP + warp));
+                    float best = -INFINITY, total = 0.f, t[kMostBlocks / 32], l[kMostBlocks / 32];
+#pragma unroll
+                    for (uint32_t i = 0; i < kMostBlocks / 32; ++i) {
+                        const uint32_t k = lane + i * 32;
+                        t[i] = k < contributors ? __ldcg(piece(k) + kAttentionRows * HDP + warp) : -INFINITY;
+                        l[i] = k < contributors ? __ldcg(piece(k) + kAttentionRows * (HDP + 1) + warp) : 0.f;
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < kMostBlocks / 32; ++i) best = fmaxf(best, t[i]);
 #pragma unroll
                     for (int off = 16; off > 0; off >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, off));
-#pragma unroll 1
-                    for (uint32_t k = lane; k < contributors; k += 32) {
-                        const float t = __ldcg(piece(k) + kAttentionRows * HDP + warp), l = __ldcg(piece(k) + kAttentionRows * (HDP + 1) + warp);
-                        const float f = t == -INFINITY ? 0.f : exp2_fast(t - best);
-                        total += t == -INFINITY ? l : l * f;
-                        factors[k * kAttentionRows + warp] = f;
+#pragma unroll
+                    for (uint32_t i = 0; i < kMostBlocks / 32; ++i) {
+                        const float f = t[i] == -INFINITY ? 0.f : exp2_fast(t[i] - best);
+                        total += t[i] == -INFINITY ? l[i] : l[i] * f;
+                        if (lane + i * 32 < contributors) factors[(lane + i * 32) * kAttentionRows + warp] = f;
                     }
 #pragma unroll
                     for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
