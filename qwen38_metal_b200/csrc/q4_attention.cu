@@ -59,7 +59,7 @@ struct Shape {
     static constexpr uint32_t kSeg = kRow < 128 ? kRow : 128;        // swizzled together
     static constexpr uint32_t kSegs = kRow / kSeg;
     static constexpr uint32_t kSub = kTileTokens * kRow;             // 16 tokens' keys or values
-    static constexpr uint32_t kOwnSubs = kRow > 128 ? 1 : 2;         // of a tile, whose scores a warp has
+    static constexpr uint32_t kOwnSubs = kRow > 256 ? 1 : 2;         // of a tile, whose scores a warp has
     static constexpr uint32_t kSubs = kWarps * kOwnSubs;             // of a tile
     static constexpr uint32_t kSlot = kSubs * kSub;                  // of the ring: keys, or values, of a tile
     static constexpr uint32_t kPieces = kSeg / 64;                   // 16-byte pieces of a segment a lane takes from a key row
@@ -77,7 +77,7 @@ struct Shape {
     static constexpr uint32_t kWeights = kSubs * 32 * 16;               // of a tile; there are two
     static constexpr uint32_t kSmall = 2048;
     static constexpr uint32_t kFit = (kSharedLimit - 1024 - kQueries - 2 * kWeights - kSmall) / (kSlot + kScales + 16);
-    static constexpr uint32_t kSlots = (kFit < 16 ? kFit : 16) & (FMT == 0 ? ~0u : ~1u);  // 8-bit: keys in even ones
+    static constexpr uint32_t kSlots = kFit < 16 ? kFit : 16;
     static constexpr uint32_t kShared = 1024 + kSlots * (kSlot + kScales + 16) + kQueries + 2 * kWeights + kSmall;
     static_assert(kSlots >= 2 && kSubs * kSegs <= 32 && 2 * kWeights >= kMostBlocks * kAttentionRows * 4, "");
 };
@@ -392,8 +392,8 @@ __device__ __forceinline__ void ask_for_tiles(const AttentionParams &p, const Ge
                         copy_16_or_zeros(sc, p.kv.k_scales + from, here);
                         copy_16_or_zeros(sc + S::kSubs * 64, p.kv.v_scales + from, here);
                     }
-                    copies_arrive(bar);
                 }
+                if (FMT != 0) copies_arrive(bar);
                 turn.next();
             }
         }
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row = lane >> 2, quad = lane & 3u;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < S::kSlots; ++i) {
-            mbar_init(full + i * 8, FMT != 0 && i % 2 == 0 ? 33 : 1);  // the tile copies; the lanes' scales
+            mbar_init(full + i * 8, FMT != 0 ? 33 : 1);  // the tile copies; the lanes' scales
             mbar_init(empty + i * 8, kWarps);
         }
         mbar_init(joined, 1);
