@@ -231,6 +231,7 @@ struct Geometry {
     uint32_t rows;    // query rows of a key head
     uint32_t group;   // query heads of a key head
     uint32_t whole_rows;  // a copy brings all segments of 16 rows, else one of them
+    uint32_t tile_shift;  // a copy brings 16 << tile_shift tokens (rows of one segment)
     AttentionPages pages;
 };
 
@@ -268,7 +269,7 @@ __device__ __forceinline__ Share share_of_block(const AttentionParams &p, const 
 #pragma unroll 1
     for (uint32_t s = mine; s < sequences; s += stride) {
         const int32_t raw = __ldcg(p.lengths + s);
-        const uint32_t t = attention_tiles(raw > most ? most : raw);
+        const uint32_t t = attention_tiles(raw > most ? most : raw, g.tile_shift);
         if ((raw < 0 || raw > most) && blockIdx.x == 0) *p.kv.input_error = 1;
         if (s == mine) own = t;
         tiles += t;
@@ -290,7 +291,7 @@ __device__ __forceinline__ Share share_of_block(const AttentionParams &p, const 
     share.any = false;
     share.at = Cursor{};
     if (tiles == 0) return share;
-    share.cut = attention_cut(tiles * g.heads, items * g.heads, longest, gridDim.x, kLeastRun);
+    share.cut = attention_cut(tiles * g.heads, items * g.heads, longest, gridDim.x, kLeastRun >> g.tile_shift, g.tile_shift);
     uint32_t target;
     if (!attention_target(share.cut, blockIdx.x, &target)) return share;
     // the sequence that holds piece or tile number `target`; every warp finds it: first eight that do, of 256 at a time, then which of them
@@ -302,7 +303,7 @@ __device__ __forceinline__ Share share_of_block(const AttentionParams &p, const 
 #pragma unroll
             for (uint32_t j = 0; j < 8; ++j) {
                 const uint32_t i = base + lane * 8 + j;
-                weight += attention_weight(share.cut, i < sequences ? attention_tiles(length_of(p, i)) : 0u, g.heads);
+                weight += attention_weight(share.cut, i < sequences ? attention_tiles(length_of(p, i), g.tile_shift) : 0u, g.heads);
             }
             const uint32_t to = before + warp_scan(weight, lane);
             hit = __ballot_sync(0xffffffffu, target >= to - weight && target - (to - weight) < weight);
@@ -316,7 +317,7 @@ __device__ __forceinline__ Share share_of_block(const AttentionParams &p, const 
         }
     }
     {
-        const uint32_t i = base + lane, t = few ? own : lane < 8 && i < sequences ? attention_tiles(length_of(p, i)) : 0u;
+        const uint32_t i = base + lane, t = few ? own : lane < 8 && i < sequences ? attention_tiles(length_of(p, i), g.tile_shift) : 0u;
         const uint32_t weight = attention_weight(share.cut, t, g.heads), to = before + warp_scan(weight, lane);
         hit = __ballot_sync(0xffffffffu, target >= to - weight && target - (to - weight) < weight);
         const uint32_t from = hit ? __ffs(hit) - 1 : 0;
@@ -358,15 +359,16 @@ __device__ __forceinline__ void ask_for_tiles(const AttentionParams &p, const Ge
     do {
         const uint32_t head = at.item / g.chunks;
         const int32_t *const table = p.kv.table + (uint64_t)at.s * p.kv.row_stride;
+        const uint32_t shift = S::kSegs == 1 ? g.tile_shift : 0, tiles = S::kSubs >> shift;  // of a slot
         uint32_t entry = g.pages.page_of(at.begin + mine);
         uint32_t page = at.begin + mine < at.end ? (uint32_t)__ldcg(table + entry) : 0u;
-        for (uint32_t tile = at.begin; tile < at.end; tile += S::kSubs) {
-            const uint32_t count = min(at.end - tile, S::kSubs);
+        for (uint32_t tile = at.begin; tile < at.end; tile += tiles) {
+            const uint32_t count = min(at.end - tile, tiles);
             const bool wanted = mine < count, there = page < p.kv.pages;
             // (a page outside the cache is outside the tensor map too: such copies bring zeros)
-            const uint32_t now = there ? page : p.kv.pages, place = (tile + mine - entry * g.pages.per) * kTileTokens;
+            const uint32_t now = there ? page : p.kv.pages, place = (tile + mine - entry * g.pages.per) * (kTileTokens << shift);
             if (wanted && !there) *p.kv.input_error = 1;
-            const uint32_t next = tile + S::kSubs + mine;
+            const uint32_t next = tile + tiles + mine;
             if (next < at.end) {
                 entry = g.pages.page_of(next);
                 page = (uint32_t)__ldcg(table + entry);
@@ -375,18 +377,19 @@ __device__ __forceinline__ void ask_for_tiles(const AttentionParams &p, const Ge
             for (uint32_t values = 0; values < 2; ++values) {
                 mbar_wait(empty + turn.slot * 8, turn.phase ^ 1u, limit_ns, p.error_flag);
                 const uint32_t bar = full + turn.slot * 8, dst = ring + turn.slot * S::kSlot;
-                if (lane == 0) mbar_expect(bar, count * S::kSub);
+                if (lane == 0) mbar_expect(bar, count * (S::kSub << shift));
                 __syncwarp();
                 if (wanted) {
                     if (S::kSegs > 1 && g.whole_rows) copy_whole_tile(dst + lane * S::kSub, values ? v_map : k_map, bar, (int)place, (int)head, (int)now);
-                    else copy_tile(dst + lane * (kTileTokens * S::kSeg), values ? v_map : k_map, bar, (int)(seg * S::kSeg / (FMT == 0 ? 2 : 1)), (int)place, (int)head, (int)now);
+                    else copy_tile(dst + lane * (kTileTokens * S::kSeg << shift), values ? v_map : k_map, bar, (int)(seg * S::kSeg / (FMT == 0 ? 2 : 1)), (int)place, (int)head, (int)now);
                 }
                 if (FMT != 0 && values == 0) {
                     // lane 4 i + j: 16-byte piece j of the scales of 16 tokens, of keys and of values
 #pragma unroll
                     for (uint32_t of = lane / 4; of < S::kSubs; of += 8) {
-                        const uint32_t of_page = __shfl_sync(0xffffffffu, now, of * per), of_place = __shfl_sync(0xffffffffu, place, of * per);
-                        const bool here = of < count && of_page < p.kv.pages;
+                        const uint32_t by = (of >> shift) * per, of_page = __shfl_sync(0xffffffffu, now, by);
+                        const uint32_t of_place = __shfl_sync(0xffffffffu, place, by) + (of & ((1u << shift) - 1)) * kTileTokens;
+                        const bool here = of >> shift < count && of_page < p.kv.pages;
                         const uint64_t from = here ? ((uint64_t)of_page * p.kv.kv_heads + head) * p.kv.page_tokens + of_place + lane % 4 * 4 : 0;
                         const uint32_t sc = scales + turn.slot * S::kScales + of * 64 + lane % 4 * 16;
                         copy_16_or_zeros(sc, p.kv.k_scales + from, here);
@@ -514,7 +517,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             more = ahead.next(lengths, p.kv.sequences, g.heads);
             if (more) load_query(ahead);
             // tokens of the segment that all rows see, that this row sees, and that exist
-            const int32_t end_token = (int32_t)(at.end * kTileTokens), existing = min(at.length, end_token);
+            const uint32_t shift = S::kSegs == 1 ? g.tile_shift : 0, end_sub = at.end << shift;
+            const int32_t end_token = (int32_t)(end_sub * kTileTokens), existing = min(at.length, end_token);
             const int32_t sure = min(at.length - (int32_t)p.q_tokens + 1, end_token);
             const uint32_t r = chunk * kAttentionRows + row;
             const bool live = r < g.rows;
@@ -528,8 +532,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             float top = kNone, sum = 0.f;                      // reference of the row's scores; sum of this lane's weights
             float weight_top = kNone, lift = 0.f, most = 0.f;  // 8-bit: reference of weights times scales, 2^(top - weight_top), and what they may be
 
-            for (uint32_t tile = at.begin; tile < at.end; tile += S::kSubs) {
-                const uint32_t count = min(at.end - tile, S::kSubs);  // of 16 tokens; this warp's scores are those of warp * kOwnSubs and on
+            for (uint32_t tile = at.begin << shift; tile < end_sub; tile += S::kSubs) {
+                const uint32_t count = min(end_sub - tile, S::kSubs);  // of 16 tokens; this warp's scores are those of warp * kOwnSubs and on
                 // ---- scores ----
                 mbar_wait(full + turn.slot * 8, turn.phase, limit_ns, p.error_flag);
                 float x[4 * S::kOwnSubs];  // tokens 2 quad, + 1, + 8, + 9 of each 16, row `row`
@@ -984,9 +988,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 
 // ---- host ----
 
-// Rows of the cache as [page][head][token][value], or [page][head][segment][token][value in it]; copies of 16 tokens by one segment, or all.
+// Rows of the cache as [page][head][token][value], or [page][head][segment][token][value in it]; copies of a tile's tokens by
+// one segment, or all.
 template <int FMT, int HDP>
-bool encode_map(EncodeTiledFn encode, CUtensorMap *map, const KvView &kv, const uint8_t *pool, bool whole_rows) {
+bool encode_map(EncodeTiledFn encode, CUtensorMap *map, const KvView &kv, const uint8_t *pool, bool whole_rows, uint32_t tile_shift) {
     using S = Shape<FMT, HDP>;
     constexpr uint32_t kSegValues = S::kSeg / (FMT == 0 ? 2 : 1);
     const CUtensorMapDataType type = FMT == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
@@ -1001,7 +1006,7 @@ bool encode_map(EncodeTiledFn encode, CUtensorMap *map, const KvView &kv, const 
     }
     const cuuint64_t dims[4] = {kv.head_dim, kv.page_tokens, kv.kv_heads, kv.pages};
     const cuuint64_t strides[3] = {kv.token_stride, kv.head_stride, kv.page_stride};
-    const cuuint32_t box[4] = {kSegValues, kTileTokens, 1, 1};
+    const cuuint32_t box[4] = {kSegValues, kTileTokens << tile_shift, 1, 1};
     return encode(map, type, 4, const_cast<uint8_t *>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1011,8 +1016,12 @@ cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t str
     using S = Shape<FMT, HDP>;
     const EncodeTiledFn encode = encode_tiled_fn();
     CUtensorMap maps[2];
+    // Rows of one segment come 64 tokens at a time where pages allow (smaller copies are more than the copy engine takes; larger ones would
+    // bring more of what lies behind a sequence's end).
+    uint32_t shift = 0;
+    while (S::kSegs == 1 && shift < 2 && p.kv.page_tokens % (2 * kTileTokens << shift) == 0) ++shift;
     const bool whole_rows = p.kv.head_dim * (FMT == 0 ? 2 : 1) % S::kSeg == 0;
-    if (!encode || !encode_map<FMT, HDP>(encode, &maps[0], p.kv, p.kv.k, whole_rows) || !encode_map<FMT, HDP>(encode, &maps[1], p.kv, p.kv.v, whole_rows)) return cudaErrorInvalidValue;
+    if (!encode || !encode_map<FMT, HDP>(encode, &maps[0], p.kv, p.kv.k, whole_rows, shift) || !encode_map<FMT, HDP>(encode, &maps[1], p.kv, p.kv.v, whole_rows, shift)) return cudaErrorInvalidValue;
     static std::atomic<uint64_t> ready{0};  // a bit for each device: the attribute is the kernel's, once set it stays
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
@@ -1028,7 +1037,8 @@ cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t str
     g.rows = g.group * p.q_tokens;
     g.chunks = (g.rows + kAttentionRows - 1) / kAttentionRows;
     g.heads = p.kv.kv_heads * g.chunks;
-    g.pages = attention_pages(p.kv.page_tokens);
+    g.tile_shift = shift;
+    g.pages = attention_pages(p.kv.page_tokens, shift);
     g.whole_rows = whole_rows || S::kSegs == 1;
     return launch_dependent(attention_kernel<FMT, HDP>, dim3(sm_count < kMostBlocks ? sm_count : kMostBlocks), kThreads, S::kShared, stream, p, g, maps[0], maps[1]);
 }

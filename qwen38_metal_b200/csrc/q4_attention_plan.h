@@ -1,7 +1,8 @@
 // How the work of an attention call is cut over its blocks; shared by the kernel and the CPU tests.
 //
-// A tile is 16 tokens of one sequence, which lie in one page. An item is what one result belongs to: a sequence, a key head and eight
-// query rows of it; it has as many tiles as its sequence. Blocks take runs of tiles, and the partial results of an item that
+// A tile is 16 tokens of one sequence, or 16 << shift where pages have a whole number of those: tokens that lie in one page and come by
+// one copy. An item is what one result belongs to: a sequence, a key head and eight query rows of it; it has as many tiles as its
+// sequence. Blocks take runs of tiles, and the partial results of an item that
 // several blocks have worked on are joined by the last of them.
 #pragma once
 #include <stdint.h>
@@ -17,15 +18,15 @@ namespace q4 {
 constexpr uint32_t kTileTokens = 16;
 constexpr uint32_t kAttentionRows = 8;  // query rows of an item
 
-Q4_PLAN_FN uint32_t attention_tiles(int64_t length) { return length > 0 ? (uint32_t)((length + kTileTokens - 1) / kTileTokens) : 0u; }
+Q4_PLAN_FN uint32_t attention_tiles(int64_t length, uint32_t shift) { return length > 0 ? (uint32_t)((length - 1) / kTileTokens >> shift) + 1 : 0u; }
 
 // tile / per for tiles below 2^27, as a product: 2^(32 + shift) / per rounded up is off by less than per <= 2^(shift + 1).
 struct AttentionPages {
     uint32_t per, inverse, shift;  // tiles of a page
     Q4_PLAN_FN uint32_t page_of(uint32_t tile) const { return per == 1 ? tile : (uint32_t)((uint64_t)tile * inverse >> 32) >> shift; }
 };
-inline AttentionPages attention_pages(uint32_t page_tokens) {
-    AttentionPages d = {page_tokens / kTileTokens, 0, 0};
+inline AttentionPages attention_pages(uint32_t page_tokens, uint32_t tile_shift) {
+    AttentionPages d = {page_tokens / (kTileTokens << tile_shift), 0, 0};
     while ((2ull << d.shift) < d.per) ++d.shift;
     if (d.per > 1) d.inverse = (uint32_t)(((1ull << (32 + d.shift)) + d.per - 1) / d.per);
     return d;
@@ -42,6 +43,7 @@ struct AttentionCut {
     uint32_t tiles;  // of all items
     uint32_t run;    // tiles of a block's run, or of a piece at most
     uint32_t mode;
+    uint32_t shift;  // of a tile's tokens
 };
 
 // `tiles`: of all items, `items`: those that have any, `longest`: tiles of the longest one.
@@ -49,8 +51,9 @@ struct AttentionCut {
 //     holds for run >= tiles / (blocks - items).
 //   * Items that are short against a run stay whole: what a block does more than another is less than joining cut items takes.
 //   * Otherwise all blocks take the same number of tiles.
-Q4_PLAN_FN AttentionCut attention_cut(uint32_t tiles, uint32_t items, uint32_t longest, uint32_t blocks, uint32_t least) {
+Q4_PLAN_FN AttentionCut attention_cut(uint32_t tiles, uint32_t items, uint32_t longest, uint32_t blocks, uint32_t least, uint32_t shift) {
     AttentionCut c;
+    c.shift = shift;
     c.tiles = tiles;
     c.mode = items <= blocks / 2 ? kEqualPieces : kEqualRuns;
     const uint32_t by = c.mode == kEqualPieces ? blocks - items : blocks;
@@ -81,7 +84,7 @@ struct AttentionCursor {
     int32_t length;
     uint32_t left;   // tiles of the share from `begin` on; whole items: where the block's run ends
     uint32_t first;  // runs: number of the sequence's first tile among the tiles of all items
-    uint32_t whole;
+    uint32_t whole, shift;
 
     Q4_PLAN_FN void close() { end = whole || tiles - begin < left ? tiles : begin + left; }
     Q4_PLAN_FN bool mine() const { return first + item * tiles + tiles / 2 < left; }  // whole items: middle in the run
@@ -94,7 +97,8 @@ struct AttentionCursor {
         const uint32_t local = target - before;
         s = sequence;
         length = (int32_t)tokens;
-        tiles = attention_tiles(tokens);
+        shift = cut.shift;
+        tiles = attention_tiles(tokens, shift);
         first = before;
         piece = 0;
         pieces = 1;
@@ -137,7 +141,7 @@ struct AttentionCursor {
                 if (++s >= sequences) return false;
                 const int64_t tokens = lengths(s);
                 length = (int32_t)tokens;
-                tiles = attention_tiles(tokens);
+                tiles = attention_tiles(tokens, shift);
             } while (tiles == 0);
         }
         if (whole && !mine()) return false;

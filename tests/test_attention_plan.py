@@ -20,14 +20,14 @@ def shim():
     subprocess.check_call(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-o", out, os.path.join(ROOT, "tests", "attention_plan_shim.cpp")])
     lib = C.CDLL(out)
     lib.shim_attention_plan.restype = C.c_uint64
-    lib.shim_attention_plan.argtypes = [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint64]
+    lib.shim_attention_plan.argtypes = [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint64]
     return lib
 
 
-def _plan(lib, lengths, items, blocks):
+def _plan(lib, lengths, items, blocks, shift=0):
     lengths = np.asarray(lengths, dtype=np.int64)
     out = np.zeros((300000, 7), dtype=np.uint64)
-    n = lib.shim_attention_plan(lengths.ctypes.data, len(lengths), items, blocks, LEAST, out.ctypes.data, len(out))
+    n = lib.shim_attention_plan(lengths.ctypes.data, len(lengths), items, blocks, LEAST >> shift, shift, out.ctypes.data, len(out))
     assert n < len(out)
     return out[:n].astype(np.int64)
 
@@ -38,8 +38,9 @@ CASES = [([1], 1), ([37], 4), ([0, 0, 5, 0], 4), ([262144], 4), ([8200], 4), ([1
 
 @pytest.mark.parametrize("blocks", [1, 2, 7, 132, 148, 160])
 @pytest.mark.parametrize("lengths,items", CASES)
-def test_every_tile_once_and_partial_results_apart(shim, lengths, items, blocks):
-    plan = _plan(shim, lengths, items, blocks)
+@pytest.mark.parametrize("shift", [0, 2])
+def test_every_tile_once_and_partial_results_apart(shim, lengths, items, blocks, shift):
+    plan = _plan(shim, lengths, items, blocks, shift)
     by_item, places, owned = defaultdict(list), set(), defaultdict(set)
     for block, s, item, begin, end, owner, count in plan.tolist():
         assert end > begin
@@ -47,7 +48,7 @@ def test_every_tile_once_and_partial_results_apart(shim, lengths, items, blocks)
     assert set(by_item) == {(s, i) for s, n in enumerate(lengths) if n > 0 for i in range(items)}
     for (s, item), parts in by_item.items():
         assert [p[2] for p in parts] == sorted(p[2] for p in parts)
-        assert parts[0][0] == 0 and parts[-1][1] == -(-lengths[s] // 16)
+        assert parts[0][0] == 0 and parts[-1][1] == -(-lengths[s] // (16 << shift))
         assert all(a[1] == b[0] for a, b in zip(parts, parts[1:]))
         if len(parts) == 1:
             continue
@@ -88,4 +89,5 @@ def test_division_by_page_size(shim):
         tiles = [0, 1, per - 1, per, per + 1, 2 ** 27 - 1, 2 ** 27 - per] + rng.integers(0, 2 ** 27, 200).tolist()
         tiles += [per * k + d for k in rng.integers(1, 2 ** 27 // per, 50).tolist() for d in (-1, 0)]
         for t in tiles:
-            assert shim.shim_attention_page_of(16 * per, int(t)) == t // per
+            for shift in (0, 2):
+                assert shim.shim_attention_page_of((16 << shift) * per, shift, int(t)) == t // per
