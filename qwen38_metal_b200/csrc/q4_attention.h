@@ -97,9 +97,9 @@ struct AttentionParams {
 }  // namespace q4
 
 extern "C" {
-cudaError_t q4k_rotary(const q4::RotaryParams *p, cudaStream_t stream);
-cudaError_t q4k_kv_write(const q4::KvTokensParams *p, cudaStream_t stream);
-cudaError_t q4k_kv_read(const q4::KvTokensParams *p, cudaStream_t stream);
+cudaError_t q4k_rotary(const q4::RotaryParams *p, uint32_t sm_count, cudaStream_t stream);
+cudaError_t q4k_kv_write(const q4::KvTokensParams *p, uint32_t sm_count, cudaStream_t stream);
+cudaError_t q4k_kv_read(const q4::KvTokensParams *p, uint32_t sm_count, cudaStream_t stream);
 size_t q4k_attention_part_floats(uint32_t sm_count);  // scratch of partial results; one counter a block, zero between launches
 cudaError_t q4k_attention(const q4::AttentionParams *p, uint32_t sm_count, cudaStream_t stream);
 }

@@ -331,7 +331,7 @@ extern "C" int q4b_rotary_device(q4b_runtime *rt, const q4b_rotary *rotary, cons
     p.out_is_f32 = out_dtype == Q4B_F32;
     std::lock_guard<std::recursive_mutex> lock(*v.mu);
     q4::DeviceGuard guard(v.device);
-    if (int st = launched(q4k_rotary(&p, (cudaStream_t)stream), "rotary launch")) return st;
+    if (int st = launched(q4k_rotary(&p, (uint32_t)v.sm_count, (cudaStream_t)stream), "rotary launch")) return st;
     ++*v.launches;
     return Q4B_OK;
 }
@@ -359,7 +359,7 @@ extern "C" int q4b_kv_write_device(q4b_runtime *rt, const q4b_kv_cache *cache, c
     p.kv.input_error = v.input_error;
     std::lock_guard<std::recursive_mutex> lock(*v.mu);
     q4::DeviceGuard guard(v.device);
-    if (int st = launched(q4k_kv_write(&p, (cudaStream_t)stream), "cache write launch")) return st;
+    if (int st = launched(q4k_kv_write(&p, (uint32_t)v.sm_count, (cudaStream_t)stream), "cache write launch")) return st;
     ++*v.launches;
     return Q4B_OK;
 }
@@ -385,7 +385,7 @@ extern "C" int q4b_kv_read_device(q4b_runtime *rt, const q4b_kv_cache *cache, co
     p.kv.input_error = v.input_error;
     std::lock_guard<std::recursive_mutex> lock(*v.mu);
     q4::DeviceGuard guard(v.device);
-    if (int st = launched(q4k_kv_read(&p, (cudaStream_t)stream), "cache read launch")) return st;
+    if (int st = launched(q4k_kv_read(&p, (uint32_t)v.sm_count, (cudaStream_t)stream), "cache read launch")) return st;
     ++*v.launches;
     return Q4B_OK;
 }
