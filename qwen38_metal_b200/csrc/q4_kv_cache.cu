@@ -10,19 +10,22 @@ namespace q4 {
 
 // ---- activations: eight values at a time, fp32 or bf16 ----
 
+__device__ __forceinline__ void unpack8_bf16(uint4 a, float (&v)[8]) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
 __device__ __forceinline__ void load8(const void *base, uint64_t at, uint32_t is_f32, float (&v)[8]) {
     if (is_f32) {
         const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
         const float4 a = p[0], b = p[1];
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else {
-        const uint4 a = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + at);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+        unpack8_bf16(*reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + at), v);
     }
 }
 
@@ -143,63 +146,77 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p, uint3
 // ---- codes ----
 
 // A code is the number nearest to x / scale, ties to even, for the exact quotient: reading back differs by whole codes where two
-// ways to divide disagree, so a product with 1 / scale alone is not enough. Scales below 2^-100 (whose reciprocal or residuals
-// leave the range of 32 bits) take a division in 64 bits.
-struct Divisor {
-    float scale, inverse, half;
-    bool tiny;
-    __device__ explicit Divisor(float s) : scale(s), inverse(1.0f / s), half(0.5f * s), tiny(s < 0x1p-100f) {}
-    // x * (1 / scale) is within 2^-16 of the quotient, so its nearest integer is off by one at most, and the residual
-    // x - q * scale, which one fused operation gives exactly, tells.
-    __device__ int int8(float x) const {
-        if (tiny) return scale > 0.f ? (int)fmin(fmax(rint((double)x / (double)scale), -127.0), 127.0) : 0;
-        float q = rintf(x * inverse);
-        const float t = fmaf(-q, scale, x);
-        const bool odd = ((int)q & 1) != 0;
-        if (t > half || (t == half && odd)) q += 1.f;
-        else if (t < -half || (t == -half && odd)) q -= 1.f;
-        return (int)q;
-    }
-    // The quotient rounded to odd: to 24 bits towards zero, the last bit set if anything was cut off. Rounding that to the 4 bits
-    // of an e4m3 number gives what rounding the exact quotient gives.
-    __device__ float odd(float x) const {
-        if (tiny) {
-            if (!(scale > 0.f)) return 0.f;
-            const double q = (double)x / (double)scale;
-            const float r = __double2float_rz(q);
-            return (double)r == q ? r : __uint_as_float(__float_as_uint(r) | 1u);
-        }
-        float r = x * inverse;
-        r = fmaf(fmaf(-r, scale, x), inverse, r);
-        const float e = fmaf(-r, scale, x);  // its sign is exact
-        uint32_t bits = __float_as_uint(r);
-        if (e == 0.f || r == 0.f) return r;
-        if ((__float_as_uint(e) ^ bits) >> 31) bits -= 1u;  // r lies beyond the quotient
-        return __uint_as_float(bits | 1u);
-    }
-};
+// ways to divide disagree, so a product with 1 / scale alone is not enough.
+constexpr float kTinyScale = 0x1p-80f;  // below it reciprocals or residuals leave the range of 32 bits
 
-__device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t format, const Divisor &by) {
+__device__ __forceinline__ uint32_t e4m3_pair(float a, float b) { return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3); }
+
+// The codes of quotients in 64 bits, which rounds no quotient of two 24-bit numbers onto or across the middle between two codes. For e4m3
+// the quotient goes to 24 bits towards zero with the last bit set if anything was cut off: rounding that to 4 bits is rounding it.
+template <int FMT>
+__device__ __noinline__ uint2 encode8_exactly(float4 a, float4 b, float scale) {
+    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     uint32_t w[2] = {0u, 0u};
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        uint32_t pair;
-        if (format == 1u) {
-            pair = ((uint32_t)by.int8(v[i]) & 0xffu) | (((uint32_t)by.int8(v[i + 1]) & 0xffu) << 8);
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+        const double q = scale > 0.f ? (double)v[i] / (double)scale : 0.0;
+        uint32_t code;
+        if (FMT == 1) {
+            code = (uint32_t)(int)fmin(fmax(rint(q), -127.0), 127.0) & 0xffu;
         } else {
-            pair = __nv_cvt_float2_to_fp8x2(make_float2(by.odd(v[i]), by.odd(v[i + 1])), __NV_SATFINITE, __NV_E4M3);
+            const float r = __double2float_rz(q);
+            code = e4m3_pair((double)r == q ? r : __uint_as_float(__float_as_uint(r) | 1u), 0.f) & 0xffu;
         }
-        w[i / 4] |= pair << (i % 4 * 8);
+        if (i < 4) w[0] |= code << (i * 8);
+        else w[1] |= code << (i * 8 - 32);
     }
     return make_uint2(w[0], w[1]);
 }
 
-__device__ __forceinline__ void decode8(uint2 c, uint32_t format, float scale, float (&v)[8]) {
+// int8: x * (1 / scale) is within 2^-22 of the quotient (relative). Where that could be on the other side of the middle between two codes, all
+// eight are done exactly: seldom (one in 10^5 values). e4m3: the middles are numbers of 5 bits, and bf16 values meet them often (every fourth
+// row has one: 3/4 of an even largest value, for one). So the product goes to the nearest number m of 5 bits; the sign of x - m * scale is
+// exact, and the number given to the conversion is on that side of m, or m itself.
+template <int FMT>
+__device__ __forceinline__ uint2 encode8(const float (&v)[8], float scale) {
+    const float inverse = 1.0f / scale;
+    bool sure = scale >= kTinyScale;
+    uint32_t w[2];
+    if (FMT == 1) {
+        // 1.5 * 2^23 + quotient: the sum is rounded to a whole number, whose low byte is the code. x - q * scale is exact.
+        uint32_t n[8];
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float m = fmaf(v[i], inverse, 12582912.f);
+            most = fmaxf(most, fabsf(fmaf(12582912.f - m, scale, v[i])));
+            n[i] = __float_as_uint(m);
+        }
+        sure = sure && most < 0.5f * scale;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[i] = __byte_perm(__byte_perm(n[4 * i], n[4 * i + 1], 0x0040), __byte_perm(n[4 * i + 2], n[4 * i + 3], 0x0040), 0x5410);
+    } else {
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float m = __uint_as_float(__float_as_uint(v[i] * inverse) + 0x40000u & 0xfff80000u), r = fmaf(-m, scale, v[i]);
+            q[i] = __fmaf_rz(r, inverse, m);
+            if (r != 0.f) q[i] = __uint_as_float(__float_as_uint(q[i]) | 1u);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[i] = e4m3_pair(q[4 * i], q[4 * i + 1]) | e4m3_pair(q[4 * i + 2], q[4 * i + 3]) << 16;
+    }
+    if (!sure) return encode8_exactly<FMT>(make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]), scale);
+    return make_uint2(w[0], w[1]);
+}
+
+template <int FMT>
+__device__ __forceinline__ void decode8(uint2 c, float scale, float (&v)[8]) {
     const uint32_t w[2] = {c.x, c.y};
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const uint32_t pair = (w[i / 4] >> (i % 4 * 8)) & 0xffffu;
-        if (format == 1u) {
+        if (FMT == 1) {
             v[i] = (float)(int8_t)(pair & 0xffu) * scale;
             v[i + 1] = (float)(int8_t)(pair >> 8) * scale;
         } else {
@@ -255,92 +272,124 @@ __device__ __forceinline__ Row row_of(uint32_t r, uint32_t kv_heads) {
 }
 
 constexpr uint32_t kMostTokens = 8;  // of a block
+constexpr uint32_t kRowsAhead = 4;   // rows that are on their way to a lane
 
 // A block writes up to kMostTokens tokens. Of several tokens with the same place the last one is kept: every block looks through the tokens
 // behind its own (most by one comparison with the range of its positions) while its first rows are on their way. Bound by memory for long
 // prompts, by latency for single tokens. (A block a token, whole warps for rows of any length: 27 us for 4096 tokens of
 // 2 x 4 x 256 fp32 values.)
-template <int LANES>
+template <int FMT, int LANES, bool TURN>
 __global__ void __launch_bounds__(256) kv_write_kernel(const KvTokensParams p, uint32_t block_tokens) {
-    __shared__ float2 cs[kMostTokens][kMaxHeadDim / 2];
+    __shared__ float2 cs[TURN ? kMostTokens : 1][kMaxHeadDim / 2];
     __shared__ Place places[kMostTokens];
     __shared__ uint32_t replaced;  // a bit a token: one behind it has the same place
     grid_dependency_wait();
     grid_dependents_launch();
     const uint64_t t0 = (uint64_t)blockIdx.x * block_tokens;
-    const uint32_t tokens = (uint32_t)min((uint64_t)block_tokens, p.tokens - t0);
+    const uint32_t tokens = (uint32_t)min((uint64_t)block_tokens, p.tokens - t0), pairs = p.rotary.pairs;
+    const uint32_t lane = threadIdx.x & 31u, part = lane % LANES, d = part * 8u, rows = tokens * 2 * p.kv.kv_heads;
+    const uint32_t step = (blockDim.x >> 5) * (32 / LANES);
+    float v[kRowsAhead][8];
+    uint32_t r0 = (threadIdx.x >> 5) * (32 / LANES);
+    const auto load_rows = [&]() {
+#pragma unroll
+        for (uint32_t k = 0; k < kRowsAhead; ++k) {
+            const uint32_t r = r0 + k * step + lane / LANES;
+            const Row row = row_of(min(r, rows - 1), p.kv.kv_heads);
+            const void *in = row.values ? p.v_in : p.k_in;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
+            if (r < rows && in && d < p.kv.head_dim) load8(in, (t0 + row.token) * (row.values ? p.v_stride : p.k_stride) + (uint64_t)row.head * p.kv.head_dim + d, p.is_f32, v[k]);
+        }
+    };
+    load_rows();
     if (threadIdx.x == 0) replaced = 0;
     if (threadIdx.x < tokens) places[threadIdx.x] = place_of(p, t0 + threadIdx.x);
     __syncthreads();
-    if (p.rotary.step && p.k_in)
-        for (uint32_t i = threadIdx.x; i < tokens * p.rotary.pairs; i += blockDim.x) {
-            const uint32_t t = i / p.rotary.pairs;
-            cs[t][i - t * p.rotary.pairs] = turn(p.rotary, i - t * p.rotary.pairs, places[t].position);
+    if (TURN)
+        for (uint32_t i = threadIdx.x; i < tokens * pairs; i += blockDim.x) {
+            const uint32_t t = i / pairs;
+            cs[t][i - t * pairs] = turn(p.rotary, i - t * pairs, places[t].position);
         }
     int32_t low = 0x7fffffff, high = -1;
     for (uint32_t t = 0; t < tokens; ++t)
         if (places[t].page != ~0u) low = min(low, places[t].position), high = max(high, places[t].position);
-#pragma unroll 8
-    for (uint64_t u = t0 + 1 + threadIdx.x; u < p.tokens; u += blockDim.x) {
-        const int32_t position = p.positions[u];
+    const auto compare = [&](uint64_t u, int32_t position) {
         if (position >= low && position <= high)
+#pragma unroll 1
             for (uint32_t t = 0; t < tokens; ++t)
                 if (position == places[t].position && u > t0 + t && sequence_of(p, u) == places[t].sequence) atomicOr(&replaced, 1u << t);
+    };
+    // the tokens behind the block's first, four at a time from the first whose position starts at 16 bytes
+    const uint64_t behind = t0 + 1, fours = min(p.tokens, behind + (0u - (uint32_t)((uintptr_t)(p.positions + behind) >> 2) & 3u)), last = fours + ((p.tokens - min(fours, p.tokens)) & ~3ull);
+    if (threadIdx.x < fours - min(behind, fours)) compare(behind + threadIdx.x, p.positions[behind + threadIdx.x]);
+    if (threadIdx.x < p.tokens - last) compare(last + threadIdx.x, p.positions[last + threadIdx.x]);
+#pragma unroll 2
+    for (uint64_t u = fours + 4 * threadIdx.x; u < last; u += 4 * blockDim.x) {
+        const int4 position = *reinterpret_cast<const int4 *>(p.positions + u);
+        if (min(min(position.x, position.y), min(position.z, position.w)) <= high && max(max(position.x, position.y), max(position.z, position.w)) >= low) {
+            compare(u, position.x);
+            compare(u + 1, position.y);
+            compare(u + 2, position.z);
+            compare(u + 3, position.w);
+        }
     }
     __syncthreads();
-    const uint32_t lane = threadIdx.x & 31u, part = lane % LANES, d = part * 8u, rows = tokens * 2 * p.kv.kv_heads;
-    const bool has = d < p.kv.head_dim;
-#pragma unroll 2
-    for (uint32_t r0 = (threadIdx.x >> 5) * (32 / LANES); r0 < rows; r0 += (blockDim.x >> 5) * (32 / LANES)) {
-        const uint32_t r = r0 + lane / LANES;
-        const Row row = row_of(min(r, rows - 1), p.kv.kv_heads);
-        const void *in = row.values ? p.v_in : p.k_in;
-        const Place a = places[row.token];
-        const bool writes = r < rows && in && a.page != ~0u && !(replaced >> row.token & 1u);
-        const uint64_t at = (t0 + row.token) * (row.values ? p.v_stride : p.k_stride) + (uint64_t)row.head * p.kv.head_dim;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (writes && has) load8(in, at + d, p.is_f32, v);
-        if (p.rotary.step && p.k_in) {
-            const bool turns = writes && !row.values && d < 2 * p.rotary.pairs;
-            if (p.rotary.interleaved) {
-                if (turns) turn_interleaved(v, d / 2, p.rotary.pairs, cs[row.token]);
-            } else if (p.rotary.pairs % 8 == 0) {
-                // the other values of the pairs are those of a lane of the same row
-                const uint32_t step = p.rotary.pairs / 8, other = (lane & ~(LANES - 1u)) + (part < step ? part + step : part - step) % LANES;
-                const uint32_t i = part < step ? d : d - p.rotary.pairs;
+#pragma unroll 1
+    for (;;) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float b = __shfl_sync(0xffffffffu, v[j], other);
-                    if (turns) v[j] = v[j] * cs[row.token][i + j].x + (part < step ? -b : b) * cs[row.token][i + j].y;
-                }
-            } else if (turns) {
+        for (uint32_t k = 0; k < kRowsAhead; ++k) {
+            const uint32_t r = r0 + k * step + lane / LANES;
+            if (r0 + k * step >= rows) break;
+            const Row row = row_of(min(r, rows - 1), p.kv.kv_heads);
+            const Place a = places[row.token];
+            const bool writes = r < rows && (row.values ? p.v_in : p.k_in) && a.page != ~0u && !(replaced >> row.token & 1u);
+            if (TURN) {
+                const bool turns = !row.values && d < 2 * pairs;
+                if (p.rotary.interleaved) {
+                    if (turns) turn_interleaved(v[k], d / 2, pairs, cs[row.token]);
+                } else if (pairs % 8 == 0) {
+                    // the other values of the pairs are those of a lane of the same row
+                    const uint32_t by = pairs / 8, other = (lane & ~(LANES - 1u)) + (part < by ? part + by : part - by) % LANES;
+                    const uint32_t i = part < by ? d : d - pairs;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t e = d + j, pairs = p.rotary.pairs;
-                    if (e < pairs) v[j] = v[j] * cs[row.token][e].x - load1(in, at + e + pairs, p.is_f32) * cs[row.token][e].y;
-                    else if (e < 2 * pairs) v[j] = v[j] * cs[row.token][e - pairs].x + load1(in, at + e - pairs, p.is_f32) * cs[row.token][e - pairs].y;
+                    for (int j = 0; j < 8; ++j) {
+                        const float b = __shfl_sync(0xffffffffu, v[k][j], other);
+                        if (turns) v[k][j] = v[k][j] * cs[row.token][i + j].x + (part < by ? -b : b) * cs[row.token][i + j].y;
+                    }
+                } else if (turns && writes) {
+                    const uint64_t at = (t0 + row.token) * p.k_stride + (uint64_t)row.head * p.kv.head_dim;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t e = d + j;
+                        if (e < pairs) v[k][j] = v[k][j] * cs[row.token][e].x - load1(p.k_in, at + e + pairs, p.is_f32) * cs[row.token][e].y;
+                        else if (e < 2 * pairs) v[k][j] = v[k][j] * cs[row.token][e - pairs].x + load1(p.k_in, at + e - pairs, p.is_f32) * cs[row.token][e - pairs].y;
+                    }
                 }
             }
-        }
-        uint8_t *const to = (row.values ? p.kv.v : p.kv.k) + (writes ? row_offset(p.kv, a, row.head) : 0);
-        if (p.kv.format == 0u) {
-            if (writes && has) *reinterpret_cast<uint4 *>(to + 2 * d) = pack8_bf16(v);
-            continue;
-        }
-        uint32_t amax = 0;
+            uint8_t *const to = (row.values ? p.kv.v : p.kv.k) + (writes ? row_offset(p.kv, a, row.head) : 0);
+            const bool has = writes && d < p.kv.head_dim;
+            if (FMT == 0) {
+                if (has) *reinterpret_cast<uint4 *>(to + 2 * d) = pack8_bf16(v[k]);
+                continue;
+            }
+            uint32_t amax = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+            for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[k][j]) & 0x7fffffffu);
 #pragma unroll
-        for (int off = LANES / 2; off > 0; off >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-        const bool finite = amax < 0x7f800000u;
-        const float scale = finite ? __fdiv_rn(__uint_as_float(amax), p.kv.format == 1u ? 127.f : 448.f) : __uint_as_float(0x7fc00000u);
-        const Divisor by(scale);
-        if (writes && has) *reinterpret_cast<uint2 *>(to + d) = finite ? encode8(v, p.kv.format, by) : make_uint2(0u, 0u);
-        if (writes && part == 0) (row.values ? p.kv.v_scales : p.kv.k_scales)[scale_index(p.kv, a, row.head)] = scale;
+            for (int off = LANES / 2; off > 0; off >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+            const bool finite = amax < 0x7f800000u;
+            const float scale = finite ? __fdiv_rn(__uint_as_float(amax), FMT == 1 ? 127.f : 448.f) : __uint_as_float(0x7fc00000u);
+            if (has) *reinterpret_cast<uint2 *>(to + d) = finite ? encode8<FMT == 0 ? 1 : FMT>(v[k], scale) : make_uint2(0u, 0u);
+            if (writes && part == 0) (row.values ? p.kv.v_scales : p.kv.k_scales)[scale_index(p.kv, a, row.head)] = scale;
+        }
+        r0 += kRowsAhead * step;
+        if (r0 >= rows) break;
+        load_rows();
     }
 }
 
-template <int LANES>
+template <int FMT, int LANES>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvTokensParams p, uint32_t block_tokens) {
     __shared__ Place places[kMostTokens];
     grid_dependency_wait();
@@ -349,30 +398,64 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvTokensParams p, ui
     const uint32_t tokens = (uint32_t)min((uint64_t)block_tokens, p.tokens - t0);
     if (threadIdx.x < tokens) places[threadIdx.x] = place_of(p, t0 + threadIdx.x);
     __syncthreads();
-    const uint32_t lane = threadIdx.x & 31u, d = lane % LANES * 8u, rows = tokens * 2 * p.kv.kv_heads;
+    const uint32_t lane = threadIdx.x & 31u, d = lane % LANES * 8u, rows = tokens * 2 * p.kv.kv_heads, step = (blockDim.x >> 5) * (32 / LANES);
     if (d >= p.kv.head_dim) return;
-#pragma unroll 4
-    for (uint32_t r = (threadIdx.x >> 5) * (32 / LANES) + lane / LANES; r < rows; r += (blockDim.x >> 5) * (32 / LANES)) {
-        const Row row = row_of(r, p.kv.kv_heads);
-        void *out = row.values ? p.v_out : p.k_out;
-        const Place a = places[row.token];
-        if (!out || a.page == ~0u) continue;
-        const uint8_t *from = (row.values ? p.kv.v : p.kv.k) + row_offset(p.kv, a, row.head);
-        float v[8];
-        if (p.kv.format == 0u) load8(from, d, 0u, v);
-        else decode8(*reinterpret_cast<const uint2 *>(from + d), p.kv.format, (row.values ? p.kv.v_scales : p.kv.k_scales)[scale_index(p.kv, a, row.head)], v);
-        store8(out, (t0 + row.token) * (row.values ? p.v_stride : p.k_stride) + (uint64_t)row.head * p.kv.head_dim + d, p.is_f32, v);
+#pragma unroll 1
+    for (uint32_t r0 = (threadIdx.x >> 5) * (32 / LANES) + lane / LANES; r0 < rows; r0 += kRowsAhead * step) {
+        uint4 held[kRowsAhead];
+        float scale[kRowsAhead];
+        bool there[kRowsAhead];
+#pragma unroll
+        for (uint32_t k = 0; k < kRowsAhead; ++k) {
+            const uint32_t r = r0 + k * step;
+            const Row row = row_of(min(r, rows - 1), p.kv.kv_heads);
+            const Place a = places[row.token];
+            there[k] = r < rows && (row.values ? p.v_out : p.k_out) && a.page != ~0u;
+            held[k] = make_uint4(0u, 0u, 0u, 0u);
+            scale[k] = 1.f;
+            if (!there[k]) continue;
+            const uint8_t *from = (row.values ? p.kv.v : p.kv.k) + row_offset(p.kv, a, row.head);
+            if (FMT == 0) {
+                held[k] = *reinterpret_cast<const uint4 *>(from + 2 * d);
+            } else {
+                const uint2 c = *reinterpret_cast<const uint2 *>(from + d);
+                held[k].x = c.x, held[k].y = c.y;
+                scale[k] = (row.values ? p.kv.v_scales : p.kv.k_scales)[scale_index(p.kv, a, row.head)];
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kRowsAhead; ++k) {
+            if (!there[k]) continue;
+            const Row row = row_of(r0 + k * step, p.kv.kv_heads);
+            float v[8];
+            if (FMT == 0) unpack8_bf16(held[k], v);
+            else decode8<FMT == 0 ? 1 : FMT>(make_uint2(held[k].x, held[k].y), scale[k], v);
+            store8(row.values ? p.v_out : p.k_out, (t0 + row.token) * (row.values ? p.v_stride : p.k_stride) + (uint64_t)row.head * p.kv.head_dim + d, p.is_f32, v);
+        }
     }
 }
 
 // Tokens of a block: few tokens go to as many blocks as there are, many in eights.
-uint32_t block_tokens(uint64_t tokens, uint32_t sm_count) { return (uint32_t)(tokens / (4ull * sm_count) < kMostTokens ? tokens / (4ull * sm_count) + 1 : kMostTokens); }
+uint32_t block_tokens(uint64_t tokens, uint32_t sm_count) { return (uint32_t)(tokens / (8ull * sm_count) < kMostTokens ? tokens / (8ull * sm_count) + 1 : kMostTokens); }
 
-template <typename Kernel>
-cudaError_t launch_tokens(Kernel lanes8, Kernel lanes16, Kernel lanes32, const KvTokensParams &p, uint32_t sm_count, cudaStream_t stream) {
+template <int FMT, int LANES>
+cudaError_t launch_tokens(const KvTokensParams &p, bool write, uint32_t sm_count, cudaStream_t stream) {
     const uint32_t each = block_tokens(p.tokens, sm_count);
-    const Kernel kernel = p.kv.head_dim <= 64 ? lanes8 : p.kv.head_dim <= 128 ? lanes16 : lanes32;
+    const auto kernel = !write ? kv_read_kernel<FMT, LANES> : p.rotary.step && p.k_in ? kv_write_kernel<FMT, LANES, true> : kv_write_kernel<FMT, LANES, false>;
     return launch_dependent(kernel, dim3((uint32_t)((p.tokens + each - 1) / each)), 256, 0, stream, p, each);
+}
+
+template <int FMT>
+cudaError_t launch_tokens(const KvTokensParams &p, bool write, uint32_t sm_count, cudaStream_t stream) {
+    if (p.kv.head_dim <= 64) return launch_tokens<FMT, 8>(p, write, sm_count, stream);
+    if (p.kv.head_dim <= 128) return launch_tokens<FMT, 16>(p, write, sm_count, stream);
+    return launch_tokens<FMT, 32>(p, write, sm_count, stream);
+}
+
+cudaError_t launch_tokens(const KvTokensParams &p, bool write, uint32_t sm_count, cudaStream_t stream) {
+    if (p.kv.format == 0u) return launch_tokens<0>(p, write, sm_count, stream);
+    if (p.kv.format == 1u) return launch_tokens<1>(p, write, sm_count, stream);
+    return launch_tokens<2>(p, write, sm_count, stream);
 }
 
 }  // namespace q4
@@ -385,9 +468,9 @@ extern "C" cudaError_t q4k_rotary(const q4::RotaryParams *p, uint32_t sm_count, 
 }
 
 extern "C" cudaError_t q4k_kv_write(const q4::KvTokensParams *p, uint32_t sm_count, cudaStream_t stream) {
-    return q4::launch_tokens(q4::kv_write_kernel<8>, q4::kv_write_kernel<16>, q4::kv_write_kernel<32>, *p, sm_count, stream);
+    return q4::launch_tokens(*p, true, sm_count, stream);
 }
 
 extern "C" cudaError_t q4k_kv_read(const q4::KvTokensParams *p, uint32_t sm_count, cudaStream_t stream) {
-    return q4::launch_tokens(q4::kv_read_kernel<8>, q4::kv_read_kernel<16>, q4::kv_read_kernel<32>, *p, sm_count, stream);
+    return q4::launch_tokens(*p, false, sm_count, stream);
 }
