@@ -313,24 +313,33 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
     int32_t low = 0x7fffffff, high = -1;
     for (uint32_t t = 0; t < tokens; ++t)
         if (places[t].stands) low = min(low, places[t].position), high = max(high, places[t].position);
+    // Tokens behind the block's first are looked through four at a time, from the first whose position starts at 16 bytes. Runs of one length
+    // end the search with the last token's own.
+    const uint64_t behind = t0 + 1, end = p.sequences ? p.tokens : min(p.tokens, (t0 + tokens - 1) / p.run * p.run + p.run);
+    const uint64_t fours = min(end, behind + (0u - (uint32_t)((uintptr_t)(p.positions + behind) >> 2) & 3u)), last = fours + ((end - min(fours, end)) & ~3ull);
     const auto compare = [&](uint64_t u, int32_t position) {
-        if (position >= low && position <= high)
+        if (position < low || position > high) return;
+        const int32_t sequence = sequence_of(p, u);
 #pragma unroll 1
-            for (uint32_t t = 0; t < tokens; ++t)
-                if (position == places[t].position && u > t0 + t && sequence_of(p, u) == places[t].sequence) atomicOr(&replaced, 1u << t);
+        for (uint32_t t = 0; t < tokens; ++t)
+            if (position == places[t].position && sequence == places[t].sequence && u > t0 + t) atomicOr(&replaced, 1u << t);
     };
-    // the tokens behind the block's first, four at a time from the first whose position starts at 16 bytes
-    const uint64_t behind = t0 + 1, fours = min(p.tokens, behind + (0u - (uint32_t)((uintptr_t)(p.positions + behind) >> 2) & 3u)), last = fours + ((p.tokens - min(fours, p.tokens)) & ~3ull);
     if (threadIdx.x < fours - min(behind, fours)) compare(behind + threadIdx.x, p.positions[behind + threadIdx.x]);
-    if (threadIdx.x < p.tokens - last) compare(last + threadIdx.x, p.positions[last + threadIdx.x]);
+    if (threadIdx.x < end - last) compare(last + threadIdx.x, p.positions[last + threadIdx.x]);
 #pragma unroll 2
     for (uint64_t u = fours + 4 * threadIdx.x; u < last; u += 4 * blockDim.x) {
         const int4 position = *reinterpret_cast<const int4 *>(p.positions + u);
-        if (min(min(position.x, position.y), min(position.z, position.w)) <= high && max(max(position.x, position.y), max(position.z, position.w)) >= low) {
-            compare(u, position.x);
-            compare(u + 1, position.y);
-            compare(u + 2, position.z);
-            compare(u + 3, position.w);
+        if (min(min(position.x, position.y), min(position.z, position.w)) > high || max(max(position.x, position.y), max(position.z, position.w)) < low) continue;
+        const int32_t at[4] = {position.x, position.y, position.z, position.w};
+        int32_t sequence[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sequence[i] = sequence_of(p, u + i);
+#pragma unroll 1
+        for (uint32_t t = 0; t < tokens; ++t) {
+            bool same = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) same = same || (at[i] == places[t].position && sequence[i] == places[t].sequence && u + i > t0 + t);
+            if (same) atomicOr(&replaced, 1u << t);
         }
     }
     __syncthreads();
