@@ -105,7 +105,7 @@ typedef struct q4b_job {
 
 /* ---- runtime ---- */
 
-/* MetalRuntime::new, src/metal_runtime.rs:642-927. Sets aside about 57 MB of device scratch. Options are latched from the environment
+/* MetalRuntime::new, src/metal_runtime.rs:642-927. Sets aside about 62 MB of device scratch. Options are latched from the environment
  * once, here (the reference reads QWEN38_* variables, :916-925): Q4B_FORCE_VARIANT. */
 int q4b_runtime_create(int device_ordinal, q4b_runtime **out);
 void q4b_runtime_destroy(q4b_runtime *rt);

@@ -3,8 +3,8 @@
 //
 //     out = sum_j p_j v_j / sum_j p_j,   p_j = e^(scale q.k_j)
 //
-// Every key and value is read once from memory for eight query rows (token, head) that share its key head: at one byte a value that is
-// 12 to 16 operations a byte, so memory is the bound, and the kernel is built around keeping loads in flight.
+// Every key and value is read once from memory for 8, 16 or 24 query rows (token, head) that share its key head: at one byte a value and 8 rows
+// that is 12 to 16 operations a byte, so memory is the bound, and the kernel is built around keeping loads in flight.
 //
 //   * One block per SM: eight warps that multiply and one that asks for tiles with tensor copies into a ring in shared memory, keys of
 //     128 tokens (256 where rows are short) and their values in turn, past the end of an item too: 190 KB are in flight while results
@@ -37,8 +37,9 @@
 
 namespace q4 {
 
-constexpr uint32_t kWarps = 8, kMultipliers = kWarps * 32, kThreads = kMultipliers + 32;  // the last warp asks for tiles
+constexpr uint32_t kWarps = 8, kMultipliers = kWarps * 32, kThreads = kMultipliers + 32, kAllWarps = kWarps + 1;  // the last warp asks for tiles
 constexpr uint32_t kMostBlocks = 256;           // of a launch
+constexpr uint32_t kMostSets = 3;               // of eight query rows that a block takes through a tile together
 constexpr uint32_t kLeastRun = 16;              // tiles: shorter runs cost more in joining than they save
 constexpr float kNone = -3.0e38f;               // a reference below all scores: the row has seen nothing
 constexpr float kHeadroom = 8.f;                // how far above its reference a score may lie, in powers of two
@@ -53,8 +54,9 @@ struct Weights {
 constexpr unsigned long long kWaitLimitNs = 200ull * 1000 * 1000, kLateLimitNs = 1000 * 1000;
 constexpr uint32_t kSharedLimit = 227 * 1024;
 
-template <int FMT, int HDP>
+template <int FMT, int HDP, int SETS>
 struct Shape {
+    static constexpr uint32_t kRows = SETS * kAttentionRows;         // query rows of an item
     static constexpr uint32_t kRow = HDP * (FMT == 0 ? 2 : 1);       // bytes of a token's row in shared memory
     static constexpr uint32_t kSeg = kRow < 128 ? kRow : 128;        // swizzled together
     static constexpr uint32_t kSegs = kRow / kSeg;
@@ -63,6 +65,7 @@ struct Shape {
     static constexpr uint32_t kSubs = kWarps * kOwnSubs;             // of a tile
     static constexpr uint32_t kSlot = kSubs * kSub;                  // of the ring: keys, or values, of a tile
     static constexpr uint32_t kPieces = kSeg / 64;                   // 16-byte pieces of a segment a lane takes from a key row
+    static constexpr uint32_t kWords = FMT == 2 ? 8 : 4;             // registers of a 16-byte piece as it is multiplied
     static constexpr uint32_t kMmas = HDP / 16;                      // per 8 tokens of scores
     static constexpr uint32_t kChunkDims = FMT == 0 ? 8 : 16;        // of a 16-byte piece
     static constexpr uint32_t kValueWarps = HDP / kChunkDims < kWarps ? HDP / kChunkDims : kWarps;  // that have dimensions of the values
@@ -70,16 +73,17 @@ struct Shape {
     static constexpr uint32_t kChunks = kWarpDims / kChunkDims;
     static constexpr uint32_t kAcc = kWarpDims / 8;                  // accumulators of four numbers
     static constexpr uint32_t kOwn = kWarpDims / 4;                  // numbers of a row's result in a lane
-    static constexpr bool kQueriesStay = HDP < 256;      // in registers
+    static constexpr bool kQueriesStay = HDP < 256 && SETS == 1;  // in registers
+    static constexpr uint32_t kTogether = SETS < 3 ? 2 * kOwnSubs : 2;   // eights of tokens whose scores are computed together
     // shared memory: ring, scales of its keys and values, weights, queries, barriers, small arrays
     static constexpr uint32_t kScales = FMT == 0 ? 0 : 2 * kSubs * 64;  // of a slot
-    static constexpr uint32_t kQueries = kMmas * 32 * 16;
-    static constexpr uint32_t kWeights = kSubs * 32 * 16;               // of a tile; there are two
-    static constexpr uint32_t kSmall = 2048;
+    static constexpr uint32_t kSetQueries = kMmas * 32 * 16, kQueries = SETS * kSetQueries;
+    static constexpr uint32_t kSetWeights = kSubs * 32 * 16, kWeights = SETS * kSetWeights;  // of a tile; there are two
+    static constexpr uint32_t kSmall = (3 * kWarps + 1) * kRows * 4 + 3 * kAllWarps * 4 + 12 * 4;
     static constexpr uint32_t kFit = (kSharedLimit - 1024 - kQueries - 2 * kWeights - kSmall) / (kSlot + kScales + 16);
     static constexpr uint32_t kSlots = kFit < 16 ? kFit : 16;
     static constexpr uint32_t kShared = 1024 + kSlots * (kSlot + kScales + 16) + kQueries + 2 * kWeights + kSmall;
-    static_assert(kSlots >= 2 && kSubs * kSegs <= 32 && 2 * kWeights >= kMostBlocks * kAttentionRows * 4, "");
+    static_assert(kSlots >= 2 && kSubs * kSegs <= 32 && 2 * kWeights >= kMostBlocks * kRows * 4 && kSmall % 4 == 0 && kShared <= kSharedLimit, "");
 };
 
 // ---- small pieces ----
@@ -226,7 +230,7 @@ __device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.a
 // ---- a block's share ----
 
 struct Geometry {
-    uint32_t chunks;  // items of a key head: eight query rows each
+    uint32_t chunks;  // items of a key head: 8, 16 or 24 query rows each
     uint32_t heads;   // items of a sequence = key heads * chunks
     uint32_t rows;    // query rows of a key head
     uint32_t group;   // query heads of a key head
@@ -256,8 +260,6 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v, uint32_t lane) {
     }
     return v;
 }
-
-constexpr uint32_t kAllWarps = kThreads / 32;
 
 // All threads. `scratch`: 3 * kAllWarps words in shared memory. Up to 32 sequences every warp finds it by itself.
 __device__ __forceinline__ Share share_of_block(const AttentionParams &p, const Geometry &g, uint32_t *scratch) {
@@ -348,10 +350,10 @@ struct Turn {
 
 // A lane brings a tile, or one segment of it where rows are not a whole number of segments; scales come in 16-byte pieces, two a lane.
 // Page numbers are read while the slot that comes next is still in use.
-template <int FMT, int HDP>
+template <int FMT, int HDP, int SETS>
 __device__ __forceinline__ void ask_for_tiles(const AttentionParams &p, const Geometry &g, Cursor at, const CUtensorMap *k_map, const CUtensorMap *v_map, uint32_t ring, uint32_t scales,
                                               uint32_t full, uint32_t empty, uint32_t lane) {
-    using S = Shape<FMT, HDP>;
+    using S = Shape<FMT, HDP, SETS>;
     const uint32_t per = g.whole_rows ? 1 : S::kSegs, mine = lane / per, seg = lane % per;
     const auto lengths = [&](uint32_t i) { return length_of(p, i); };
     unsigned long long limit_ns = kWaitLimitNs;
@@ -406,18 +408,18 @@ __device__ __forceinline__ void ask_for_tiles(const AttentionParams &p, const Ge
 
 // ---- the kernel ----
 
-template <int FMT, int HDP>
+template <int FMT, int HDP, int SETS>
 __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ Geometry g, const __grid_constant__ CUtensorMap k_map,
                                                                 const __grid_constant__ CUtensorMap v_map) {
-    using S = Shape<FMT, HDP>;
+    using S = Shape<FMT, HDP, SETS>;
     extern __shared__ uint8_t shared_raw[];
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(shared_raw), pad = (1024u - (raw & 1023u)) & 1023u;
     const uint32_t ring = raw + pad, scales = ring + S::kSlots * S::kSlot, weights = scales + S::kSlots * S::kScales, queries = weights + 2 * S::kWeights,
                    full = queries + S::kQueries, empty = full + S::kSlots * 8, joined = empty + S::kSlots * 8;
     float *const small = reinterpret_cast<float *>(shared_raw + (joined + 16 - raw));
-    float *const highs = small, *const weight_highs = small + kWarps * kAttentionRows, *const sums = small + 2 * kWarps * kAttentionRows;  // [warp][row]
-    float *const row_scales = small + 3 * kWarps * kAttentionRows;                                                                         // [row] scale of the scores, in powers of two
-    uint32_t *const scratch = reinterpret_cast<uint32_t *>(row_scales + kAttentionRows), *const joins = scratch + 3 * kAllWarps;  // joins: 2 of 6 words
+    float *const highs = small, *const weight_highs = small + kWarps * S::kRows, *const sums = small + 2 * kWarps * S::kRows;  // [warp][row]
+    float *const row_scales = small + 3 * kWarps * S::kRows;                                                                         // [row] scale of the scores, in powers of two
+    uint32_t *const scratch = reinterpret_cast<uint32_t *>(row_scales + S::kRows), *const joins = scratch + 3 * kAllWarps;  // joins: 2 of 6 words
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row = lane >> 2, quad = lane & 3u;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < S::kSlots; ++i) {
@@ -434,47 +436,53 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const Share share = share_of_block(p, g, scratch);
     const auto lengths = [&](uint32_t i) { return length_of(p, i); };
     if (share.any && warp == kWarps) {
-        ask_for_tiles<FMT, HDP>(p, g, share.at, &k_map, &v_map, ring, scales, full, empty, lane);
+        ask_for_tiles<FMT, HDP, SETS>(p, g, share.at, &k_map, &v_map, ring, scales, full, empty, lane);
     } else if (share.any) {
         Turn<S::kSlots> turn;
         unsigned long long limit_ns = kWaitLimitNs;
         uint32_t weights_at = weights;  // one of two
         Cursor at = share.at;
-        // eight values of query row `warp` of an item
-        float q[8];
+        // eight values of query row `warp` of each set of eight; those of the next item are on their way meanwhile where registers allow
+        constexpr bool kAhead = SETS == 1;
+        float q[SETS][8];
         const auto load_query = [&](const Cursor &c) {
-            const uint32_t r = c.item % g.chunks * kAttentionRows + warp, d = lane * 8;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = 0.f;
-            if (r < g.rows && d < p.kv.head_dim) {
-                const uint64_t base = ((uint64_t)c.s * p.q_tokens + r / g.group) * p.q_stride + ((uint64_t)(c.item / g.chunks) * g.group + r % g.group) * p.kv.head_dim + d;
-                if (p.q_is_f32) {
-                    const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + base);
-                    const float4 v = __ldcg(f), w = __ldcg(f + 1);
-                    q[0] = v.x, q[1] = v.y, q[2] = v.z, q[3] = v.w, q[4] = w.x, q[5] = w.y, q[6] = w.z, q[7] = w.w;
-                } else {
-                    const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + base));
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            for (uint32_t set = 0; set < SETS; ++set) {
+                const uint32_t r = c.item % g.chunks * S::kRows + set * kAttentionRows + warp, d = lane * 8;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) q[2 * i] = __uint_as_float(w[i] << 16), q[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                for (int i = 0; i < 8; ++i) q[set][i] = 0.f;
+                if (r < g.rows && d < p.kv.head_dim) {
+                    const uint64_t base = ((uint64_t)c.s * p.q_tokens + r / g.group) * p.q_stride + ((uint64_t)(c.item / g.chunks) * g.group + r % g.group) * p.kv.head_dim + d;
+                    if (p.q_is_f32) {
+                        const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + base);
+                        const float4 v = __ldcg(f), w = __ldcg(f + 1);
+                        q[set][0] = v.x, q[set][1] = v.y, q[set][2] = v.z, q[set][3] = v.w, q[set][4] = w.x, q[set][5] = w.y, q[set][6] = w.z, q[set][7] = w.w;
+                    } else {
+                        const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + base));
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) q[set][2 * i] = __uint_as_float(w[i] << 16), q[set][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                    }
                 }
             }
         };
-        load_query(at);
-        constexpr uint32_t kPart = kAttentionRows * (kMaxHeadDim + 2);  // numbers of a partial result: rows, then maxima, then sums
+        if (kAhead) load_query(at);
+        constexpr uint32_t kPart = S::kRows * (kMaxHeadDim + 2);  // numbers of a partial result: rows, then maxima, then sums
         uint32_t left_parts = 0;  // partial results this block has left: two at most
         bool more;
         do {
             // ---- queries of the item: warp w splits row w into halves, or digits, in the order in which key rows are read ----
             const uint32_t head = at.item / g.chunks, chunk = at.item % g.chunks;
-            {
+            if (!kAhead) load_query(at);
+#pragma unroll
+            for (uint32_t set = 0; set < SETS; ++set) {
                 const uint32_t d = lane * 8;
                 float unit = 1.f, row_scale = p.scale * 1.4426950408889634f;
                 if (FMT != 0) {
                     // fp16 halves, whole numbers: the row is scaled by a power of two that brings its largest value into [1, 2)
                     uint32_t amax = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(q[i]) & 0x7fffffffu);
+                    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(q[set][i]) & 0x7fffffffu);
                     amax = __reduce_max_sync(0xffffffffu, amax);
                     const uint32_t e = min(max(amax >> 23, 1u), 254u);
                     unit = e == 254u ? __uint_as_float(0x00400000u) : __uint_as_float((254u - e) << 23);
@@ -486,212 +494,267 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     // a lane's part of an MMA is four values, of a whole-number one eight; a 16-byte piece of a key row holds 8 or 16
                     constexpr uint32_t kPer = S::kChunkDims / 4;
                     const uint32_t piece = d / S::kChunkDims, seg = piece / (S::kSeg / 16), in_seg = piece % (S::kSeg / 16);
-                    const uint32_t m = (seg * S::kPieces + in_seg % S::kPieces) * kPer + d % S::kChunkDims / 4, to = queries + (m * 32 + warp * 4 + in_seg / S::kPieces) * 16;
+                    const uint32_t m = (seg * S::kPieces + in_seg % S::kPieces) * kPer + d % S::kChunkDims / 4, to = queries + set * S::kSetQueries + (m * 32 + warp * 4 + in_seg / S::kPieces) * 16;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) q[i] *= unit;
+                    for (int i = 0; i < 8; ++i) q[set][i] *= unit;
                     uint4 a, b;
                     if (FMT == 1) {
-                        split_digits(q, a, b);
+                        split_digits(q[set], a, b);
                     } else {
-                        split<FMT>(q[0], q[1], a.x, a.y);
-                        split<FMT>(q[2], q[3], a.z, a.w);
-                        split<FMT>(q[4], q[5], b.x, b.y);
-                        split<FMT>(q[6], q[7], b.z, b.w);
+                        split<FMT>(q[set][0], q[set][1], a.x, a.y);
+                        split<FMT>(q[set][2], q[set][3], a.z, a.w);
+                        split<FMT>(q[set][4], q[set][5], b.x, b.y);
+                        split<FMT>(q[set][6], q[set][7], b.z, b.w);
                     }
                     sts_v4(to, a);
                     sts_v4(to + 512, b);
                 }
-                if (lane == 0) row_scales[warp] = row_scale;
+                if (lane == 0) row_scales[set * kAttentionRows + warp] = row_scale;
             }
             multipliers_sync();
-            const float row_scale = row_scales[row];
+            float row_scale[SETS];
+#pragma unroll
+            for (uint32_t set = 0; set < SETS; ++set) row_scale[set] = row_scales[set * kAttentionRows + row];
             uint32_t qa[S::kMmas][4];  // (where registers are short, read again for every tile)
-            const auto fetch_query = [&](uint32_t m) {
-                const uint4 w = lds_v4(queries + (m * 32 + lane) * 16);
+            const auto fetch_query = [&](uint32_t set, uint32_t m) {
+                const uint4 w = lds_v4(queries + set * S::kSetQueries + (m * 32 + lane) * 16);
                 qa[m][0] = w.x, qa[m][1] = w.y, qa[m][2] = w.z, qa[m][3] = w.w;
             };
             if (S::kQueriesStay)
 #pragma unroll
-                for (uint32_t m = 0; m < S::kMmas; ++m) fetch_query(m);
+                for (uint32_t m = 0; m < S::kMmas; ++m) fetch_query(0, m);
             Cursor ahead = at;
             more = ahead.next(lengths, p.kv.sequences, g.heads);
-            if (more) load_query(ahead);
+            if (kAhead && more) load_query(ahead);
             // tokens of the segment that all rows see, that this row sees, and that exist
             const uint32_t shift = S::kSegs == 1 ? g.tile_shift : 0, end_sub = at.end << shift;
             const int32_t end_token = (int32_t)(end_sub * kTileTokens), existing = min(at.length, end_token);
             const int32_t sure = min(at.length - (int32_t)p.q_tokens + 1, end_token);
-            const uint32_t r = chunk * kAttentionRows + row;
-            const bool live = r < g.rows;
-            const int32_t limit = live ? min(at.length - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group), end_token) : 0;
+            const auto row_of = [&](uint32_t set) { return chunk * S::kRows + set * kAttentionRows + row; };
+            int32_t limit[SETS];
+#pragma unroll
+            for (uint32_t set = 0; set < SETS; ++set) limit[set] = row_of(set) < g.rows ? min(at.length - (int32_t)p.q_tokens + 1 + (int32_t)(row_of(set) / g.group), end_token) : 0;
             // Results. int8: o itself, from whole-number accumulators of a tile; else accumulators of the upper and lower halves
-            float o[FMT == 1 ? S::kOwn : 1], acc[FMT == 1 ? 1 : S::kAcc][4];
+            float o[SETS][FMT == 1 ? S::kOwn : 1], acc[SETS][FMT == 1 ? 1 : S::kAcc][4];
+            float top[SETS], sum[SETS];                          // reference of the row's scores; sum of this lane's weights
+            float weight_top[SETS], lift[SETS], most[SETS];      // 8-bit: reference of weights times scales, 2^(top - weight_top), and what they may be
 #pragma unroll
-            for (uint32_t i = 0; i < (FMT == 1 ? S::kOwn : 1); ++i) o[i] = 0.f;
+            for (uint32_t set = 0; set < SETS; ++set) {
+                top[set] = weight_top[set] = kNone;
+                sum[set] = lift[set] = most[set] = 0.f;
 #pragma unroll
-            for (uint32_t i = 0; i < (FMT == 1 ? 1 : S::kAcc); ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-            float top = kNone, sum = 0.f;                      // reference of the row's scores; sum of this lane's weights
-            float weight_top = kNone, lift = 0.f, most = 0.f;  // 8-bit: reference of weights times scales, 2^(top - weight_top), and what they may be
+                for (uint32_t i = 0; i < (FMT == 1 ? S::kOwn : 1); ++i) o[set][i] = 0.f;
+#pragma unroll
+                for (uint32_t i = 0; i < (FMT == 1 ? 1 : S::kAcc); ++i) acc[set][i][0] = acc[set][i][1] = acc[set][i][2] = acc[set][i][3] = 0.f;
+            }
 
             for (uint32_t tile = at.begin << shift; tile < end_sub; tile += S::kSubs) {
                 const uint32_t count = min(end_sub - tile, S::kSubs);  // of 16 tokens; this warp's scores are those of warp * kOwnSubs and on
                 // ---- scores ----
                 mbar_wait(full + turn.slot * 8, turn.phase, limit_ns, p.error_flag);
-                float x[4 * S::kOwnSubs];  // tokens 2 quad, + 1, + 8, + 9 of each 16, row `row`
-                float value_scale[4 * S::kOwnSubs];
+                float x[SETS][4 * S::kOwnSubs];  // tokens 2 quad, + 1, + 8, + 9 of each 16, row `row`
+                float value_scale[SETS][4 * S::kOwnSubs];
 #pragma unroll
-                for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) x[i] = -INFINITY, value_scale[i] = 0.f;
+                for (uint32_t set = 0; set < SETS; ++set)
+#pragma unroll
+                    for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) x[set][i] = -INFINITY, value_scale[set][i] = 0.f;
                 if (warp * S::kOwnSubs < count) {
                     // (the last warp may multiply 16 tokens that are not there; they are left out below)
                     const uint32_t keys = ring + turn.slot * S::kSlot + warp * S::kOwnSubs * S::kSub;
-                    float s[2 * S::kOwnSubs][4];
-                    int upper[2 * S::kOwnSubs][4], lower[2 * S::kOwnSubs][4];  // int8: products with digits 3 and 2, and with 1 and 0
 #pragma unroll
-                    for (uint32_t n = 0; n < 2 * S::kOwnSubs; ++n) {
-                        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-                        upper[n][0] = upper[n][1] = upper[n][2] = upper[n][3] = lower[n][0] = lower[n][1] = lower[n][2] = lower[n][3] = 0;
-                    }
+                    for (uint32_t n0 = 0; n0 < 2 * S::kOwnSubs; n0 += S::kTogether) {
+                        float s[SETS][S::kTogether][4];
+                        int upper[SETS][S::kTogether][4], lower[SETS][S::kTogether][4];  // int8: products with digits 3 and 2, and with 1 and 0
 #pragma unroll
-                    for (uint32_t seg = 0; seg < S::kSegs; ++seg)
+                        for (uint32_t set = 0; set < SETS; ++set)
 #pragma unroll
-                        for (uint32_t c = 0; c < S::kPieces; ++c) {
-                            const uint32_t piece = quad * S::kPieces + c, swap = S::kSeg == 128 ? row : row >> 1 & 3u;
-                            const uint32_t from = keys + seg * (kTileTokens * S::kSeg) + row * S::kSeg + ((piece ^ swap) << 4);
-                            constexpr uint32_t kPer = S::kChunkDims / 4;
-                            const uint32_t m = (seg * S::kPieces + c) * kPer;
-                            if (!S::kQueriesStay)
+                            for (uint32_t n = 0; n < S::kTogether; ++n)
 #pragma unroll
-                                for (uint32_t i = 0; i < kPer; ++i) fetch_query(m + i);
+                                for (int j = 0; j < 4; ++j) s[set][n][j] = 0.f, upper[set][n][j] = lower[set][n][j] = 0;
 #pragma unroll
-                            for (uint32_t n = 0; n < 2 * S::kOwnSubs; ++n) {
-                                const uint4 w = lds_v4(from + n / 2 * S::kSub + n % 2 * 8 * S::kSeg);
-                                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+                        for (uint32_t seg = 0; seg < S::kSegs; ++seg)
 #pragma unroll
-                                for (uint32_t i = 0; i < kPer; ++i) {
-                                    if (FMT == 0) mma<FMT>(s[n], qa[m + i], word[2 * i % 4], word[(2 * i + 1) % 4]);
-                                    else if (FMT == 1) mma_s8s8_16832(i % 2 == 0 ? upper[n] : lower[n], qa[m + i][0], qa[m + i][1], qa[m + i][2], qa[m + i][3], word[i / 2 * 2], word[i / 2 * 2 + 1]);
-                                    else mma<FMT>(s[n], qa[m + i], e4m3_pair(word[i]), e4m3_pair(word[i] >> 16));
+                            for (uint32_t c = 0; c < S::kPieces; ++c) {
+                                const uint32_t piece = quad * S::kPieces + c, swap = S::kSeg == 128 ? row : row >> 1 & 3u;
+                                const uint32_t from = keys + seg * (kTileTokens * S::kSeg) + row * S::kSeg + ((piece ^ swap) << 4);
+                                constexpr uint32_t kPer = S::kChunkDims / 4;
+                                const uint32_t m = (seg * S::kPieces + c) * kPer;
+                                uint32_t word[S::kTogether][S::kWords];
+#pragma unroll
+                                for (uint32_t n = 0; n < S::kTogether; ++n) {
+                                    const uint4 w = lds_v4(from + (n0 + n) / 2 * S::kSub + (n0 + n) % 2 * 8 * S::kSeg);
+                                    const uint32_t part[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                                    for (uint32_t i = 0; i < 4; ++i) {
+                                        if (FMT == 2) word[n][2 * i % S::kWords] = e4m3_pair(part[i]), word[n][(2 * i + 1) % S::kWords] = e4m3_pair(part[i] >> 16);
+                                        else word[n][i] = part[i];
+                                    }
+                                }
+#pragma unroll
+                                for (uint32_t set = 0; set < SETS; ++set) {
+                                    if (!S::kQueriesStay)
+#pragma unroll
+                                        for (uint32_t i = 0; i < kPer; ++i) fetch_query(set, m + i);
+#pragma unroll
+                                    for (uint32_t n = 0; n < S::kTogether; ++n)
+#pragma unroll
+                                        for (uint32_t i = 0; i < kPer; ++i) {
+                                            if (FMT == 1) mma_s8s8_16832(i % 2 == 0 ? upper[set][n] : lower[set][n], qa[m + i][0], qa[m + i][1], qa[m + i][2], qa[m + i][3], word[n][i / 2 * 2], word[n][i / 2 * 2 + 1]);
+                                            else mma<FMT>(s[set][n], qa[m + i], word[n][2 * i % S::kWords], word[n][(2 * i + 1) % S::kWords]);
+                                        }
                                 }
                             }
-                        }
-                    const uint32_t sc = scales + turn.slot * S::kScales + warp * S::kOwnSubs * 64 + quad * 8;
+                        const uint32_t sc = scales + turn.slot * S::kScales + warp * S::kOwnSubs * 64 + quad * 8;
 #pragma unroll
-                    for (uint32_t n = 0; n < 2 * S::kOwnSubs; ++n) {
-                        if (FMT == 1) {
+                        for (uint32_t n = 0; n < S::kTogether; ++n) {
+                            uint2 k, v;
+                            if (FMT != 0) k = lds_v2(sc + (n0 + n) * 32), v = lds_v2(sc + S::kSubs * 64 + (n0 + n) * 32);
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) x[2 * n + j] = of_digits(upper[n][j], upper[n][j + 2], lower[n][j], lower[n][j + 2]) * row_scale;
-                        } else {
-                            x[2 * n] = (s[n][0] + s[n][2]) * row_scale;
-                            x[2 * n + 1] = (s[n][1] + s[n][3]) * row_scale;
-                        }
-                        if (FMT != 0) {
-                            const uint2 k = lds_v2(sc + n * 32), v = lds_v2(sc + S::kSubs * 64 + n * 32);
-                            x[2 * n] *= __uint_as_float(k.x), x[2 * n + 1] *= __uint_as_float(k.y);
-                            value_scale[2 * n] = __uint_as_float(v.x), value_scale[2 * n + 1] = __uint_as_float(v.y);
+                            for (uint32_t set = 0; set < SETS; ++set) {
+                                float *const to = x[set] + 2 * (n0 + n), *const scale_to = value_scale[set] + 2 * (n0 + n);
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    if (FMT == 1) to[j] = of_digits(upper[set][n][j], upper[set][n][j + 2], lower[set][n][j], lower[set][n][j + 2]) * row_scale[set];
+                                    else to[j] = (s[set][n][j] + s[set][n][j + 2]) * row_scale[set];
+                                }
+                                if (FMT != 0) {
+                                    to[0] *= __uint_as_float(k.x), to[1] *= __uint_as_float(k.y);
+                                    scale_to[0] = __uint_as_float(v.x), scale_to[1] = __uint_as_float(v.y);
+                                }
+                            }
                         }
                     }
                     const int32_t token = (int32_t)((tile + warp * S::kOwnSubs) * kTileTokens);
                     if (token + (int32_t)(S::kOwnSubs * kTileTokens) > sure)  // some rows do not see all of it
 #pragma unroll
-                        for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i)
-                            if (token + (int32_t)(quad * 2 + i % 2 + i / 2 * 8) >= limit) {
-                                x[i] = -INFINITY;
-                                value_scale[i] = 0.f;  // (it may be anything)
-                            }
+                        for (uint32_t set = 0; set < SETS; ++set)
+#pragma unroll
+                            for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i)
+                                if (token + (int32_t)(quad * 2 + i % 2 + i / 2 * 8) >= limit[set]) {
+                                    x[set][i] = -INFINITY;
+                                    value_scale[set][i] = 0.f;  // (it may be anything)
+                                }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty + turn.slot * 8);
                 turn.next();
                 // ---- weights ----
-                float high = x[0], weight[4 * S::kOwnSubs], of_tile;
+                float high[SETS], of_tile[SETS];
 #pragma unroll
-                for (uint32_t i = 1; i < 4 * S::kOwnSubs; ++i) high = fmaxf(high, x[i]);
+                for (uint32_t set = 0; set < SETS; ++set) {
+                    high[set] = x[set][0];
+#pragma unroll
+                    for (uint32_t i = 1; i < 4 * S::kOwnSubs; ++i) high[set] = fmaxf(high[set], x[set][i]);
+                }
 #pragma unroll 1
                 for (bool again = false;; again = true) {
                     // as if the references were high enough; if they are not, for any warp, they are raised and all is done again
-                    float weight_high = 0.f;
-                    of_tile = 0.f;
+                    bool raise = false;
 #pragma unroll
-                    for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) {
-                        weight[i] = exp2_fast(x[i] - top);
-                        if (FMT != 0) weight_high = fmaxf(weight_high, weight[i] * value_scale[i]);
-                    }
+                    for (uint32_t set = 0; set < SETS; ++set) {
+                        float weight[4 * S::kOwnSubs], weight_high = 0.f;
+                        of_tile[set] = 0.f;
 #pragma unroll
-                    for (uint32_t t = 0; t < S::kOwnSubs; ++t) {
-                        const uint32_t sub = warp * S::kOwnSubs + t;
-                        float w[4];
-#pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) {
-                            w[i] = FMT == 0 ? weight[4 * t + i] : weight[4 * t + i] * (value_scale[4 * t + i] * lift);
-                            if (FMT != 0) of_tile += weight[4 * t + i];
+                        for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) {
+                            weight[i] = exp2_fast(x[set][i] - top[set]);
+                            if (FMT != 0) weight_high = fmaxf(weight_high, weight[i] * value_scale[set][i]);
                         }
-                        uint32_t a[4];
-                        if (FMT == 1) {
-                            // of two 16s, one MMA's left operand: digits 3 and 2 of the first, of the second; another one's: digits 1 and 0.
-                            // What is no number spoils the sum of the weights, and with it the row.
-                            weight_digits(w, a);
-                            const uint32_t to = weights_at + sub / 2 * 1024 + lane * 16 + sub % 2 * 8;
-                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(a[0]), "r"(a[1]) : "memory");
-                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + 512), "r"(a[2]), "r"(a[3]) : "memory");
 #pragma unroll
-                            for (uint32_t i = 0; i < 4; ++i)
-                                if (!(w[i] <= Weights<1>::kMost)) of_tile = __uint_as_float(0x7fc00000u);
-                        } else {
-                            split<FMT>(w[0], w[1], a[0], a[1]);
-                            split<FMT>(w[2], w[3], a[2], a[3]);
-                            if (FMT == 0) {
-                                // bf16: the weights as they are multiplied, so that they add up to one whatever the halves cut off
+                        for (uint32_t t = 0; t < S::kOwnSubs; ++t) {
+                            const uint32_t sub = warp * S::kOwnSubs + t, weights_to = weights_at + set * S::kSetWeights;
+                            float w[4];
 #pragma unroll
-                                for (int j = 0; j < 4; j += 2)
-                                    of_tile += (__uint_as_float(a[j] << 16) + __uint_as_float(a[j + 1] << 16)) + (__uint_as_float(a[j] & 0xffff0000u) + __uint_as_float(a[j + 1] & 0xffff0000u));
+                            for (uint32_t i = 0; i < 4; ++i) {
+                                w[i] = FMT == 0 ? weight[4 * t + i] : weight[4 * t + i] * (value_scale[set][4 * t + i] * lift[set]);
+                                if (FMT != 0) of_tile[set] += weight[4 * t + i];
                             }
-                            sts_v4(weights_at + (sub * 32 + lane) * 16, make_uint4(a[0], a[1], a[2], a[3]));
-                        }
-                    }
-                    if (!multipliers_any(!again && (high - top > kHeadroom || (FMT != 0 && weight_high > most)))) break;
-                    float now = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
-                    now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 2));
-                    if (quad == 0) highs[warp * kAttentionRows + row] = now;
-                    multipliers_sync();
-                    now = -INFINITY;
+                            uint32_t a[4];
+                            if (FMT == 1) {
+                                // of two 16s, one MMA's left operand: digits 3 and 2 of the first, of the second; another one's: digits 1 and 0.
+                                // What is no number spoils the sum of the weights, and with it the row.
+                                weight_digits(w, a);
+                                const uint32_t to = weights_to + sub / 2 * 1024 + lane * 16 + sub % 2 * 8;
+                                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(a[0]), "r"(a[1]) : "memory");
+                                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + 512), "r"(a[2]), "r"(a[3]) : "memory");
 #pragma unroll
-                    for (uint32_t w = 0; w < kWarps; ++w) now = fmaxf(now, highs[w * kAttentionRows + row]);
-                    float keep = 1.f;
-                    if (now - top > kHeadroom) {
-                        now = ceilf(now);
-                        keep = exp2_fast(top - now);
-                        sum *= keep;
-                        top = now;
+                                for (uint32_t i = 0; i < 4; ++i)
+                                    if (!(w[i] <= Weights<1>::kMost)) of_tile[set] = __uint_as_float(0x7fc00000u);
+                            } else {
+                                split<FMT>(w[0], w[1], a[0], a[1]);
+                                split<FMT>(w[2], w[3], a[2], a[3]);
+                                if (FMT == 0) {
+                                    // bf16: the weights as they are multiplied, so that they add up to one whatever the halves cut off
+#pragma unroll
+                                    for (int j = 0; j < 4; j += 2)
+                                        of_tile[set] += (__uint_as_float(a[j] << 16) + __uint_as_float(a[j + 1] << 16)) + (__uint_as_float(a[j] & 0xffff0000u) + __uint_as_float(a[j + 1] & 0xffff0000u));
+                                }
+                                sts_v4(weights_to + (sub * 32 + lane) * 16, make_uint4(a[0], a[1], a[2], a[3]));
+                            }
+                        }
+                        raise = raise || high[set] - top[set] > kHeadroom || (FMT != 0 && weight_high > most[set]);
+                    }
+                    if (!multipliers_any(!again && raise)) break;
+#pragma unroll
+                    for (uint32_t set = 0; set < SETS; ++set) {
+                        float now = fmaxf(high[set], __shfl_xor_sync(0xffffffffu, high[set], 1));
+                        now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 2));
+                        if (quad == 0) highs[warp * S::kRows + set * kAttentionRows + row] = now;
+                    }
+                    multipliers_sync();
+                    float keep[SETS];
+#pragma unroll
+                    for (uint32_t set = 0; set < SETS; ++set) {
+                        float now = -INFINITY;
+#pragma unroll
+                        for (uint32_t w = 0; w < kWarps; ++w) now = fmaxf(now, highs[w * S::kRows + set * kAttentionRows + row]);
+                        keep[set] = 1.f;
+                        if (now - top[set] > kHeadroom) {
+                            now = ceilf(now);
+                            keep[set] = exp2_fast(top[set] - now);
+                            sum[set] *= keep[set];
+                            top[set] = now;
+                        }
                     }
                     if (FMT != 0) {
-                        weight_high = 0.f;
 #pragma unroll
-                        for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) weight_high = fmaxf(weight_high, exp2_fast(x[i] - top) * value_scale[i]);
-                        weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 1));
-                        weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 2));
-                        if (quad == 0) weight_highs[warp * kAttentionRows + row] = weight_high;
-                        multipliers_sync();
-                        weight_high = 0.f;
+                        for (uint32_t set = 0; set < SETS; ++set) {
+                            float weight_high = 0.f;
 #pragma unroll
-                        for (uint32_t w = 0; w < kWarps; ++w) weight_high = fmaxf(weight_high, weight_highs[w * kAttentionRows + row]);
-                        lift = weight_top == kNone ? 0.f : exp2_fast(top - weight_top);
-                        keep = 1.f;
-                        if (weight_high * lift > Weights<FMT>::kMost || (lift == 0.f && weight_high > 0.f)) {
-                            const int e = (int)(__float_as_uint(weight_high) >> 23) - 126;  // weight_high < 2^e
-                            const float next = top + (float)max(e - Weights<FMT>::kExponent, -100);
-                            keep = weight_top == kNone ? 0.f : exp2_fast(weight_top - next);
-                            weight_top = next;
-                            lift = exp2_fast(top - weight_top);
+                            for (uint32_t i = 0; i < 4 * S::kOwnSubs; ++i) weight_high = fmaxf(weight_high, exp2_fast(x[set][i] - top[set]) * value_scale[set][i]);
+                            weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 1));
+                            weight_high = fmaxf(weight_high, __shfl_xor_sync(0xffffffffu, weight_high, 2));
+                            if (quad == 0) weight_highs[warp * S::kRows + set * kAttentionRows + row] = weight_high;
                         }
-                        most = lift > 0.f ? Weights<FMT>::kMost / lift : 0.f;
+                        multipliers_sync();
+#pragma unroll
+                        for (uint32_t set = 0; set < SETS; ++set) {
+                            float weight_high = 0.f;
+#pragma unroll
+                            for (uint32_t w = 0; w < kWarps; ++w) weight_high = fmaxf(weight_high, weight_highs[w * S::kRows + set * kAttentionRows + row]);
+                            lift[set] = weight_top[set] == kNone ? 0.f : exp2_fast(top[set] - weight_top[set]);
+                            keep[set] = 1.f;
+                            if (weight_high * lift[set] > Weights<FMT>::kMost || (lift[set] == 0.f && weight_high > 0.f)) {
+                                const int e = (int)(__float_as_uint(weight_high) >> 23) - 126;  // weight_high < 2^e
+                                const float next = top[set] + (float)max(e - Weights<FMT>::kExponent, -100);
+                                keep[set] = weight_top[set] == kNone ? 0.f : exp2_fast(weight_top[set] - next);
+                                weight_top[set] = next;
+                                lift[set] = exp2_fast(top[set] - weight_top[set]);
+                            }
+                            most[set] = lift[set] > 0.f ? Weights<FMT>::kMost / lift[set] : 0.f;
+                        }
                     }
 #pragma unroll
-                    for (uint32_t i = 0; i < (FMT == 1 ? S::kOwn : 1); ++i) o[i] *= keep;
+                    for (uint32_t set = 0; set < SETS; ++set) {
 #pragma unroll
-                    for (uint32_t i = 0; i < (FMT == 1 ? 1 : S::kAcc); ++i)
+                        for (uint32_t i = 0; i < (FMT == 1 ? S::kOwn : 1); ++i) o[set][i] *= keep[set];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[i][j] *= keep;
+                        for (uint32_t i = 0; i < (FMT == 1 ? 1 : S::kAcc); ++i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) acc[set][i][j] *= keep[set];
+                    }
                 }
-                sum += of_tile;
+#pragma unroll
+                for (uint32_t set = 0; set < SETS; ++set) sum[set] += of_tile[set];
                 // ---- values: this warp's dimensions, all tokens of the tile ----
                 mbar_wait(full + turn.slot * 8, turn.phase, limit_ns, p.error_flag);
                 if (warp < S::kValueWarps) {
@@ -713,13 +776,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     };
                     if constexpr (FMT == 1) {
                         // 32 tokens to an MMA; those without a weight count as nothing whatever their codes are
-                        int upper[S::kAcc][4], lower[S::kAcc][4];
+                        int upper[SETS][S::kAcc][4], lower[SETS][S::kAcc][4];
 #pragma unroll
-                        for (uint32_t i = 0; i < S::kAcc; ++i)
+                        for (uint32_t set = 0; set < SETS; ++set)
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) upper[i][j] = lower[i][j] = 0;
+                            for (uint32_t i = 0; i < S::kAcc; ++i)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) upper[set][i][j] = lower[set][i][j] = 0;
                         const auto add_pair = [&](uint32_t t) {
-                            const uint4 a = lds_v4(weights_at + (t * 64 + lane) * 16), b = lds_v4(weights_at + (t * 64 + 32 + lane) * 16);
+                            uint4 a[SETS], b[SETS];
+#pragma unroll
+                            for (uint32_t set = 0; set < SETS; ++set) {
+                                const uint32_t weights_of = weights_at + set * S::kSetWeights + (t * 64 + lane) * 16;
+                                a[set] = lds_v4(weights_of), b[set] = lds_v4(weights_of + 512);
+                            }
                             uint32_t v[kPairs][4], w[kPairs][4];
                             fetch(v, 2 * t);
                             fetch(w, 2 * t + 1);
@@ -729,8 +799,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll
                                 for (uint32_t i = 0; i < 2; ++i) {
                                     const uint32_t pick = i == 0 ? 0x6420 : 0x7531, b0 = __byte_perm(v0, v1, pick), b1 = __byte_perm(w0, w1, pick);
-                                    mma_s8s8_16832(upper[2 * c + i], a.x, a.y, a.z, a.w, b0, b1);
-                                    mma_s8s8_16832(lower[2 * c + i], b.x, b.y, b.z, b.w, b0, b1);
+#pragma unroll
+                                    for (uint32_t set = 0; set < SETS; ++set) {
+                                        mma_s8s8_16832(upper[set][2 * c + i], a[set].x, a[set].y, a[set].z, a[set].w, b0, b1);
+                                        mma_s8s8_16832(lower[set][2 * c + i], b[set].x, b[set].y, b[set].z, b[set].w, b0, b1);
+                                    }
                                 }
                             }
                         };
@@ -742,14 +815,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             for (uint32_t t = 0; 2 * t < count; ++t) add_pair(t);
                         }
 #pragma unroll
-                        for (uint32_t i = 0; i < S::kOwn; ++i) {
-                            const uint32_t m = i / 4 * 2 + i % 2, j = i / 2 % 2;  // dimensions 4 quad ... + 3 of each 16: even, odd, even, odd
-                            o[i] += of_digits(upper[m][j], upper[m][j + 2], lower[m][j], lower[m][j + 2]);
-                        }
+                        for (uint32_t set = 0; set < SETS; ++set)
+#pragma unroll
+                            for (uint32_t i = 0; i < S::kOwn; ++i) {
+                                const uint32_t m = i / 4 * 2 + i % 2, j = i / 2 % 2;  // dimensions 4 quad ... + 3 of each 16: even, odd, even, odd
+                                o[set][i] += of_digits(upper[set][m][j], upper[set][m][j + 2], lower[set][m][j], lower[set][m][j + 2]);
+                            }
                     } else {
                         const auto add_sub = [&](uint32_t t, bool edge) {
-                            const uint4 w = lds_v4(weights_at + (t * 32 + lane) * 16);
-                            const uint32_t wa[4] = {w.x, w.y, w.z, w.w};
+                            uint32_t wa[SETS][4];
+#pragma unroll
+                            for (uint32_t set = 0; set < SETS; ++set) {
+                                const uint4 w = lds_v4(weights_at + set * S::kSetWeights + (t * 32 + lane) * 16);
+                                wa[set][0] = w.x, wa[set][1] = w.y, wa[set][2] = w.z, wa[set][3] = w.w;
+                            }
                             uint32_t v[kPairs][4];
                             fetch(v, t);
                             const int32_t first = (int32_t)((tile + t) * kTileTokens);
@@ -773,19 +852,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                                                 }
                                     }
                                 if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+                                    for (uint32_t set = 0; set < SETS; ++set)
 #pragma unroll 1
-                                    for (int32_t k = 0; k < (int32_t)kTileTokens && first + k < limit; ++k) {
-                                        const uint32_t turned = S::kSeg == 128 ? (uint32_t)k & 7u : (uint32_t)k >> 1 & 3u, at_token = held + t * S::kSub + (uint32_t)k * S::kSeg;
+                                        for (int32_t k = 0; k < (int32_t)kTileTokens && first + k < limit[set]; ++k) {
+                                            const uint32_t turned = S::kSeg == 128 ? (uint32_t)k & 7u : (uint32_t)k >> 1 & 3u, at_token = held + t * S::kSub + (uint32_t)k * S::kSeg;
 #pragma unroll
-                                        for (uint32_t i = 0; i < S::kAcc; ++i)
+                                            for (uint32_t i = 0; i < S::kAcc; ++i)
 #pragma unroll
-                                            for (uint32_t j = 0; j < 2; ++j) {
-                                                const uint32_t d = warp * S::kWarpDims + (FMT == 0 ? i * 8 + quad * 2 + j : i / 2 * 16 + quad * 4 + j * 2 + (i & 1u));
-                                                const uint32_t byte = d * (FMT == 0 ? 2 : 1), piece = byte % S::kSeg / 16;
-                                                const uint32_t e = lds_u32((at_token + byte / S::kSeg * (kTileTokens * S::kSeg) + ((piece ^ turned) << 4) + byte % 16) & ~3u);
-                                                if (not_finite<FMT>(e, byte & 3u)) acc[i][j] += FMT == 0 ? __uint_as_float((e >> ((byte & 3u) * 8)) << 16) : __uint_as_float(0x7fc00000u);
-                                            }
-                                    }
+                                                for (uint32_t j = 0; j < 2; ++j) {
+                                                    const uint32_t d = warp * S::kWarpDims + (FMT == 0 ? i * 8 + quad * 2 + j : i / 2 * 16 + quad * 4 + j * 2 + (i & 1u));
+                                                    const uint32_t byte = d * (FMT == 0 ? 2 : 1), piece = byte % S::kSeg / 16;
+                                                    const uint32_t e = lds_u32((at_token + byte / S::kSeg * (kTileTokens * S::kSeg) + ((piece ^ turned) << 4) + byte % 16) & ~3u);
+                                                    if (not_finite<FMT>(e, byte & 3u)) acc[set][i][j] += FMT == 0 ? __uint_as_float((e >> ((byte & 3u) * 8)) << 16) : __uint_as_float(0x7fc00000u);
+                                                }
+                                        }
                                     __syncwarp();
                                 }
                             }
@@ -793,10 +874,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             for (uint32_t c = 0; c < S::kChunks; ++c) {
                                 const uint32_t b0 = v[c / 2][c % 2 * 2], b1 = v[c / 2][c % 2 * 2 + 1];
                                 if (FMT == 0) {
-                                    mma<FMT>(acc[c], wa, b0, b1);
+#pragma unroll
+                                    for (uint32_t set = 0; set < SETS; ++set) mma<FMT>(acc[set][c], wa[set], b0, b1);
                                 } else {
-                                    mma<FMT>(acc[2 * c], wa, e4m3_pair(__byte_perm(b0, 0, 0x4420)), e4m3_pair(__byte_perm(b1, 0, 0x4420)));
-                                    mma<FMT>(acc[2 * c + 1], wa, e4m3_pair(__byte_perm(b0, 0, 0x4431)), e4m3_pair(__byte_perm(b1, 0, 0x4431)));
+                                    const uint32_t even[2] = {e4m3_pair(__byte_perm(b0, 0, 0x4420)), e4m3_pair(__byte_perm(b1, 0, 0x4420))};
+                                    const uint32_t odd[2] = {e4m3_pair(__byte_perm(b0, 0, 0x4431)), e4m3_pair(__byte_perm(b1, 0, 0x4431))};
+#pragma unroll
+                                    for (uint32_t set = 0; set < SETS; ++set) {
+                                        mma<FMT>(acc[set][2 * c], wa[set], even[0], even[1]);
+                                        mma<FMT>(acc[set][2 * c + 1], wa[set], odd[0], odd[1]);
+                                    }
                                 }
                             }
                         };
@@ -817,48 +904,76 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             }
 
             // ---- the segment's result ----
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (quad == 0) sums[warp * kAttentionRows + row] = sum;
-            // numbers of the row: bf16: dimensions 8 i + 2 quad, + 1; 8-bit: 16 i + 4 quad ... + 3, from the warp's first on
-            const bool holds = live && warp < S::kValueWarps;
-            float mine[S::kOwn];
-            {
-                const float unlift = FMT == 0 ? 1.f : weight_top == kNone ? 0.f : exp2_fast(weight_top - top);
 #pragma unroll
-                for (uint32_t i = 0; i < S::kOwn; ++i) {
-                    if constexpr (FMT == 1) {
-                        mine[i] = o[i] * unlift;
-                    } else {
-                        const uint32_t m = FMT == 0 ? i / 2 : i / 4 * 2 + i % 2, j = FMT == 0 ? i % 2 : i / 2 % 2;
-                        mine[i] = (acc[m][j] + acc[m][j + 2]) * unlift;
+            for (uint32_t set = 0; set < SETS; ++set) {
+                sum[set] += __shfl_xor_sync(0xffffffffu, sum[set], 1);
+                sum[set] += __shfl_xor_sync(0xffffffffu, sum[set], 2);
+                if (quad == 0) sums[warp * S::kRows + set * kAttentionRows + row] = sum[set];
+            }
+            multipliers_sync();
+            const bool whole = at.whole_item();
+            uint32_t owner = 0, contributors = 0;
+            if (!whole) at.contributors(share.cut, blockIdx.x, &owner, &contributors);
+            float *const part = p.parts + ((uint64_t)blockIdx.x * 2 + (blockIdx.x == owner ? 1 : 0)) * kPart;
+            constexpr uint32_t kBeside = FMT == 0 ? 2 : 4;  // numbers beside each other
+            const auto dim_of = [&](uint32_t i) { return warp * S::kWarpDims + i / kBeside * (4 * kBeside) + quad * kBeside + i % kBeside; };
+#pragma unroll
+            for (uint32_t set = 0; set < SETS; ++set) {
+                // numbers of the row: bf16: dimensions 8 i + 2 quad, + 1; 8-bit: 16 i + 4 quad ... + 3, from the warp's first on
+                const uint32_t in_item = set * kAttentionRows + row, r = row_of(set);
+                const bool holds = r < g.rows && warp < S::kValueWarps;
+                float mine[S::kOwn];
+                {
+                    const float unlift = FMT == 0 ? 1.f : weight_top[set] == kNone ? 0.f : exp2_fast(weight_top[set] - top[set]);
+#pragma unroll
+                    for (uint32_t i = 0; i < S::kOwn; ++i) {
+                        if constexpr (FMT == 1) {
+                            mine[i] = o[set][i] * unlift;
+                        } else {
+                            const uint32_t m = FMT == 0 ? i / 2 : i / 4 * 2 + i % 2, j = FMT == 0 ? i % 2 : i / 2 % 2;
+                            mine[i] = (acc[set][m][j] + acc[set][m][j + 2]) * unlift;
+                        }
+                    }
+                }
+                float total = 0.f;
+#pragma unroll
+                for (uint32_t w = 0; w < kWarps; ++w) total += sums[w * S::kRows + in_item];
+                if (!whole) {
+                    // ---- a partial result; the block that is the last to leave one of an item joins them below ----
+                    if (holds)
+#pragma unroll
+                        for (uint32_t i = 0; i < S::kOwn; i += kBeside) {
+                            float *const to = part + in_item * HDP + dim_of(i);
+                            if (FMT == 0) *reinterpret_cast<float2 *>(to) = make_float2(mine[i], mine[i + 1]);
+                            else *reinterpret_cast<float4 *>(to) = make_float4(mine[i], mine[i + 1], mine[(i + 2) % S::kOwn], mine[(i + 3) % S::kOwn]);
+                        }
+                    if (warp == 0 && quad == 0) {
+                        part[S::kRows * HDP + in_item] = top[set] == kNone ? -INFINITY : top[set];
+                        part[S::kRows * (HDP + 1) + in_item] = total;
+                    }
+                } else if (holds) {
+                    const bool none = at.length - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group) <= 0;
+                    const float by = 1.f / total;
+                    const uint64_t base = ((uint64_t)at.s * p.q_tokens + r / g.group) * p.out_stride + ((uint64_t)head * g.group + r % g.group) * p.kv.head_dim;
+#pragma unroll
+                    for (uint32_t i = 0; i < S::kOwn; ++i) mine[i] = none ? 0.f : mine[i] * by;
+#pragma unroll
+                    for (uint32_t i = 0; i < S::kOwn; i += kBeside) {
+                        const uint32_t d = dim_of(i);
+                        if (d >= p.kv.head_dim) continue;
+                        if (p.out_is_f32) {
+                            float *const to = static_cast<float *>(p.out) + base + d;
+                            if (FMT == 0) *reinterpret_cast<float2 *>(to) = make_float2(mine[i], mine[i + 1]);
+                            else *reinterpret_cast<float4 *>(to) = make_float4(mine[i], mine[i + 1], mine[(i + 2) % S::kOwn], mine[(i + 3) % S::kOwn]);
+                        } else {
+                            uint16_t *const to = static_cast<uint16_t *>(p.out) + base + d;
+                            if (FMT == 0) *reinterpret_cast<uint32_t *>(to) = pack_bf16(mine[i], mine[i + 1]);
+                            else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16(mine[i], mine[i + 1]), pack_bf16(mine[(i + 2) % S::kOwn], mine[(i + 3) % S::kOwn]));
+                        }
                     }
                 }
             }
-            if (top == kNone) top = -INFINITY;
-            constexpr uint32_t kBeside = FMT == 0 ? 2 : 4;  // numbers beside each other
-            const auto dim_of = [&](uint32_t i) { return warp * S::kWarpDims + i / kBeside * (4 * kBeside) + quad * kBeside + i % kBeside; };
-            const auto put = [&](float *row_at, const float (&v)[S::kOwn]) {
-#pragma unroll
-                for (uint32_t i = 0; i < S::kOwn; i += kBeside) {
-                    if (FMT == 0) *reinterpret_cast<float2 *>(row_at + dim_of(i)) = make_float2(v[i], v[i + 1]);
-                    else *reinterpret_cast<float4 *>(row_at + dim_of(i)) = make_float4(v[i], v[i + 1], v[(i + 2) % S::kOwn], v[(i + 3) % S::kOwn]);
-                }
-            };
-            multipliers_sync();
-            float total = 0.f;
-#pragma unroll
-            for (uint32_t w = 0; w < kWarps; ++w) total += sums[w * kAttentionRows + row];
-            if (!at.whole_item()) {
-                // ---- a partial result; the block that is the last to leave one of an item joins them below ----
-                uint32_t owner, contributors;
-                at.contributors(share.cut, blockIdx.x, &owner, &contributors);
-                float *const part = p.parts + ((uint64_t)blockIdx.x * 2 + (blockIdx.x == owner ? 1 : 0)) * kPart;
-                if (holds) put(part + row * HDP, mine);
-                if (warp == 0 && quad == 0) {
-                    part[kAttentionRows * HDP + row] = top;
-                    part[kAttentionRows * (HDP + 1) + row] = total;
-                }
+            if (!whole) {
                 __threadfence();
                 multipliers_sync();
                 if (threadIdx.x == 0) {
@@ -868,26 +983,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     to[0] = last, to[1] = owner, to[2] = contributors, to[3] = at.s, to[4] = at.item, to[5] = (uint32_t)at.length;
                 }
                 ++left_parts;
-            } else if (holds) {
-                const bool none = at.length - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group) <= 0;
-                const float by = 1.f / total;
-                const uint64_t base = ((uint64_t)at.s * p.q_tokens + r / g.group) * p.out_stride + ((uint64_t)head * g.group + r % g.group) * p.kv.head_dim;
-#pragma unroll
-                for (uint32_t i = 0; i < S::kOwn; ++i) mine[i] = none ? 0.f : mine[i] * by;
-#pragma unroll
-                for (uint32_t i = 0; i < S::kOwn; i += kBeside) {
-                    const uint32_t d = dim_of(i);
-                    if (d >= p.kv.head_dim) continue;
-                    if (p.out_is_f32) {
-                        float *const to = static_cast<float *>(p.out) + base + d;
-                        if (FMT == 0) *reinterpret_cast<float2 *>(to) = make_float2(mine[i], mine[i + 1]);
-                        else *reinterpret_cast<float4 *>(to) = make_float4(mine[i], mine[i + 1], mine[(i + 2) % S::kOwn], mine[(i + 3) % S::kOwn]);
-                    } else {
-                        uint16_t *const to = static_cast<uint16_t *>(p.out) + base + d;
-                        if (FMT == 0) *reinterpret_cast<uint32_t *>(to) = pack_bf16(mine[i], mine[i + 1]);
-                        else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16(mine[i], mine[i + 1]), pack_bf16(mine[(i + 2) % S::kOwn], mine[(i + 3) % S::kOwn]));
-                    }
-                }
             }
             at = ahead;
         } while (more);
@@ -902,11 +997,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             const uint32_t *const job = joins + n * 6;
             if (!job[0]) continue;
             const uint32_t owner = job[1], contributors = job[2], seq = job[3], head = job[4] / g.chunks, chunk = job[4] % g.chunks;
-            const uint32_t rows = min(g.rows - chunk * kAttentionRows, kAttentionRows), bytes = rows * HDP * 4, room = S::kSlots * S::kSlot / bytes;
+            const uint32_t rows = min(g.rows - chunk * S::kRows, S::kRows), bytes = rows * HDP * 4, room = S::kSlots * S::kSlot / bytes;
             // piece k lies 2 k - 1 places behind the owner's, which is the first one
             const float *const first = p.parts + ((uint64_t)owner * 2 + 1) * kPart;
             const auto piece = [&](uint32_t k) { return first + (k == 0 ? 0 : 2 * k - 1) * kPart; };
-            float4 sums_of[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};  // 16 bytes of the item's rows, and those 256 x 16 behind
+            float4 sums_of[2 * SETS];  // 16 bytes of the item's rows, and those 256 x 16 behind them
+#pragma unroll
+            for (uint32_t j = 0; j < 2 * SETS; ++j) sums_of[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
             for (uint32_t done = 0; done < contributors; done += room) {
                 const uint32_t now = min(room, contributors - done);
@@ -918,32 +1015,35 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 }
                 if (done == 0) {
                     // a warp for each row; pieces that saw nothing have zeros, rows whose scores are NaNs keep those
-                    float best = -INFINITY, total = 0.f, t[kMostBlocks / 32], l[kMostBlocks / 32];
+#pragma unroll 1
+                    for (uint32_t of = warp; of < S::kRows; of += kWarps) {
+                        float best = -INFINITY, total = 0.f, t[kMostBlocks / 32], l[kMostBlocks / 32];
 #pragma unroll
-                    for (uint32_t i = 0; i < kMostBlocks / 32; ++i) {
-                        const uint32_t k = lane + i * 32;
-                        t[i] = k < contributors ? __ldcg(piece(k) + kAttentionRows * HDP + warp) : -INFINITY;
-                        l[i] = k < contributors ? __ldcg(piece(k) + kAttentionRows * (HDP + 1) + warp) : 0.f;
+                        for (uint32_t i = 0; i < kMostBlocks / 32; ++i) {
+                            const uint32_t k = lane + i * 32;
+                            t[i] = k < contributors ? __ldcg(piece(k) + S::kRows * HDP + of) : -INFINITY;
+                            l[i] = k < contributors ? __ldcg(piece(k) + S::kRows * (HDP + 1) + of) : 0.f;
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < kMostBlocks / 32; ++i) best = fmaxf(best, t[i]);
+#pragma unroll
+                        for (int off = 16; off > 0; off >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, off));
+#pragma unroll
+                        for (uint32_t i = 0; i < kMostBlocks / 32; ++i) {
+                            const float f = t[i] == -INFINITY ? 0.f : exp2_fast(t[i] - best);
+                            total += t[i] == -INFINITY ? l[i] : l[i] * f;
+                            if (lane + i * 32 < contributors) factors[(lane + i * 32) * S::kRows + of] = f;
+                        }
+#pragma unroll
+                        for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+                        if (lane == 0) sums[of] = total;
                     }
-#pragma unroll
-                    for (uint32_t i = 0; i < kMostBlocks / 32; ++i) best = fmaxf(best, t[i]);
-#pragma unroll
-                    for (int off = 16; off > 0; off >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, off));
-#pragma unroll
-                    for (uint32_t i = 0; i < kMostBlocks / 32; ++i) {
-                        const float f = t[i] == -INFINITY ? 0.f : exp2_fast(t[i] - best);
-                        total += t[i] == -INFINITY ? l[i] : l[i] * f;
-                        if (lane + i * 32 < contributors) factors[(lane + i * 32) * kAttentionRows + warp] = f;
-                    }
-#pragma unroll
-                    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-                    if (lane == 0) sums[warp] = total;
                     multipliers_sync();
                 }
                 mbar_wait(joined, phase, limit_ns, p.error_flag);
                 phase ^= 1u;
 #pragma unroll
-                for (uint32_t j = 0; j < 2; ++j) {
+                for (uint32_t j = 0; j < 2 * SETS; ++j) {
                     const uint32_t i = threadIdx.x + j * kMultipliers;
                     if (i * 16 >= bytes) continue;
                     const uint32_t of = i / (HDP / 4);
@@ -951,7 +1051,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll 4
                     for (uint32_t k = 0; k < now; ++k) {
                         const uint4 w = lds_v4(ring + k * bytes + i * 16);
-                        const float f = factors[(done + k) * kAttentionRows + of];
+                        const float f = factors[(done + k) * S::kRows + of];
                         o4.x = fmaf(__uint_as_float(w.x), f, o4.x), o4.y = fmaf(__uint_as_float(w.y), f, o4.y);
                         o4.z = fmaf(__uint_as_float(w.z), f, o4.z), o4.w = fmaf(__uint_as_float(w.w), f, o4.w);
                     }
@@ -959,10 +1059,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 }
             }
 #pragma unroll
-            for (uint32_t j = 0; j < 2; ++j) {
+            for (uint32_t j = 0; j < 2 * SETS; ++j) {
                 const uint32_t i = threadIdx.x + j * kMultipliers, of = i / (HDP / 4), d = i % (HDP / 4) * 4;
                 if (i * 16 >= bytes || d >= p.kv.head_dim) continue;
-                const uint32_t r = chunk * kAttentionRows + of;
+                const uint32_t r = chunk * S::kRows + of;
                 const bool none = (int32_t)job[5] - (int32_t)p.q_tokens + 1 + (int32_t)(r / g.group) <= 0;
                 const float by = 1.f / sums[of];
                 const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sums_of[j].x * by, sums_of[j].y * by, sums_of[j].z * by, sums_of[j].w * by);
@@ -992,7 +1092,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 // one segment, or all.
 template <int FMT, int HDP>
 bool encode_map(EncodeTiledFn encode, CUtensorMap *map, const KvView &kv, const uint8_t *pool, bool whole_rows, uint32_t tile_shift) {
-    using S = Shape<FMT, HDP>;
+    using S = Shape<FMT, HDP, 1>;
     constexpr uint32_t kSegValues = S::kSeg / (FMT == 0 ? 2 : 1);
     const CUtensorMapDataType type = FMT == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const CUtensorMapSwizzle swizzle = S::kSeg == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
@@ -1011,9 +1111,9 @@ bool encode_map(EncodeTiledFn encode, CUtensorMap *map, const KvView &kv, const 
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int FMT, int HDP>
+template <int FMT, int HDP, int SETS>
 cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t stream) {
-    using S = Shape<FMT, HDP>;
+    using S = Shape<FMT, HDP, SETS>;
     const EncodeTiledFn encode = encode_tiled_fn();
     CUtensorMap maps[2];
     // Rows of one segment come 64 tokens at a time where pages allow (smaller copies are more than the copy engine takes; larger ones would
@@ -1028,31 +1128,46 @@ cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t str
     if (e != cudaSuccess) return e;
     const uint64_t bit = device < 64 ? 1ull << device : 0;
     if (!(ready.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(attention_kernel<FMT, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kShared);
+        e = cudaFuncSetAttribute(attention_kernel<FMT, HDP, SETS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kShared);
         if (e != cudaSuccess) return e;
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
     Geometry g;
     g.group = p.heads / p.kv.kv_heads;
     g.rows = g.group * p.q_tokens;
-    g.chunks = (g.rows + kAttentionRows - 1) / kAttentionRows;
+    g.chunks = (g.rows + S::kRows - 1) / S::kRows;
     g.heads = p.kv.kv_heads * g.chunks;
     g.tile_shift = shift;
     g.pages = attention_pages(p.kv.page_tokens, shift);
     g.whole_rows = whole_rows || S::kSegs == 1;
-    return launch_dependent(attention_kernel<FMT, HDP>, dim3(sm_count < kMostBlocks ? sm_count : kMostBlocks), kThreads, S::kShared, stream, p, g, maps[0], maps[1]);
+    return launch_dependent(attention_kernel<FMT, HDP, SETS>, dim3(sm_count < kMostBlocks ? sm_count : kMostBlocks), kThreads, S::kShared, stream, p, g, maps[0], maps[1]);
+}
+
+// Eights of rows that an item has together read and convert every key and value once; each has more registers and less of the ring. Measured on
+// 51,000 tokens in four sequences, 4 key heads, us with 1 / 2 / 3 eights an item: bf16 of 256 with 12 rows 62 / 57 / 65, with 24 rows
+// 74 / 72 / 68, with 48 rows 176 / 94 / 96; bf16 of 128 with 32 rows 66 / 51 / 59; e4m3 of 128 with 16 rows 39 / 31 / 45; int8 of 64 with 16 rows
+// 35 / 29 / 35; but int8 of 256 with 24 rows 59 / 74 / 70, e4m3 63 / 72 / 72: the digits, or fp16 pairs, of more rows do not fit the registers.
+template <int FMT, int HDP>
+cudaError_t launch_sets(const AttentionParams &p, uint32_t sm_count, cudaStream_t stream) {
+    const uint32_t sets = (p.heads / p.kv.kv_heads * p.q_tokens + kAttentionRows - 1) / kAttentionRows;
+    if constexpr (FMT == 0 || HDP < 256) {
+        if constexpr (HDP == 256)
+            if (sets > 1 && sets % 2 == 1) return launch<FMT, HDP, 3>(p, sm_count, stream);
+        if (sets > 1) return launch<FMT, HDP, 2>(p, sm_count, stream);
+    }
+    return launch<FMT, HDP, 1>(p, sm_count, stream);
 }
 
 template <int FMT>
 cudaError_t launch_dim(const AttentionParams &p, uint32_t sm_count, cudaStream_t stream) {
-    if (p.kv.head_dim <= 64) return launch<FMT, 64>(p, sm_count, stream);
-    if (p.kv.head_dim <= 128) return launch<FMT, 128>(p, sm_count, stream);
-    return launch<FMT, 256>(p, sm_count, stream);
+    if (p.kv.head_dim <= 64) return launch_sets<FMT, 64>(p, sm_count, stream);
+    if (p.kv.head_dim <= 128) return launch_sets<FMT, 128>(p, sm_count, stream);
+    return launch_sets<FMT, 256>(p, sm_count, stream);
 }
 
 }  // namespace q4
 
-extern "C" size_t q4k_attention_part_floats(uint32_t sm_count) { return (size_t)sm_count * 2 * q4::kAttentionRows * (q4::kMaxHeadDim + 2); }
+extern "C" size_t q4k_attention_part_floats(uint32_t sm_count) { return (size_t)sm_count * 2 * q4::kMostSets * q4::kAttentionRows * (q4::kMaxHeadDim + 2); }
 
 extern "C" cudaError_t q4k_attention(const q4::AttentionParams *p, uint32_t sm_count, cudaStream_t stream) {
     if (p->kv.format == 0u) return q4::launch_dim<0>(*p, sm_count, stream);

@@ -63,6 +63,44 @@ def test_long_contexts_are_split_and_joined(runtime, fmt, lengths, heads, kv_hea
     _case(runtime, fmt, lengths, 1, heads, kv_heads, dim, page, ("f32", "f32"), q_gain=2.0)
 
 
+# 9 to 48 query rows of a key head, which are multiplied 16 or 24 at a time, the last of them partly empty
+WIDE = [("bf16", 2, 24, 4, 256), ("bf16", 4, 24, 4, 256), ("bf16", 5, 8, 1, 256), ("bf16", 3, 8, 2, 128), ("bf16", 16, 3, 1, 48), ("e4m3", 4, 8, 2, 128), ("e4m3", 3, 5, 1, 64),
+        ("int8", 9, 2, 1, 64), ("int8", 2, 24, 3, 128), ("int8", 3, 24, 4, 256), ("e4m3", 3, 24, 4, 256)]
+
+
+@pytest.mark.parametrize("fmt,q_tokens,heads,kv_heads,dim", WIDE)
+def test_more_rows_of_a_key_head(runtime, fmt, q_tokens, heads, kv_heads, dim):
+    _case(runtime, fmt, RAGGED, q_tokens, heads, kv_heads, dim, 16, ("f32", "f32"))
+    _case(runtime, fmt, [20011, 7, 1031], q_tokens, heads, kv_heads, dim, 64, ("bf16", "bf16"), q_gain=2.0)
+
+
+@pytest.mark.parametrize("fmt,q_tokens,heads,kv_heads,dim", WIDE)
+def test_numbers_that_are_not_finite_among_more_rows(runtime, fmt, q_tokens, heads, kv_heads, dim):
+    import torch
+
+    group, n = heads // kv_heads, 40
+    for where in ("k", "v", "q"):
+        cache, lengths, q, out, scale = _case(runtime, fmt, [n, n], q_tokens, heads, kv_heads, dim, 16, ("f32", "f32"))
+        page, slot = cache.place(torch.tensor([0], device="cuda"), torch.tensor([n - 2], device="cuda"))
+        good, last = out.clone(), kv_heads - 1
+        if where == "q":
+            q[1, heads - 1, 5] = math.nan
+        elif fmt == "bf16":
+            cache.pools["kv".index(where)][page, last, slot, 3] = math.nan
+        else:
+            cache.scales["kv".index(where)][page, last, slot] = math.nan
+        _attend(runtime, cache, lengths, q, q_tokens, scale, out, ("f32", "f32"), heads)
+        runtime.device_status()
+        bad = torch.zeros_like(out, dtype=torch.bool)
+        if where == "q":
+            bad[1, heads - 1] = True
+        else:
+            # the last two tokens of sequence 0 see position n - 2
+            bad[max(q_tokens - 2, 0):q_tokens, last * group:(last + 1) * group, slice(3, 4) if where == "v" and fmt == "bf16" else slice(None)] = True
+        assert torch.equal(torch.isnan(out), bad)
+        assert torch.equal(out[~bad], good[~bad])
+
+
 @pytest.mark.parametrize("names", [("f32", "bf16"), ("bf16", "f32")])
 def test_many_sequences(runtime, names):
     lengths = [(i * 37) % 150 for i in range(700)]
