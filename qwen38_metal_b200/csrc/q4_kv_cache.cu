@@ -278,7 +278,7 @@ template <int FMT, int LANES, bool TURN>
 __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p, uint32_t block_tokens) {
     __shared__ float2 cs[TURN ? kMostTokens : 1][kMaxHeadDim / 2];
     __shared__ Place places[kMostTokens];
-    __shared__ uint32_t replaced;  // a bit a token: one behind it has the same place
+    __shared__ uint32_t found[8];  // a bit a token: one behind it has the same place
     grid_dependency_wait();
     grid_dependents_launch();
     const uint64_t t0 = (uint64_t)blockIdx.x * block_tokens;
@@ -302,19 +302,21 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
         }
     };
     load_rows();
-    if (threadIdx.x == 0) replaced = 0;
     if (threadIdx.x < tokens) places[threadIdx.x] = place_of(p, t0 + threadIdx.x);
-    __syncthreads();
     if (TURN)
         for (uint32_t i = threadIdx.x; i < tokens * pairs; i += blockDim.x) {
             const uint32_t t = i / pairs;
-            cs[t][i - t * pairs] = turn(p.rotary, i - t * pairs, places[t].position);
+            cs[t][i - t * pairs] = turn(p.rotary, i - t * pairs, p.positions[t0 + t]);
         }
-    int32_t low = 0x7fffffff, high = -1;
-    for (uint32_t t = 0; t < tokens; ++t)
-        if (places[t].stands) low = min(low, places[t].position), high = max(high, places[t].position);
     // Tokens behind the block's first are looked through four at a time, from the first whose position starts at 16 bytes. Runs of one length
     // end the search with the last token's own.
+    int32_t low = 0x7fffffff, high = -1;
+#pragma unroll 1
+    for (uint32_t t = 0; t < tokens; ++t) {
+        const int32_t position = p.positions[t0 + t];
+        if (position >= 0) low = min(low, position), high = max(high, position);
+    }
+    uint32_t replaced = 0;
     const uint64_t behind = t0 + 1, end = p.sequences ? p.tokens : min(p.tokens, (t0 + tokens - 1) / p.run * p.run + p.run);
     const uint64_t fours = min(end, behind + (0u - (uint32_t)((uintptr_t)(p.positions + behind) >> 2) & 3u)), last = fours + ((end - min(fours, end)) & ~3ull);
     const auto compare = [&](uint64_t u, int32_t position) {
@@ -322,7 +324,7 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
         const int32_t sequence = sequence_of(p, u);
 #pragma unroll 1
         for (uint32_t t = 0; t < tokens; ++t)
-            if (position == places[t].position && sequence == places[t].sequence && u > t0 + t) atomicOr(&replaced, 1u << t);
+            if (position == p.positions[t0 + t] && sequence == sequence_of(p, t0 + t) && u > t0 + t) replaced |= 1u << t;
     };
     if (threadIdx.x < fours - min(behind, fours)) compare(behind + threadIdx.x, p.positions[behind + threadIdx.x]);
     if (threadIdx.x < end - last) compare(last + threadIdx.x, p.positions[last + threadIdx.x]);
@@ -336,13 +338,16 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
         for (int i = 0; i < 4; ++i) sequence[i] = sequence_of(p, u + i);
 #pragma unroll 1
         for (uint32_t t = 0; t < tokens; ++t) {
-            bool same = false;
+            const int32_t own = p.positions[t0 + t], own_sequence = sequence_of(p, t0 + t);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) same = same || (at[i] == places[t].position && sequence[i] == places[t].sequence && u + i > t0 + t);
-            if (same) atomicOr(&replaced, 1u << t);
+            for (int i = 0; i < 4; ++i)
+                if (at[i] == own && sequence[i] == own_sequence && u + i > t0 + t) replaced |= 1u << t;
         }
     }
+    replaced = __reduce_or_sync(0xffffffffu, replaced);
+    if (lane == 0) found[threadIdx.x >> 5] = replaced;
     __syncthreads();
+    replaced = __reduce_or_sync(0xffffffffu, lane < 8 ? found[lane] : 0u);
 #pragma unroll 1
     for (;;) {
 #pragma unroll
