@@ -256,7 +256,7 @@ __device__ __forceinline__ Place place_of(const KvTokensParams &p, uint64_t t) {
     return a;
 }
 
-// Rows of a block's tokens: keys and values of every head. Each has LANES lanes, eight values a lane; a warp takes 32 / LANES rows at a time.
+// Rows of a block's tokens: keys and values of every head; a warp takes 32 / LANES rows at a time.
 struct Row {
     uint32_t token, i;  // token of the block; head, or kv_heads + head for values
     __device__ __forceinline__ Row(uint32_t r, uint32_t a_token) : token(r / a_token), i(r % a_token) {}
@@ -268,13 +268,15 @@ struct Row {
 };
 
 constexpr uint32_t kMostTokens = 8;  // of a block
-constexpr uint32_t kRowsAhead = 4;   // rows that are on their way to a lane
+constexpr uint32_t kRowsAhead = 4;   // eights of values that are on their way to a lane
 
 // A block writes up to kMostTokens tokens. Of several tokens with the same place the last one is kept: every block looks through the tokens
-// behind its own (most by one comparison with the range of its positions) while its first rows are on their way. Bound by memory for long
-// prompts, by latency for single tokens. With the read kernel, for 4096 tokens of 2 x 4 x 256 fp32 values in int8: 30 us (84 MB, 12.8 us at the
-// peak); a block a token with whole warps for every row 54 us; rows loaded behind the scan 36 us; registers for three blocks an SM 34 us.
-template <int FMT, int LANES, bool TURN>
+// behind its own (most by one comparison with the range of its positions) while its first rows are on their way. A row is LANES lanes with
+// EIGHTS eights of values each: two where keys are not turned (the other value of a pair is an eight of another lane), which halves what a
+// row costs beside its values. Bound by instructions for long prompts, which keep the issue slots half busy, and by latency for single tokens.
+// With the read kernel, for 4096 tokens of 2 x 4 x 256 fp32 values in int8: 28 us (84 MB, 12.8 us at the peak), with one eight a lane 30 us;
+// rows loaded behind the scan 36 us; registers for three blocks an SM 34 us; a block a token with whole warps for every row 54 us.
+template <int FMT, int LANES, int EIGHTS, bool TURN>
 __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p, uint32_t block_tokens) {
     __shared__ float2 cs[TURN ? kMostTokens : 1][kMaxHeadDim / 2];
     __shared__ Place places[kMostTokens];
@@ -283,22 +285,27 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
     grid_dependents_launch();
     const uint64_t t0 = (uint64_t)blockIdx.x * block_tokens;
     const uint32_t tokens = (uint32_t)min((uint64_t)block_tokens, p.tokens - t0), pairs = p.rotary.pairs;
-    const uint32_t lane = threadIdx.x & 31u, part = lane % LANES, d = part * 8u, rows = tokens * 2 * p.kv.kv_heads;
+    constexpr uint32_t kAhead = kRowsAhead / EIGHTS;
+    const uint32_t lane = threadIdx.x & 31u, part = lane % LANES, rows = tokens * 2 * p.kv.kv_heads;
     const uint32_t step = (blockDim.x >> 5) * (32 / LANES);
     const uint32_t kv_heads = p.kv.kv_heads;
-    float v[kRowsAhead][8];
+    float v[kAhead][EIGHTS][8];  // values (part + e * LANES) * 8 and on
     uint32_t r0 = (threadIdx.x >> 5) * (32 / LANES);
     const Row by(step, 2 * kv_heads);
     Row loads(r0 + lane / LANES, 2 * kv_heads), row = loads;
     const auto load_rows = [&]() {
 #pragma unroll
-        for (uint32_t k = 0; k < kRowsAhead; ++k, loads.advance(by, 2 * kv_heads)) {
+        for (uint32_t k = 0; k < kAhead; ++k, loads.advance(by, 2 * kv_heads)) {
             const bool values = loads.i >= kv_heads;
             const void *in = values ? p.v_in : p.k_in;
+            const bool has = loads.token < tokens && in;
+            const uint64_t from = (t0 + loads.token) * (values ? p.v_stride : p.k_stride) + (loads.i - (values ? kv_heads : 0u)) * p.kv.head_dim + part * 8;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
-            if (loads.token < tokens && in && d < p.kv.head_dim)
-                load8(in, (t0 + loads.token) * (values ? p.v_stride : p.k_stride) + (loads.i - (values ? kv_heads : 0u)) * p.kv.head_dim + d, p.is_f32, v[k]);
+            for (uint32_t e = 0; e < EIGHTS; ++e) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[k][e][j] = 0.f;
+                if (has && (part + e * LANES) * 8 < p.kv.head_dim) load8(in, from + e * LANES * 8, p.is_f32, v[k][e]);
+            }
         }
     };
     load_rows();
@@ -351,51 +358,57 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
 #pragma unroll 1
     for (;;) {
 #pragma unroll
-        for (uint32_t k = 0; k < kRowsAhead; ++k, row.advance(by, 2 * kv_heads)) {
+        for (uint32_t k = 0; k < kAhead; ++k, row.advance(by, 2 * kv_heads)) {
             if (r0 + k * step >= rows) break;
             const bool values = row.i >= kv_heads;
             const uint32_t head = row.i - (values ? kv_heads : 0u), at = min(row.token, tokens - 1);
             const bool writes = row.token < tokens && (values ? p.v_in : p.k_in) && places[at].stands && !(replaced >> at & 1u);
             if (TURN) {
+                const uint32_t d = part * 8;
                 const bool turns = !values && d < 2 * pairs;
                 if (p.rotary.interleaved) {
-                    if (turns) turn_interleaved(v[k], d / 2, pairs, cs[at]);
+                    if (turns) turn_interleaved(v[k][0], d / 2, pairs, cs[at]);
                 } else if (pairs % 8 == 0) {
                     // the other values of the pairs are those of a lane of the same row
                     const uint32_t by = pairs / 8, other = (lane & ~(LANES - 1u)) + (part < by ? part + by : part - by) % LANES;
                     const uint32_t i = part < by ? d : d - pairs;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float b = __shfl_sync(0xffffffffu, v[k][j], other);
-                        if (turns) v[k][j] = v[k][j] * cs[at][i + j].x + (part < by ? -b : b) * cs[at][i + j].y;
+                        const float b = __shfl_sync(0xffffffffu, v[k][0][j], other);
+                        if (turns) v[k][0][j] = v[k][0][j] * cs[at][i + j].x + (part < by ? -b : b) * cs[at][i + j].y;
                     }
                 } else if (turns && writes) {
                     const uint64_t key = (t0 + at) * p.k_stride + head * p.kv.head_dim;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const uint32_t e = d + j;
-                        if (e < pairs) v[k][j] = v[k][j] * cs[at][e].x - load1(p.k_in, key + e + pairs, p.is_f32) * cs[at][e].y;
-                        else if (e < 2 * pairs) v[k][j] = v[k][j] * cs[at][e - pairs].x + load1(p.k_in, key + e - pairs, p.is_f32) * cs[at][e - pairs].y;
+                        if (e < pairs) v[k][0][j] = v[k][0][j] * cs[at][e].x - load1(p.k_in, key + e + pairs, p.is_f32) * cs[at][e].y;
+                        else if (e < 2 * pairs) v[k][0][j] = v[k][0][j] * cs[at][e - pairs].x + load1(p.k_in, key + e - pairs, p.is_f32) * cs[at][e - pairs].y;
                     }
                 }
             }
-            uint8_t *const to = (values ? p.kv.v : p.kv.k) + places[at].row + head * p.kv.head_stride;
-            const bool has = writes && d < p.kv.head_dim;
+            uint8_t *const to = (values ? p.kv.v : p.kv.k) + places[at].row + head * p.kv.head_stride + part * (FMT == 0 ? 16 : 8);
             if (FMT == 0) {
-                if (has) *reinterpret_cast<uint4 *>(to + 2 * d) = pack8_bf16(v[k]);
+#pragma unroll
+                for (uint32_t e = 0; e < EIGHTS; ++e)
+                    if (writes && (part + e * LANES) * 8 < p.kv.head_dim) *reinterpret_cast<uint4 *>(to + e * LANES * 16) = pack8_bf16(v[k][e]);
                 continue;
             }
             uint32_t amax = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[k][j]) & 0x7fffffffu);
+            for (uint32_t e = 0; e < EIGHTS; ++e)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[k][e][j]) & 0x7fffffffu);
 #pragma unroll
             for (int off = LANES / 2; off > 0; off >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, off));
             const bool finite = amax < 0x7f800000u;
             const float scale = finite ? __fdiv_rn(__uint_as_float(amax), FMT == 1 ? 127.f : 448.f) : __uint_as_float(0x7fc00000u);
-            if (has) *reinterpret_cast<uint2 *>(to + d) = finite ? encode8<FMT == 0 ? 1 : FMT>(v[k], scale) : make_uint2(0u, 0u);
+#pragma unroll
+            for (uint32_t e = 0; e < EIGHTS; ++e)
+                if (writes && (part + e * LANES) * 8 < p.kv.head_dim) *reinterpret_cast<uint2 *>(to + e * LANES * 8) = finite ? encode8<FMT == 0 ? 1 : FMT>(v[k][e], scale) : make_uint2(0u, 0u);
             if (writes && part == 0) (values ? p.kv.v_scales : p.kv.k_scales)[places[at].scale + head * p.kv.page_tokens] = scale;
         }
-        r0 += kRowsAhead * step;
+        r0 += kAhead * step;
         if (r0 >= rows) break;
         load_rows();
     }
@@ -455,7 +468,7 @@ uint32_t block_tokens(uint64_t tokens, uint32_t sm_count) { return (uint32_t)(to
 template <int FMT, int LANES>
 cudaError_t launch_tokens(const KvTokensParams &p, bool write, uint32_t sm_count, cudaStream_t stream) {
     const uint32_t each = block_tokens(p.tokens, sm_count);
-    const auto kernel = !write ? kv_read_kernel<FMT, LANES> : p.rotary.step && p.k_in ? kv_write_kernel<FMT, LANES, true> : kv_write_kernel<FMT, LANES, false>;
+    const auto kernel = !write ? kv_read_kernel<FMT, LANES> : p.rotary.step && p.k_in ? kv_write_kernel<FMT, LANES, 1, true> : kv_write_kernel<FMT, LANES / 2, 2, false>;
     return launch_dependent(kernel, dim3((uint32_t)((p.tokens + each - 1) / each)), 256, 0, stream, p, each);
 }
 
