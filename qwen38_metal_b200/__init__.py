@@ -8,5 +8,13 @@ B200, constructing a runtime raises.
 from .runtime import (CudaRuntime, DeviceBuffer, KvCache, KvTable, MappedQ4AffineJob, Q4RuntimeError, Rotary,  # noqa: F401
                       rotary_frequencies)
 
-__all__ = ["CudaRuntime", "DeviceBuffer", "KvCache", "KvTable", "MappedQ4AffineJob", "Q4RuntimeError", "Rotary",
+__all__ = ["AttentionLayer", "CudaRuntime", "DeviceBuffer", "KvCache", "KvTable", "MappedQ4AffineJob", "Q4RuntimeError", "Rotary",
            "rotary_frequencies"]
+
+
+def __getattr__(name):  # (needs torch, which the calls over host buffers do not)
+    if name == "AttentionLayer":
+        from .attention import AttentionLayer
+
+        return AttentionLayer
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
