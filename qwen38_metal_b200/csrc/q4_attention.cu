@@ -442,27 +442,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         unsigned long long limit_ns = kWaitLimitNs;
         uint32_t weights_at = weights;  // one of two
         Cursor at = share.at;
-        // eight values of query row `warp` of each set of eight; those of the next item are on their way meanwhile where registers allow
+        // eight values of query row `warp` of each set of eight, as they lie in memory; those of the next item are on their way meanwhile where registers allow
         constexpr bool kAhead = SETS == 1;
-        float q[SETS][8];
+        uint4 rows_in[SETS][2];
         const auto load_query = [&](const Cursor &c) {
 #pragma unroll
             for (uint32_t set = 0; set < SETS; ++set) {
                 const uint32_t r = c.item % g.chunks * S::kRows + set * kAttentionRows + warp, d = lane * 8;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q[set][i] = 0.f;
+                rows_in[set][0] = rows_in[set][1] = make_uint4(0u, 0u, 0u, 0u);
                 if (r < g.rows && d < p.kv.head_dim) {
                     const uint64_t base = ((uint64_t)c.s * p.q_tokens + r / g.group) * p.q_stride + ((uint64_t)(c.item / g.chunks) * g.group + r % g.group) * p.kv.head_dim + d;
-                    if (p.q_is_f32) {
-                        const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + base);
-                        const float4 v = __ldcg(f), w = __ldcg(f + 1);
-                        q[set][0] = v.x, q[set][1] = v.y, q[set][2] = v.z, q[set][3] = v.w, q[set][4] = w.x, q[set][5] = w.y, q[set][6] = w.z, q[set][7] = w.w;
-                    } else {
-                        const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + base));
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) q[set][2 * i] = __uint_as_float(w[i] << 16), q[set][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-                    }
+                    const uint4 *const from = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(p.q) + base * (p.q_is_f32 ? 4 : 2));
+                    rows_in[set][0] = __ldcg(from);
+                    if (p.q_is_f32) rows_in[set][1] = __ldcg(from + 1);
                 }
             }
         };
@@ -476,13 +468,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             if (!kAhead) load_query(at);
 #pragma unroll
             for (uint32_t set = 0; set < SETS; ++set) {
-                const uint32_t d = lane * 8;
+                const uint32_t d = lane * 8, w[8] = {rows_in[set][0].x, rows_in[set][0].y, rows_in[set][0].z, rows_in[set][0].w, rows_in[set][1].x, rows_in[set][1].y, rows_in[set][1].z, rows_in[set][1].w};
+                float q[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q[i] = __uint_as_float(p.q_is_f32 ? w[i] : i % 2 == 0 ? w[i / 2] << 16 : w[i / 2] & 0xffff0000u);
                 float unit = 1.f, row_scale = p.scale * 1.4426950408889634f;
                 if (FMT != 0) {
                     // fp16 halves, whole numbers: the row is scaled by a power of two that brings its largest value into [1, 2)
                     uint32_t amax = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(q[set][i]) & 0x7fffffffu);
+                    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(q[i]) & 0x7fffffffu);
                     amax = __reduce_max_sync(0xffffffffu, amax);
                     const uint32_t e = min(max(amax >> 23, 1u), 254u);
                     unit = e == 254u ? __uint_as_float(0x00400000u) : __uint_as_float((254u - e) << 23);
@@ -496,15 +491,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     const uint32_t piece = d / S::kChunkDims, seg = piece / (S::kSeg / 16), in_seg = piece % (S::kSeg / 16);
                     const uint32_t m = (seg * S::kPieces + in_seg % S::kPieces) * kPer + d % S::kChunkDims / 4, to = queries + set * S::kSetQueries + (m * 32 + warp * 4 + in_seg / S::kPieces) * 16;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) q[set][i] *= unit;
+                    for (int i = 0; i < 8; ++i) q[i] *= unit;
                     uint4 a, b;
                     if (FMT == 1) {
-                        split_digits(q[set], a, b);
+                        split_digits(q, a, b);
                     } else {
-                        split<FMT>(q[set][0], q[set][1], a.x, a.y);
-                        split<FMT>(q[set][2], q[set][3], a.z, a.w);
-                        split<FMT>(q[set][4], q[set][5], b.x, b.y);
-                        split<FMT>(q[set][6], q[set][7], b.z, b.w);
+                        split<FMT>(q[0], q[1], a.x, a.y);
+                        split<FMT>(q[2], q[3], a.z, a.w);
+                        split<FMT>(q[4], q[5], b.x, b.y);
+                        split<FMT>(q[6], q[7], b.z, b.w);
                     }
                     sts_v4(to, a);
                     sts_v4(to + 512, b);
