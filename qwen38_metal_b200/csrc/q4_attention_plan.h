@@ -47,19 +47,31 @@ struct AttentionCut {
 };
 
 // `tiles`: of all items, `items`: those that have any, `longest`: tiles of the longest one.
+//   * Items stay whole where that costs a block no more than four times `least` tiles: what joining cut items takes. Where each has a block of its
+//     own a piece is as long as the longest; more of them go by where their middles lie. (Int8, 4 key heads of 256, whole against cut: 128 items of
+//     800 / 1600 / 3600 tokens 22.5 / 32.8 / 57.3 us against 26.6 / 36.9 / 61.4; 52 items of 800 / 1600 / 3600 tokens 18.4 / 26.6 / 45.1 against
+//     22.5 / 26.6 / 36.9; 240 items of 800 / 3600 tokens 38.9 / 104.4 against 43.0 / 102.4. Few items leave most blocks idle, and joining is all
+//     that goes on: 4 items of 300 / 600 / 1000 tokens 14.3 / 16.4 / 18.4 against 16.3 / 16.4 / 16.4.)
 //   * Few items are cut into pieces: no block has a second start or an uneven rest. pieces <= tiles / run + items <= blocks
 //     holds for run >= tiles / (blocks - items). (Above a third of the blocks the longer runs cost more: 64 items 74 us, in equal runs 55 us.)
-//   * Items that are short against a run stay whole: what a block does more than another is less than joining cut items takes.
 //   * Otherwise all blocks take the same number of tiles.
 Q4_PLAN_FN AttentionCut attention_cut(uint32_t tiles, uint32_t items, uint32_t longest, uint32_t blocks, uint32_t least, uint32_t shift) {
     AttentionCut c;
     c.shift = shift;
     c.tiles = tiles;
-    c.mode = items <= blocks / 3 ? kEqualPieces : kEqualRuns;
-    const uint32_t by = c.mode == kEqualPieces ? blocks - items : blocks;
-    c.run = (tiles - 1) / by + 1;
-    if (c.mode == kEqualRuns && (longest <= 2 * least || longest <= c.run / 16)) c.mode = kWholeItems;
-    if (c.mode != kWholeItems && c.run < least) c.run = least;
+    const uint32_t even = (tiles - 1) / blocks + 1, more = longest > even ? longest - even : 0;
+    const bool few = items <= blocks / 3;
+    if (items <= blocks && more <= (few ? 2 : 4) * least) {
+        c.mode = kEqualPieces;
+        c.run = longest;
+    } else if (few) {
+        c.mode = kEqualPieces;
+        c.run = (tiles - 1) / (blocks - items) + 1;
+        if (c.run < least) c.run = least;
+    } else {
+        c.mode = longest <= 4 * least || longest <= even / 16 ? kWholeItems : kEqualRuns;
+        c.run = even < least && c.mode == kEqualRuns ? least : even;
+    }
     return c;
 }
 
