@@ -8,7 +8,7 @@
  *
  * The conventions are those of the `_device` calls of q4b200.h: device pointers, work enqueued on the stream that is given,
  * no synchronisation, outputs untouched when a call returns an error, calls on one runtime ordered on the device (they share
- * its scratch; a captured graph may be replayed as long as the runtime lives). None of these calls allocates.
+ * its scratch; a captured graph may be replayed as long as the runtime lives). None of the `_device` calls allocates.
  *
  * Activations are rows of a token: heads x head_dim values, heads behind each other, `stride` VALUES from one token to the
  * next. Types Q4B_F32 and Q4B_BF16. Addresses are multiples of 16 bytes and so are strides in bytes, else
@@ -104,7 +104,8 @@ typedef struct q4b_kv_cache {
 } q4b_kv_cache;
 
 /* Which pages hold a sequence: token at position p is in page pages_dev[sequence * row_stride + p / page_tokens]. Entries that
- * no token needs are not read. row_stride 0 stands for pages_per_sequence. Sequences may share pages for reading. */
+ * no token needs are not read. row_stride 0 stands for pages_per_sequence. Sequences may share pages for reading; one call may not write
+ * a place of a shared page twice (through two sequences, or two entries of one). */
 typedef struct q4b_kv_table {
     const int32_t *pages_dev;
     uint32_t sequences;
@@ -138,7 +139,8 @@ int q4b_kv_read_device(q4b_runtime *rt, const q4b_kv_cache *cache, const q4b_kv_
  * factors of each product to 16 bits or more (8-bit caches: queries to 2^-25 of the row's largest one at least, weights times scales
  * to 2^-26 of the largest one). A number that is not finite, in a query or in keys and values, reaches the rows that
  * see it and no others. What lies behind a sequence's length in its last page is not looked at, whatever it is.
- * The same call on the same data gives the same bits; another batch around a sequence may change its last bits. */
+ * The same call on the same data gives the same bits; another batch around a sequence may change its last bits. Tables that could
+ * hold 2^32 or more 16s of tokens, over all sequences, key heads and eights of their query rows, are Q4B_DIMENSION_OVERFLOW. */
 int q4b_attention_device(q4b_runtime *rt, const q4b_kv_cache *cache, const q4b_kv_table *table, const int32_t *lengths_dev,
                          const void *q_dev, int q_dtype, uint64_t q_stride, uint32_t heads, uint32_t q_tokens, float scale,
                          void *out_dev, int out_dtype, uint64_t out_stride, void *stream);
