@@ -35,6 +35,12 @@ class AttentionLayer:
         for name, job, rows in (("q", q, heads * head_dim), ("k", k, kv_heads * head_dim), ("v", v, kv_heads * head_dim), ("o", o, hidden)):
             if job.output_rows != rows:
                 raise Q4RuntimeError(6, f"{name} projection has {job.output_rows} elements, expected {rows}")
+        if not 1 <= tokens <= 16:
+            raise Q4RuntimeError(7, f"tokens {tokens} is not a number from 1 to 16")
+        if sequences < 1 or pages_per_sequence < 1 or page_tokens < 16 or page_tokens % 16:
+            raise Q4RuntimeError(13, "an attention layer needs sequences, pages and pages of a multiple of 16 tokens")
+        if heads % kv_heads:
+            raise Q4RuntimeError(6, f"heads has {heads} elements, expected a multiple of {kv_heads}")
         if cache_format not in _POOLS:
             raise Q4RuntimeError(13, f"unknown cache format {cache_format}")
         self.rt, self.q, self.k, self.v, self.o = rt, q, k, v, o

@@ -2,6 +2,7 @@
 // launches of the kernels in q4_kv_cache.cu and q4_attention.cu.
 #include "../../include/q4b_attention.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -31,8 +32,9 @@ int fail(int status, const char *fmt, ...) {
 }
 
 int launched(cudaError_t e, const char *what) {
-    if (e != cudaSuccess) return fail(Q4B_CUDA_ERROR, "CUDA call failed in %s: %s", what, cudaGetErrorString(e));
-    return Q4B_OK;
+    if (e == cudaSuccess) return Q4B_OK;
+    cudaGetLastError();  // (or the next call's launch would report it again)
+    return fail(Q4B_CUDA_ERROR, "CUDA call failed in %s: %s", what, cudaGetErrorString(e));
 }
 
 // A range of device memory that a call reads or writes: [begin, end).
@@ -153,6 +155,28 @@ int check_cache(const q4b_kv_cache *c, const q4b_kv_table *t, bool need_k, bool 
     view->per_sequence = t->pages_per_sequence;
     view->row_stride = entries;
     return Q4B_OK;
+}
+
+// Whether a row of the keys and one of the values share memory. Tokens, heads and pages lie inside one another, so that along each of them,
+// from the widest on, only the two steps nearest to the distance come near enough.
+bool rows_meet(const q4::KvView &kv, int64_t apart) {
+    struct Axis {
+        int64_t stride, count;
+    } axis[3] = {{(int64_t)kv.token_stride, kv.page_tokens}, {(int64_t)kv.head_stride, kv.kv_heads}, {(int64_t)kv.page_stride, kv.pages}};
+    std::sort(axis, axis + 3, [](const Axis &a, const Axis &b) { return a.stride > b.stride; });
+    const int64_t row = (int64_t)kv.head_dim * value_bytes(kv.format);
+    for (int pick = 0; pick < 8; ++pick) {
+        int64_t left = apart;
+        bool there = true;
+        for (int i = 0; i < 3; ++i) {
+            if (axis[i].count == 1) continue;
+            int64_t step = left / axis[i].stride - (left % axis[i].stride < 0) + (pick >> i & 1);
+            there = there && step < axis[i].count && -step < axis[i].count;
+            left -= step * axis[i].stride;
+        }
+        if (there && left < row && -left < row) return true;
+    }
+    return false;
 }
 
 int check_index(const char *name, const int32_t *ptr, uint64_t count, Span *span) {
@@ -347,7 +371,8 @@ extern "C" int q4b_kv_write_device(q4b_runtime *rt, const q4b_kv_cache *cache, c
     CacheSpans spans;
     Span rows[2], index[2];
     if (int st = check_kv_tokens(cache, table, positions_dev, sequences_dev, tokens, k_dev, k_stride, v_dev, v_stride, dtype, &p, &spans, rows, index)) return st;
-    if (k_dev && v_dev && cache->k == cache->v) return fail(Q4B_INVALID_ARGUMENT, "keys and values of the cache share memory");
+    if (k_dev && v_dev && (rows_meet(p.kv, (int64_t)((uintptr_t)cache->v - (uintptr_t)cache->k)) || spans.k_scales.meets(spans.v_scales)))
+        return fail(Q4B_INVALID_ARGUMENT, "keys and values of the cache share memory");
     if (spans.meets(rows[0]) || spans.meets(rows[1]) || spans.meets(index[0]) || spans.meets(index[1]) || spans.meets(spans.table))
         return fail(Q4B_INVALID_ARGUMENT, "cache shares memory with an input");
     if (int st = check_rt(rt)) return st;
@@ -374,7 +399,7 @@ extern "C" int q4b_kv_read_device(q4b_runtime *rt, const q4b_kv_cache *cache, co
         // keys and values of a token may stand beside each other in rows of one stride
         const uint64_t size = dtype == Q4B_F32 ? 4 : 2, width = (uint64_t)cache->kv_heads * cache->head_dim * size, step = k_stride * size;
         const uint64_t apart = rows[0].begin < rows[1].begin ? rows[1].begin - rows[0].begin : rows[0].begin - rows[1].begin;
-        if (k_stride != v_stride || apart % step < width || step - apart % step < width) return fail(Q4B_INVALID_ARGUMENT, "outputs share memory");
+        if (tokens == 1 || k_stride != v_stride || apart % step < width || step - apart % step < width) return fail(Q4B_INVALID_ARGUMENT, "outputs share memory");
     }
     for (const Span &out : {rows[0], rows[1]})
         if (spans.meets(out) || index[0].meets(out) || index[1].meets(out) || spans.table.meets(out)) return fail(Q4B_INVALID_ARGUMENT, "output shares memory with an input");

@@ -791,7 +791,7 @@ extern "C" int q4b_runtime_create(int device_ordinal, q4b_runtime **out) {
     if (e == cudaSuccess) e = rt->gemm_parts.ensure(q4_gemm_most_partial_floats((uint32_t)rt->sm_count / 2u) * 4, true);
     if (e == cudaSuccess) e = rt->gemm_counters.ensure((size_t)q4_gemm_most_counters((uint32_t)rt->sm_count / 2u) * 4);
     if (e == cudaSuccess) e = cudaMemset(rt->gemm_counters.ptr, 0, rt->gemm_counters.capacity);
-    // partial results of attention items that are cut over blocks (two 8 KB slots a block)
+    // partial results of attention items that are cut over blocks (two 24 KB slots a block)
     if (e == cudaSuccess) e = rt->attention_parts.ensure(q4k_attention_part_floats((uint32_t)rt->sm_count) * 4, true);
     if (e == cudaSuccess) e = rt->attention_counters.ensure((size_t)rt->sm_count * 4);
     if (e == cudaSuccess) e = cudaMemset(rt->attention_counters.ptr, 0, rt->attention_counters.capacity);

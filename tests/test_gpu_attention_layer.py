@@ -168,3 +168,6 @@ def test_wrong_projections_are_refused(runtime):
     for jobs, fmt in (((q, kv, q, o), "int8"), ((kv, kv, kv, o), "int8"), ((q, kv, kv, q), "int8"), ((q, kv, kv, o), "int4")):
         with pytest.raises(Q4RuntimeError):
             AttentionLayer(runtime, *jobs, HIDDEN, 2, 1, 64, 1, 1, cache_format=fmt)
+    for more in (dict(tokens=0), dict(tokens=17), dict(sequences=0), dict(page_tokens=24)):
+        with pytest.raises(Q4RuntimeError):
+            AttentionLayer(runtime, q, kv, kv, o, HIDDEN, 2, 1, 64, **{"sequences": 1, "pages_per_sequence": 1, "page_tokens": 16, **more})

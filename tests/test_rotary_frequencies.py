@@ -215,6 +215,31 @@ def test_shared_memory_is_refused(lib):
     assert _attend(lib, cache=_cache(v=K)) == NO_RUNTIME  # reading one pool as both is allowed
 
 
+def test_one_token_has_no_step_from_one_row_to_the_next(lib):
+    share = lambda got: got[0] == "InvalidArgument" and "share" in got[1]  # noqa: E731
+    one = dict(tokens=1, k_stride=0, v_stride=0)
+    assert _read(lib, **one) == NO_RUNTIME and _write(lib, **one) == NO_RUNTIME
+    assert share(_read(lib, k=Q, v=Q, **one)) and share(_read(lib, k=Q, v=Q + 16, **one)) and share(_read(lib, k=Q + 4080, v=Q, **one))
+    assert _read(lib, k=Q, v=Q + 4096, **one) == NO_RUNTIME
+
+
+def test_keys_and_values_that_would_be_written_over_each_other_are_refused(lib):
+    share = lambda got: got[0] == "InvalidArgument" and "share" in got[1]  # noqa: E731
+    page = 4 * 16 * 256
+    for off in (16, 240, 256, 4096, page, 63 * page + 16, 64 * page - 256):
+        assert share(_write(lib, cache=_cache(v=K + off))) and share(_write(lib, cache=_cache(k=V + off))), off
+    assert _write(lib, cache=_cache(v=K + 64 * page)) == NO_RUNTIME
+    # pages of keys, then of values; heads of both in turn; rows of both in turn
+    for strides, off in ((dict(token_stride=256, head_stride=4096, page_stride=2 * page), page), (dict(token_stride=256, head_stride=8192, page_stride=2 * page), 4096),
+                         (dict(token_stride=512, head_stride=8192, page_stride=2 * page), 256), (dict(token_stride=2048, head_stride=512, page_stride=2 * page), 256)):
+        assert _write(lib, cache=_cache(v=K + off, **strides)) == NO_RUNTIME
+        assert _write(lib, cache=_cache(k=V + off, **strides)) == NO_RUNTIME
+        assert _write(lib, cache=_cache(v=K + off + 2 * page, **strides)) == NO_RUNTIME
+        assert share(_write(lib, cache=_cache(v=K + off - 16, **strides))) and share(_write(lib, cache=_cache(v=K + off + 2 * page + 240, **strides)))
+    assert share(_write(lib, cache=_cache(v_scales=KS))) and share(_write(lib, cache=_cache(v_scales=KS + 16)))
+    assert _write(lib, k=None, cache=_cache(k=V + 16, k_scales=VS)) == NO_RUNTIME  # one side alone
+
+
 def test_rotary_refusals(lib):
     def call(rotary=None, x=Q, x_dtype=0, x_stride=6144, tokens=4, heads=24, head_dim=256, pos=POS, out=OUT, out_dtype=0, out_stride=6144):
         return _status(lib, "q4b_rotary_device", None, rotary, x, x_dtype, x_stride, tokens, heads, head_dim, pos, out, out_dtype, out_stride, None)
