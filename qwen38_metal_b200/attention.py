@@ -36,7 +36,7 @@ class AttentionLayer:
             if job.output_rows != rows:
                 raise Q4RuntimeError(6, f"{name} projection has {job.output_rows} elements, expected {rows}")
         if not 1 <= tokens <= 16:
-            raise Q4RuntimeError(7, f"tokens {tokens} is not a number from 1 to 16")
+            raise Q4RuntimeError(14, f"tokens {tokens} is not a number from 1 to 16")
         if sequences < 1 or pages_per_sequence < 1 or page_tokens < 16 or page_tokens % 16:
             raise Q4RuntimeError(13, "an attention layer needs sequences, pages and pages of a multiple of 16 tokens")
         if heads % kv_heads:

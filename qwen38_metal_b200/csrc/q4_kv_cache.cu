@@ -267,6 +267,21 @@ struct Row {
     }
 };
 
+// The eight values of a lane: two fours. Of fp32 rows they lie apart, so that what a warp asks for, or stores, at once has no gaps (4096 tokens of
+// int8 written and read back 28 us with them side by side).
+struct Fours {
+    uint32_t a, b;
+};
+template <int LANES>
+__device__ __forceinline__ Fours fours_of(uint32_t part, uint32_t e, bool apart) {
+    const uint32_t a = apart ? (2 * e * LANES + part) * 4 : (e * LANES + part) * 8;
+    return {a, a + (apart ? LANES * 4 : 4)};
+}
+__device__ __forceinline__ void load4(const void *base, uint64_t at, float *v) {
+    const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+}
+
 constexpr uint32_t kMostTokens = 8;  // of a block
 constexpr uint32_t kRowsAhead = 4;   // eights of values that are on their way to a lane
 
@@ -274,9 +289,9 @@ constexpr uint32_t kRowsAhead = 4;   // eights of values that are on their way t
 // behind its own (most by one comparison with the range of its positions) while its first rows are on their way. A row is LANES lanes with
 // EIGHTS eights of values each: two where keys are not turned (the other value of a pair is an eight of another lane), which halves what a
 // row costs beside its values. Bound by instructions for long prompts, which keep the issue slots half busy, and by latency for single tokens.
-// With the read kernel, for 4096 tokens of 2 x 4 x 256 fp32 values in int8: 28 us (84 MB, 12.8 us at the peak), with one eight a lane 30 us;
+// With the read kernel, for 4096 tokens of 2 x 4 x 256 fp32 values in int8: 25 us (84 MB, 12.8 us at the peak); with one eight a lane 2 us more;
 // rows loaded behind the scan 36 us; registers for three blocks an SM 34 us; a block a token with whole warps for every row 54 us.
-template <int FMT, int LANES, int EIGHTS, bool TURN>
+template <int FMT, int LANES, int EIGHTS, bool TURN, bool F32>
 __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p, uint32_t block_tokens) {
     __shared__ float2 cs[TURN ? kMostTokens : 1][kMaxHeadDim / 2];
     __shared__ Place places[kMostTokens];
@@ -289,7 +304,7 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
     const uint32_t lane = threadIdx.x & 31u, part = lane % LANES, rows = tokens * 2 * p.kv.kv_heads;
     const uint32_t step = (blockDim.x >> 5) * (32 / LANES);
     const uint32_t kv_heads = p.kv.kv_heads;
-    float v[kAhead][EIGHTS][8];  // values (part + e * LANES) * 8 and on
+    float v[kAhead][EIGHTS][8];  // fours_of(part, e)
     uint32_t r0 = (threadIdx.x >> 5) * (32 / LANES);
     const Row by(step, 2 * kv_heads);
     Row loads(r0 + lane / LANES, 2 * kv_heads), row = loads;
@@ -299,12 +314,18 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
             const bool values = loads.i >= kv_heads;
             const void *in = values ? p.v_in : p.k_in;
             const bool has = loads.token < tokens && in;
-            const uint64_t from = (t0 + loads.token) * (values ? p.v_stride : p.k_stride) + (loads.i - (values ? kv_heads : 0u)) * p.kv.head_dim + part * 8;
+            const uint64_t from = (t0 + loads.token) * (values ? p.v_stride : p.k_stride) + (loads.i - (values ? kv_heads : 0u)) * p.kv.head_dim;
 #pragma unroll
             for (uint32_t e = 0; e < EIGHTS; ++e) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[k][e][j] = 0.f;
-                if (has && (part + e * LANES) * 8 < p.kv.head_dim) load8(in, from + e * LANES * 8, p.is_f32, v[k][e]);
+                const Fours at = fours_of<LANES>(part, e, F32);
+                if (has && F32) {
+                    if (at.a < p.kv.head_dim) load4(in, from + at.a, v[k][e]);
+                    if (at.b < p.kv.head_dim) load4(in, from + at.b, v[k][e] + 4);
+                } else if (has && at.a < p.kv.head_dim) {
+                    load8(in, from + at.a, TURN ? p.is_f32 : 0u, v[k][e]);
+                }
             }
         }
     };
@@ -387,11 +408,19 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
                     }
                 }
             }
-            uint8_t *const to = (values ? p.kv.v : p.kv.k) + places[at].row + head * p.kv.head_stride + part * (FMT == 0 ? 16 : 8);
+            uint8_t *const to = (values ? p.kv.v : p.kv.k) + places[at].row + head * p.kv.head_stride;
             if (FMT == 0) {
 #pragma unroll
-                for (uint32_t e = 0; e < EIGHTS; ++e)
-                    if (writes && (part + e * LANES) * 8 < p.kv.head_dim) *reinterpret_cast<uint4 *>(to + e * LANES * 16) = pack8_bf16(v[k][e]);
+                for (uint32_t e = 0; e < EIGHTS; ++e) {
+                    const Fours to_of = fours_of<LANES>(part, e, F32);
+                    const uint4 w = pack8_bf16(v[k][e]);
+                    if (!F32) {
+                        if (writes && to_of.a < p.kv.head_dim) *reinterpret_cast<uint4 *>(to + to_of.a * 2) = w;
+                        continue;
+                    }
+                    if (writes && to_of.a < p.kv.head_dim) *reinterpret_cast<uint2 *>(to + to_of.a * 2) = make_uint2(w.x, w.y);
+                    if (writes && to_of.b < p.kv.head_dim) *reinterpret_cast<uint2 *>(to + to_of.b * 2) = make_uint2(w.z, w.w);
+                }
                 continue;
             }
             uint32_t amax = 0;
@@ -404,8 +433,17 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
             const bool finite = amax < 0x7f800000u;
             const float scale = finite ? __fdiv_rn(__uint_as_float(amax), FMT == 1 ? 127.f : 448.f) : __uint_as_float(0x7fc00000u);
 #pragma unroll
-            for (uint32_t e = 0; e < EIGHTS; ++e)
-                if (writes && (part + e * LANES) * 8 < p.kv.head_dim) *reinterpret_cast<uint2 *>(to + e * LANES * 8) = finite ? encode8<FMT == 0 ? 1 : FMT>(v[k][e], scale) : make_uint2(0u, 0u);
+            for (uint32_t e = 0; e < EIGHTS; ++e) {
+                const Fours to_of = fours_of<LANES>(part, e, F32);
+                if (!writes || to_of.a >= p.kv.head_dim) continue;
+                const uint2 w = finite ? encode8<FMT == 0 ? 1 : FMT>(v[k][e], scale) : make_uint2(0u, 0u);
+                if (!F32) {
+                    *reinterpret_cast<uint2 *>(to + to_of.a) = w;
+                    continue;
+                }
+                *reinterpret_cast<uint32_t *>(to + to_of.a) = w.x;
+                if (to_of.b < p.kv.head_dim) *reinterpret_cast<uint32_t *>(to + to_of.b) = w.y;
+            }
             if (writes && part == 0) (values ? p.kv.v_scales : p.kv.k_scales)[places[at].scale + head * p.kv.page_tokens] = scale;
         }
         r0 += kAhead * step;
@@ -414,7 +452,7 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
     }
 }
 
-template <int FMT, int LANES>
+template <int FMT, int LANES, bool F32>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvTokensParams p, uint32_t block_tokens) {
     __shared__ Place places[kMostTokens];
     grid_dependency_wait();
@@ -423,8 +461,10 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvTokensParams p, ui
     const uint32_t tokens = (uint32_t)min((uint64_t)block_tokens, p.tokens - t0);
     if (threadIdx.x < tokens) places[threadIdx.x] = place_of(p, t0 + threadIdx.x);
     __syncthreads();
-    const uint32_t lane = threadIdx.x & 31u, d = lane % LANES * 8u, step = (blockDim.x >> 5) * (32 / LANES);
-    if (d >= p.kv.head_dim) return;
+    const uint32_t lane = threadIdx.x & 31u, step = (blockDim.x >> 5) * (32 / LANES);
+    const Fours d = fours_of<LANES>(lane % LANES, 0, F32);
+    const bool second = !F32 || d.b < p.kv.head_dim;
+    if (d.a >= p.kv.head_dim) return;
     const uint32_t kv_heads = p.kv.kv_heads;
     const Row by(step, 2 * kv_heads);
     Row loads((threadIdx.x >> 5) * (32 / LANES) + lane / LANES, 2 * kv_heads), row = loads;
@@ -443,10 +483,20 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvTokensParams p, ui
             if (!there[k]) continue;
             const uint8_t *from = (values ? p.kv.v : p.kv.k) + places[loads.token].row + head * p.kv.head_stride;
             if (FMT == 0) {
-                held[k] = *reinterpret_cast<const uint4 *>(from + 2 * d);
+                if (!F32) {
+                    held[k] = *reinterpret_cast<const uint4 *>(from + 2 * d.a);
+                    continue;
+                }
+                const uint2 a = *reinterpret_cast<const uint2 *>(from + 2 * d.a), b = second ? *reinterpret_cast<const uint2 *>(from + 2 * d.b) : make_uint2(0u, 0u);
+                held[k] = make_uint4(a.x, a.y, b.x, b.y);
             } else {
-                const uint2 c = *reinterpret_cast<const uint2 *>(from + d);
-                held[k].x = c.x, held[k].y = c.y;
+                if (!F32) {
+                    const uint2 c = *reinterpret_cast<const uint2 *>(from + d.a);
+                    held[k].x = c.x, held[k].y = c.y;
+                } else {
+                    held[k].x = *reinterpret_cast<const uint32_t *>(from + d.a);
+                    if (second) held[k].y = *reinterpret_cast<const uint32_t *>(from + d.b);
+                }
                 scale[k] = (values ? p.kv.v_scales : p.kv.k_scales)[places[loads.token].scale + head * p.kv.page_tokens];
             }
         }
@@ -457,7 +507,14 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvTokensParams p, ui
             float v[8];
             if (FMT == 0) unpack8_bf16(held[k], v);
             else decode8<FMT == 0 ? 1 : FMT>(make_uint2(held[k].x, held[k].y), scale[k], v);
-            store8(values ? p.v_out : p.k_out, (t0 + row.token) * (values ? p.v_stride : p.k_stride) + (row.i - (values ? kv_heads : 0u)) * p.kv.head_dim + d, p.is_f32, v);
+            const uint64_t to = (t0 + row.token) * (values ? p.v_stride : p.k_stride) + (row.i - (values ? kv_heads : 0u)) * p.kv.head_dim;
+            if (F32) {
+                float *const out = static_cast<float *>(values ? p.v_out : p.k_out) + to;
+                *reinterpret_cast<float4 *>(out + d.a) = make_float4(v[0], v[1], v[2], v[3]);
+                if (second) *reinterpret_cast<float4 *>(out + d.b) = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+                store8(values ? p.v_out : p.k_out, to + d.a, 0, v);
+            }
         }
     }
 }
@@ -468,7 +525,10 @@ uint32_t block_tokens(uint64_t tokens, uint32_t sm_count) { return (uint32_t)(to
 template <int FMT, int LANES>
 cudaError_t launch_tokens(const KvTokensParams &p, bool write, uint32_t sm_count, cudaStream_t stream) {
     const uint32_t each = block_tokens(p.tokens, sm_count);
-    const auto kernel = !write ? kv_read_kernel<FMT, LANES> : p.rotary.step && p.k_in ? kv_write_kernel<FMT, LANES, 1, true> : kv_write_kernel<FMT, LANES / 2, 2, false>;
+    const auto kernel = !write                     ? (p.is_f32 ? kv_read_kernel<FMT, LANES, true> : kv_read_kernel<FMT, LANES, false>)
+                        : p.rotary.step && p.k_in ? kv_write_kernel<FMT, LANES, 1, true, false>
+                        : p.is_f32                ? kv_write_kernel<FMT, LANES / 2, 2, false, true>
+                                                  : kv_write_kernel<FMT, LANES / 2, 2, false, false>;
     return launch_dependent(kernel, dim3((uint32_t)((p.tokens + each - 1) / each)), 256, 0, stream, p, each);
 }
 
