@@ -162,10 +162,9 @@ __device__ __forceinline__ void weight_digits(const float (&w)[4], uint32_t (&di
     digit[1] = __byte_perm(high01, high23, 0x5410) ^ 0x80808080u;
     digit[0] = __byte_perm(high01, high23, 0x7632);
 }
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {  // the lower two bytes
-    uint32_t r;
-    asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
-    return r;
+// Four e4m3 numbers as fp16, exactly.
+__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t &lower, uint32_t &upper) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lower), "=r"(upper) : "r"(w));
 }
 
 __device__ __forceinline__ void ldmatrix_x2_trans(uint32_t (&r)[4], uint32_t addr) {
@@ -581,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                                     const uint32_t part[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                                     for (uint32_t i = 0; i < 4; ++i) {
-                                        if (FMT == 2) word[n][2 * i % S::kWords] = e4m3_pair(part[i]), word[n][(2 * i + 1) % S::kWords] = e4m3_pair(part[i] >> 16);
+                                        if (FMT == 2) e4m3_pairs(part[i], word[n][2 * i % S::kWords], word[n][(2 * i + 1) % S::kWords]);
                                         else word[n][i] = part[i];
                                     }
                                 }
@@ -872,8 +871,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll
                                     for (uint32_t set = 0; set < SETS; ++set) mma<FMT>(acc[set][c], wa[set], b0, b1);
                                 } else {
-                                    const uint32_t even[2] = {e4m3_pair(__byte_perm(b0, 0, 0x4420)), e4m3_pair(__byte_perm(b1, 0, 0x4420))};
-                                    const uint32_t odd[2] = {e4m3_pair(__byte_perm(b0, 0, 0x4431)), e4m3_pair(__byte_perm(b1, 0, 0x4431))};
+                                    uint32_t even[2], odd[2];
+                                    e4m3_pairs(__byte_perm(b0, 0, 0x3120), even[0], odd[0]);
+                                    e4m3_pairs(__byte_perm(b1, 0, 0x3120), even[1], odd[1]);
 #pragma unroll
                                     for (uint32_t set = 0; set < SETS; ++set) {
                                         mma<FMT>(acc[set][2 * c], wa[set], even[0], even[1]);
