@@ -985,14 +985,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         // ---- partial results of cut items that are complete, joined in the order of the tiles ----
         // They come by bulk copies into the ring, which is free now: plain loads took 14000 cycles for 36 pieces of 6 KB, copies 3000.
         multipliers_sync();
-        float *const factors = reinterpret_cast<float *>(shared_raw + (weights - raw));  // [piece][row]
         uint32_t phase = 0;
 #pragma unroll 1
         for (uint32_t n = 0; n < left_parts; ++n) {
             const uint32_t *const job = joins + n * 6;
             if (!job[0]) continue;
             const uint32_t owner = job[1], contributors = job[2], seq = job[3], head = job[4] / g.chunks, chunk = job[4] % g.chunks;
-            const uint32_t rows = min(g.rows - chunk * S::kRows, S::kRows), bytes = rows * HDP * 4, room = S::kSlots * S::kSlot / bytes;
+            const uint32_t rows = min(g.rows - chunk * S::kRows, S::kRows), bytes = rows * HDP * 4;
+            // the pieces lie from the ring's start on, factors [piece][row] behind them, in what was there for scales, weights and queries
+            const uint32_t factors_at = full - contributors * S::kRows * 4, room = (factors_at - ring) / bytes;
+            float *const factors = reinterpret_cast<float *>(shared_raw + (factors_at - raw));
             // piece k lies 2 k - 1 places behind the owner's, which is the first one
             const float *const first = p.parts + ((uint64_t)owner * 2 + 1) * kPart;
             const auto piece = [&](uint32_t k) { return first + (k == 0 ? 0 : 2 * k - 1) * kPart; };
