@@ -26,6 +26,10 @@
 //     that they stay in range whatever the scales are.
 //   * The work of all sequences is cut into equal shares by every block for itself (q4_attention_plan.h), from the lengths in device memory:
 //     a captured graph follows them. Results of an item cut over several blocks are joined in order by the last one.
+//
+// Measured, 24 query heads on 4 key heads of 256: one sequence of 262144 int8 tokens 93 to 98 us (545 MB, 5.6 to 5.8 TB/s), of 8200 tokens 13.1 us, 32
+// sequences of 500 to 8000 tokens 58 us (277 MB); four sequences of 9001 to 20011 bf16 tokens with four new ones each 52.8 us (214 MB, 35 us of it in
+// the loop at 6.1 TB/s, the rest is start and joining); 32 heads on 8 of 128, 128 sequences of 3100 to 5100 e4m3 tokens 221 us (1.11 GB, 5.0 TB/s).
 #include <cuda_fp8.h>
 
 #include <atomic>
@@ -983,7 +987,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         } while (more);
 
         // ---- partial results of cut items that are complete, joined in the order of the tiles ----
-        // They come by bulk copies into the ring, which is free now: plain loads took 14000 cycles for 36 pieces of 6 KB, copies 3000.
+        // They come by bulk copies into the ring, which is free now: plain loads took 14000 cycles for 36 pieces of 6 KB, copies 3000. (Adding up a first
+        // half or quarter while the others arrive was slower: 13.7 us in place of 13.1 for 8200 tokens.)
         multipliers_sync();
         uint32_t phase = 0;
 #pragma unroll 1

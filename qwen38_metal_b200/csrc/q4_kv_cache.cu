@@ -452,6 +452,8 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
     }
 }
 
+// The reverse, number = code * scale rounded to the output's type. Bound by memory for long prompts (4096 int8 tokens of 2 x 4 x 256 values to fp32,
+// 42 MB: 10 us, 6.4 at the peak), else by the latencies of position, page number and row, which depend on one another.
 template <int FMT, int LANES, bool F32>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvTokensParams p, uint32_t block_tokens) {
     __shared__ Place places[kMostTokens];
