@@ -49,7 +49,8 @@ constexpr float kNone = -3.0e38f;               // a reference below all scores:
 constexpr float kHeadroom = 8.f;                // how far above its reference a score may lie, in powers of two
 // 8-bit caches: a weight times scale is brought below 2^11 (int8: 2^26) when it becomes the reference and may grow to 2^15 (2^30). As fp16
 // halves, up to the end of fp16's range, weights keep 16 bits down to 2^-19 of the largest one (and 2^-35 of it below); as whole
-// numbers they are off by half at most, 2^-26 of the largest one.
+// numbers they are off by half at most, 2^-26 of the largest one. The factor that brings them there is 2^126 at most, whose reciprocal 32 bits
+// hold: largest ones below 2^-100 (int8) keep fewer bits.
 template <int FMT>
 struct Weights {
     static constexpr int kExponent = FMT == 1 ? 26 : 11;
@@ -663,7 +664,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             float w[4];
 #pragma unroll
                             for (uint32_t i = 0; i < 4; ++i) {
-                                w[i] = FMT == 0 ? weight[4 * t + i] : weight[4 * t + i] * (value_scale[set][4 * t + i] * lift[set]);
+                                // (weight times scale first: the scale of a token that hardly counts may be far above those that set the lift)
+                                w[i] = FMT == 0 ? weight[4 * t + i] : weight[4 * t + i] * value_scale[set][4 * t + i] * lift[set];
                                 if (FMT != 0) of_tile[set] += weight[4 * t + i];
                             }
                             uint32_t a[4];
@@ -733,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             keep[set] = 1.f;
                             if (weight_high * lift[set] > Weights<FMT>::kMost || (lift[set] == 0.f && weight_high > 0.f)) {
                                 const int e = (int)(__float_as_uint(weight_high) >> 23) - 126;  // weight_high < 2^e
-                                const float next = top[set] + (float)max(e - Weights<FMT>::kExponent, -100);
+                                const float next = top[set] + (float)max(e - Weights<FMT>::kExponent, -126);
                                 keep[set] = weight_top[set] == kNone ? 0.f : exp2_fast(weight_top[set] - next);
                                 weight_top[set] = next;
                                 lift[set] = exp2_fast(top[set] - weight_top[set]);
