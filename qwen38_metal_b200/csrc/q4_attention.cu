@@ -47,6 +47,7 @@ constexpr uint32_t kMostSets = 3;               // of eight query rows that a bl
 constexpr uint32_t kLeastRun = 16;              // tiles: shorter runs cost more in joining than they save
 constexpr float kNone = -3.0e38f;               // a reference below all scores: the row has seen nothing
 constexpr float kHeadroom = 8.f;                // how far above its reference a score may lie, in powers of two
+constexpr float kMostLift = 126.f;              // of weights times scales, in powers of two: its reciprocal is a number of 32 bits
 // 8-bit caches: a weight times scale is brought below 2^11 (int8: 2^26) when it becomes the reference and may grow to 2^15 (2^30). As fp16
 // halves, up to the end of fp16's range, weights keep 16 bits down to 2^-19 of the largest one (and 2^-35 of it below); as whole
 // numbers they are off by half at most, 2^-26 of the largest one. The factor that brings them there is 2^126 at most, whose reciprocal 32 bits
@@ -536,10 +537,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             // Results. int8: o itself, from whole-number accumulators of a tile; else accumulators of the upper and lower halves
             float o[SETS][FMT == 1 ? S::kOwn : 1], acc[SETS][FMT == 1 ? 1 : S::kAcc][4];
             float top[SETS], sum[SETS];                          // reference of the row's scores; sum of this lane's weights
-            float weight_top[SETS], lift[SETS], most[SETS];      // 8-bit: reference of weights times scales, 2^(top - weight_top), and what they may be
+            // 8-bit: weights times scales are multiplied by `lift`, a power of two, none yet: 0; and what they may be before that. The lift is kept,
+            // not a second reference as a number: it has to follow jumps of the scores, whose difference may leave the range of 32 bits.
+            float lift[SETS], most[SETS];
 #pragma unroll
             for (uint32_t set = 0; set < SETS; ++set) {
-                top[set] = weight_top[set] = kNone;
+                top[set] = kNone;
                 sum[set] = lift[set] = most[set] = 0.f;
 #pragma unroll
                 for (uint32_t i = 0; i < (FMT == 1 ? S::kOwn : 1); ++i) o[set][i] = 0.f;
@@ -701,16 +704,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         if (quad == 0) highs[warp * S::kRows + set * kAttentionRows + row] = now;
                     }
                     multipliers_sync();
-                    float keep[SETS];
+                    float keep[SETS], raised[SETS];
 #pragma unroll
                     for (uint32_t set = 0; set < SETS; ++set) {
                         float now = -INFINITY;
 #pragma unroll
                         for (uint32_t w = 0; w < kWarps; ++w) now = fmaxf(now, highs[w * S::kRows + set * kAttentionRows + row]);
                         keep[set] = 1.f;
+                        raised[set] = 0.f;
                         if (now - top[set] > kHeadroom) {
                             now = ceilf(now);
-                            keep[set] = exp2_fast(top[set] - now);
+                            raised[set] = now - top[set];
+                            keep[set] = exp2_fast(-raised[set]);
                             sum[set] *= keep[set];
                             top[set] = now;
                         }
@@ -731,14 +736,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             float weight_high = 0.f;
 #pragma unroll
                             for (uint32_t w = 0; w < kWarps; ++w) weight_high = fmaxf(weight_high, weight_highs[w * S::kRows + set * kAttentionRows + row]);
-                            lift[set] = weight_top[set] == kNone ? 0.f : exp2_fast(top[set] - weight_top[set]);
                             keep[set] = 1.f;
-                            if (weight_high * lift[set] > Weights<FMT>::kMost || (lift[set] == 0.f && weight_high > 0.f)) {
-                                const int e = (int)(__float_as_uint(weight_high) >> 23) - 126;  // weight_high < 2^e
-                                const float next = top[set] + (float)max(e - Weights<FMT>::kExponent, -126);
-                                keep[set] = weight_top[set] == kNone ? 0.f : exp2_fast(weight_top[set] - next);
-                                weight_top[set] = next;
-                                lift[set] = exp2_fast(top[set] - weight_top[set]);
+                            if (lift[set] > 0.f || weight_high > 0.f) {
+                                // what has been added up stays as it is with a lift of 2^same, unless that is too much for this tile, or for 32 bits
+                                const float same = lift[set] > 0.f ? (float)((int)(__float_as_uint(lift[set]) >> 23) - 127) + raised[set] : INFINITY;
+                                float next = same;
+                                if (same > kMostLift || weight_high * exp2_fast(same) > Weights<FMT>::kMost) {
+                                    const int e = (int)(__float_as_uint(weight_high) >> 23) - 126;  // weight_high < 2^e
+                                    next = weight_high > 0.f ? fminf((float)(Weights<FMT>::kExponent - e), kMostLift) : kMostLift;
+                                    keep[set] = exp2_fast(next - same);
+                                }
+                                lift[set] = exp2_fast(next);
                             }
                             most[set] = lift[set] > 0.f ? Weights<FMT>::kMost / lift[set] : 0.f;
                         }
@@ -925,7 +933,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 const bool holds = r < g.rows && warp < S::kValueWarps;
                 float mine[S::kOwn];
                 {
-                    const float unlift = FMT == 0 ? 1.f : weight_top[set] == kNone ? 0.f : exp2_fast(weight_top[set] - top[set]);
+                    const float unlift = FMT == 0 ? 1.f : lift[set] > 0.f ? 1.f / lift[set] : 0.f;
 #pragma unroll
                     for (uint32_t i = 0; i < S::kOwn; ++i) {
                         if constexpr (FMT == 1) {

@@ -104,3 +104,67 @@ def test_a_large_value_that_hardly_counts_among_small_ones(runtime, fmt, dim):
         for fall in (60, 90, 110, 125):
             scores[large] = -fall * LN2
             _check(runtime, _cache(fmt, dim, scores, values), n, q)
+
+
+# one block's second step of 256 tokens with one token and with many; items that several blocks work on, in one step and in two
+PLACES = [(257, 256), (300, 270), (9000, 8999), (60011, 330), (60011, 60010)]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim,q_tokens", [(64, 1), (64, 4), (128, 6), (256, 1), (256, 4)])
+@pytest.mark.parametrize("zero", [True, False])
+def test_a_score_that_jumps(runtime, fmt, dim, q_tokens, zero):
+    """A token far above those before it, in powers of two; its value is all zeros or like the others."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(dim + q_tokens)
+    q = _queries(dim, q_tokens)
+    for n, peak in PLACES:
+        scores = torch.rand(n, generator=gen, device="cuda")
+        values = torch.randn(n, 1, dim, generator=gen, device="cuda")
+        if zero:
+            values[peak] = 0.0
+        for jump in (30, 60, 97, 100, 120, 128, 160, 200, 1000):
+            scores[peak] = jump * LN2
+            _check(runtime, _cache(fmt, dim, scores, values), n, q)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_nothing_but_zeros_at_the_top(runtime, fmt, dim):
+    """Scores that rise from step to step with values of zeros, then ordinary values again, and only zeros."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    n = 520  # three steps of one block
+    scores = torch.rand(n, generator=gen, device="cuda") + (torch.arange(n, device="cuda") // 100) * 40 * LN2
+    q = _queries(dim, 2)
+    for first, last in ((256, 512), (256, n), (0, 256), (0, n)):
+        values = torch.randn(n, 1, dim, generator=gen, device="cuda")
+        values[first:last] = 0.0
+        _check(runtime, _cache(fmt, dim, scores, values), n, q)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3", "bf16"])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_scores_that_24_bits_hold_in_steps_above_one(runtime, fmt, dim):
+    """The peak takes all where it is seen from above, and nothing (the others are equal) where its score is negative."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    q = _queries(dim, 1)
+    for n, peak in PLACES + [(300, 3), (9000, 5)]:
+        values = torch.randn(n, 1, dim, generator=gen, device="cuda")
+        for size in (2.0 ** 24, 2.0 ** 27, 2.0 ** 31, 2.0 ** 40, 2.0 ** 100):
+            scores = torch.zeros(n, device="cuda")
+            scores[peak] = size
+            cache = _cache(fmt, dim, scores, values)
+            out = _attend(runtime, cache, n, q)
+            at = torch.arange(n, dtype=torch.int32, device="cuda")
+            held = cache.held(1, torch.zeros_like(at), at)[0][:, 0]
+            # a weight of its own: two roundings of it, three of the sum of digits, or two of halves, and those of the quotient
+            off = (out[0, [0, 1, 3]].double() - held[peak]).abs()
+            assert bool((off <= 2.0 ** -16 * held[peak].abs()).all()), (n, peak, size)
+            others = torch.cat([held[:peak], held[peak + 1:]])
+            off = (out[0, 2].double() - others.mean(0)).abs()
+            assert bool((off <= 2.0 ** -15 * others.abs().mean(0)).all()), (n, peak, size)
