@@ -988,7 +988,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 if (threadIdx.x == 0) {
                     uint32_t *const to = joins + left_parts * 6;
                     const bool last = atomicAdd(p.counters + owner, 1u) + 1 == contributors;
-                    if (last) p.counters[owner] = 0;
+                    if (last) {
+                        __threadfence();  // the others' partial results are read behind the barrier below
+                        p.counters[owner] = 0;
+                    }
                     to[0] = last, to[1] = owner, to[2] = contributors, to[3] = at.s, to[4] = at.item, to[5] = (uint32_t)at.length;
                 }
                 ++left_parts;
