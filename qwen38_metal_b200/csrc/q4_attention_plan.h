@@ -18,6 +18,9 @@ namespace q4 {
 constexpr uint32_t kTileTokens = 16;
 constexpr uint32_t kAttentionRows = 8;  // query rows that are multiplied together
 
+// Scales lie [page][key head][token of the page]: number of a head's, `first` being that of head 0. Heads times tokens may pass 32 bits.
+Q4_PLAN_FN uint64_t kv_scale_index(uint64_t first, uint32_t head, uint32_t page_tokens) { return first + (uint64_t)head * page_tokens; }
+
 Q4_PLAN_FN uint32_t attention_tiles(int64_t length, uint32_t shift) { return length > 0 ? (uint32_t)((length - 1) / kTileTokens >> shift) + 1 : 0u; }
 
 // tile / per for tiles below 2^27, as a product: 2^(32 + shift) / per rounded up is off by less than per <= 2^(shift + 1).

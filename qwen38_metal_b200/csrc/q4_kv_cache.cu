@@ -1,6 +1,7 @@
 // Rotary positions, and a paged cache of keys and values that is quantised as it is written. Counterparts in the reference:
 // src/metal_runtime.rs:5171-5475, 7298-7457, shaders/qwen38.metal:4761-5323 (rotary preparation, int8 append).
 #include "q4_attention.h"
+#include "q4_attention_plan.h"
 
 #include <cuda_fp8.h>
 
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p
                 *reinterpret_cast<uint32_t *>(to + to_of.a) = w.x;
                 if (to_of.b < p.kv.head_dim) *reinterpret_cast<uint32_t *>(to + to_of.b) = w.y;
             }
-            if (writes && part == 0) (values ? p.kv.v_scales : p.kv.k_scales)[places[at].scale + head * p.kv.page_tokens] = scale;
+            if (writes && part == 0) (values ? p.kv.v_scales : p.kv.k_scales)[kv_scale_index(places[at].scale, head, p.kv.page_tokens)] = scale;
         }
         r0 += kAhead * step;
         if (r0 >= rows) break;
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvTokensParams p, ui
                     held[k].x = *reinterpret_cast<const uint32_t *>(from + d.a);
                     if (second) held[k].y = *reinterpret_cast<const uint32_t *>(from + d.b);
                 }
-                scale[k] = (values ? p.kv.v_scales : p.kv.k_scales)[places[loads.token].scale + head * p.kv.page_tokens];
+                scale[k] = (values ? p.kv.v_scales : p.kv.k_scales)[kv_scale_index(places[loads.token].scale, head, p.kv.page_tokens)];
             }
         }
 #pragma unroll
