@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         }
                     }
                     const int32_t token = (int32_t)((tile + warp * S::kOwnSubs) * kTileTokens);
-                    if (token + (int32_t)(S::kOwnSubs * kTileTokens) > sure)  // some rows do not see all of it
+                    if (attention_some_hidden(token, (int32_t)(S::kOwnSubs * kTileTokens), sure))
 #pragma unroll
                         for (uint32_t set = 0; set < SETS; ++set)
 #pragma unroll

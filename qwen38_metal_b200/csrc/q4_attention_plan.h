@@ -35,6 +35,10 @@ inline AttentionPages attention_pages(uint32_t page_tokens, uint32_t tile_shift)
     return d;
 }
 
+// Whether some rows do not see all of `tokens` tokens from `token` on, the first `sure` ones being seen by all. (The last token's number plus one
+// step may pass 31 bits.)
+Q4_PLAN_FN bool attention_some_hidden(int32_t token, int32_t tokens, int32_t sure) { return token > sure - tokens; }
+
 enum AttentionMode : uint32_t {
     kEqualRuns = 0,    // blocks take equal runs through the tiles of all items
     kEqualPieces = 1,  // every item is cut into equal pieces, a block takes one
