@@ -23,7 +23,7 @@ _POOLS = {"bf16": torch.bfloat16, "int8": torch.int8, "e4m3": torch.float8_e4m3f
 class AttentionLayer:
     """`q`, `k`, `v`, `o`: jobs of the four projections (q: heads * head_dim outputs of `hidden` inputs, k and v: kv_heads * head_dim, o:
     `hidden` outputs of heads * head_dim inputs). `sequences` of up to `pages_per_sequence * page_tokens` tokens each; `forward` takes
-    `tokens` (1...16) new ones of every sequence.
+    `tokens` (1...16) new ones of every sequence. Its buffers are on the runtime's device.
 
     The caller keeps up to date, on the device: `table` [sequences][pages_per_sequence] (numbers of the `pages` pages; each sequence has its
     own to begin with), `positions` [sequences * tokens] of the new tokens (negative: padded, for a sequence with fewer of them; they stand in
@@ -31,7 +31,11 @@ class AttentionLayer:
 
     def __init__(self, rt: CudaRuntime, q: MappedQ4AffineJob, k: MappedQ4AffineJob, v: MappedQ4AffineJob, o: MappedQ4AffineJob, hidden: int, heads: int,
                  kv_heads: int, head_dim: int, sequences: int, pages_per_sequence: int, page_tokens: int = 16, cache_format: str = "int8", rotary_dim: int = 64,
-                 rotary_base: float = 1e7, rotary_scaling: dict | None = None, tokens: int = 1, scale: float | None = None, device: int = 0):
+                 rotary_base: float = 1e7, rotary_scaling: dict | None = None, tokens: int = 1, scale: float | None = None, device: int | None = None):
+        if device is None:
+            device = rt.device
+        if device != rt.device:
+            raise Q4RuntimeError(13, f"buffers on device {device}, the runtime is on {rt.device}")
         for name, job, rows in (("q", q, heads * head_dim), ("k", k, kv_heads * head_dim), ("v", v, kv_heads * head_dim), ("o", o, hidden)):
             if job.output_rows != rows:
                 raise Q4RuntimeError(6, f"{name} projection has {job.output_rows} elements, expected {rows}")
