@@ -168,3 +168,20 @@ def test_scores_that_24_bits_hold_in_steps_above_one(runtime, fmt, dim):
             others = torch.cat([held[:peak], held[peak + 1:]])
             off = (out[0, 2].double() - others.mean(0)).abs()
             assert bool((off <= 2.0 ** -15 * others.abs().mean(0)).all()), (n, peak, size)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3", "bf16"])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("size", [-90, -40, 60, 100])
+def test_queries_far_from_one(runtime, fmt, dim, size):
+    """Queries of 2^size times the usual and keys of as much less: the scores are what they always are."""
+    import torch
+
+    from attention_helpers import Cache
+
+    n, q_tokens, heads = 400, 3, 6
+    cache = Cache(fmt, 1, dim, 16, 1, n // 16)
+    cache.fill([n], dim, k_gain=2.0 ** -size)
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    q = torch.randn(q_tokens, heads, dim, generator=gen, device="cuda") * 2.0 ** size * dim ** -0.5
+    _check(runtime, cache, n, q)
