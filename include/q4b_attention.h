@@ -8,7 +8,8 @@
  *
  * The conventions are those of the `_device` calls of q4b200.h: device pointers, work enqueued on the stream that is given,
  * no synchronisation, outputs untouched when a call returns an error, calls on one runtime ordered on the device (they share
- * its scratch; a captured graph may be replayed as long as the runtime lives). None of the `_device` calls allocates.
+ * its scratch; a captured graph may be replayed as long as the runtime, the rotary handles that its calls were given and the
+ * caller's buffers live). None of the `_device` calls allocates.
  *
  * Activations are rows of a token: heads x head_dim values, heads behind each other, `stride` VALUES from one token to the
  * next. Types Q4B_F32 and Q4B_BF16. Addresses are multiples of 16 bytes and so are strides in bytes, else
@@ -64,7 +65,8 @@ typedef struct q4b_rotary q4b_rotary;
 
 /* Keeps the frequencies (rotary_dim / 2 finite numbers, those of q4b_rotary_frequencies or the caller's own) on the device as
  * fractions of a turn in 64 bits: the angle of any int32 position is exact modulo a turn to 2^-33. rotary_dim is even, 2...256.
- * q4b_rotary_destroy waits for the device. */
+ * q4b_rotary_destroy waits for the device and frees them: a graph that has captured a call with the handle may not be replayed
+ * behind it. */
 int q4b_rotary_create(q4b_runtime *rt, const double *inv_freq, uint32_t rotary_dim, int layout, double attention_factor,
                       q4b_rotary **out);
 void q4b_rotary_destroy(q4b_rotary *rotary);

@@ -73,7 +73,8 @@ class AttentionLayer:
         self.positions.copy_(at.reshape(-1))
 
     def forward(self, x_ptr: int, stream: int = 0) -> None:
-        """x [sequences * tokens][hidden] bf16, row s * tokens + i for token i of sequence s; results in `out`."""
+        """x [sequences * tokens][hidden] bf16, row s * tokens + i for token i of sequence s; results in `out`. `stream` is ordered behind what
+        set x, `table`, `positions` and `lengths`."""
         rt, rows, d, f32 = self.rt, self.sequences * self.tokens, self.head_dim, capi.Q4B_F32
         rt.matmul_batch_device(x_ptr, capi.Q4B_BF16, rows, self.hidden, [self.q, self.k, self.v], [t.data_ptr() for t in (self.queries, self.keys, self.values)], 0, stream)
         rt.rotary_device(self.rotary, self.queries.data_ptr(), f32, self.heads * d, rows, self.heads, d, self.positions.data_ptr(), self.queries.data_ptr(), f32, self.heads * d, stream)
@@ -84,4 +85,6 @@ class AttentionLayer:
         rt.matmul_batch_device(self.attended.data_ptr(), capi.Q4B_BF16, rows, self.heads * d, [self.o], [self.out.data_ptr()], 0, stream)
 
     def close(self) -> None:
+        """Frees the rotary frequencies: graphs that have captured `forward` may not be replayed behind it, nor without the layer, whose
+        buffers they use."""
         self.rotary.close()

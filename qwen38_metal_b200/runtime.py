@@ -130,7 +130,8 @@ def rotary_frequencies(rotary_dim: int, base: float, scaling: dict | None = None
 
 
 class Rotary:
-    """Rotary frequencies kept on a device (q4b_rotary)."""
+    """Rotary frequencies kept on a device (q4b_rotary). Calls that a graph has captured read them when it is replayed: keep the object as long
+    as such a graph."""
 
     def __init__(self, rt: "CudaRuntime", handle):
         self._lib, self._h = rt._lib, handle
