@@ -139,8 +139,8 @@ int q4b_kv_read_device(q4b_runtime *rt, const q4b_kv_cache *cache, const q4b_kv_
  *     out = sum_j e^(scale q.k_j) v_j / sum_j e^(scale q.k_j).
  * A row that sees nothing (a length of 0 is a padded sequence) is zero. Products, maxima and sums are held in 32 bits, the
  * factors of each product to 16 bits or more (8-bit caches: queries to 2^-25 of the row's largest one at least, if that one
- * lies between 2^-90 and 2^100; weights times scales to 2^-26 of the largest one or to 2^-127, whichever is more). Weights
- * below 2^-126 of the row's largest one count as nothing. A number that is not finite, in a query or in keys and values,
+ * lies between 2^-90 and 2^100; weights times scales to 2^-26 of the largest one or to 2^-126, whichever is more). Weights
+ * below 2^-125 of the row's largest one count as nothing. A number that is not finite, in a query or in keys and values,
  * reaches the rows that see it and no others. What lies behind a sequence's length in its last page is not looked at,
  * whatever it is.
  * The same call on the same data gives the same bits; another batch around a sequence may change its last bits. Tables that could

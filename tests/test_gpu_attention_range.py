@@ -55,8 +55,9 @@ def _attend(rt, cache, n, q, scale=1.0):
 
 
 def _check(rt, cache, n, q):
-    """Two things are added to the bound: weights below 2^-126 of the row's largest one count as nothing, which takes that much of all values from
-    the result at most; and weights times scales, multiplied by 2^126 at most, are whole numbers (int8) off by half, or e4m3 halves off by 2^-25."""
+    """Two things are added to the bound. Weights are relative to a whole power of two, which lies up to one power above the row's largest score:
+    those below 2^-126 count as nothing, which takes 2^-125 of all values from the result at most. Weights times scales, multiplied by 2^126 at
+    most, are whole numbers (int8) off by half, 2^-127, or e4m3 halves off by 2^-25, 2^-151: twice that of the largest weight."""
     import torch
 
     from attention_helpers import POOLS, attention64, rounded
@@ -65,8 +66,8 @@ def _check(rt, cache, n, q):
     ref, bound = attention64(cache, [n], q, q.shape[0], 1.0)
     at = torch.arange(n, dtype=torch.int32, device="cuda")
     values, raw, _ = cache.held(1, torch.zeros_like(at), at)
-    nothing = 2.0 ** -126 * values.abs().sum(0)
-    steps = 2.0 ** (-127 if cache.fmt == "int8" else -151) * raw.view(POOLS[cache.fmt]).double().abs().sum(0)
+    nothing = 2.0 ** -125 * values.abs().sum(0)
+    steps = 2.0 ** (-126 if cache.fmt == "int8" else -150) * raw.view(POOLS[cache.fmt]).double().abs().sum(0)
     off, most = (out.double() - ref).abs(), rounded(bound + nothing + steps, ref, "f32") - 1e-37 + 1e-43
     assert bool((off <= most).all()), (float((off / most).max()), out.isnan().sum().item())
 
