@@ -22,14 +22,14 @@
 //     lane takes whole 16-byte pieces of a key row; values are read transposed as pairs of bytes, which gives the lane a pair of
 //     dimensions, one for each of two MMAs, and a byte permutation for each brings four tokens into a register.
 //   * One pass: sums and results are relative to a power of two for each row that is raised when a score lies 8 above it, which is seldom
-//     after the first tiles. The scale of a token's values goes into its weight; weights times scales have a reference of their own, so
-//     that they stay in range whatever the scales are.
+//     after the first tiles. The scale of a token's values goes into its weight; weights times scales are lifted by a power of two of their
+//     own, so that they stay in range whatever the scales are, and whatever values lie behind a score that jumps.
 //   * The work of all sequences is cut into equal shares by every block for itself (q4_attention_plan.h), from the lengths in device memory:
 //     a captured graph follows them. Results of an item cut over several blocks are joined in order by the last one.
 //
-// Measured, 24 query heads on 4 key heads of 256: one sequence of 262144 int8 tokens 93 to 98 us (545 MB, 5.6 to 5.8 TB/s), of 8200 tokens 13.1 us, 32
-// sequences of 500 to 8000 tokens 58 us (277 MB); four sequences of 9001 to 20011 bf16 tokens with four new ones each 52.8 us (214 MB, 35 us of it in
-// the loop at 6.1 TB/s, the rest is start and joining); 32 heads on 8 of 128, 128 sequences of 3100 to 5100 e4m3 tokens 221 us (1.11 GB, 5.0 TB/s).
+// Measured, 24 query heads on 4 key heads of 256: one sequence of 262144 int8 tokens 93 to 99 us (545 MB, 5.5 to 5.8 TB/s), of 8200 tokens 13.2 us, 32
+// sequences of 500 to 8000 tokens 58 to 61 us (277 MB); four sequences of 9001 to 20011 bf16 tokens with four new ones each 53 us (214 MB, 35 us of it in
+// the loop at 6.1 TB/s, the rest is start and joining); 32 heads on 8 of 128, 128 sequences of 3100 to 5100 e4m3 tokens 221 to 227 us (1.11 GB, 5.0 TB/s).
 #include <cuda_fp8.h>
 
 #include <atomic>
@@ -48,7 +48,7 @@ constexpr uint32_t kLeastRun = 16;              // tiles: shorter runs cost more
 constexpr float kNone = -3.0e38f;               // a reference below all scores: the row has seen nothing
 constexpr float kHeadroom = 8.f;                // how far above its reference a score may lie, in powers of two
 constexpr float kMostLift = 126.f;              // of weights times scales, in powers of two: its reciprocal is a number of 32 bits
-// 8-bit caches: a weight times scale is brought below 2^11 (int8: 2^26) when it becomes the reference and may grow to 2^15 (2^30). As fp16
+// 8-bit caches: the largest weight times scale is brought below 2^11 (int8: 2^26) when the lift is set and may grow to 2^15 (2^30). As fp16
 // halves, up to the end of fp16's range, weights keep 16 bits down to 2^-19 of the largest one (and 2^-35 of it below); as whole
 // numbers they are off by half at most, 2^-26 of the largest one. The factor that brings them there is 2^126 at most, whose reciprocal 32 bits
 // hold: largest ones below 2^-100 (int8) keep fewer bits.
@@ -1162,6 +1162,9 @@ cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t str
 // 51,000 tokens in four sequences, 4 key heads, us with 1 / 2 / 3 eights an item: bf16 of 256 with 12 rows 62 / 57 / 65, with 24 rows
 // 74 / 72 / 68, with 48 rows 176 / 94 / 96; bf16 of 128 with 32 rows 66 / 51 / 59; e4m3 of 128 with 16 rows 39 / 31 / 45; int8 of 64 with 16 rows
 // 35 / 29 / 35; but int8 of 256 with 24 rows 59 / 74 / 70, e4m3 63 / 72 / 72: the digits, or fp16 pairs, of more rows do not fit the registers.
+// More rows of bf16 of 256, same tokens, 2 / 3 eights an item: 40 rows 102 / 86, 48 rows 102 / 86, 56 and 72 rows 126 / 139, 80 rows 127 / 146,
+// 88 rows 171 / 145: how the items fall on the blocks counts as much as their width, and the rule is on the wrong side by up to a fifth at 48, 56
+// and 72 rows. (Spills of the forms kept: 20 bytes of e4m3 of 64 with two eights, 4 of bf16 of 64 with two and of 256 with three.)
 template <int FMT, int HDP>
 cudaError_t launch_sets(const AttentionParams &p, uint32_t sm_count, cudaStream_t stream) {
     const uint32_t sets = (p.heads / p.kv.kv_heads * p.q_tokens + kAttentionRows - 1) / kAttentionRows;

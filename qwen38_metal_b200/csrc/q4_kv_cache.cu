@@ -96,7 +96,8 @@ __host__ __device__ inline uint32_t head_units(const RotaryView &r, uint32_t hea
 // A block turns `heads` heads of one token; the grid is [tokens][groups of heads]. Bound by memory. A thread has one unit, whose loads go out
 // before the block's turns are computed. (2048 tokens of 24 x 256 values, 64 of them turned, fp32 in and bf16 out: a thread a pair 36 us;
 // a block a token, whose threads take several units in turn, 21 us; this 15.8 us, 18.0 us with registers for five blocks an SM, 21 us for
-// eight, which spill. 11.5 us at the peak.)
+// eight, which spill. 11.5 us at the peak. Halves that are not a multiple of eight values have a value a thread, whose loads and stores of two or
+// four bytes are the bound: the same tokens with 36 to 130 values turned 71 to 75 us; interleaved pairs need no such form, 15 us.)
 __global__ void __launch_bounds__(kRotaryThreads, 6) rotary_kernel(const RotaryParams p, uint32_t heads) {
     __shared__ float2 cs[kMaxHeadDim / 2];
     grid_dependency_wait();
@@ -292,6 +293,10 @@ constexpr uint32_t kRowsAhead = 4;   // eights of values that are on their way t
 // row costs beside its values. Bound by instructions for long prompts, which keep the issue slots half busy, and by latency for single tokens.
 // With the read kernel, for 4096 tokens of 2 x 4 x 256 fp32 values in int8: 25 us (84 MB, 12.8 us at the peak); with one eight a lane 2 us more;
 // rows loaded behind the scan 36 us; registers for three blocks an SM 34 us; a block a token with whole warps for every row 54 us.
+// Writing 4096 tokens of 2 x 4 x 256, us for fp32 / bf16 in: int8 16 / 20, with 64 values of a key turned 20 / 26, with all turned 26 / 30; e4m3
+// 16 / 14, 20 / 21, 26 / 27; bf16 14 / 12, 17 / 17, 23 / 23. Looking through the tokens behind a block's own grows with the square of a call's: int8 from
+// bf16 of 32768 / 65536 / 131072 / 262144 tokens of one sequence 122 / 274 / 743 / 2280 us, in 16 equal runs without sequence numbers, where a run ends
+// the search, 114 / 217 / 431 / 878. (The quantising forms for fp32 rows spill 36 bytes at the 64 registers of four blocks an SM, others up to 8.)
 template <int FMT, int LANES, int EIGHTS, bool TURN, bool F32>
 __global__ void __launch_bounds__(256, 4) kv_write_kernel(const KvTokensParams p, uint32_t block_tokens) {
     __shared__ float2 cs[TURN ? kMostTokens : 1][kMaxHeadDim / 2];
