@@ -2101,12 +2101,14 @@ extern "C" int q4b_device_status(q4b_runtime *rt) {
     DeviceGuard guard(rt->device);
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return fail(Q4B_COMMAND_FAILED, "CUDA command failed: %s", cudaGetErrorString(e));
-    if (int st = finish(rt, rt->stream)) return st;
-    int input = 0;
-    int *word = (int *)rt->error_flag.ptr + kInputErrorWord;
-    Q4B_CUDA(cudaMemcpy(&input, word, sizeof input, cudaMemcpyDeviceToHost), "status download");
-    if (!input) return Q4B_OK;
-    Q4B_CUDA(cudaMemset(word, 0, sizeof input), "status reset");
+    int flags[kInputErrorWord + 1];
+    e = cudaMemcpy(flags, rt->error_flag.ptr, sizeof flags, cudaMemcpyDeviceToHost);
+    if (e != cudaSuccess) return fail(Q4B_COMMAND_FAILED, "CUDA command failed: %s", cudaGetErrorString(e));
+    if (flags[0]) return device_gave_up(rt);
+    if (!flags[kInputErrorWord]) return Q4B_OK;
+    // (waited for: the reset returns before it is done, and would take away what a call on another stream reports behind it)
+    Q4B_CUDA(cudaMemset((int *)rt->error_flag.ptr + kInputErrorWord, 0, sizeof(int)), "status reset");
+    Q4B_CUDA(cudaStreamSynchronize(cudaStreamLegacy), "status reset");
     return fail(Q4B_TENSOR_OUT_OF_RANGE, "a sequence, position, length or page number of an attention call is outside its page table or cache");
 }
 
