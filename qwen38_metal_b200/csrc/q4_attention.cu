@@ -534,8 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             int32_t limit[SETS];
 #pragma unroll
             for (uint32_t set = 0; set < SETS; ++set) limit[set] = row_of(set) < g.rows ? min(at.length - (int32_t)p.q_tokens + 1 + (int32_t)(row_of(set) / g.group), end_token) : 0;
-            // Results. int8: o itself, from whole-number accumulators of a tile; else accumulators of the upper and lower halves
-            float o[SETS][FMT == 1 ? S::kOwn : 1], acc[SETS][FMT == 1 ? 1 : S::kAcc][4];
+            float o[SETS][S::kOwn];  // results: sums of what the tiles' accumulators hold
             float top[SETS], sum[SETS];                          // reference of the row's scores; sum of this lane's weights
             // 8-bit: weights times scales are multiplied by `lift`, a power of two, none yet: 0; and what they may be before that. The lift is kept,
             // not a second reference as a number: it has to follow jumps of the scores, whose difference may leave the range of 32 bits.
@@ -545,9 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 top[set] = kNone;
                 sum[set] = lift[set] = most[set] = 0.f;
 #pragma unroll
-                for (uint32_t i = 0; i < (FMT == 1 ? S::kOwn : 1); ++i) o[set][i] = 0.f;
-#pragma unroll
-                for (uint32_t i = 0; i < (FMT == 1 ? 1 : S::kAcc); ++i) acc[set][i][0] = acc[set][i][1] = acc[set][i][2] = acc[set][i][3] = 0.f;
+                for (uint32_t i = 0; i < S::kOwn; ++i) o[set][i] = 0.f;
             }
 
             for (uint32_t tile = at.begin << shift; tile < end_sub; tile += S::kSubs) {
@@ -752,14 +749,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         }
                     }
 #pragma unroll
-                    for (uint32_t set = 0; set < SETS; ++set) {
+                    for (uint32_t set = 0; set < SETS; ++set)
 #pragma unroll
-                        for (uint32_t i = 0; i < (FMT == 1 ? S::kOwn : 1); ++i) o[set][i] *= keep[set];
-#pragma unroll
-                        for (uint32_t i = 0; i < (FMT == 1 ? 1 : S::kAcc); ++i)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) acc[set][i][j] *= keep[set];
-                    }
+                        for (uint32_t i = 0; i < S::kOwn; ++i) o[set][i] *= keep[set];
                 }
 #pragma unroll
                 for (uint32_t set = 0; set < SETS; ++set) sum[set] += of_tile[set];
@@ -830,6 +822,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                                 o[set][i] += of_digits(upper[set][m][j], upper[set][m][j + 2], lower[set][m][j], lower[set][m][j + 2]);
                             }
                     } else {
+                        // Accumulators of the upper and lower halves, for one tile: an MMA cuts its sum off, so that it falls short by up to 2^-23 with
+                        // every 16 tokens (30,000 tokens in one accumulator were off by 1.6e-4, with a sum a tile it is 2^-24 for its addition).
+                        float acc[SETS][S::kAcc][4];
+#pragma unroll
+                        for (uint32_t set = 0; set < SETS; ++set)
+#pragma unroll
+                            for (uint32_t i = 0; i < S::kAcc; ++i) acc[set][i][0] = acc[set][i][1] = acc[set][i][2] = acc[set][i][3] = 0.f;
                         const auto add_sub = [&](uint32_t t, bool edge) {
                             uint32_t wa[SETS][4];
 #pragma unroll
@@ -904,6 +903,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll 1
                             for (uint32_t t = 0; t < count; ++t) add_sub(t, t >= plain);
                         }
+#pragma unroll
+                        for (uint32_t set = 0; set < SETS; ++set)
+#pragma unroll
+                            for (uint32_t i = 0; i < S::kOwn; ++i) {
+                                const uint32_t m = FMT == 0 ? i / 2 : i / 4 * 2 + i % 2, j = FMT == 0 ? i % 2 : i / 2 % 2;
+                                o[set][i] += acc[set][m][j] + acc[set][m][j + 2];
+                            }
                     }
                 }
                 __syncwarp();
@@ -935,14 +941,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 {
                     const float unlift = FMT == 0 ? 1.f : lift[set] > 0.f ? 1.f / lift[set] : 0.f;
 #pragma unroll
-                    for (uint32_t i = 0; i < S::kOwn; ++i) {
-                        if constexpr (FMT == 1) {
-                            mine[i] = o[set][i] * unlift;
-                        } else {
-                            const uint32_t m = FMT == 0 ? i / 2 : i / 4 * 2 + i % 2, j = FMT == 0 ? i % 2 : i / 2 % 2;
-                            mine[i] = (acc[set][m][j] + acc[set][m][j + 2]) * unlift;
-                        }
-                    }
+                    for (uint32_t i = 0; i < S::kOwn; ++i) mine[i] = o[set][i] * unlift;
                 }
                 float total = 0.f;
 #pragma unroll

@@ -186,3 +186,38 @@ def test_queries_far_from_one(runtime, fmt, dim, size):
     gen = torch.Generator(device="cuda").manual_seed(dim)
     q = torch.randn(q_tokens, heads, dim, generator=gen, device="cuda") * 2.0 ** size * dim ** -0.5
     _check(runtime, cache, n, q)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3", "bf16"])
+@pytest.mark.parametrize("dim,heads", [(64, 1), (64, 16), (128, 1), (128, 16), (256, 1), (256, 16), (256, 24)])
+def test_sums_over_many_tokens_of_one_block(runtime, fmt, dim, heads):
+    """More long sequences than blocks, all reading the same pages. Queries of zero: weights of exactly one, so that the result is the mean of positive
+    values, and off by what its sum loses: steps of 256 tokens at most, in which 16 additions of 16 tokens or less lose a last place of 24
+    bits each, 2^-23; the sum of steps, n / 128 additions that are rounded, 2^-24 each; 2^-21 for joining, the quotient and a weight's halves."""
+    import torch
+
+    from attention_helpers import POOLS, Cache
+
+    n, sequences = 30000, 160
+    cache = Cache(fmt, 1, dim, 16, sequences, n // 16, share=True)
+    at = torch.arange(n, dtype=torch.int32, device="cuda")
+    pages, slots = cache.place(torch.zeros_like(at), at)
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    # of very different size, so that their sum does not fit 24 bits
+    values = (8 + torch.randint(0, 8, (n, 1, dim), generator=gen, device="cuda")) * torch.exp2(-torch.randint(0, 9, (n, 1, dim), generator=gen, device="cuda").float())
+    for side, x in ((0, torch.ones_like(values)), (1, values)):
+        codes = (x.ceil() if fmt == "int8" else x).to(POOLS[fmt])
+        cache.pools[side].view(torch.int16 if fmt == "bf16" else torch.uint8)[pages, :, slots] = codes.view(torch.int16 if fmt == "bf16" else torch.uint8)
+        if cache.scales:
+            cache.scales[side][pages, :, slots] = 0.3
+    want = cache.held(1, torch.zeros_like(at), at)[0].mean(0)[0]
+    from attention_helpers import kind
+
+    q = torch.zeros(sequences, heads, dim, device="cuda")
+    out = torch.full_like(q, math.nan)
+    lengths = torch.full((sequences,), n, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    runtime.attention_device(cache.c, cache.t, lengths.data_ptr(), q.data_ptr(), kind("f32"), heads * dim, heads, 1, 1.0, out.data_ptr(), kind("f32"), heads * dim)
+    runtime.device_status()
+    off = ((out.double() - want) / want).abs().max().item()
+    assert off <= 16 * 2.0 ** -23 + n / 128 * 2.0 ** -24 + 2.0 ** -21, off
