@@ -29,7 +29,7 @@
 //
 // Measured, 24 query heads on 4 key heads of 256: one sequence of 262144 int8 tokens 93 to 99 us (545 MB, 5.5 to 5.8 TB/s), of 8200 tokens 13.2 us, 32
 // sequences of 500 to 8000 tokens 58 to 61 us (277 MB); four sequences of 9001 to 20011 bf16 tokens with four new ones each 53 us (214 MB, 35 us of it in
-// the loop at 6.1 TB/s, the rest is start and joining); 32 heads on 8 of 128, 128 sequences of 3100 to 5100 e4m3 tokens 221 to 227 us (1.11 GB, 5.0 TB/s).
+// the loop at 6.1 TB/s, the rest is start and joining; 2.8e-6 from 64 bits, 1.8e-6 of it by the weights' two halves; sums in 32 bits 2.1e-6); 32 heads on 8 of 128, 128 sequences of 3100 to 5100 e4m3 tokens 221 to 227 us (1.11 GB, 5.0 TB/s).
 #include <cuda_fp8.h>
 
 #include <atomic>
@@ -1158,12 +1158,13 @@ cudaError_t launch(const AttentionParams &p, uint32_t sm_count, cudaStream_t str
 }
 
 // Eights of rows that an item has together read and convert every key and value once; each has more registers and less of the ring. Measured on
-// 51,000 tokens in four sequences, 4 key heads, us with 1 / 2 / 3 eights an item: bf16 of 256 with 12 rows 62 / 57 / 65, with 24 rows
-// 74 / 72 / 68, with 48 rows 176 / 94 / 96; bf16 of 128 with 32 rows 66 / 51 / 59; e4m3 of 128 with 16 rows 39 / 31 / 45; int8 of 64 with 16 rows
-// 35 / 29 / 35; but int8 of 256 with 24 rows 59 / 74 / 70, e4m3 63 / 72 / 72: the digits, or fp16 pairs, of more rows do not fit the registers.
-// More rows of bf16 of 256, same tokens, 2 / 3 eights an item: 40 rows 102 / 86, 48 rows 102 / 86, 56 and 72 rows 126 / 139, 80 rows 127 / 146,
-// 88 rows 171 / 145: how the items fall on the blocks counts as much as their width, and the rule is on the wrong side by up to a fifth at 48, 56
-// and 72 rows. (Spills of the forms kept: 20 bytes of e4m3 of 64 with two eights, 4 of bf16 of 64 with two and of 256 with three.)
+// 51,000 tokens in four sequences, 4 key heads, us with 1 / 2 / 3 eights an item: bf16 of 256 with 12 rows 49 / 44 / 51, with 24 rows
+// 75 / 64 / 55; bf16 of 128 with 32 rows 46 / 42 / 52; e4m3 of 128 with 16 rows 34 / 26 / 35, with 32 rows 52 / 40 / 57; int8 of 128 with 16 rows
+// 32 / 28 / 38; of 64 with 16 rows bf16 27 / 21 / 26, e4m3 31 / 22 / 26, int8 31 / 23 / 30; of 256 with 24 rows int8 63 / 67 / 60, e4m3 62 / 58 / 62:
+// there the digits, or fp16 pairs, of more rows do not fit the registers, and one eight is kept. More rows of bf16 of 256, 2 / 3 eights an item:
+// 40 and 48 rows 104 / 87, 56 and 72 rows 125 to 133 / 143, 80 rows 128 to 142 / 146, 88 rows 175 / 146: how the items fall on the blocks counts as
+// much as their width, and the rule is on the wrong side by up to a fifth at 48, 56 and 72 rows. (Bf16 of 256 with three
+// eights spills 104 bytes.)
 template <int FMT, int HDP>
 cudaError_t launch_sets(const AttentionParams &p, uint32_t sm_count, cudaStream_t stream) {
     const uint32_t sets = (p.heads / p.kv.kv_heads * p.q_tokens + kAttentionRows - 1) / kAttentionRows;
