@@ -136,6 +136,12 @@ class Rotary:
     def __init__(self, rt: "CudaRuntime", handle):
         self._lib, self._h = rt._lib, handle
 
+    @property
+    def handle(self):
+        if self._h is None:
+            raise Q4RuntimeError(13, "rotary handle has been closed")
+        return self._h
+
     def close(self) -> None:
         if getattr(self, "_h", None):
             self._lib.q4b_rotary_destroy(self._h)
@@ -350,7 +356,7 @@ class CudaRuntime:
     def rotary_device(self, rotary: Rotary, x_ptr: int, x_dtype: int, x_stride: int, tokens: int, heads: int, head_dim: int,
                       positions_ptr: int, out_ptr: int, out_dtype: int, out_stride: int, stream: int = 0) -> None:
         """Turn the queries (or keys) of `tokens` tokens by their positions; strides in values. In place if out_ptr is x_ptr."""
-        _check(self._lib.q4b_rotary_device(self._h, rotary._h, x_ptr, x_dtype, x_stride, tokens, heads, head_dim, positions_ptr,
+        _check(self._lib.q4b_rotary_device(self._h, rotary.handle, x_ptr, x_dtype, x_stride, tokens, heads, head_dim, positions_ptr,
                                            out_ptr, out_dtype, out_stride, stream))
 
     def kv_write_device(self, cache: KvCache, table: KvTable, positions_ptr: int, sequences_ptr: int, tokens: int, k_ptr: int,
@@ -358,7 +364,7 @@ class CudaRuntime:
         """Quantise new keys (turned first if `rotary` is given) and values into the cache. sequences_ptr 0: the table's sequences
         have equal runs of tokens; k_ptr or v_ptr 0: that side is left alone."""
         _check(self._lib.q4b_kv_write_device(self._h, cache.c, table.c, positions_ptr, sequences_ptr or None, tokens, k_ptr or None,
-                                             k_stride, v_ptr or None, v_stride, dtype, rotary._h if rotary is not None else None, stream))
+                                             k_stride, v_ptr or None, v_stride, dtype, rotary.handle if rotary is not None else None, stream))
 
     def kv_read_device(self, cache: KvCache, table: KvTable, positions_ptr: int, sequences_ptr: int, tokens: int, k_ptr: int,
                        k_stride: int, v_ptr: int, v_stride: int, dtype: int, stream: int = 0) -> None:
